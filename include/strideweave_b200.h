@@ -516,6 +516,61 @@ int sw_map_f32(int op, int rank, const int64_t* shape,
                float* out, int64_t out_offset, const int64_t* out_stride, int64_t out_size,
                float scalar, void* stream);
 
+/* ---- losses of a linear head --------------------------------------------- */
+
+#define SW_HEAD_F32 0
+#define SW_HEAD_BF16 1
+#define SW_HEAD_NONE 0 /* loss [tokens], upstream [tokens]                            */
+#define SW_HEAD_MEAN 1 /* loss [1]: mean over the rows that count; upstream [1]       */
+#define SW_MAX_TEACHER 256 /* teacher entries of a row                               */
+
+/* A linear head: states h [tokens, dim], weights w [vocab, dim] (both of
+ * `dtype`, element strides), logits s = c h w^T in Float32.  The gradients dh
+ * and dw have the dtype of h and w and strides of their own. */
+typedef struct {
+  int32_t dtype;     /* SW_HEAD_F32 or SW_HEAD_BF16 */
+  int32_t reduction; /* SW_HEAD_NONE or SW_HEAD_MEAN */
+  int64_t tokens, dim, vocab;
+  int64_t h_row, h_col, w_row, w_col;
+  int64_t dh_row, dh_col, dw_row, dw_col;
+  int64_t workspace_limit; /* bytes the pieces of the vocabulary may take (0: the default, 2 GiB) */
+} sw_linear_head;
+
+/* Softmax cross entropy of a linear head, without keeping the logits:
+ *   lse_t = log sum_v exp(s_tv),  loss_t = lse_t - s_{t, targets_t},  c = logit_scale,
+ * and, where dh / dw are given, the gradients of sum_t upstream_t loss_t (or of
+ * upstream times the mean loss); upstream NULL means 1.  A row whose target is
+ * ignore_index has loss 0, lse 0 and no gradient, and its states are not read.
+ * Any other target outside [0, vocab) makes its loss (and the mean) NaN,
+ * leaves the row out of the gradients and sets the device error word to
+ * SW_ERR_INVALID.
+ *
+ * `loss` is Float32 [tokens] or [1]; `lse` is Float32 [tokens] and optional.
+ * With loss NULL the call computes only gradients, from the `lse` an earlier
+ * call returned (the backward node of an autograd graph).  Scratch comes from
+ * the device's stream-ordered pool.  No reference counterpart: the reference's
+ * losses take whole predictions (src/strideweave/nn/modules.py:129-200). */
+int sw_linear_xent(const sw_linear_head* plan, const void* h, const void* w,
+                   const int32_t* targets, int32_t ignore_index, float logit_scale,
+                   float* loss, float* lse, const float* upstream,
+                   void* dh, void* dw, void* stream);
+
+/* Distillation of a linear head from a teacher's top logits.  Row t has top_k
+ * entries: columns index[t, k] with logits[t, k] ([tokens, top_k], row-major);
+ * an entry with a negative index or a logit of -infinity is not one (an index
+ * >= vocab is not one either and sets the device error word).  With
+ * p_t = softmax over the row's entries of logits / temperature and
+ * c = 1 / temperature,
+ *   loss_t = temperature^2 (sum_k p_tk (log p_tk - s_{t, index_tk}) + lse_t),
+ * the Kullback-Leibler divergence of the head's whole softmax from the
+ * teacher's, scaled as usual.  A column may occur twice in a row.  A row
+ * without entries has loss 0, lse 0 and no gradient.  Everything else is as
+ * in sw_linear_xent. */
+int sw_linear_distill(const sw_linear_head* plan, const void* h, const void* w,
+                      const int32_t* index, const float* logits, int32_t top_k,
+                      float temperature, float* loss, float* lse, const float* upstream,
+                      void* dh, void* dw, void* stream);
+
 #if defined(__GNUC__)
 #pragma GCC visibility pop
 #endif

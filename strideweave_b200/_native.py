@@ -55,6 +55,11 @@ SW_XF_GELU = 1
 SW_XF_GELU_GRAD = 2
 SW_NCCL_ID_BYTES = 128
 SW_IPC_HANDLE_BYTES = 64
+SW_HEAD_F32 = 0
+SW_HEAD_BF16 = 1
+SW_HEAD_NONE = 0
+SW_HEAD_MEAN = 1
+SW_MAX_TEACHER = 256
 
 
 class DeviceTimeout(RuntimeError):
@@ -78,6 +83,14 @@ class ReducePlan(ctypes.Structure):
         ("swizzle_base", c_int32 * SW_MAX_SWIZZLE),
         ("swizzle_shift", c_int32 * SW_MAX_SWIZZLE),
     ]
+
+
+class LinearHead(ctypes.Structure):
+    """Mirror of ``sw_linear_head``."""
+
+    _fields_ = [("dtype", c_int32), ("reduction", c_int32)] + [
+        (name, c_int64) for name in ("tokens", "dim", "vocab", "h_row", "h_col", "w_row", "w_col", "dh_row", "dh_col",
+                                     "dw_row", "dw_col", "workspace_limit")]
 
 
 # name -> (restype, argtypes); exactly the functions the header declares.
@@ -198,6 +211,14 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         c_int,
         [c_int, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, POINTER(c_void_p), c_int, c_int64, c_int64,
          c_int, c_int64, c_int64, c_int64, c_int, c_void_p],
+    ),
+    "sw_linear_xent": (
+        c_int, [POINTER(LinearHead), c_void_p, c_void_p, c_void_p, c_int32, ctypes.c_float, c_void_p, c_void_p,
+                c_void_p, c_void_p, c_void_p, c_void_p],
+    ),
+    "sw_linear_distill": (
+        c_int, [POINTER(LinearHead), c_void_p, c_void_p, c_void_p, c_void_p, c_int32, ctypes.c_float, c_void_p,
+                c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
     ),
     "sw_map_f32": (
         c_int,

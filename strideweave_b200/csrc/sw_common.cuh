@@ -20,6 +20,10 @@ int fail(int code, const char* fmt, ...);
 // Clears the calling thread's last-error message and returns SW_OK.
 int ok();
 
+// Lets the device's default memory pool keep what stream-ordered allocations
+// release (defined in sw_runtime.cu): scratch of one call is the next call's.
+int keep_pool_memory(int device);
+
 // Converts a CUDA error into SW_ERR_CUDA with context.
 inline int cuda_fail(cudaError_t err, const char* what) {
     return fail(SW_ERR_CUDA, "%s: %s", what, cudaGetErrorString(err));

@@ -1,0 +1,844 @@
+// sw_linear_head.cu - losses of a linear head over a large vocabulary, with
+// their gradients and without keeping the logits.
+//
+//   s[t, v] = c sum_d h[t, d] w[v, d]       lse_t = log sum_v exp(s[t, v])
+//   cross entropy  loss_t = lse_t - s[t, y_t]
+//   distillation   loss_t = tau^2 (sum_k p_tk (log p_tk - s[t, i_tk]) + lse_t),   c = 1 / tau,
+//                  p_t = softmax of the teacher's entries / tau
+//   dlogits  G[t, v] = g_t c f (exp(s[t, v] - lse_t) - sum_k p_tk [v = i_tk])     (f = 1 or tau^2)
+//   dh = G w,  dw = G^T h
+//
+// Cross entropy is the case of one entry with p = 1, so both run the same
+// kernels.  The rows that count are gathered first (a row that is ignored, or
+// whose teacher has no entry, costs nothing and its states are never read);
+// the contractions of sw_head_gemm.cuh then run over the compact rows.  The
+// forward keeps a (max, sum, target term) triple per row and column tile; the
+// backward walks the vocabulary in pieces: the piece's logits are computed
+// again, their gradient is rounded once to the operand type, and two more
+// contractions take it to dh (summed over the pieces in fp32) and dw.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+
+#include "sw_common.cuh"
+#include "sw_head_gemm.cuh"
+#include "sw_ptx.cuh"
+#include "sw_tma.cuh"
+
+namespace sw {
+namespace head {
+namespace {
+
+constexpr int kMaxTeacher = SW_MAX_TEACHER;
+constexpr int64_t kDefaultWorkspace = int64_t(2) << 30;
+
+__device__ __forceinline__ float warp_max(float v) {
+    for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+__device__ __forceinline__ float warp_sum(float v) {
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+__device__ __forceinline__ bool entry_counts(int index, float logit, int64_t V) {
+    return index >= 0 && index < V && logit != -INFINITY;
+}
+
+// ---- preparation ---------------------------------------------------------------
+
+// flags[t] = 1 when the teacher's row has an entry (a warp per row).
+__global__ void teacher_flags_kernel(const int* index, const float* logits, int64_t T, int K, int64_t V,
+                                     uint8_t* flags) {
+    pdl_enter();
+    const int64_t t = int64_t(blockIdx.x) * (blockDim.x / 32) + threadIdx.x / 32;
+    const int lane = threadIdx.x & 31;
+    if (t >= T) return;
+    bool any = false;
+    for (int k = lane; k < K; k += 32) {
+        const int i = index[t * K + k];
+        if (i >= V) report_device_error(SW_ERR_INVALID);
+        any |= entry_counts(i, logits[t * K + k], V);
+    }
+    any = __any_sync(0xffffffffu, any);
+    if (lane == 0) flags[t] = any;
+}
+
+struct RowsArgs {
+    const int* targets;      // cross entropy, or null
+    int ignore_index;
+    const uint8_t* flags;    // distillation
+    int64_t T, V;
+    const float* upstream;   // null: 1
+    int mean;
+    float factor;            // c f
+    const float* lse;        // a kept lse to start from, or null
+    int* row_map;            // compact rows, then the rows that do not count
+    int* ent_idx;            // cross entropy: the compact rows' targets
+    float* coef;
+    float* lse2;
+    HeadState* state;
+};
+
+// One CTA ranks the rows: row_map[0, count) are the rows that count, in order,
+// row_map[count, T) the others.  Then the factor of each compact row's gradient.
+__global__ void __launch_bounds__(1024) rows_kernel(const RowsArgs a) {
+    __shared__ int warp_n[32];
+    __shared__ int total;
+    pdl_enter();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    int kept = 0, bad = 0;
+    for (int64_t base = 0; base < a.T; base += 1024) {
+        const int64_t t = base + tid;
+        bool keep = false;
+        int y = 0;
+        if (t < a.T) {
+            if (a.targets) {
+                y = a.targets[t];
+                keep = y != a.ignore_index;
+                if (keep && (y < 0 || y >= a.V)) {
+                    keep = false;
+                    bad = 1;
+                }
+            } else {
+                keep = a.flags[t] != 0;
+            }
+        }
+        const uint32_t votes = __ballot_sync(0xffffffffu, keep);
+        if (lane == 0) warp_n[warp] = __popc(votes);
+        __syncthreads();
+        if (warp == 0) {
+            int n = warp_n[lane];
+            for (int o = 1; o < 32; o <<= 1) {
+                const int up = __shfl_up_sync(0xffffffffu, n, o);
+                if (lane >= o) n += up;
+            }
+            warp_n[lane] = n;
+            if (lane == 31) total = n;
+        }
+        __syncthreads();
+        const int before = kept + (warp ? warp_n[warp - 1] : 0) + __popc(votes & ((1u << lane) - 1));
+        if (t < a.T) {
+            if (keep) {
+                a.row_map[before] = int(t);
+                if (a.targets) a.ent_idx[before] = y;
+            } else {
+                a.row_map[a.T - 1 - (t - before)] = int(t);
+            }
+        }
+        kept += total;
+        __syncthreads();
+    }
+    bad = __syncthreads_or(bad);
+    if (tid == 0) {
+        a.state->count = kept;
+        a.state->bad = bad;
+        if (bad) report_device_error(SW_ERR_INVALID);
+        // what every row's gradient is multiplied by stays out of the 16-bit
+        // logits' gradient: a target's -1 is exact there, where the common
+        // factor would round it the same way in every row
+        a.state->grad_scale = a.factor * (a.mean ? (a.upstream ? a.upstream[0] : 1.0f) / float(max(kept, 1)) : 1.0f);
+    }
+    __syncthreads();  // row_map is read back by other threads of this CTA
+    uint32_t top = 0;
+    for (int i = tid; i < kept; i += 1024) {
+        const int t = a.row_map[i];
+        if (a.coef) {
+            const float g = a.mean || !a.upstream ? 1.0f : a.upstream[t];
+            a.coef[i] = g;
+            if (isfinite(g)) top = max(top, __float_as_uint(fabsf(g)));
+        }
+        if (a.lse) a.lse2[i] = a.lse[t] * kLog2e;
+    }
+    if (a.coef && top) atomicMax(&a.state->amax[2], top);
+}
+
+// A warp per compact row: its teacher's probabilities and its entries in
+// ascending column order, the row's sum of p log p, and the first entry of
+// every kEntryTile columns.
+__global__ void teacher_sort_kernel(const int* index, const float* logits, int K, int64_t V, float inv_tau,
+                                    const int* row_map, const HeadState* state, int rows_pad, int tiles,
+                                    int* ent_idx, float* ent_p, float* entropy, uint16_t* offs) {
+    __shared__ int s_idx[4][kMaxTeacher];
+    __shared__ int s_sorted[4][kMaxTeacher];
+    pdl_enter();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int i = blockIdx.x * 4 + warp;
+    if (i >= state->count) return;
+    const int64_t t = row_map[i];
+    float top = -INFINITY;
+    for (int k = lane; k < K; k += 32) {
+        const int col = index[t * K + k];
+        const float x = logits[t * K + k];
+        const bool ok = entry_counts(col, x, V);
+        s_idx[warp][k] = ok ? col : INT_MAX;
+        if (ok) top = fmaxf(top, x * inv_tau);
+    }
+    top = warp_max(top);
+    __syncwarp();
+    float sum = 0.0f;
+    for (int k = lane; k < K; k += 32)
+        if (s_idx[warp][k] != INT_MAX) sum += expf(logits[t * K + k] * inv_tau - top);
+    sum = warp_sum(sum);
+    const float log_sum = logf(sum);
+    float ent = 0.0f;
+    int n = 0;
+    for (int k = lane; k < K; k += 32) {
+        const int col = s_idx[warp][k];
+        int rank = 0;
+        for (int j = 0; j < K; ++j) {
+            const int o = s_idx[warp][j];
+            rank += (o < col) || (o == col && j < k);
+        }
+        float p = 0.0f;
+        if (col != INT_MAX) {
+            const float x = logits[t * K + k] * inv_tau - top;
+            p = expf(x) / sum;
+            if (p > 0.0f || p != p) ent += p * (x - log_sum);
+            ++n;
+        }
+        s_sorted[warp][rank] = col;
+        ent_idx[int64_t(i) * K + rank] = col;
+        ent_p[int64_t(i) * K + rank] = p;
+    }
+    ent = warp_sum(ent);
+    if (lane == 0) entropy[i] = ent;
+    for (int o = 16; o; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+    __syncwarp();
+    for (int tile = lane; tile <= tiles; tile += 32) {
+        const int64_t col0 = int64_t(tile) * kEntryTile;
+        int lo = 0, hi = n;  // entries [0, n) are the real ones
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (s_sorted[warp][mid] < col0) lo = mid + 1;
+            else hi = mid;
+        }
+        offs[int64_t(tile) * rows_pad + i] = uint16_t(lo);
+    }
+}
+
+// Largest finite magnitude of a matrix (the rows of row_map when it is given).
+__global__ void amax_kernel(const float* x, int64_t rows, int64_t cols, int64_t sr, int64_t sc, const int* row_map,
+                            const HeadState* count_from, uint32_t* out) {
+    pdl_enter();
+    if (count_from) rows = count_from->count;
+    const int64_t n = rows * cols;
+    uint32_t top = 0;
+    const bool by_rows = sr == 1 && sc != 1;  // walk the unit stride fastest
+    for (int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; i < n; i += int64_t(gridDim.x) * blockDim.x) {
+        int64_t r = by_rows ? i % rows : i / cols;
+        const int64_t c = by_rows ? i / rows : i % cols;
+        if (row_map) r = row_map[r];
+        const float v = fabsf(x[r * sr + c * sc]);
+        if (v <= 3.402823466e38f) top = max(top, __float_as_uint(v));
+    }
+    for (int o = 16; o; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if ((threadIdx.x & 31) == 0 && top) atomicMax(out, top);
+}
+
+// Gathers rows into the contraction's operand: [rows_pad][ld] 16-bit, a copy
+// of bf16 values, or two f16 planes of a Float32 value times 2^q (hi rounded
+// to nearest, lo the rest).  Rows past the ones that count are zero.
+template <bool kF32>
+__global__ void pack_kernel(const void* src, int64_t rows, int64_t cols, int64_t sr, int64_t sc, const int* row_map,
+                            const HeadState* state, int use_count, int scale_of, uint16_t* dst, int64_t ld,
+                            int64_t rows_pad) {
+    __shared__ float tile[32][33];
+    pdl_enter();
+    const int64_t valid = use_count ? min(rows, int64_t(state->count)) : rows;
+    const float scale = kF32 ? pow2i(scale_exponent(state->amax[scale_of])) : 1.0f;
+    const int64_t r0 = int64_t(blockIdx.x) * 32, c0 = int64_t(blockIdx.y) * 32;
+    const bool by_rows = sr == 1 && sc != 1;
+    const int x = threadIdx.x & 31, y0 = threadIdx.x >> 5;
+    for (int y = y0; y < 32; y += 8) {
+        const int64_t r = r0 + (by_rows ? x : y), c = c0 + (by_rows ? y : x);
+        float v = 0.0f;
+        if (r < valid && c < cols) {
+            const int64_t at = (row_map ? int64_t(row_map[r]) : r) * sr + c * sc;
+            v = kF32 ? static_cast<const float*>(src)[at] : __bfloat162float(static_cast<const __nv_bfloat16*>(src)[at]);
+        }
+        tile[by_rows ? x : y][by_rows ? y : x] = v;
+    }
+    __syncthreads();
+    for (int y = y0; y < 32; y += 8) {
+        const int64_t r = r0 + y, c = c0 + x;
+        if (r >= rows_pad || c >= ld) continue;
+        const float v = tile[y][x];
+        if (kF32) {
+            const float s = v * scale;
+            const __half hi = __float2half_rn(s);
+            dst[r * ld + c] = __half_as_ushort(hi);
+            dst[(rows_pad + r) * ld + c] = __half_as_ushort(__float2half_rn(s - __half2float(hi)));
+        } else {
+            const __nv_bfloat16 b = __float2bfloat16_rn(v);
+            dst[r * ld + c] = __bfloat16_as_ushort(b);
+        }
+    }
+}
+
+// ---- after the forward ---------------------------------------------------------
+
+struct MergeArgs {
+    const float4* partial;
+    int tiles, rows_pad;
+    int64_t T, V;
+    const HeadState* state;
+    const int* row_map;
+    const int* targets;
+    int ignore_index;
+    const float* entropy;    // distillation, or null
+    float factor;            // f
+    float* row_loss;         // compact
+    float* lse2;             // compact
+    float* loss;             // per row, or null
+    float* lse;              // per row, or null
+};
+
+// 32 rows x 8 slices of the tiles per CTA.
+__global__ void __launch_bounds__(256) merge_kernel(const MergeArgs a) {
+    __shared__ float4 part[8][32];
+    pdl_enter();
+    const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
+    const int64_t i = int64_t(blockIdx.x) * 32 + lane;
+    const int count = a.state->count;
+    float ref = -INFINITY, sum = 0.0f, dot = 0.0f;
+    if (i < count) {
+        for (int t = slice; t < a.tiles; t += 8) {
+            const float4 p = a.partial[int64_t(t) * a.rows_pad + i];
+            const float next = fmaxf(ref, p.x), base = next == -INFINITY ? 0.0f : next;
+            sum = sum * ex2(ref - base) + p.y * ex2(p.x - base);
+            ref = next;
+            dot += p.z;
+        }
+    }
+    part[slice][lane] = make_float4(ref, sum, dot, 0.0f);
+    __syncthreads();
+    if (slice || i >= a.T) return;
+    const int64_t row = a.row_map[i];
+    if (i >= count) {
+        float v = 0.0f;
+        if (a.targets && a.targets[row] != a.ignore_index) v = NAN;  // a target outside the vocabulary
+        if (a.loss) a.loss[row] = v;
+        if (a.lse) a.lse[row] = 0.0f;
+        return;
+    }
+    for (int s = 1; s < 8; ++s) {
+        const float4 p = part[s][lane];
+        const float next = fmaxf(ref, p.x), base = next == -INFINITY ? 0.0f : next;
+        sum = sum * ex2(ref - base) + p.y * ex2(p.x - base);
+        ref = next;
+        dot += p.z;
+    }
+    const float l2 = ref + log2f(sum);
+    const float v = a.factor * ((a.entropy ? a.entropy[i] : 0.0f) + (l2 - dot) * kLn2);
+    a.lse2[i] = l2;
+    a.row_loss[i] = v;
+    if (a.loss) a.loss[row] = v;
+    if (a.lse) a.lse[row] = l2 * kLn2;
+}
+
+// loss = mean of the compact rows' losses, summed in a fixed order.
+__global__ void __launch_bounds__(1024) mean_kernel(const float* row_loss, const HeadState* state, float* loss) {
+    __shared__ float part[32];
+    pdl_enter();
+    const int n = state->count;
+    float s = 0.0f;
+    for (int i = threadIdx.x; i < n; i += 1024) s += row_loss[i];
+    s = warp_sum(s);
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s;
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        s = warp_sum(part[threadIdx.x]);
+        if (threadIdx.x == 0) *loss = state->bad ? NAN : s / float(n);
+    }
+}
+
+// Zeroes the gradient of the rows that do not count.
+__global__ void zero_rows_kernel(void* dst, int f32, int64_t T, int64_t D, int64_t sr, int64_t sc, const int* row_map,
+                                 const HeadState* state) {
+    pdl_enter();
+    for (int64_t i = state->count + blockIdx.x; i < T; i += gridDim.x) {
+        const int64_t at = int64_t(row_map[i]) * sr;
+        for (int64_t d = threadIdx.x; d < D; d += blockDim.x) {
+            if (f32) static_cast<float*>(dst)[at + d * sc] = 0.0f;
+            else static_cast<uint16_t*>(dst)[at + d * sc] = 0;
+        }
+    }
+}
+
+// ---- host ----------------------------------------------------------------------
+
+// 2-D map over rows x cols 16-bit elements (pitch ld elements), 64 x box_rows
+// boxes, 128-byte swizzle; what lies outside reads as zero.
+int make_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t ld, uint32_t box_rows) {
+    auto fn = tensor_map_encoder();
+    if (!fn) return fail(SW_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+    cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)(ld * 2)};
+    cuuint32_t box[2] = {(cuuint32_t)kBK, box_rows};
+    cuuint32_t estr[2] = {1, 1};
+    CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(base), dims, strides, box, estr,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(SW_ERR_CUDA, "cuTensorMapEncodeTiled (linear head) failed (%d)", (int)r);
+    return SW_OK;
+}
+
+// A contraction operand: `rows` x `cols` 16-bit elements in memory, pitch ld,
+// `planes` of them `plane` rows apart.
+struct Operand {
+    const uint16_t* ptr;
+    int64_t rows, cols, ld;
+    int planes;
+    int64_t plane;
+};
+
+template <bool kBf16, bool kAMn, bool kBMn, int kEpi>
+int gemm(const Operand& a, const Operand& b, GemmArgs args, cudaStream_t stream) {
+    constexpr int BN = 256, kStages = 4;
+    using Cf = Cfg<BN, kStages>;
+    CUtensorMap ma, mb;
+    // the rows of a plane past its extent belong to the next plane or to
+    // nothing: tiles that reach there read other finite values, whose products
+    // meet only result rows or columns that are not stored, or (along K) zeros
+    int rc = make_map(&ma, a.ptr, a.planes > 1 ? a.plane * (a.planes - 1) + a.rows : a.rows, a.cols, a.ld,
+                      kAMn ? kBK : kBM);
+    if (rc != SW_OK) return rc;
+    rc = make_map(&mb, b.ptr, b.planes > 1 ? b.plane * (b.planes - 1) + b.rows : b.rows, b.cols, b.ld,
+                  kBMn ? kBK : BN);
+    if (rc != SW_OK) return rc;
+    args.terms = a.planes > 1 ? 3 : 1;
+    args.a_plane = (int)a.plane;
+    args.b_plane = (int)b.plane;
+    constexpr bool kChunked = !kBf16 || kEpi == kEpiLse;
+    auto kernel = head_gemm_kernel<BN, kStages, kBf16, kAMn, kBMn, kEpi, kChunked>;
+    SW_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cf::kSmemBytes),
+                "linear head smem");
+    int dev = 0, sms = 148;
+    SW_CUDA_TRY(cudaGetDevice(&dev), "cudaGetDevice");
+    SW_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev), "SM count");
+    const int64_t tiles = int64_t((args.M + kBM - 1) / kBM) * ((args.N + BN - 1) / BN);
+    if (tiles == 0) return SW_OK;
+    SW_CUDA_TRY(launch_pdl(kernel, dim3((unsigned)std::min<int64_t>(tiles, sms)), dim3(Cf::kThreads), Cf::kSmemBytes,
+                           stream, ma, mb, args),
+                "linear head contraction");
+    return SW_OK;
+}
+
+struct Bump {
+    uint8_t* base;
+    int64_t used;
+    template <class T>
+    T* take(int64_t n) {
+        used = (used + 255) / 256 * 256;
+        T* p = base ? reinterpret_cast<T*>(base + used) : nullptr;
+        used += n * (int64_t)sizeof(T);
+        return p;
+    }
+};
+
+int64_t round_up(int64_t x, int64_t q) { return (x + q - 1) / q * q; }
+
+struct Call {
+    const sw_linear_head* plan;
+    const void* h;
+    const void* w;
+    const int32_t* targets;
+    int32_t ignore_index;
+    const int32_t* teacher_index;
+    const float* teacher_logits;
+    int top_k;
+    float scale, factor;     // c, f
+    float* loss;
+    float* lse;
+    const float* upstream;
+    void* dh;
+    void* dw;
+};
+
+// Everything the call needs in device memory, as offsets into one block.
+struct Layout {
+    HeadState* state;
+    uint8_t* flags;
+    int* row_map;
+    int* ent_idx;
+    float* ent_p;
+    float* entropy;
+    uint16_t* offs;
+    float* coef;
+    float* lse2;
+    float* row_loss;
+    uint16_t* hc;
+    float4* partial;
+    float* accum;
+    uint16_t* wp;
+    uint16_t* grad;
+};
+
+struct Shape {
+    int64_t T, D, V, rows_pad, ld_h, ld_w, piece, tiles;
+    bool f32, pack_w, grads;
+    int planes;
+};
+
+Layout lay_out(Bump& b, const Call& c, const Shape& s) {
+    Layout l;
+    memset(&l, 0, sizeof(l));
+    const int64_t K = c.targets ? 1 : c.top_k;
+    l.state = b.take<HeadState>(1);
+    l.row_map = b.take<int>(s.T);
+    l.ent_idx = b.take<int>(s.rows_pad * K);
+    if (!c.targets) {
+        l.flags = b.take<uint8_t>(s.T);
+        l.ent_p = b.take<float>(s.rows_pad * K);
+        l.entropy = b.take<float>(s.rows_pad);
+        l.offs = b.take<uint16_t>(s.rows_pad * ((s.V + kEntryTile - 1) / kEntryTile + 1));
+    }
+    l.coef = b.take<float>(s.rows_pad);
+    l.lse2 = b.take<float>(s.rows_pad);
+    l.row_loss = b.take<float>(s.rows_pad);
+    l.hc = b.take<uint16_t>(s.planes * s.rows_pad * s.ld_h);
+    if (c.loss) l.partial = b.take<float4>(s.tiles * s.rows_pad);
+    if (s.grads && c.dh && s.piece < s.V) l.accum = b.take<float>(s.T * s.D);
+    if (s.pack_w) l.wp = b.take<uint16_t>(s.planes * round_up(s.piece, kBK) * s.ld_w);
+    if (s.grads) l.grad = b.take<uint16_t>(s.planes * s.rows_pad * round_up(s.piece, 64));
+    return l;
+}
+
+template <bool kF32>
+int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
+    const sw_linear_head& p = *c.plan;
+    constexpr bool kBf16 = !kF32;
+    const int esize = kF32 ? 4 : 2;
+    const unsigned row_blocks = (unsigned)((s.rows_pad + 31) / 32);
+    SW_CUDA_TRY(cudaMemsetAsync(l.state, 0, sizeof(HeadState), stream), "linear head state");
+    if (!c.targets)
+        SW_CUDA_TRY(launch_pdl(teacher_flags_kernel, dim3((unsigned)std::max<int64_t>((s.T + 7) / 8, 1)), dim3(256), 0, stream,
+                               c.teacher_index, c.teacher_logits, s.T, c.top_k, s.V, l.flags),
+                    "teacher rows");
+    RowsArgs ra;
+    memset(&ra, 0, sizeof(ra));
+    ra.targets = c.targets;
+    ra.ignore_index = c.ignore_index;
+    ra.flags = l.flags;
+    ra.T = s.T;
+    ra.V = s.V;
+    ra.upstream = c.upstream;
+    ra.mean = p.reduction == SW_HEAD_MEAN;
+    ra.factor = c.scale * c.factor;
+    ra.lse = c.loss ? nullptr : c.lse;
+    ra.row_map = l.row_map;
+    ra.ent_idx = l.ent_idx;
+    ra.coef = s.grads ? l.coef : nullptr;
+    ra.lse2 = l.lse2;
+    ra.state = l.state;
+    SW_CUDA_TRY(launch_pdl(rows_kernel, dim3(1), dim3(1024), 0, stream, ra), "linear head rows");
+    if (!c.targets)
+        SW_CUDA_TRY(launch_pdl(teacher_sort_kernel, dim3((unsigned)std::max<int64_t>((s.T + 3) / 4, 1)), dim3(128), 0, stream,
+                               c.teacher_index, c.teacher_logits, c.top_k, s.V, c.scale, l.row_map, l.state,
+                               (int)s.rows_pad, (int)((s.V + kEntryTile - 1) / kEntryTile), l.ent_idx, l.ent_p,
+                               l.entropy, l.offs),
+                    "teacher entries");
+    if (kF32) {
+        SW_CUDA_TRY(launch_pdl(amax_kernel, dim3(592), dim3(256), 0, stream, (const float*)c.h, s.T, s.D, p.h_row,
+                               p.h_col, l.row_map, l.state, &l.state->amax[0]),
+                    "linear head scale");
+        SW_CUDA_TRY(launch_pdl(amax_kernel, dim3(592), dim3(256), 0, stream, (const float*)c.w, s.V, s.D, p.w_row,
+                               p.w_col, (const int*)nullptr, (const HeadState*)nullptr, &l.state->amax[1]),
+                    "linear head scale");
+    }
+    SW_CUDA_TRY(launch_pdl(pack_kernel<kF32>, dim3(row_blocks, (unsigned)((s.ld_h + 31) / 32)), dim3(256), 0, stream,
+                           c.h, s.T, s.D, p.h_row, p.h_col, l.row_map, l.state, 1, 0, l.hc, s.ld_h, s.rows_pad),
+                "linear head states");
+    const Operand hk{l.hc, s.rows_pad, s.D, s.ld_h, s.planes, s.rows_pad};
+
+    GemmArgs g;
+    memset(&g, 0, sizeof(g));
+    g.state = l.state;
+    g.logit_scale = c.scale;
+    g.ent_idx = l.ent_idx;
+    g.ent_p = l.ent_p;
+    g.offs = l.offs;
+    g.ent_k = c.targets ? 1 : c.top_k;
+    g.rows_pad = (int)s.rows_pad;
+    g.partial = l.partial;
+    g.lse2 = l.lse2;
+    g.coef = l.coef;
+    g.grad = l.grad;
+    g.ld_grad = round_up(s.piece, 64);
+    g.split = kF32;
+    g.accum = l.accum;
+    g.ld_accum = s.D;
+
+    // the weights of columns [v0, v0 + n): in place, or packed into the workspace
+    auto weights = [&](int64_t v0, int64_t n, Operand* out) -> int {
+        const uint8_t* at = static_cast<const uint8_t*>(c.w) + v0 * p.w_row * esize;
+        if (!s.pack_w) {
+            *out = Operand{reinterpret_cast<const uint16_t*>(at), n, s.D, p.w_row, 1, 0};
+            return SW_OK;
+        }
+        // zero rows up to whole K stages: a tail of G's zeros must not meet the next plane
+        const int64_t rows = round_up(n, kBK);
+        SW_CUDA_TRY(launch_pdl(pack_kernel<kF32>, dim3((unsigned)((rows + 31) / 32), (unsigned)((s.ld_w + 31) / 32)),
+                               dim3(256), 0, stream, (const void*)at, n, s.D, p.w_row, p.w_col, (const int*)nullptr,
+                               l.state, 0, 1, l.wp, s.ld_w, rows),
+                    "linear head weights");
+        *out = Operand{l.wp, rows, s.D, s.ld_w, s.planes, rows};
+        return SW_OK;
+    };
+
+    if (c.loss) {
+        const int64_t step = s.pack_w ? s.piece : s.V;
+        for (int64_t v0 = 0; v0 < s.V; v0 += step) {
+            const int64_t n = std::min(step, s.V - v0);
+            Operand w;
+            int rc = weights(v0, n, &w);
+            if (rc != SW_OK) return rc;
+            GemmArgs a = g;
+            a.M = (int)s.T;
+            a.N = (int)n;
+            a.K = (int)s.D;
+            a.count_is = kCountM;
+            a.scale_a = kF32 ? 0 : -1;
+            a.scale_b = kF32 ? 1 : -1;
+            a.v0 = v0;
+            rc = gemm<kBf16, false, false, kEpiLse>(hk, w, a, stream);
+            if (rc != SW_OK) return rc;
+        }
+        MergeArgs m;
+        memset(&m, 0, sizeof(m));
+        m.partial = l.partial;
+        m.tiles = (int)s.tiles;
+        m.rows_pad = (int)s.rows_pad;
+        m.T = s.T;
+        m.V = s.V;
+        m.state = l.state;
+        m.row_map = l.row_map;
+        m.targets = c.targets;
+        m.ignore_index = c.ignore_index;
+        m.entropy = l.entropy;
+        m.factor = c.factor;
+        m.row_loss = l.row_loss;
+        m.lse2 = l.lse2;
+        m.loss = p.reduction == SW_HEAD_MEAN ? nullptr : c.loss;
+        m.lse = c.lse;
+        SW_CUDA_TRY(launch_pdl(merge_kernel, dim3((unsigned)std::max<int64_t>((s.T + 31) / 32, 1)), dim3(256), 0, stream, m),
+                    "linear head loss");
+        if (p.reduction == SW_HEAD_MEAN)
+            SW_CUDA_TRY(launch_pdl(mean_kernel, dim3(1), dim3(1024), 0, stream, l.row_loss, l.state, c.loss),
+                        "linear head mean loss");
+    }
+    if (!s.grads) return SW_OK;
+    if (c.dh && s.T > 0)
+        SW_CUDA_TRY(launch_pdl(zero_rows_kernel, dim3((unsigned)std::min<int64_t>(s.T, 1184)), dim3(256), 0, stream,
+                               c.dh, (int)kF32, s.T, s.D, p.dh_row, p.dh_col, l.row_map, l.state),
+                    "linear head ignored rows");
+    for (int64_t v0 = 0; v0 < s.V; v0 += s.piece) {
+        const int64_t n = std::min(s.piece, s.V - v0);
+        Operand w;
+        int rc = weights(v0, n, &w);
+        if (rc != SW_OK) return rc;
+        GemmArgs a = g;
+        a.M = (int)s.T;
+        a.N = (int)n;
+        a.K = (int)s.D;
+        a.count_is = kCountM;
+        a.scale_a = kF32 ? 0 : -1;
+        a.scale_b = kF32 ? 1 : -1;
+        a.v0 = v0;
+        rc = gemm<kBf16, false, false, kEpiGrad>(hk, w, a, stream);
+        if (rc != SW_OK) return rc;
+        const Operand gr{l.grad, s.rows_pad, n, g.ld_grad, s.planes, s.rows_pad};
+        a.dst_f32 = kF32;
+        if (c.dh) {
+            a.M = (int)s.T;
+            a.N = (int)s.D;
+            a.K = (int)n;
+            a.count_is = kCountM;
+            a.scale_a = kF32 ? 2 : -1;
+            a.scale_b = kF32 ? 1 : -1;
+            a.first = v0 == 0;
+            a.last = v0 + n == s.V;
+            a.dst = c.dh;
+            a.dst_row = p.dh_row;
+            a.dst_col = p.dh_col;
+            a.row_map = l.row_map;
+            rc = gemm<kBf16, false, true, kEpiOut>(gr, w, a, stream);
+            if (rc != SW_OK) return rc;
+        }
+        if (c.dw) {
+            a.M = (int)n;
+            a.N = (int)s.D;
+            a.K = (int)s.T;
+            a.count_is = kCountK;
+            a.scale_a = kF32 ? 2 : -1;
+            a.scale_b = kF32 ? 0 : -1;
+            a.accum = nullptr;
+            a.row_map = nullptr;
+            a.dst = static_cast<uint8_t*>(c.dw) + v0 * p.dw_row * esize;
+            a.dst_row = p.dw_row;
+            a.dst_col = p.dw_col;
+            rc = gemm<kBf16, true, true, kEpiOut>(gr, hk, a, stream);
+            if (rc != SW_OK) return rc;
+        }
+    }
+    return SW_OK;
+}
+
+// A matrix's strides must reach each element once (gradients) and fit 63 bits.
+bool strides_ok(int64_t rows, int64_t cols, int64_t sr, int64_t sc, bool distinct) {
+    if (sr < 0 || sc < 0) return false;
+    const int64_t lim = int64_t(1) << 52;
+    if ((rows > 1 && sr > lim / rows) || (cols > 1 && sc > lim / cols)) return false;
+    if (!distinct) return true;
+    if (rows > 1 && sr == 0) return false;
+    if (cols > 1 && sc == 0) return false;
+    if (rows == 1 || cols == 1) return true;
+    return sr <= sc ? sc > (rows - 1) * sr : sr > (cols - 1) * sc;
+}
+
+int check_and_run(const char* name, Call& c, void* stream_ptr) {
+    const sw_linear_head* p = c.plan;
+    if (!p) return fail(SW_ERR_INVALID, "%s: null plan", name);
+    if (p->dtype != SW_HEAD_F32 && p->dtype != SW_HEAD_BF16)
+        return fail(SW_ERR_INVALID, "%s: unknown dtype %d", name, (int)p->dtype);
+    if (p->reduction != SW_HEAD_NONE && p->reduction != SW_HEAD_MEAN)
+        return fail(SW_ERR_INVALID, "%s: unknown reduction %d", name, (int)p->reduction);
+    if (p->tokens < 0 || p->dim < 1 || p->vocab < 1)
+        return fail(SW_ERR_INVALID, "%s: tokens must be >= 0, dim and vocab positive (got %lld, %lld, %lld)", name,
+                    (long long)p->tokens, (long long)p->dim, (long long)p->vocab);
+    const int64_t lim = int64_t(1) << 30;
+    if (p->tokens > lim || p->dim > lim || p->vocab > lim)
+        return fail(SW_ERR_UNSUPPORTED, "%s: extents above 2^30 are not supported", name);
+    if (((p->tokens + kBM - 1) / kBM) * ((p->vocab + 63) / 64) > INT32_MAX ||
+        ((p->vocab + kBM - 1) / kBM) * ((p->dim + 63) / 64) > INT32_MAX || (p->dim + 31) / 32 > 65535)
+        return fail(SW_ERR_UNSUPPORTED, "%s: too many tiles", name);
+    if (p->workspace_limit < 0) return fail(SW_ERR_INVALID, "%s: negative workspace limit", name);
+    if (!(c.scale > 0.0f) || !std::isfinite(c.scale) || !std::isfinite(c.factor))
+        return fail(SW_ERR_INVALID, "%s: the logit scale or temperature must be positive and finite", name);
+    const bool grads = c.dh || c.dw;
+    // (the vectors of no rows may be null)
+    if (!c.loss && !grads && p->tokens == 0 && p->reduction == SW_HEAD_NONE) return ok();
+    if (!c.loss && !grads) return fail(SW_ERR_INVALID, "%s: neither a loss nor a gradient is asked for", name);
+    if (!c.loss && !c.lse && p->tokens > 0)
+        return fail(SW_ERR_INVALID, "%s: a gradient without the loss needs the kept lse", name);
+    const int64_t T = p->tokens, D = p->dim, V = p->vocab;
+    if (T > 0 && !c.h) return fail(SW_ERR_INVALID, "%s: null states", name);
+    if (!c.w) return fail(SW_ERR_INVALID, "%s: null weights", name);
+    if (!strides_ok(T, D, p->h_row, p->h_col, false) || !strides_ok(V, D, p->w_row, p->w_col, false))
+        return fail(SW_ERR_INVALID, "%s: bad strides of the states or weights", name);
+    if (c.dh && !strides_ok(T, D, p->dh_row, p->dh_col, true))
+        return fail(SW_ERR_INVALID, "%s: the strides of dh must reach every element once", name);
+    if (c.dw && !strides_ok(V, D, p->dw_row, p->dw_col, true))
+        return fail(SW_ERR_INVALID, "%s: the strides of dw must reach every element once", name);
+    const uintptr_t align = p->dtype == SW_HEAD_F32 ? 3 : 1;
+    if ((reinterpret_cast<uintptr_t>(c.h) | reinterpret_cast<uintptr_t>(c.w) | reinterpret_cast<uintptr_t>(c.dh) |
+         reinterpret_cast<uintptr_t>(c.dw)) & align)
+        return fail(SW_ERR_INVALID, "%s: a matrix is not aligned to its elements", name);
+    if ((reinterpret_cast<uintptr_t>(c.loss) | reinterpret_cast<uintptr_t>(c.lse) |
+         reinterpret_cast<uintptr_t>(c.upstream) | reinterpret_cast<uintptr_t>(c.targets) |
+         reinterpret_cast<uintptr_t>(c.teacher_index) | reinterpret_cast<uintptr_t>(c.teacher_logits)) & 3)
+        return fail(SW_ERR_INVALID, "%s: a vector is not aligned to its elements", name);
+    cudaStream_t stream = (cudaStream_t)stream_ptr;
+
+    Shape s;
+    s.T = T;
+    s.D = D;
+    s.V = V;
+    s.f32 = p->dtype == SW_HEAD_F32;
+    s.planes = s.f32 ? 2 : 1;
+    s.rows_pad = std::max<int64_t>(round_up(T, kBM), kBM);
+    s.ld_h = s.ld_w = round_up(D, 8);
+    s.grads = grads;
+    s.tiles = (V + 255) / 256 * 2;  // half tiles, each with its own partial statistics
+    // weights are read in place when TMA can: bf16, unit stride, 16-byte rows
+    s.pack_w = s.f32 || p->w_col != 1 || p->w_row % 8 != 0 || p->w_row < D ||
+               (reinterpret_cast<uintptr_t>(c.w) & 15) != 0;
+    // the piece of the vocabulary: as wide as the workspace limit allows, in
+    // whole 256-column tiles
+    const int64_t per_column = (grads ? s.planes * s.rows_pad * 2 : 0) + (s.pack_w ? s.planes * s.ld_w * 2 : 0);
+    const int64_t budget = p->workspace_limit > 0 ? p->workspace_limit : kDefaultWorkspace;
+    s.piece = round_up(V, 256);
+    if (per_column > 0) s.piece = std::min(s.piece, std::max<int64_t>(budget / per_column / 256 * 256, 256));
+
+    Bump measure{nullptr, 0};
+    lay_out(measure, c, s);
+    void* ws = nullptr;
+    int dev = 0;
+    SW_CUDA_TRY(cudaGetDevice(&dev), "cudaGetDevice");
+    const int pooled = keep_pool_memory(dev);
+    if (pooled != SW_OK) return pooled;
+    cudaError_t err = cudaMallocAsync(&ws, (size_t)measure.used, stream);
+    if (err == cudaErrorMemoryAllocation) {
+        cudaGetLastError();
+        return fail(SW_ERR_NOMEM, "%s: out of device memory for %lld bytes of workspace", name,
+                    (long long)measure.used);
+    }
+    SW_CUDA_TRY(err, "cudaMallocAsync (linear head workspace)");
+    Bump real{static_cast<uint8_t*>(ws), 0};
+    const Layout l = lay_out(real, c, s);
+    const int rc = s.f32 ? run<true>(c, s, l, stream) : run<false>(c, s, l, stream);
+    const cudaError_t freed = cudaFreeAsync(ws, stream);
+    if (rc != SW_OK) return rc;
+    SW_CUDA_TRY(freed, "cudaFreeAsync (linear head workspace)");
+    return ok();
+}
+
+}  // namespace
+}  // namespace head
+}  // namespace sw
+
+extern "C" int sw_linear_xent(const sw_linear_head* plan, const void* h, const void* w, const int32_t* targets,
+                              int32_t ignore_index, float logit_scale, float* loss, float* lse, const float* upstream,
+                              void* dh, void* dw, void* stream) {
+    using namespace sw;
+    if (plan && plan->tokens > 0 && !targets) return fail(SW_ERR_INVALID, "sw_linear_xent: null targets");
+    static const int32_t none = 0;  // no rows: the list is never read
+    head::Call c;
+    memset(&c, 0, sizeof(c));
+    c.plan = plan;
+    c.h = h;
+    c.w = w;
+    c.targets = targets ? targets : &none;
+    c.ignore_index = ignore_index;
+    c.top_k = 1;
+    c.scale = logit_scale;
+    c.factor = 1.0f;
+    c.loss = loss;
+    c.lse = lse;
+    c.upstream = upstream;
+    c.dh = dh;
+    c.dw = dw;
+    return head::check_and_run("sw_linear_xent", c, stream);
+}
+
+extern "C" int sw_linear_distill(const sw_linear_head* plan, const void* h, const void* w, const int32_t* index,
+                                 const float* logits, int32_t top_k, float temperature, float* loss, float* lse,
+                                 const float* upstream, void* dh, void* dw, void* stream) {
+    using namespace sw;
+    if (plan && plan->tokens > 0 && (!index || !logits))
+        return fail(SW_ERR_INVALID, "sw_linear_distill: null teacher entries");
+    if (top_k < 1 || top_k > SW_MAX_TEACHER)
+        return fail(SW_ERR_INVALID, "sw_linear_distill: 1 to %d teacher entries a row (got %d)", SW_MAX_TEACHER,
+                    (int)top_k);
+    if (!(temperature > 0.0f) || !std::isfinite(temperature))
+        return fail(SW_ERR_INVALID, "sw_linear_distill: the temperature must be positive and finite");
+    head::Call c;
+    memset(&c, 0, sizeof(c));
+    c.plan = plan;
+    c.h = h;
+    c.w = w;
+    c.teacher_index = index;
+    c.teacher_logits = logits;
+    c.top_k = top_k;
+    c.scale = 1.0f / temperature;
+    c.factor = temperature * temperature;
+    c.loss = loss;
+    c.lse = lse;
+    c.upstream = upstream;
+    c.dh = dh;
+    c.dw = dw;
+    return head::check_and_run("sw_linear_distill", c, stream);
+}

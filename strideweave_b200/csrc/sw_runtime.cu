@@ -91,6 +91,12 @@ static int ensure_pool(int device) {
     return SW_OK;
 }
 
+}  // extern "C"
+
+int sw::keep_pool_memory(int device) { return ensure_pool(device); }
+
+extern "C" {
+
 int sw_alloc(void** ptr, int64_t bytes) {
     if (!ptr) return fail(SW_ERR_INVALID, "sw_alloc: null output");
     *ptr = nullptr;

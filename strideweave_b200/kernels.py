@@ -194,3 +194,55 @@ def matmul_f32(a_ptr: int, sam: int, sak: int, b_ptr: int, sbn: int, sbk: int, c
     N.check(N.lib.sw_matmul_f32_batched_ex(c_void_p(a_ptr), 0, sam, sak, c_void_p(b_ptr), 0, sbn, sbk,
                                            c_void_p(c_ptr), 0, scm, scn, 1, M, N_, K,
                                            N.SW_ACC_F64 if acc64 else N.SW_ACC_F32, c_void_p(stream)))
+
+
+HEAD_DTYPES = {"Float32": N.SW_HEAD_F32, "BFloat16": N.SW_HEAD_BF16}
+HEAD_REDUCTIONS = {"none": N.SW_HEAD_NONE, "mean": N.SW_HEAD_MEAN}
+
+
+def _linear_head(dtype: str, h_strides: Sequence[int], w_strides: Sequence[int], tokens: int, vocab: int, dim: int,
+                 reduction: str, dh_strides: Sequence[int] | None, dw_strides: Sequence[int] | None,
+                 workspace_limit: int) -> N.LinearHead:
+    if dtype not in HEAD_DTYPES:
+        raise NotImplementedError(f"no linear head kernel for dtype {dtype!r}")
+    if reduction not in HEAD_REDUCTIONS:
+        raise ValueError(f"unknown reduction {reduction!r}")
+    dh = (dim, 1) if dh_strides is None else dh_strides
+    dw = (dim, 1) if dw_strides is None else dw_strides
+    return N.LinearHead(HEAD_DTYPES[dtype], HEAD_REDUCTIONS[reduction], tokens, dim, vocab, *h_strides, *w_strides,
+                        *dh, *dw, workspace_limit)
+
+
+def linear_cross_entropy(dtype: str, h_ptr: int, h_strides: Sequence[int], w_ptr: int, w_strides: Sequence[int],
+                         tokens: int, vocab: int, dim: int, targets_ptr: int, *, ignore_index: int = -100,
+                         logit_scale: float = 1.0, reduction: str = "none", loss_ptr: int = 0, lse_ptr: int = 0,
+                         upstream_ptr: int = 0, dh_ptr: int = 0, dh_strides: Sequence[int] | None = None,
+                         dw_ptr: int = 0, dw_strides: Sequence[int] | None = None, workspace_limit: int = 0,
+                         stream: int = 0) -> None:
+    """Cross entropy of logit_scale * h w^T against Int32 targets, h [tokens, dim]
+    and w [vocab, dim] of ``dtype`` ("Float32" or "BFloat16", element strides),
+    and its gradients where ``dh_ptr`` / ``dw_ptr`` are given (row-major unless
+    strides say otherwise).  With ``loss_ptr`` 0 the gradients start from the
+    lse at ``lse_ptr``.  See sw_linear_xent."""
+    plan = _linear_head(dtype, h_strides, w_strides, tokens, vocab, dim, reduction, dh_strides, dw_strides,
+                        workspace_limit)
+    N.check(N.lib.sw_linear_xent(byref(plan), h_ptr or None, w_ptr or None, targets_ptr or None, ignore_index,
+                                 logit_scale, loss_ptr or None, lse_ptr or None, upstream_ptr or None, dh_ptr or None,
+                                 dw_ptr or None, stream or None))
+
+
+def linear_distillation(dtype: str, h_ptr: int, h_strides: Sequence[int], w_ptr: int, w_strides: Sequence[int],
+                        tokens: int, vocab: int, dim: int, index_ptr: int, logits_ptr: int, top_k: int, *,
+                        temperature: float = 1.0, reduction: str = "none", loss_ptr: int = 0, lse_ptr: int = 0,
+                        upstream_ptr: int = 0, dh_ptr: int = 0, dh_strides: Sequence[int] | None = None,
+                        dw_ptr: int = 0, dw_strides: Sequence[int] | None = None, workspace_limit: int = 0,
+                        stream: int = 0) -> None:
+    """Distillation of the head h w^T from a teacher's ``top_k`` logits a row:
+    Int32 columns and Float32 logits, both [tokens, top_k] row-major, an absent
+    entry marked by a negative column.  The other arguments are those of
+    ``linear_cross_entropy``.  See sw_linear_distill."""
+    plan = _linear_head(dtype, h_strides, w_strides, tokens, vocab, dim, reduction, dh_strides, dw_strides,
+                        workspace_limit)
+    N.check(N.lib.sw_linear_distill(byref(plan), h_ptr or None, w_ptr or None, index_ptr or None, logits_ptr or None,
+                                    top_k, temperature, loss_ptr or None, lse_ptr or None, upstream_ptr or None,
+                                    dh_ptr or None, dw_ptr or None, stream or None))
