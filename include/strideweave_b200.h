@@ -533,7 +533,7 @@ typedef struct {
   int64_t tokens, dim, vocab;
   int64_t h_row, h_col, w_row, w_col;
   int64_t dh_row, dh_col, dw_row, dw_col;
-  int64_t workspace_limit; /* bytes the pieces of the vocabulary may take (0: the default, 2 GiB) */
+  int64_t workspace_limit; /* bytes that logits' gradients and packed weights may take (0: the default, 4 GiB) */
 } sw_linear_head;
 
 /* Softmax cross entropy of a linear head, without keeping the logits:

@@ -68,12 +68,21 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+// Placement of an operand's 64-element blocks and of its lo plane, in TMA
+// coordinates: block b of plane p starts at element b x_block + p x_plane of a
+// row, row r at row r + p y_plane.
+struct Plane {
+    int x_block, x_plane, y_plane;
+};
+
 struct GemmArgs {
     int M, N, K;
     int count_is;            // which extent the device-side row count bounds
     const HeadState* state;
+    int row0;                // first compact row of this launch (the count starts there)
     int terms;               // plane pairs walked: 1, or 3 for Float32
-    int a_plane, b_plane;    // rows from the hi to the lo plane of each operand
+    Plane pa, pb;            // where each operand's lo plane and 64-element blocks lie
+    int splits;              // parts of the K walk, each with its own slot of `accum`
     int scale_a, scale_b;    // indexes into HeadState::amax of the operands' scales (-1: none)
     // logits epilogues
     float logit_scale;
@@ -84,14 +93,15 @@ struct GemmArgs {
     int ent_k;
     int rows_pad;
     float4* partial;         // kEpiLse: [half tile][rows_pad] (max, sum, target term, -) in base-2 units
+    float* ent_s;            // kEpiLse: base-2 logit of every target entry (null: not kept)
+    int keep;                // kEpiLse: write exp2(logit - half tile's max) where the logits' gradient will be
     const float* lse2;       // kEpiGrad: per compact row
     const float* coef;
-    uint16_t* grad;          // [planes][rows_pad][ld_grad]
-    int64_t ld_grad;
-    int split;               // kEpiGrad: write hi and lo planes
+    uint16_t* grad;          // [rows_pad][ld_grad]; Float32: every 64 columns as 64 hi then 64 lo values
+    int64_t ld_grad;         // 16-bit elements
     // kEpiOut
-    float* accum;            // fp32 running sum [M][ld_accum] (null: none)
-    int64_t ld_accum;
+    float* accum;            // fp32 running sums [splits][M][ld_accum] (null: none)
+    int64_t ld_accum, slot;
     int first, last;         // first: nothing to add yet; last: write dst
     void* dst;
     int dst_f32;
@@ -196,40 +206,6 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     return *reinterpret_cast<uint32_t*>(&v);
 }
 
-// A row's softmax statistics over the columns seen so far, in base-2 units:
-// sum of exp2(k2 z - ref) with ref the running maximum of k2 z, and the target
-// term sum p z.
-struct LseState {
-    float ref = -INFINITY, sum = 0.0f, dot = 0.0f;
-};
-
-__device__ __forceinline__ void lse_part(LseState& st, EntryCursor& cur, int64_t col0, int ncols, float k2,
-                                         float (&r)[32]) {
-    cur.walk(col0, [&](int rel, float p) {
-        float v = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-            if (j == rel) v = r[j];
-        if (rel >= 0) st.dot += p * v;
-    });
-    if (ncols < 32) {
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-            if (j >= ncols) r[j] = -INFINITY;
-    }
-    float top = r[0];
-#pragma unroll
-    for (int j = 1; j < 32; ++j) top = fmaxf(top, r[j]);
-    const float next = fmaxf(st.ref, top * k2);
-    // columns of nothing but -inf add nothing (and must not make -inf minus -inf)
-    const float base = next == -INFINITY ? 0.0f : next;
-    float s = st.sum * ex2(st.ref - base);
-#pragma unroll
-    for (int j = 0; j < 32; ++j) s += ex2(fmaf(r[j], k2, -base));
-    st.sum = s;
-    st.ref = next;
-}
-
 template <bool kBf16>
 __device__ __forceinline__ void store_row32(uint16_t* dst, const float (&r)[32]) {
     uint4* d = reinterpret_cast<uint4*>(dst);
@@ -239,11 +215,78 @@ __device__ __forceinline__ void store_row32(uint16_t* dst, const float (&r)[32])
                           pack2<kBf16>(r[8 * v + 4], r[8 * v + 5]), pack2<kBf16>(r[8 * v + 6], r[8 * v + 7]));
 }
 
-// Gradient with respect to 32 logits of a row: softmax minus target in fp32,
-// rounded once to the type the next contractions read.
+// Where 32 columns of a row's logits' gradient are: column n0 of the row, and
+// in Float32 its hi values (the lo values 64 elements further).
 template <bool kBf16>
-__device__ __forceinline__ void grad_part(const GemmArgs& args, EntryCursor& cur, int64_t m, int64_t n0, bool row_in,
-                                          float k2, float lse2, float coef, float (&r)[32]) {
+__device__ __forceinline__ uint16_t* grad_at(const GemmArgs& args, int64_t m, int64_t n0) {
+    return args.grad + m * args.ld_grad + (kBf16 ? n0 : (n0 & ~int64_t(63)) * 2 + (n0 & 63));
+}
+
+// Softmax statistics of a row over the half tile in registers, in base-2
+// units: ref = max k2 z, sum of exp2(k2 z - ref), target term sum p z.  With
+// `keep` the exponentials are stored too, for the gradient: as f16 times 2^15
+// (11 bits down to 2^-29 of the half tile's largest; the later rounding to
+// bf16 is the one that counts) or, for Float32, as they are.
+template <bool kBf16, int kParts>
+__device__ __forceinline__ float4 lse_tile(const GemmArgs& args, EntryCursor& cur, int64_t m, int64_t n0, bool row_in,
+                                           float k2, float (&r)[kParts][32]) {
+    float dot = 0.0f, top = -INFINITY;
+#pragma unroll
+    for (int c = 0; c < kParts; ++c) {
+        cur.walk(args.v0 + n0 + c * 32, [&](int rel, float p) {
+            float v = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+                if (j == rel) v = r[c][j];
+            if (rel >= 0) {
+                dot += p * v;
+                if (args.ent_s) args.ent_s[m * args.ent_k + cur.e] = v * k2;
+            }
+        });
+        const int ncols = (int)min(int64_t(32), int64_t(args.N) - (n0 + c * 32));
+        if (ncols < 32) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+                if (j >= ncols) r[c][j] = -INFINITY;
+        }
+#pragma unroll
+        for (int j = 0; j < 32; ++j) top = fmaxf(top, r[c][j]);
+    }
+    const float ref = top * k2;
+    // columns of nothing but -inf add nothing (and must not make -inf minus -inf)
+    const float base = ref == -INFINITY ? 0.0f : ref;
+    float sum = 0.0f;
+#pragma unroll
+    for (int c = 0; c < kParts; ++c) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+            r[c][j] = ex2(fmaf(r[c][j], k2, -base));
+            sum += r[c][j];
+        }
+        // (Float32 blocks of 64 columns are written whole: the K walk reads them whole)
+        if (args.keep && n0 + c * 32 < (kBf16 ? int64_t(args.N) : (int64_t(args.N) + 63) / 64 * 64)) {
+            if (kBf16) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) r[c][j] = row_in ? r[c][j] * 32768.0f : 0.0f;
+                store_row32<false>(grad_at<true>(args, m, n0 + c * 32), r[c]);
+            } else {
+                float4* d = reinterpret_cast<float4*>(args.grad + m * args.ld_grad + 2 * (n0 + c * 32));
+#pragma unroll
+                for (int v = 0; v < 8; ++v)
+                    d[v] = row_in ? make_float4(r[c][4 * v], r[c][4 * v + 1], r[c][4 * v + 2], r[c][4 * v + 3])
+                                  : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            }
+        }
+    }
+    return make_float4(ref, sum, dot * k2, 0.0f);
+}
+
+// Gradient with respect to 32 logits of a row: softmax minus target in fp32,
+// rounded once to the type the next contractions read.  Float32: zeros up to
+// the end of a 64-column block, which the K walk reads whole.
+template <bool kBf16>
+__device__ __forceinline__ void grad_part(const GemmArgs& args, EntryCursor& cur, int64_t m, int64_t n0, int ncols,
+                                          bool row_in, float k2, float lse2, float coef, float (&r)[32]) {
 #pragma unroll
     for (int j = 0; j < 32; ++j) r[j] = ex2(fmaf(r[j], k2, -lse2));
     cur.walk(args.v0 + n0, [&](int rel, float p) {
@@ -252,32 +295,51 @@ __device__ __forceinline__ void grad_part(const GemmArgs& args, EntryCursor& cur
             if (j == rel) r[j] -= p;
     });
 #pragma unroll
-    for (int j = 0; j < 32; ++j) r[j] = row_in ? r[j] * coef : 0.0f;
-    store_row32<kBf16>(args.grad + m * args.ld_grad + n0, r);
-    if (!kBf16 && args.split) {
+    for (int j = 0; j < 32; ++j) r[j] = row_in && j < ncols ? r[j] * coef : 0.0f;
+    uint16_t* d = grad_at<kBf16>(args, m, n0);
+    store_row32<kBf16>(d, r);
+    if (!kBf16) {
 #pragma unroll
         for (int j = 0; j < 32; ++j) r[j] -= __half2float(__float2half_rn(r[j]));
-        store_row32<kBf16>(args.grad + (int64_t(args.rows_pad) + m) * args.ld_grad + n0, r);
+        store_row32<kBf16>(d + 64, r);
     }
 }
 
 // 32 columns of a result row: scaled, added to the running fp32 sum, and the
 // last time written in the result's type.
-__device__ __forceinline__ void out_part(const GemmArgs& args, int64_t m, int64_t n0, int ncols, float scale,
-                                         float (&r)[32]) {
+__device__ __forceinline__ void out_part(const GemmArgs& args, int split, int64_t m, int64_t n0, int ncols,
+                                         float scale, float (&r)[32]) {
 #pragma unroll
     for (int j = 0; j < 32; ++j) r[j] *= scale;
     if (args.accum) {
-        float* a = args.accum + m * args.ld_accum + n0;
+        float* a = args.accum + split * args.slot + m * args.ld_accum + n0;
+        const bool whole = ncols == 32 && (reinterpret_cast<uintptr_t>(a) & 15) == 0;
         if (!args.first) {
+            if (whole) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-                if (j < ncols) r[j] += a[j];
+                for (int v = 0; v < 8; ++v) {
+                    const float4 o = reinterpret_cast<const float4*>(a)[v];
+                    r[4 * v] += o.x;
+                    r[4 * v + 1] += o.y;
+                    r[4 * v + 2] += o.z;
+                    r[4 * v + 3] += o.w;
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                    if (j < ncols) r[j] += a[j];
+            }
         }
         if (!args.last) {
+            if (whole) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-                if (j < ncols) a[j] = r[j];
+                for (int v = 0; v < 8; ++v)
+                    reinterpret_cast<float4*>(a)[v] = make_float4(r[4 * v], r[4 * v + 1], r[4 * v + 2], r[4 * v + 3]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                    if (j < ncols) a[j] = r[j];
+            }
             return;
         }
     }
@@ -346,17 +408,22 @@ __global__ void __launch_bounds__(320, 1)
     const uint32_t tmem = *tmem_slot;
     pdl_enter();
 
-    const int count = args.count_is == kCountNone ? 0 : args.state->count;
+    const int count = args.count_is == kCountNone ? 0 : max(args.state->count - args.row0, 0);
     const int M = args.count_is == kCountM ? min(args.M, count) : args.M;
     const int K = args.count_is == kCountK ? min(args.K, count) : args.K;
     const int num_m = (M + kBM - 1) / kBM;
     const int num_n = (args.N + BN - 1) / BN;
     const int num_tiles = num_m * num_n;
+    const int num_items = num_tiles * args.splits;
     const int k_steps = (K + kBK - 1) / kBK;
-    const int chunk_steps = kChunked ? kChunkSteps : max(k_steps, 1);
-    const int chunks = kChunked ? (k_steps + chunk_steps - 1) / chunk_steps : 1;
+    const int split_steps = (k_steps + args.splits - 1) / args.splits;
     constexpr int kGroup = 16;
-    auto tile_coords = [&](int t, int& mb, int& nb) {
+    // Work item `t`: a tile and its share [k0, k1) of the K stages.
+    auto item = [&](int t, int& mb, int& nb, int& split, int& k0, int& k1) {
+        split = t / num_tiles;
+        t -= split * num_tiles;
+        k0 = min(split * split_steps, k_steps);
+        k1 = min(k0 + split_steps, k_steps);
         const int per_group = kGroup * num_n;
         const int g = t / per_group;
         const int first = g * kGroup;
@@ -365,6 +432,7 @@ __global__ void __launch_bounds__(320, 1)
         mb = first + r % gsize;
         nb = r / gsize;
     };
+    auto chunk_end = [&](int k0, int k1) { return kChunked ? min(k0 + kChunkSteps, k1) : k1; };
 
     if (warp == 0) {
         if (lane == 0) {
@@ -372,16 +440,18 @@ __global__ void __launch_bounds__(320, 1)
             uint32_t phase = 0;
             uint32_t issued[kStages] = {0};
             bool alive = true;
-            for (int t = blockIdx.x; t < num_tiles && alive; t += gridDim.x) {
-                int mb, nb;
-                tile_coords(t, mb, nb);
-                for (int k0 = 0; k0 < k_steps && alive; k0 += chunk_steps)
+            for (int t = blockIdx.x; t < num_items && alive; t += gridDim.x) {
+                int mb, nb, split, k0, k1;
+                item(t, mb, nb, split, k0, k1);
+                for (int c0 = k0; c0 < k1 && alive; c0 = chunk_end(c0, k1))
                     for (int term = 0; term < args.terms && alive; ++term) {
                         // plane pairs, the small products first: (hi, lo), (lo, hi), (hi, hi)
-                        const int pa = args.terms == 3 && term == 1 ? args.a_plane : 0;
-                        const int pb = args.terms == 3 && term == 0 ? args.b_plane : 0;
-                        const int k1 = min(k0 + chunk_steps, k_steps);
-                        for (int ks = k0; ks < k1; ++ks) {
+                        const int pa = args.terms == 3 && term == 1;
+                        const int pb = args.terms == 3 && term == 0;
+                        const int xa = pa * args.pa.x_plane, ya = pa * args.pa.y_plane;
+                        const int xb = pb * args.pb.x_plane, yb = pb * args.pb.y_plane;
+                        const int c1 = chunk_end(c0, k1);
+                        for (int ks = c0; ks < c1; ++ks) {
                             if (!ptx::mbar_wait(bar_empty + 8 * stage, phase ^ 1)) { alive = false; break; }
                             const uint32_t full = bar_full + 8 * stage;
                             const uint32_t sa = sbase + stage * C::kStageBytes;
@@ -390,16 +460,18 @@ __global__ void __launch_bounds__(320, 1)
                             if (kAMn) {
 #pragma unroll
                                 for (int g = 0; g < kBM / 64; ++g)
-                                    ptx::tma_load_2d(sa + g * 8192, &tmap_a, mb * kBM + g * 64, pa + ks * kBK, full);
+                                    ptx::tma_load_2d(sa + g * 8192, &tmap_a,
+                                                     (mb * (kBM / 64) + g) * args.pa.x_block + xa, ya + ks * kBK, full);
                             } else {
-                                ptx::tma_load_2d(sa, &tmap_a, ks * kBK, pa + mb * kBM, full);
+                                ptx::tma_load_2d(sa, &tmap_a, ks * args.pa.x_block + xa, ya + mb * kBM, full);
                             }
                             if (kBMn) {
 #pragma unroll
                                 for (int g = 0; g < BN / 64; ++g)
-                                    ptx::tma_load_2d(sb + g * 8192, &tmap_b, nb * BN + g * 64, pb + ks * kBK, full);
+                                    ptx::tma_load_2d(sb + g * 8192, &tmap_b,
+                                                     (nb * (BN / 64) + g) * args.pb.x_block + xb, yb + ks * kBK, full);
                             } else {
-                                ptx::tma_load_2d(sb, &tmap_b, ks * kBK, pb + nb * BN, full);
+                                ptx::tma_load_2d(sb, &tmap_b, ks * args.pb.x_block + xb, yb + nb * BN, full);
                             }
                             issued[stage] += 1;
                             if (++stage == kStages) { stage = 0; phase ^= 1; }
@@ -415,13 +487,15 @@ __global__ void __launch_bounds__(320, 1)
             int stage = 0;
             uint32_t phase = 0, it = 0;
             bool alive = true;
-            for (int t = blockIdx.x; t < num_tiles && alive; t += gridDim.x) {
-                for (int c = 0; c < chunks && alive; ++c, ++it) {
+            for (int t = blockIdx.x; t < num_items && alive; t += gridDim.x) {
+                int mb, nb, split, k0, k1;
+                item(t, mb, nb, split, k0, k1);
+                for (int c0 = k0; c0 < k1; c0 = chunk_end(c0, k1), ++it) {
                     const uint32_t buf = it & 1;
                     if (!ptx::mbar_wait(bar_tmem_empty + 8 * buf, ((it >> 1) & 1) ^ 1)) { alive = false; break; }
                     ptx::tc_fence_after();
                     const uint32_t acc = tmem + buf * BN;
-                    const int steps = min(chunk_steps, k_steps - c * chunk_steps) * args.terms;
+                    const int steps = (chunk_end(c0, k1) - c0) * args.terms;
                     for (int ks = 0; ks < steps; ++ks) {
                         if (!ptx::mbar_wait(bar_full + 8 * stage, phase)) { alive = false; break; }
                         ptx::tc_fence_after();
@@ -459,18 +533,17 @@ __global__ void __launch_bounds__(320, 1)
         if (args.scale_a >= 0) inv *= pow2i(-scale_exponent(args.state->amax[args.scale_a]));
         if (args.scale_b >= 0) inv *= pow2i(-scale_exponent(args.state->amax[args.scale_b]));
         const float k2 = args.logit_scale * kLog2e * inv;
-        const float gscale = kEpi == kEpiGrad && args.split ? pow2i(scale_exponent(args.state->amax[2])) : 1.0f;
+        const float gscale = kEpi == kEpiGrad && !kBf16 ? pow2i(scale_exponent(args.state->amax[2])) : 1.0f;
         const float out_scale = kEpi == kEpiOut ? inv * args.state->grad_scale : 1.0f;
         uint32_t it = 0;
         bool alive = true;
-        for (int t = blockIdx.x; t < num_tiles && alive; t += gridDim.x) {
-            int mb, nb;
-            tile_coords(t, mb, nb);
+        for (int t = blockIdx.x; t < num_items && alive; t += gridDim.x) {
+            int mb, nb, split, k0, k1;
+            item(t, mb, nb, split, k0, k1);
             const int64_t m = int64_t(mb) * kBM + row_in_tile;
             const bool row_in = m < M;
             const int64_t ncol0 = int64_t(nb) * BN + half * kCols;
             EntryCursor cur;
-            LseState lse;
             float lse2 = 0.0f, coef = 0.0f;
             if (kEpi != kEpiOut) cur.begin(args, m, row_in, args.v0 + ncol0);
             if (kEpi == kEpiGrad && row_in) {
@@ -480,11 +553,13 @@ __global__ void __launch_bounds__(320, 1)
             // one 32-column part of the finished accumulator
             auto part = [&](int c, float (&r)[32]) {
                 const int64_t n0 = ncol0 + c * 32;
-                const int ncols = (int)min(int64_t(32), int64_t(args.N) - n0);
-                if (ncols <= 0) return;
-                if (kEpi == kEpiLse) lse_part(lse, cur, args.v0 + n0, ncols, k2, r);
-                else if (kEpi == kEpiGrad) grad_part<kBf16>(args, cur, m, n0, row_in, k2, lse2, coef, r);
-                else if (row_in) out_part(args, m, n0, ncols, out_scale, r);
+                const int ncols = (int)max(int64_t(0), min(int64_t(32), int64_t(args.N) - n0));
+                if (kEpi == kEpiGrad) {
+                    if (n0 < (int64_t(args.N) + 63) / 64 * 64)
+                        grad_part<kBf16>(args, cur, m, n0, ncols, row_in, k2, lse2, coef, r);
+                } else if (kEpi == kEpiOut) {
+                    if (row_in && ncols) out_part(args, split, m, n0, ncols, out_scale, r);
+                }
             };
             if (kChunked) {
                 float sum[kParts][32];
@@ -492,7 +567,7 @@ __global__ void __launch_bounds__(320, 1)
                 for (int c = 0; c < kParts; ++c)
 #pragma unroll
                     for (int j = 0; j < 32; ++j) sum[c][j] = 0.0f;
-                for (int k = 0; k < chunks; ++k, ++it) {
+                for (int c0 = k0; c0 < k1; c0 = chunk_end(c0, k1), ++it) {
                     const uint32_t buf = it & 1;
                     if (!ptx::mbar_wait(bar_tmem_full + 8 * buf, (it >> 1) & 1)) { alive = false; break; }
                     __syncwarp();
@@ -510,14 +585,20 @@ __global__ void __launch_bounds__(320, 1)
                     ptx::mbar_arrive(bar_tmem_empty + 8 * buf);
                 }
                 if (!alive) break;
+                if (kEpi == kEpiLse) {
+                    const float4 st = lse_tile<kBf16, kParts>(args, cur, m, ncol0, row_in, k2, sum);
+                    args.partial[(args.v0 + ncol0) / kCols * args.rows_pad + m] = st;
+                } else {
 #pragma unroll
-                for (int c = 0; c < kParts; ++c) {
-                    part(c, sum[c]);
+                    for (int c = 0; c < kParts; ++c) part(c, sum[c]);
                 }
             } else {
                 const uint32_t buf = it & 1;
-                if (!ptx::mbar_wait(bar_tmem_full + 8 * buf, (it >> 1) & 1)) break;
-                ptx::tc_fence_after();
+                const bool any = k0 < k1;  // an empty share has no accumulator: zeros
+                if (any) {
+                    if (!ptx::mbar_wait(bar_tmem_full + 8 * buf, (it >> 1) & 1)) break;
+                    ptx::tc_fence_after();
+                }
                 const uint32_t acc = tmem + buf * BN + half * kCols + (uint32_t(quarter * 32) << 16);
 #pragma unroll 1
                 for (int c = 0; c < kParts; ++c) {
@@ -527,16 +608,14 @@ __global__ void __launch_bounds__(320, 1)
                     ptx::tmem_ld_32x32b_x32(acc + c * 32, u);
                     ptx::tmem_ld_wait();
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) r[j] = k_steps == 0 ? 0.0f : __uint_as_float(u[j]);
+                    for (int j = 0; j < 32; ++j) r[j] = any ? __uint_as_float(u[j]) : 0.0f;
                     part(c, r);
                 }
-                ptx::tc_fence_before();
-                ptx::mbar_arrive(bar_tmem_empty + 8 * buf);
-                ++it;
-            }
-            if (kEpi == kEpiLse && m < args.rows_pad) {
-                const int64_t slot = (args.v0 + ncol0) / kCols;
-                args.partial[slot * args.rows_pad + m] = make_float4(lse.ref, lse.sum, lse.dot * k2, 0.0f);
+                if (any) {
+                    ptx::tc_fence_before();
+                    ptx::mbar_arrive(bar_tmem_empty + 8 * buf);
+                    ++it;
+                }
             }
         }
     }

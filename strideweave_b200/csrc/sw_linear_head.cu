@@ -33,7 +33,7 @@ namespace head {
 namespace {
 
 constexpr int kMaxTeacher = SW_MAX_TEACHER;
-constexpr int64_t kDefaultWorkspace = int64_t(2) << 30;
+constexpr int64_t kDefaultWorkspace = int64_t(4) << 30;
 
 __device__ __forceinline__ float warp_max(float v) {
     for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
@@ -283,7 +283,7 @@ __global__ void pack_kernel(const void* src, int64_t rows, int64_t cols, int64_t
 struct MergeArgs {
     const float4* partial;
     int tiles, rows_pad;
-    int64_t T, V;
+    int64_t row0, T, V;      // compact rows [row0, T)
     const HeadState* state;
     const int* row_map;
     const int* targets;
@@ -301,7 +301,7 @@ __global__ void __launch_bounds__(256) merge_kernel(const MergeArgs a) {
     __shared__ float4 part[8][32];
     pdl_enter();
     const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
-    const int64_t i = int64_t(blockIdx.x) * 32 + lane;
+    const int64_t i = a.row0 + int64_t(blockIdx.x) * 32 + lane;
     const int count = a.state->count;
     float ref = -INFINITY, sum = 0.0f, dot = 0.0f;
     if (i < count) {
@@ -355,6 +355,127 @@ __global__ void __launch_bounds__(1024) mean_kernel(const float* row_loss, const
     }
 }
 
+// The kept exponentials of the logits become their gradient, in place:
+// exp2(k2 z - ref) 2^(ref - lse2) is the softmax, and the target entries are
+// written from their own Float32 logits (where the softmax is near p, the
+// stored 11 bits of it would not be enough).  A CTA takes kScaleCols columns of
+// a row; a thread 8 columns (bf16), a half warp 32 columns (Float32: hi and lo
+// values replace the 64-column block they were computed from).
+constexpr int kScaleCols = 8192;
+struct ScaleArgs {
+    uint16_t* grad;
+    int64_t ld_grad, V;
+    const float4* partial;
+    int rows_pad, row0;
+    const HeadState* state;
+    const float* lse2;
+    const float* coef;
+    const int* ent_idx;
+    const float* ent_p;
+    const float* ent_s;
+    int ent_k;
+};
+template <bool kF32>
+__global__ void __launch_bounds__(256) scale_kernel(const ScaleArgs a) {
+    __shared__ float factor[kScaleCols / 128];
+    pdl_enter();
+    const int64_t i = blockIdx.x;
+    if (i >= a.state->count - a.row0) return;
+    const int64_t c0 = int64_t(blockIdx.y) * kScaleCols;
+    const int64_t c1 = min(c0 + kScaleCols, a.V);
+    const float lse2 = a.lse2[i];
+    const float coef = a.coef[i] * (kF32 ? pow2i(scale_exponent(a.state->amax[2])) : 1.0f);
+    const int halves = int((c1 - c0 + 127) / 128);
+    for (int t = threadIdx.x; t < halves; t += 256) {
+        const float ref = a.partial[(c0 / 128 + t) * a.rows_pad + i].x;
+        // (a half tile of nothing but -inf stored zeros)
+        factor[t] = ref == -INFINITY ? 0.0f : ex2(ref - lse2) * coef * (kF32 ? 1.0f : 1.0f / 32768.0f);
+    }
+    __syncthreads();
+    uint16_t* row = a.grad + i * a.ld_grad;
+    if (kF32) {
+        const int lane = threadIdx.x & 31;
+        for (int64_t b = c0 + (threadIdx.x >> 5) * 64; b < c1; b += 8 * 64) {
+            float2 v = reinterpret_cast<const float2*>(row + 2 * b)[lane];
+            const float f = factor[(b - c0) / 128];
+            v.x = b + 2 * lane < a.V ? v.x * f : 0.0f;
+            v.y = b + 2 * lane + 1 < a.V ? v.y * f : 0.0f;
+            const __half2 hi = __floats2half2_rn(v.x, v.y);
+            const __half2 lo = __floats2half2_rn(v.x - __low2float(hi), v.y - __high2float(hi));
+            __syncwarp();
+            reinterpret_cast<__half2*>(row + 2 * b)[lane] = hi;
+            reinterpret_cast<__half2*>(row + 2 * b + 64)[lane] = lo;
+            __syncwarp();
+        }
+    } else {
+        for (int64_t c = c0 + threadIdx.x * 8; c < c1; c += 256 * 8) {
+            uint4 v = *reinterpret_cast<const uint4*>(row + c);
+            const float f = factor[(c - c0) / 128];
+            uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float2 e = __half22float2(*reinterpret_cast<__half2*>(&w[j]));
+                w[j] = pack2<true>(e.x * f, e.y * f);
+            }
+            *reinterpret_cast<uint4*>(row + c) = v;
+        }
+    }
+    __syncthreads();  // the entries overwrite what the loop above wrote
+    for (int k = threadIdx.x; k < a.ent_k; k += 256) {
+        const int64_t at = i * a.ent_k + k;
+        const int col = a.ent_idx[at];
+        if (col < c0 || col >= c1 || (k > 0 && a.ent_idx[at - 1] == col)) continue;
+        float p = a.ent_p ? a.ent_p[at] : 1.0f;
+        for (int j = 1; k + j < a.ent_k && a.ent_idx[at + j] == col; ++j) p += a.ent_p[at + j];
+        const float g = (ex2(a.ent_s[at] - lse2) - p) * coef;
+        if (kF32) {
+            uint16_t* d = row + (col & ~63) * int64_t(2) + (col & 63);
+            const __half hi = __float2half_rn(g);
+            d[0] = __half_as_ushort(hi);
+            d[64] = __half_as_ushort(__float2half_rn(g - __half2float(hi)));
+        } else {
+            row[col] = __bfloat16_as_ushort(__float2bfloat16_rn(g));
+        }
+    }
+}
+
+// Result rows from the K walk's parts, added in order.
+struct SlotsArgs {
+    const float* accum;
+    int64_t ld_accum, slot;
+    int splits;
+    int64_t rows, cols;
+    const HeadState* state;
+    int by_count, row0;
+    const int* row_map;
+    void* dst;
+    int64_t dst_row, dst_col;
+};
+template <bool kF32>
+__global__ void __launch_bounds__(256) sum_slots_kernel(const SlotsArgs a) {
+    pdl_enter();
+    const int64_t rows = a.by_count ? min(a.rows, int64_t(max(a.state->count - a.row0, 0))) : a.rows;
+    const int64_t per_row = (a.cols + 3) / 4;
+    for (int64_t u = int64_t(blockIdx.x) * 256 + threadIdx.x; u < rows * per_row; u += int64_t(gridDim.x) * 256) {
+        const int64_t m = u / per_row, c = (u - m * per_row) * 4;
+        const float* p = a.accum + m * a.ld_accum + c;  // ld_accum is whole groups of four
+        float4 s = *reinterpret_cast<const float4*>(p);
+        for (int k = 1; k < a.splits; ++k) {
+            const float4 v = *reinterpret_cast<const float4*>(p + k * a.slot);
+            s.x += v.x;
+            s.y += v.y;
+            s.z += v.z;
+            s.w += v.w;
+        }
+        const int64_t at = (a.row_map ? int64_t(a.row_map[m]) : m) * a.dst_row + c * a.dst_col;
+        const float r[4] = {s.x, s.y, s.z, s.w};
+        for (int j = 0; j < 4 && c + j < a.cols; ++j) {
+            if (kF32) static_cast<float*>(a.dst)[at + j * a.dst_col] = r[j];
+            else static_cast<__nv_bfloat16*>(a.dst)[at + j * a.dst_col] = __float2bfloat16_rn(r[j]);
+        }
+    }
+}
+
 // Zeroes the gradient of the rows that do not count.
 __global__ void zero_rows_kernel(void* dst, int f32, int64_t T, int64_t D, int64_t sr, int64_t sc, const int* row_map,
                                  const HeadState* state) {
@@ -386,43 +507,65 @@ int make_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int
     return SW_OK;
 }
 
-// A contraction operand: `rows` x `cols` 16-bit elements in memory, pitch ld,
-// `planes` of them `plane` rows apart.
+// A contraction operand: `rows` x `cols` 16-bit elements in memory, pitch ld
+// (every plane of them), and where its lo plane lies.
 struct Operand {
     const uint16_t* ptr;
     int64_t rows, cols, ld;
-    int planes;
-    int64_t plane;
+    Plane plane;
 };
+
+// Parts of the K walk of a contraction whose tiles alone do not fill the SMs:
+// the smallest estimate of waves x (stages + a tile's fixed cost) plus the
+// traffic of writing and adding the parts.  A stage of 128 x 256 x 64 takes
+// 0.27 us, a tile's fill and drain about 2 us, the adding launch 3 us.
+int choose_splits(int64_t M, int64_t N, int64_t K, int terms, int sms) {
+    const int64_t tiles = ((M + kBM - 1) / kBM) * ((N + 255) / 256), steps = (K + kBK - 1) / kBK;
+    int best = 1;
+    double best_us = 1e30;
+    for (int s = 1; s <= 64 && (s == 1 || steps / s >= 4); ++s) {
+        const int64_t waves = (tiles * s + sms - 1) / sms, share = (steps + s - 1) / s;
+        double us = double(waves) * (double(share * terms) * 0.27 + 2.0);
+        if (s > 1) us += 3.0 + double(s) * double(M) * double(N) * 8.0 / 6.0e6;
+        if (us < best_us * 0.97) {
+            best_us = us;
+            best = s;
+        }
+    }
+    return best;
+}
+
+int device_sms() {
+    static int sms[64] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+    if (!sms[dev] && cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+        sms[dev] = 148;
+    return sms[dev];
+}
 
 template <bool kBf16, bool kAMn, bool kBMn, int kEpi>
 int gemm(const Operand& a, const Operand& b, GemmArgs args, cudaStream_t stream) {
     constexpr int BN = 256, kStages = 4;
     using Cf = Cfg<BN, kStages>;
+    const int64_t tiles = int64_t((args.M + kBM - 1) / kBM) * ((args.N + BN - 1) / BN);
+    if (tiles == 0) return SW_OK;
     CUtensorMap ma, mb;
-    // the rows of a plane past its extent belong to the next plane or to
-    // nothing: tiles that reach there read other finite values, whose products
-    // meet only result rows or columns that are not stored, or (along K) zeros
-    int rc = make_map(&ma, a.ptr, a.planes > 1 ? a.plane * (a.planes - 1) + a.rows : a.rows, a.cols, a.ld,
-                      kAMn ? kBK : kBM);
+    int rc = make_map(&ma, a.ptr, a.rows, a.cols, a.ld, kAMn ? kBK : kBM);
     if (rc != SW_OK) return rc;
-    rc = make_map(&mb, b.ptr, b.planes > 1 ? b.plane * (b.planes - 1) + b.rows : b.rows, b.cols, b.ld,
-                  kBMn ? kBK : BN);
+    rc = make_map(&mb, b.ptr, b.rows, b.cols, b.ld, kBMn ? kBK : BN);
     if (rc != SW_OK) return rc;
-    args.terms = a.planes > 1 ? 3 : 1;
-    args.a_plane = (int)a.plane;
-    args.b_plane = (int)b.plane;
+    args.terms = kBf16 ? 1 : 3;
+    args.pa = a.plane;
+    args.pb = b.plane;
+    if (args.splits < 1) args.splits = 1;
     constexpr bool kChunked = !kBf16 || kEpi == kEpiLse;
     auto kernel = head_gemm_kernel<BN, kStages, kBf16, kAMn, kBMn, kEpi, kChunked>;
     SW_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cf::kSmemBytes),
                 "linear head smem");
-    int dev = 0, sms = 148;
-    SW_CUDA_TRY(cudaGetDevice(&dev), "cudaGetDevice");
-    SW_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev), "SM count");
-    const int64_t tiles = int64_t((args.M + kBM - 1) / kBM) * ((args.N + BN - 1) / BN);
-    if (tiles == 0) return SW_OK;
-    SW_CUDA_TRY(launch_pdl(kernel, dim3((unsigned)std::min<int64_t>(tiles, sms)), dim3(Cf::kThreads), Cf::kSmemBytes,
-                           stream, ma, mb, args),
+    const int64_t items = tiles * args.splits;
+    SW_CUDA_TRY(launch_pdl(kernel, dim3((unsigned)std::min<int64_t>(items, device_sms())), dim3(Cf::kThreads),
+                           Cf::kSmemBytes, stream, ma, mb, args),
                 "linear head contraction");
     return SW_OK;
 }
@@ -470,17 +613,29 @@ struct Layout {
     float* coef;
     float* lse2;
     float* row_loss;
+    float* ent_s;
     uint16_t* hc;
     float4* partial;
-    float* accum;
+    float* dh_accum;
+    float* dw_accum;
     uint16_t* wp;
     uint16_t* grad;
 };
 
 struct Shape {
-    int64_t T, D, V, rows_pad, ld_h, ld_w, piece, tiles;
+    int64_t T, D, V, rows_pad, ld_h, ld_w;
+    int64_t half_tiles;      // 128-column pieces of the vocabulary, each with its statistics
     bool f32, pack_w, grads;
     int planes;
+    // Gradients: `keep`: the forward's exponentials of `rows` compact rows at a
+    // time stay in the workspace and become the logits' gradient.  Otherwise
+    // the logits are computed again, `piece` columns of the vocabulary at a
+    // time.  Packed weights are laid out `piece` columns at a time too.
+    bool keep;
+    int64_t rows, piece;
+    int dh_splits, dw_splits;
+    bool dh_sums, dw_sums;   // fp32 running sums are needed
+    int64_t ld_acc;
 };
 
 Layout lay_out(Bump& b, const Call& c, const Shape& s) {
@@ -500,10 +655,12 @@ Layout lay_out(Bump& b, const Call& c, const Shape& s) {
     l.lse2 = b.take<float>(s.rows_pad);
     l.row_loss = b.take<float>(s.rows_pad);
     l.hc = b.take<uint16_t>(s.planes * s.rows_pad * s.ld_h);
-    if (c.loss) l.partial = b.take<float4>(s.tiles * s.rows_pad);
-    if (s.grads && c.dh && s.piece < s.V) l.accum = b.take<float>(s.T * s.D);
+    if (c.loss) l.partial = b.take<float4>(s.half_tiles * s.rows_pad);
+    if (s.keep) l.ent_s = b.take<float>(s.rows_pad * K);
+    if (s.dh_sums) l.dh_accum = b.take<float>(s.dh_splits * s.T * s.ld_acc);
+    if (s.dw_sums) l.dw_accum = b.take<float>(s.dw_splits * (s.keep ? s.V : s.piece) * s.ld_acc);
     if (s.pack_w) l.wp = b.take<uint16_t>(s.planes * round_up(s.piece, kBK) * s.ld_w);
-    if (s.grads) l.grad = b.take<uint16_t>(s.planes * s.rows_pad * round_up(s.piece, 64));
+    if (s.grads) l.grad = b.take<uint16_t>(s.planes * s.rows * round_up(s.piece, 64));
     return l;
 }
 
@@ -552,67 +709,71 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
     SW_CUDA_TRY(launch_pdl(pack_kernel<kF32>, dim3(row_blocks, (unsigned)((s.ld_h + 31) / 32)), dim3(256), 0, stream,
                            c.h, s.T, s.D, p.h_row, p.h_col, l.row_map, l.state, 1, 0, l.hc, s.ld_h, s.rows_pad),
                 "linear head states");
-    const Operand hk{l.hc, s.rows_pad, s.D, s.ld_h, s.planes, s.rows_pad};
+    const Plane dense{kBK, 0, 0};
+    // rows [r0, r0 + n) of the gathered states
+    auto states = [&](int64_t r0, int64_t n) {
+        return Operand{l.hc + r0 * s.ld_h, kF32 ? s.rows_pad + n : n, s.D, s.ld_h, Plane{kBK, 0, (int)s.rows_pad}};
+    };
+    const int64_t ld_grad = s.planes * round_up(s.piece, 64);
 
     GemmArgs g;
     memset(&g, 0, sizeof(g));
     g.state = l.state;
     g.logit_scale = c.scale;
-    g.ent_idx = l.ent_idx;
     g.ent_p = l.ent_p;
-    g.offs = l.offs;
     g.ent_k = c.targets ? 1 : c.top_k;
     g.rows_pad = (int)s.rows_pad;
-    g.partial = l.partial;
-    g.lse2 = l.lse2;
-    g.coef = l.coef;
-    g.grad = l.grad;
-    g.ld_grad = round_up(s.piece, 64);
-    g.split = kF32;
-    g.accum = l.accum;
-    g.ld_accum = s.D;
+    g.ld_grad = ld_grad;
+    g.ld_accum = s.ld_acc;
 
     // the weights of columns [v0, v0 + n): in place, or packed into the workspace
+    int64_t packed = -1;
     auto weights = [&](int64_t v0, int64_t n, Operand* out) -> int {
         const uint8_t* at = static_cast<const uint8_t*>(c.w) + v0 * p.w_row * esize;
         if (!s.pack_w) {
-            *out = Operand{reinterpret_cast<const uint16_t*>(at), n, s.D, p.w_row, 1, 0};
+            *out = Operand{reinterpret_cast<const uint16_t*>(at), n, s.D, p.w_row, dense};
             return SW_OK;
         }
         // zero rows up to whole K stages: a tail of G's zeros must not meet the next plane
         const int64_t rows = round_up(n, kBK);
-        SW_CUDA_TRY(launch_pdl(pack_kernel<kF32>, dim3((unsigned)((rows + 31) / 32), (unsigned)((s.ld_w + 31) / 32)),
-                               dim3(256), 0, stream, (const void*)at, n, s.D, p.w_row, p.w_col, (const int*)nullptr,
-                               l.state, 0, 1, l.wp, s.ld_w, rows),
-                    "linear head weights");
-        *out = Operand{l.wp, rows, s.D, s.ld_w, s.planes, rows};
+        if (packed != v0)
+            SW_CUDA_TRY(launch_pdl(pack_kernel<kF32>,
+                                   dim3((unsigned)((rows + 31) / 32), (unsigned)((s.ld_w + 31) / 32)), dim3(256), 0,
+                                   stream, (const void*)at, n, s.D, p.w_row, p.w_col, (const int*)nullptr, l.state, 0, 1,
+                                   l.wp, s.ld_w, rows),
+                        "linear head weights");
+        packed = v0;
+        *out = Operand{l.wp, s.planes * rows, s.D, s.ld_w, Plane{kBK, 0, (int)rows}};
         return SW_OK;
     };
-
-    if (c.loss) {
-        const int64_t step = s.pack_w ? s.piece : s.V;
-        for (int64_t v0 = 0; v0 < s.V; v0 += step) {
-            const int64_t n = std::min(step, s.V - v0);
-            Operand w;
-            int rc = weights(v0, n, &w);
-            if (rc != SW_OK) return rc;
-            GemmArgs a = g;
-            a.M = (int)s.T;
-            a.N = (int)n;
-            a.K = (int)s.D;
-            a.count_is = kCountM;
-            a.scale_a = kF32 ? 0 : -1;
-            a.scale_b = kF32 ? 1 : -1;
-            a.v0 = v0;
-            rc = gemm<kBf16, false, false, kEpiLse>(hk, w, a, stream);
-            if (rc != SW_OK) return rc;
-        }
+    // logits of compact rows [r0, r0 + n) and columns [v0, v0 + nv)
+    auto logits = [&](int64_t r0, int64_t n, int64_t v0, int64_t nv) {
+        GemmArgs a = g;
+        a.M = (int)n;
+        a.N = (int)nv;
+        a.K = (int)s.D;
+        a.count_is = kCountM;
+        a.row0 = (int)r0;
+        a.scale_a = kF32 ? 0 : -1;
+        a.scale_b = kF32 ? 1 : -1;
+        a.v0 = v0;
+        a.ent_idx = l.ent_idx + r0 * g.ent_k;
+        a.ent_p = l.ent_p ? l.ent_p + r0 * g.ent_k : nullptr;
+        a.offs = l.offs ? l.offs + r0 : nullptr;
+        a.partial = l.partial + r0;
+        a.lse2 = l.lse2 + r0;
+        a.coef = l.coef + r0;
+        a.grad = l.grad;
+        return a;
+    };
+    auto merge = [&](int64_t r0, int64_t n) -> int {
         MergeArgs m;
         memset(&m, 0, sizeof(m));
         m.partial = l.partial;
-        m.tiles = (int)s.tiles;
+        m.tiles = (int)s.half_tiles;
         m.rows_pad = (int)s.rows_pad;
-        m.T = s.T;
+        m.row0 = r0;
+        m.T = std::min(s.T, r0 + n);
         m.V = s.V;
         m.state = l.state;
         m.row_map = l.row_map;
@@ -624,65 +785,158 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
         m.lse2 = l.lse2;
         m.loss = p.reduction == SW_HEAD_MEAN ? nullptr : c.loss;
         m.lse = c.lse;
-        SW_CUDA_TRY(launch_pdl(merge_kernel, dim3((unsigned)std::max<int64_t>((s.T + 31) / 32, 1)), dim3(256), 0, stream, m),
+        SW_CUDA_TRY(launch_pdl(merge_kernel, dim3((unsigned)std::max<int64_t>((n + 31) / 32, 1)), dim3(256), 0, stream,
+                               m),
                     "linear head loss");
-        if (p.reduction == SW_HEAD_MEAN)
-            SW_CUDA_TRY(launch_pdl(mean_kernel, dim3(1), dim3(1024), 0, stream, l.row_loss, l.state, c.loss),
-                        "linear head mean loss");
-    }
-    if (!s.grads) return SW_OK;
-    if (c.dh && s.T > 0)
-        SW_CUDA_TRY(launch_pdl(zero_rows_kernel, dim3((unsigned)std::min<int64_t>(s.T, 1184)), dim3(256), 0, stream,
-                               c.dh, (int)kF32, s.T, s.D, p.dh_row, p.dh_col, l.row_map, l.state),
-                    "linear head ignored rows");
-    for (int64_t v0 = 0; v0 < s.V; v0 += s.piece) {
-        const int64_t n = std::min(s.piece, s.V - v0);
-        Operand w;
-        int rc = weights(v0, n, &w);
-        if (rc != SW_OK) return rc;
+        return SW_OK;
+    };
+    // dh of compact rows [r0, r0 + n) += G[:, 0..nv) w;  dw of columns [v0, v0 + nv) += G^T h
+    auto gradients = [&](int64_t r0, int64_t n, int64_t v0, int64_t nv, const Operand& w, bool first_v, bool last_v,
+                         bool first_r, bool last_r) -> int {
+        const Plane gp = kF32 ? Plane{2 * kBK, kBK, 0} : dense;
+        const Operand gr{l.grad, s.rows, kF32 ? 2 * round_up(nv, 64) : nv, ld_grad, gp};
         GemmArgs a = g;
-        a.M = (int)s.T;
-        a.N = (int)n;
-        a.K = (int)s.D;
-        a.count_is = kCountM;
-        a.scale_a = kF32 ? 0 : -1;
-        a.scale_b = kF32 ? 1 : -1;
-        a.v0 = v0;
-        rc = gemm<kBf16, false, false, kEpiGrad>(hk, w, a, stream);
-        if (rc != SW_OK) return rc;
-        const Operand gr{l.grad, s.rows_pad, n, g.ld_grad, s.planes, s.rows_pad};
+        a.row0 = (int)r0;
         a.dst_f32 = kF32;
-        if (c.dh) {
-            a.M = (int)s.T;
+        SlotsArgs sa;
+        memset(&sa, 0, sizeof(sa));
+        sa.ld_accum = s.ld_acc;
+        sa.cols = s.D;
+        sa.state = l.state;
+        sa.row0 = (int)r0;
+        const unsigned slot_ctas = (unsigned)(8 * device_sms());
+        if (c.dh && n > 0) {
+            a.M = (int)n;
             a.N = (int)s.D;
-            a.K = (int)n;
+            a.K = (int)nv;
             a.count_is = kCountM;
             a.scale_a = kF32 ? 2 : -1;
             a.scale_b = kF32 ? 1 : -1;
-            a.first = v0 == 0;
-            a.last = v0 + n == s.V;
+            a.splits = s.dh_splits;
+            a.accum = s.dh_sums ? l.dh_accum + r0 * s.ld_acc : nullptr;
+            a.slot = s.T * s.ld_acc;
+            a.first = first_v;
+            a.last = last_v && s.dh_splits == 1;
             a.dst = c.dh;
             a.dst_row = p.dh_row;
             a.dst_col = p.dh_col;
-            a.row_map = l.row_map;
-            rc = gemm<kBf16, false, true, kEpiOut>(gr, w, a, stream);
+            a.row_map = l.row_map + r0;
+            int rc = gemm<kBf16, false, true, kEpiOut>(gr, w, a, stream);
             if (rc != SW_OK) return rc;
+            if (last_v && s.dh_splits > 1) {
+                sa.accum = a.accum;
+                sa.slot = a.slot;
+                sa.splits = s.dh_splits;
+                sa.rows = n;
+                sa.by_count = 1;
+                sa.row_map = a.row_map;
+                sa.dst = c.dh;
+                sa.dst_row = p.dh_row;
+                sa.dst_col = p.dh_col;
+                SW_CUDA_TRY(launch_pdl(sum_slots_kernel<kF32>, dim3(slot_ctas), dim3(256), 0, stream, sa),
+                            "linear head dh");
+            }
         }
         if (c.dw) {
-            a.M = (int)n;
+            a.M = (int)nv;
             a.N = (int)s.D;
-            a.K = (int)s.T;
+            a.K = (int)n;
             a.count_is = kCountK;
             a.scale_a = kF32 ? 2 : -1;
             a.scale_b = kF32 ? 0 : -1;
-            a.accum = nullptr;
+            a.splits = s.dw_splits;
+            a.accum = s.dw_sums ? l.dw_accum : nullptr;
+            a.slot = (s.keep ? s.V : s.piece) * s.ld_acc;
+            a.first = first_r;
+            a.last = last_r && s.dw_splits == 1;
             a.row_map = nullptr;
             a.dst = static_cast<uint8_t*>(c.dw) + v0 * p.dw_row * esize;
             a.dst_row = p.dw_row;
             a.dst_col = p.dw_col;
-            rc = gemm<kBf16, true, true, kEpiOut>(gr, hk, a, stream);
+            int rc = gemm<kBf16, true, true, kEpiOut>(gr, states(r0, round_up(std::max<int64_t>(n, 1), kBM)), a, stream);
+            if (rc != SW_OK) return rc;
+            if (last_r && s.dw_splits > 1) {
+                sa.accum = a.accum;
+                sa.slot = a.slot;
+                sa.splits = s.dw_splits;
+                sa.rows = nv;
+                sa.by_count = 0;
+                sa.row_map = nullptr;
+                sa.dst = a.dst;
+                sa.dst_row = p.dw_row;
+                sa.dst_col = p.dw_col;
+                SW_CUDA_TRY(launch_pdl(sum_slots_kernel<kF32>, dim3(slot_ctas), dim3(256), 0, stream, sa),
+                            "linear head dw");
+            }
+        }
+        return SW_OK;
+    };
+    auto mean = [&]() -> int {
+        if (c.loss && p.reduction == SW_HEAD_MEAN)
+            SW_CUDA_TRY(launch_pdl(mean_kernel, dim3(1), dim3(1024), 0, stream, l.row_loss, l.state, c.loss),
+                        "linear head mean loss");
+        return SW_OK;
+    };
+    if (c.dh && s.T > 0)
+        SW_CUDA_TRY(launch_pdl(zero_rows_kernel, dim3((unsigned)std::min<int64_t>(s.T, 1184)), dim3(256), 0, stream,
+                               c.dh, (int)kF32, s.T, s.D, p.dh_row, p.dh_col, l.row_map, l.state),
+                    "linear head ignored rows");
+
+    int rc;
+    if (s.keep) {
+        Operand w;
+        if ((rc = weights(0, s.V, &w)) != SW_OK) return rc;
+        for (int64_t r0 = 0; r0 == 0 || r0 < s.T; r0 += s.rows) {
+            const int64_t n = std::min(s.rows, s.T - r0);
+            GemmArgs a = logits(r0, n, 0, s.V);
+            a.keep = 1;
+            a.ent_s = l.ent_s + r0 * g.ent_k;
+            if ((rc = gemm<kBf16, false, false, kEpiLse>(states(r0, round_up(std::max<int64_t>(n, 1), kBM)), w, a, stream)) != SW_OK) return rc;
+            if ((rc = merge(r0, n)) != SW_OK) return rc;
+            ScaleArgs sc;
+            memset(&sc, 0, sizeof(sc));
+            sc.grad = l.grad;
+            sc.ld_grad = ld_grad;
+            sc.V = s.V;
+            sc.partial = a.partial;
+            sc.rows_pad = (int)s.rows_pad;
+            sc.row0 = (int)r0;
+            sc.state = l.state;
+            sc.lse2 = a.lse2;
+            sc.coef = a.coef;
+            sc.ent_idx = a.ent_idx;
+            sc.ent_p = a.ent_p;
+            sc.ent_s = a.ent_s;
+            sc.ent_k = g.ent_k;
+            if (n > 0)
+                SW_CUDA_TRY(launch_pdl(scale_kernel<kF32>,
+                                       dim3((unsigned)n, (unsigned)((s.V + kScaleCols - 1) / kScaleCols)), dim3(256), 0,
+                                       stream, sc),
+                            "linear head logits' gradient");
+            if ((rc = gradients(r0, n, 0, s.V, w, true, true, r0 == 0, r0 + s.rows >= s.T)) != SW_OK) return rc;
+        }
+        return mean();
+    }
+    if (c.loss) {
+        const int64_t step = s.pack_w ? s.piece : s.V;
+        for (int64_t v0 = 0; v0 < s.V; v0 += step) {
+            const int64_t n = std::min(step, s.V - v0);
+            Operand w;
+            if ((rc = weights(v0, n, &w)) != SW_OK) return rc;
+            rc = gemm<kBf16, false, false, kEpiLse>(states(0, s.rows_pad), w, logits(0, s.T, v0, n), stream);
             if (rc != SW_OK) return rc;
         }
+        if ((rc = merge(0, s.T)) != SW_OK) return rc;
+        if ((rc = mean()) != SW_OK) return rc;
+    }
+    if (!s.grads) return SW_OK;
+    for (int64_t v0 = 0; v0 < s.V; v0 += s.piece) {
+        const int64_t n = std::min(s.piece, s.V - v0);
+        Operand w;
+        if ((rc = weights(v0, n, &w)) != SW_OK) return rc;
+        rc = gemm<kBf16, false, false, kEpiGrad>(states(0, s.rows_pad), w, logits(0, s.T, v0, n), stream);
+        if (rc != SW_OK) return rc;
+        if ((rc = gradients(0, s.T, v0, n, w, v0 == 0, v0 + n == s.V, true, true)) != SW_OK) return rc;
     }
     return SW_OK;
 }
@@ -752,16 +1006,39 @@ int check_and_run(const char* name, Call& c, void* stream_ptr) {
     s.rows_pad = std::max<int64_t>(round_up(T, kBM), kBM);
     s.ld_h = s.ld_w = round_up(D, 8);
     s.grads = grads;
-    s.tiles = (V + 255) / 256 * 2;  // half tiles, each with its own partial statistics
+    s.half_tiles = (V + 255) / 256 * 2;
+    s.ld_acc = round_up(D, 4);
     // weights are read in place when TMA can: bf16, unit stride, 16-byte rows
     s.pack_w = s.f32 || p->w_col != 1 || p->w_row % 8 != 0 || p->w_row < D ||
                (reinterpret_cast<uintptr_t>(c.w) & 15) != 0;
-    // the piece of the vocabulary: as wide as the workspace limit allows, in
-    // whole 256-column tiles
-    const int64_t per_column = (grads ? s.planes * s.rows_pad * 2 : 0) + (s.pack_w ? s.planes * s.ld_w * 2 : 0);
     const int64_t budget = p->workspace_limit > 0 ? p->workspace_limit : kDefaultWorkspace;
+    const int64_t packed = s.pack_w ? s.planes * round_up(V, kBK) * s.ld_w * 2 : 0;
+    const int64_t grad_row = s.planes * round_up(V, 256) * 2;
+    const int terms = s.f32 ? 3 : 1, sms = device_sms();
+    // One call for the loss and the gradients keeps the logits' exponentials
+    // of as many rows as the workspace limit allows (6 T V D operations and one
+    // more pass over them); from a kept lse, or where not even 1024 rows (or
+    // all) fit, the logits are computed again (8 T V D).
+    s.rows = s.rows_pad;
+    s.keep = false;
+    if (c.loss && grads && packed < budget) {
+        const int64_t fit = (budget - packed) / grad_row / kBM * kBM;
+        if (fit >= std::min<int64_t>(s.rows_pad, 1024)) {
+            s.keep = true;
+            const int64_t chunks = (s.rows_pad + fit - 1) / fit;
+            s.rows = std::min(s.rows_pad, round_up((s.rows_pad + chunks - 1) / chunks, kBM));
+        }
+    }
     s.piece = round_up(V, 256);
-    if (per_column > 0) s.piece = std::min(s.piece, std::max<int64_t>(budget / per_column / 256 * 256, 256));
+    if (!s.keep) {
+        // as wide as the limit allows, in whole 256-column tiles
+        const int64_t per_column = (grads ? s.planes * s.rows_pad * 2 : 0) + (s.pack_w ? s.planes * s.ld_w * 2 : 0);
+        if (per_column > 0) s.piece = std::min(s.piece, std::max<int64_t>(budget / per_column / 256 * 256, 256));
+    }
+    s.dh_splits = c.dh ? choose_splits(std::min(s.rows, T), D, std::min(s.piece, V), terms, sms) : 1;
+    s.dw_splits = c.dw ? choose_splits(std::min(s.piece, V), D, std::min(s.rows, T), terms, sms) : 1;
+    s.dh_sums = c.dh && (s.dh_splits > 1 || s.piece < V);
+    s.dw_sums = c.dw && (s.dw_splits > 1 || s.rows < T);
 
     Bump measure{nullptr, 0};
     lay_out(measure, c, s);

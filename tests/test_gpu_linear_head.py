@@ -323,6 +323,27 @@ def test_pieces_of_the_vocabulary(limit, op, dtype):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("op", ["xent", "distill"])
+def test_blocks_of_rows(op, dtype):
+    """A workspace limit under which the rows are taken about 1100 at a time, with blocks that no row reaches."""
+    T, V, D = 3000, 300, 72
+    h, w, y = states(T, V, D, dtype)
+    kw = dict(targets=y)
+    limit = 1_200_000 if dtype == torch.bfloat16 else 2_500_000
+    up = torch.rand(T, device="cuda") + 0.5
+    for ignored in (slice(5, 9), slice(700, 3000)):
+        if op == "distill":
+            index, logits = teacher(T, V, 20)
+            index[ignored] = -1
+            kw = dict(index=index, logits=logits, tau=2.0)
+        else:
+            kw = dict(targets=y.clone())
+            kw["targets"][ignored] = IGNORE
+        check(call(h, w, up=up, limit=limit, **kw), reference(h, w, up, **kw), dtype)
+        check(call(h, w, up=up[:1], mean=True, limit=limit, **kw), reference(h, w, up[:1], mean=True, **kw), dtype, True)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("op", ["xent", "distill"])
 @pytest.mark.parametrize("mean", [False, True])
 def test_gradients_from_a_kept_lse(op, dtype, mean):
     T, V, D = 140, 900, 72
