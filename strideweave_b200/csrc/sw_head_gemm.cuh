@@ -9,18 +9,23 @@
 //             rounded once to the operand type
 //   kEpiOut   the product itself: a gradient of the states or of the weights
 //
-// One persistent CTA per SM walks 128 x BN tiles.  Warp 0 feeds a ring of
-// 64-deep K stages by TMA (128-byte swizzle), one thread of warp 1 issues the
-// MMAs, warps 2-9 drain one of two TMEM accumulators while the other is being
-// filled: warp w reads TMEM sub-partition w % 4 (32 rows) and one half of the
-// tile's columns.  Float32 operands come as two f16 planes (hi + lo of a
+// A persistent CTA (kPair false) walks 128 x 256 tiles, or a pair of CTAs on
+// neighbouring SMs (kPair) walks 256 x 256 tiles with tcgen05 cta_group::2: each
+// CTA holds its 128 rows of A and half of B in shared memory and its 128 rows
+// of the accumulator in TMEM, so a stage moves 32 KiB per SM instead of 48.
+// Warp 0 feeds a ring of 64-deep K stages by TMA (128-byte swizzle), one thread
+// of warp 1 (of the pair's first CTA) issues the MMAs, warps 2-9 drain one of
+// two TMEM accumulators while the other is being filled: warp w reads TMEM
+// sub-partition w % 4 (32 rows) and one half of the tile's columns.  Results
+// pass through 4 KiB of shared memory per warp, so that they leave as whole
+// 128-byte row segments.  Float32 operands come as two f16 planes (hi + lo of a
 // power-of-two multiple of the value): the K walk then runs over three plane
 // pairs, hi lo + lo hi + hi hi, which keeps 22 bits of each factor.
 //
 // The tensor core's fp32 accumulator drops the bits below its last place, so a
 // long K walk drifts: measured 1.3e-9 per K element, 1.5e-4 over 128000.  Where
-// the result is Float32 (kChunked) the walk is cut into kChunkSteps stages, and
-// the epilogue adds the pieces in registers, rounded to nearest.
+// the result is Float32 (kChunked) the walk is cut into 8 or 16 stages, and the
+// epilogue adds the pieces in registers, rounded to nearest.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -36,7 +41,7 @@ namespace head {
 
 constexpr int kBM = 128;
 constexpr int kBK = 64;                 // K elements of a stage: one 128-byte swizzle row
-constexpr int kChunkSteps = 8;          // K stages between two register sums (512 elements of K)
+constexpr int kBN = 256;
 constexpr int kEntryTile = 256;         // columns per entry of the target offset table
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -109,28 +114,104 @@ struct GemmArgs {
     const int* row_map;      // destination row of each row (null: itself)
 };
 
-template <int BN, int kStages>
+template <bool kPair>
 struct Cfg {
     static constexpr int kThreads = 64 + 256;
+    static constexpr int kTileM = kPair ? 2 * kBM : kBM;
+    static constexpr int kBRows = kPair ? kBN / 2 : kBN;  // rows of B that one CTA holds
     static constexpr int kABytes = kBM * kBK * 2;
-    static constexpr int kBBytes = BN * kBK * 2;
+    static constexpr int kBBytes = kBRows * kBK * 2;
     static constexpr int kStageBytes = kABytes + kBBytes;
-    static constexpr int kOffBar = kStages * kStageBytes;
+    static constexpr int kStages = kPair ? 6 : 4;
+    static constexpr int kOffOut = kStages * kStageBytes;  // 4 KiB per epilogue warp
+    static constexpr int kOffBar = kOffOut + 8 * 4096;
     static constexpr int kNumBars = 2 * kStages + 5;
     static constexpr int kOffSlot = kOffBar + kNumBars * 8;
     static constexpr int kSmemBytes = kOffSlot + 16 + 1024;
-    static constexpr int kTmemCols = 2 * BN;
+    static constexpr int kTmemCols = 2 * kBN;
     static_assert(kSmemBytes <= 232448, "shared memory budget");
 };
 
 // D[tmem] (+)= A[smem] B[smem], 16-bit operands, fp32 accumulation.
+template <bool kPair>
 __device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
                                         uint32_t accumulate) {
-    asm volatile(
-        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-        : "memory");
+    if (kPair)
+        asm volatile(
+            "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+            "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d_tmem),
+            "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d_tmem),
+            "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+            : "memory");
+}
+
+// Arrive on the barrier (of both CTAs of a pair) once every MMA issued so far is done.
+template <bool kPair>
+__device__ __forceinline__ void commit(uint32_t bar) {
+    if (kPair)
+        asm volatile(
+            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+                bar),
+            "h"((uint16_t)3)
+            : "memory");
+    else
+        ptx::tc_commit(bar);
+}
+
+template <bool kPair>
+__device__ __forceinline__ void tmem_alloc(uint32_t slot_smem, uint32_t ncols) {
+    if (kPair) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot_smem), "r"(ncols));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    } else {
+        ptx::tmem_alloc(slot_smem, ncols);
+        ptx::tmem_relinquish();
+    }
+}
+template <bool kPair>
+__device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t ncols) {
+    if (kPair)
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols));
+    else
+        ptx::tmem_dealloc(taddr, ncols);
+}
+
+// A TMA load into this CTA's shared memory that completes on `bar`, which with
+// kPair lies in the pair's first CTA (a shared::cluster address).
+template <bool kPair>
+__device__ __forceinline__ void tma_load(uint32_t dst, const void* tmap, int32_t x, int32_t y, uint32_t bar) {
+    if (kPair)
+        asm volatile(
+            "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
+            "%3}], [%4];" ::"r"(dst),
+            "l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(y), "r"(bar)
+            : "memory");
+    else
+        ptx::tma_load_2d(dst, tmap, x, y, bar);
+}
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+// Shared-memory address of the same variable in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t mapa(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void arrive_cluster(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // Instruction descriptor of kind::f16: fp32 D; both operands bf16 or both f16;
@@ -206,20 +287,41 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     return *reinterpret_cast<uint32_t*>(&v);
 }
 
-template <bool kBf16>
-__device__ __forceinline__ void store_row32(uint16_t* dst, const float (&r)[32]) {
-    uint4* d = reinterpret_cast<uint4*>(dst);
+// Hands 32 rows x 128 bytes, a row per lane in registers, to `emit(row, unit,
+// 16 bytes)` so that eight lanes hold one row's 128 bytes: through the warp's
+// 4 KiB of shared memory, 16-byte units swizzled by row % 8 (conflict-free both
+// ways).
+template <class F>
+__device__ __forceinline__ void transpose_rows(uint8_t* box, int lane, const uint32_t (&w)[32], F&& emit) {
+    __syncwarp();
 #pragma unroll
-    for (int v = 0; v < 4; ++v)
-        d[v] = make_uint4(pack2<kBf16>(r[8 * v], r[8 * v + 1]), pack2<kBf16>(r[8 * v + 2], r[8 * v + 3]),
-                          pack2<kBf16>(r[8 * v + 4], r[8 * v + 5]), pack2<kBf16>(r[8 * v + 6], r[8 * v + 7]));
+    for (int u = 0; u < 8; ++u)
+        *reinterpret_cast<uint4*>(box + lane * 128 + (u ^ (lane & 7)) * 16) =
+            make_uint4(w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int row = i * 4 + (lane >> 3), unit = lane & 7;
+        emit(row, unit, *reinterpret_cast<const uint4*>(box + row * 128 + (unit ^ (row & 7)) * 16));
+    }
 }
 
-// Where 32 columns of a row's logits' gradient are: column n0 of the row, and
-// in Float32 its hi values (the lo values 64 elements further).
-template <bool kBf16>
-__device__ __forceinline__ uint16_t* grad_at(const GemmArgs& args, int64_t m, int64_t n0) {
-    return args.grad + m * args.ld_grad + (kBf16 ? n0 : (n0 & ~int64_t(63)) * 2 + (n0 & 63));
+// What an epilogue warp knows about its 32 rows of a tile.
+struct WarpRows {
+    uint8_t* box;   // its 4 KiB of shared memory
+    int lane;
+    int64_t m0;     // first row; lane holds row m0 + lane
+    int64_t M;      // rows that exist
+    bool row_in;
+};
+
+// 128 bytes of each of the warp's rows of the logits' gradient (all rows of a
+// tile are written: the ones that do not exist as zeros).
+__device__ __forceinline__ void put_grad(const GemmArgs& args, const WarpRows& wr, int64_t element, uint32_t (&w)[32]) {
+    uint16_t* base = args.grad + wr.m0 * args.ld_grad + element;
+    transpose_rows(wr.box, wr.lane, w, [&](int row, int unit, const uint4& v) {
+        reinterpret_cast<uint4*>(base + row * args.ld_grad)[unit] = v;
+    });
 }
 
 // Softmax statistics of a row over the half tile in registers, in base-2
@@ -227,17 +329,18 @@ __device__ __forceinline__ uint16_t* grad_at(const GemmArgs& args, int64_t m, in
 // `keep` the exponentials are stored too, for the gradient: as f16 times 2^15
 // (11 bits down to 2^-29 of the half tile's largest; the later rounding to
 // bf16 is the one that counts) or, for Float32, as they are.
-template <bool kBf16, int kParts>
-__device__ __forceinline__ float4 lse_tile(const GemmArgs& args, EntryCursor& cur, int64_t m, int64_t n0, bool row_in,
-                                           float k2, float (&r)[kParts][32]) {
+template <bool kBf16, int kBlocks>
+__device__ __forceinline__ float4 lse_tile(const GemmArgs& args, const WarpRows& wr, EntryCursor& cur, int64_t n0,
+                                           float k2, float (&r)[kBlocks][2][32]) {
+    const int64_t m = wr.m0 + wr.lane;
     float dot = 0.0f, top = -INFINITY;
 #pragma unroll
-    for (int c = 0; c < kParts; ++c) {
+    for (int c = 0; c < 2 * kBlocks; ++c) {
         cur.walk(args.v0 + n0 + c * 32, [&](int rel, float p) {
             float v = 0.0f;
 #pragma unroll
             for (int j = 0; j < 32; ++j)
-                if (j == rel) v = r[c][j];
+                if (j == rel) v = r[c / 2][c % 2][j];
             if (rel >= 0) {
                 dot += p * v;
                 if (args.ent_s) args.ent_s[m * args.ent_k + cur.e] = v * k2;
@@ -247,131 +350,186 @@ __device__ __forceinline__ float4 lse_tile(const GemmArgs& args, EntryCursor& cu
         if (ncols < 32) {
 #pragma unroll
             for (int j = 0; j < 32; ++j)
-                if (j >= ncols) r[c][j] = -INFINITY;
+                if (j >= ncols) r[c / 2][c % 2][j] = -INFINITY;
         }
 #pragma unroll
-        for (int j = 0; j < 32; ++j) top = fmaxf(top, r[c][j]);
+        for (int j = 0; j < 32; ++j) top = fmaxf(top, r[c / 2][c % 2][j]);
     }
     const float ref = top * k2;
     // columns of nothing but -inf add nothing (and must not make -inf minus -inf)
     const float base = ref == -INFINITY ? 0.0f : ref;
     float sum = 0.0f;
 #pragma unroll
-    for (int c = 0; c < kParts; ++c) {
+    for (int c = 0; c < 2 * kBlocks; ++c) {
 #pragma unroll
         for (int j = 0; j < 32; ++j) {
-            r[c][j] = ex2(fmaf(r[c][j], k2, -base));
-            sum += r[c][j];
+            r[c / 2][c % 2][j] = ex2(fmaf(r[c / 2][c % 2][j], k2, -base));
+            sum += r[c / 2][c % 2][j];
         }
-        // (Float32 blocks of 64 columns are written whole: the K walk reads them whole)
-        if (args.keep && n0 + c * 32 < (kBf16 ? int64_t(args.N) : (int64_t(args.N) + 63) / 64 * 64)) {
+    }
+    if (args.keep) {
+        const float up = !wr.row_in ? 0.0f : kBf16 ? 32768.0f : 1.0f;
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b) {
+            if (n0 + b * 64 >= args.N) break;  // (blocks of 64 columns are written whole)
             if (kBf16) {
+                uint32_t w[32];
 #pragma unroll
-                for (int j = 0; j < 32; ++j) r[c][j] = row_in ? r[c][j] * 32768.0f : 0.0f;
-                store_row32<false>(grad_at<true>(args, m, n0 + c * 32), r[c]);
+                for (int j = 0; j < 32; ++j) {
+                    const float (&x)[32] = r[b][j / 16];
+                    w[j] = pack2<false>(x[2 * (j % 16)] * up, x[2 * (j % 16) + 1] * up);
+                }
+                put_grad(args, wr, n0 + b * 64, w);
             } else {
-                float4* d = reinterpret_cast<float4*>(args.grad + m * args.ld_grad + 2 * (n0 + c * 32));
 #pragma unroll
-                for (int v = 0; v < 8; ++v)
-                    d[v] = row_in ? make_float4(r[c][4 * v], r[c][4 * v + 1], r[c][4 * v + 2], r[c][4 * v + 3])
-                                  : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                for (int c = 2 * b; c < 2 * b + 2; ++c) {
+                    uint32_t w[32];
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) w[j] = wr.row_in ? __float_as_uint(r[c / 2][c % 2][j]) : 0u;
+                    put_grad(args, wr, 2 * (n0 + c * 32), w);
+                }
             }
         }
     }
     return make_float4(ref, sum, dot * k2, 0.0f);
 }
 
-// Gradient with respect to 32 logits of a row: softmax minus target in fp32,
-// rounded once to the type the next contractions read.  Float32: zeros up to
-// the end of a 64-column block, which the K walk reads whole.
+// Gradient with respect to 64 logits of a row: softmax minus target in fp32,
+// rounded once to the type the next contractions read.
 template <bool kBf16>
-__device__ __forceinline__ void grad_part(const GemmArgs& args, EntryCursor& cur, int64_t m, int64_t n0, int ncols,
-                                          bool row_in, float k2, float lse2, float coef, float (&r)[32]) {
+__device__ __forceinline__ void grad_block(const GemmArgs& args, const WarpRows& wr, EntryCursor& cur, int64_t n0,
+                                           float k2, float lse2, float coef, float (&r)[2][32]) {
+    uint32_t hi[32];
 #pragma unroll
-    for (int j = 0; j < 32; ++j) r[j] = ex2(fmaf(r[j], k2, -lse2));
-    cur.walk(args.v0 + n0, [&](int rel, float p) {
+    for (int c = 0; c < 2; ++c) {
+        const int ncols = (int)min(int64_t(32), int64_t(args.N) - (n0 + c * 32));
 #pragma unroll
-        for (int j = 0; j < 32; ++j)
-            if (j == rel) r[j] -= p;
-    });
+        for (int j = 0; j < 32; ++j) r[c][j] = ex2(fmaf(r[c][j], k2, -lse2));
+        cur.walk(args.v0 + n0 + c * 32, [&](int rel, float p) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j) r[j] = row_in && j < ncols ? r[j] * coef : 0.0f;
-    uint16_t* d = grad_at<kBf16>(args, m, n0);
-    store_row32<kBf16>(d, r);
+            for (int j = 0; j < 32; ++j)
+                if (j == rel) r[c][j] -= p;
+        });
+#pragma unroll
+        for (int j = 0; j < 32; ++j) r[c][j] = wr.row_in && j < ncols ? r[c][j] * coef : 0.0f;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) hi[c * 16 + j] = pack2<kBf16>(r[c][2 * j], r[c][2 * j + 1]);
+    }
+    put_grad(args, wr, kBf16 ? n0 : 2 * n0, hi);
     if (!kBf16) {
+        uint32_t lo[32];
 #pragma unroll
-        for (int j = 0; j < 32; ++j) r[j] -= __half2float(__float2half_rn(r[j]));
-        store_row32<kBf16>(d + 64, r);
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi[c * 16 + j]));
+                lo[c * 16 + j] = pack2<false>(r[c][2 * j] - h.x, r[c][2 * j + 1] - h.y);
+            }
+        put_grad(args, wr, 2 * n0 + 64, lo);
     }
 }
 
-// 32 columns of a result row: scaled, added to the running fp32 sum, and the
-// last time written in the result's type.
-__device__ __forceinline__ void out_part(const GemmArgs& args, int split, int64_t m, int64_t n0, int ncols,
-                                         float scale, float (&r)[32]) {
-#pragma unroll
-    for (int j = 0; j < 32; ++j) r[j] *= scale;
-    if (args.accum) {
-        float* a = args.accum + split * args.slot + m * args.ld_accum + n0;
-        const bool whole = ncols == 32 && (reinterpret_cast<uintptr_t>(a) & 15) == 0;
-        if (!args.first) {
-            if (whole) {
-#pragma unroll
-                for (int v = 0; v < 8; ++v) {
-                    const float4 o = reinterpret_cast<const float4*>(a)[v];
-                    r[4 * v] += o.x;
-                    r[4 * v + 1] += o.y;
-                    r[4 * v + 2] += o.z;
-                    r[4 * v + 3] += o.w;
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 32; ++j)
-                    if (j < ncols) r[j] += a[j];
+// Where out_block writes, as far as a launch fixes it.
+struct OutPlan {
+    bool vec;  // whole 16-byte units: unit column stride, aligned rows
+};
+
+// 32 Float32 columns (or, for a bf16 result that is not summed, 64 columns) of
+// the warp's rows: added to the running fp32 sum, and the last time written in
+// the result's type.
+template <bool kWide>
+__device__ __forceinline__ void out_words(const GemmArgs& args, const WarpRows& wr, const OutPlan& plan, int split,
+                                          int64_t n0, const uint32_t (&w)[32], int dst_row_of_lane) {
+    constexpr int kUnit = kWide ? 8 : 4;  // columns of 16 bytes
+    if (n0 >= args.N) return;
+    transpose_rows(wr.box, wr.lane, w, [&](int row, int unit, uint4 v) {
+        const int dst_row = __shfl_sync(0xffffffffu, dst_row_of_lane, row);
+        const int64_t m = wr.m0 + row, n = n0 + unit * kUnit;
+        const int ncols = (int)min(int64_t(kUnit), int64_t(args.N) - n);
+        if (m >= wr.M || ncols <= 0) return;
+        if (!kWide && args.accum) {
+            // (rows of the running sums are whole groups of four)
+            float4* a = reinterpret_cast<float4*>(args.accum + split * args.slot + m * args.ld_accum + n);
+            float4 x = make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z),
+                                   __uint_as_float(v.w));
+            if (!args.first) {
+                const float4 o = *a;
+                x.x += o.x;
+                x.y += o.y;
+                x.z += o.z;
+                x.w += o.w;
             }
-        }
-        if (!args.last) {
-            if (whole) {
-#pragma unroll
-                for (int v = 0; v < 8; ++v)
-                    reinterpret_cast<float4*>(a)[v] = make_float4(r[4 * v], r[4 * v + 1], r[4 * v + 2], r[4 * v + 3]);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 32; ++j)
-                    if (j < ncols) a[j] = r[j];
+            if (!args.last) {
+                *a = x;
+                return;
             }
-            return;
+            v = make_uint4(__float_as_uint(x.x), __float_as_uint(x.y), __float_as_uint(x.z), __float_as_uint(x.w));
         }
-    }
-    const int64_t row = args.row_map ? args.row_map[m] : m;
-    if (args.dst_f32) {
-        float* d = static_cast<float*>(args.dst) + row * args.dst_row + n0 * args.dst_col;
-        if (ncols == 32 && args.dst_col == 1 && (reinterpret_cast<uintptr_t>(d) & 15) == 0) {
+        const int64_t at = int64_t(dst_row) * args.dst_row + n * args.dst_col;
+        if (kWide) {
+            uint16_t* d = static_cast<uint16_t*>(args.dst) + at;
+            if (plan.vec && ncols == 8) {
+                *reinterpret_cast<uint4*>(d) = v;
+            } else {
+                const uint32_t q[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-            for (int v = 0; v < 8; ++v)
-                reinterpret_cast<float4*>(d)[v] = make_float4(r[4 * v], r[4 * v + 1], r[4 * v + 2], r[4 * v + 3]);
+                for (int j = 0; j < 8; ++j)
+                    if (j < ncols) d[j * args.dst_col] = uint16_t(q[j / 2] >> (j % 2 * 16));
+            }
+        } else if (args.dst_f32) {
+            float* d = static_cast<float*>(args.dst) + at;
+            if (plan.vec && ncols == 4) {
+                *reinterpret_cast<uint4*>(d) = v;
+            } else {
+                const uint32_t q[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (j < ncols) d[j * args.dst_col] = __uint_as_float(q[j]);
+            }
         } else {
+            __nv_bfloat16* d = static_cast<__nv_bfloat16*>(args.dst) + at;
+            const float q[4] = {__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z),
+                                __uint_as_float(v.w)};
+            if (plan.vec && ncols == 4) {
+                *reinterpret_cast<uint2*>(d) = make_uint2(pack2<true>(q[0], q[1]), pack2<true>(q[2], q[3]));
+            } else {
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-                if (j < ncols) d[j * args.dst_col] = r[j];
+                for (int j = 0; j < 4; ++j)
+                    if (j < ncols) d[j * args.dst_col] = __float2bfloat16_rn(q[j]);
+            }
+        }
+    });
+}
+
+// 64 columns of the warp's rows, in registers as two parts of 32.
+template <bool kF32>
+__device__ __forceinline__ void out_block(const GemmArgs& args, const WarpRows& wr, const OutPlan& plan, int split,
+                                          int64_t n0, float scale, float (&r)[2][32], int dst_row_of_lane) {
+    uint32_t w[32];
+    if (kF32 || args.accum) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) w[j] = __float_as_uint(r[c][j] * scale);
+            out_words<false>(args, wr, plan, split, n0 + c * 32, w, dst_row_of_lane);
         }
     } else {
-        __nv_bfloat16* d = static_cast<__nv_bfloat16*>(args.dst) + row * args.dst_row + n0 * args.dst_col;
-        if (ncols == 32 && args.dst_col == 1 && (reinterpret_cast<uintptr_t>(d) & 15) == 0) {
-            store_row32<true>(reinterpret_cast<uint16_t*>(d), r);
-        } else {
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-                if (j < ncols) d[j * args.dst_col] = __float2bfloat16_rn(r[j]);
-        }
+        for (int j = 0; j < 32; ++j)
+            w[j] = pack2<true>(r[j / 16][2 * (j % 16)] * scale, r[j / 16][2 * (j % 16) + 1] * scale);
+        out_words<true>(args, wr, plan, split, n0, w, dst_row_of_lane);
     }
 }
 
-template <int BN, int kStages, bool kBf16, bool kAMn, bool kBMn, int kEpi, bool kChunked>
+template <bool kPair, bool kBf16, bool kAMn, bool kBMn, int kEpi>
 __global__ void __launch_bounds__(320, 1)
     head_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                      const GemmArgs args) {
-    using C = Cfg<BN, kStages>;
+    using C = Cfg<kPair>;
+    constexpr bool kChunked = !kBf16 || kEpi == kEpiLse;
+    // K stages between two register sums: 512 elements; 1024 in bf16, whose logits need 1e-6
+    constexpr int kChunkSteps = kBf16 ? 16 : 8;
+    constexpr int kStages = C::kStages;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const uint32_t sbase = ptx::smem_addr(smem);
@@ -383,6 +541,9 @@ __global__ void __launch_bounds__(320, 1)
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kOffSlot);
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
+    // of a pair, the first CTA holds the barriers that the MMA thread waits on
+    const uint32_t rank = kPair ? cluster_rank() : 0;
+    const int worker = kPair ? blockIdx.x >> 1 : blockIdx.x, workers = kPair ? gridDim.x >> 1 : gridDim.x;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
@@ -391,19 +552,18 @@ __global__ void __launch_bounds__(320, 1)
         }
         for (int b = 0; b < 2; ++b) {
             ptx::mbar_init(bar_tmem_full + 8 * b, 1);
-            ptx::mbar_init(bar_tmem_empty + 8 * b, 256);
+            ptx::mbar_init(bar_tmem_empty + 8 * b, kPair ? 16 : 8);  // a lane of every epilogue warp
         }
         ptx::mbar_init(bar_drain, 1);
         ptx::fence_barrier_init();
         ptx::prefetch_tmap(&tmap_a);
         ptx::prefetch_tmap(&tmap_b);
     }
-    if (warp == 1) {
-        ptx::tmem_alloc(ptx::smem_addr(tmem_slot), C::kTmemCols);
-        ptx::tmem_relinquish();
-    }
+    if (warp == 1) tmem_alloc<kPair>(ptx::smem_addr(tmem_slot), C::kTmemCols);
     ptx::tc_fence_before();
     __syncthreads();
+    __syncwarp();
+    if (kPair) cluster_sync();  // the other CTA's barriers are initialised
     ptx::tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     pdl_enter();
@@ -411,13 +571,13 @@ __global__ void __launch_bounds__(320, 1)
     const int count = args.count_is == kCountNone ? 0 : max(args.state->count - args.row0, 0);
     const int M = args.count_is == kCountM ? min(args.M, count) : args.M;
     const int K = args.count_is == kCountK ? min(args.K, count) : args.K;
-    const int num_m = (M + kBM - 1) / kBM;
-    const int num_n = (args.N + BN - 1) / BN;
+    const int num_m = (M + C::kTileM - 1) / C::kTileM;
+    const int num_n = (args.N + kBN - 1) / kBN;
     const int num_tiles = num_m * num_n;
     const int num_items = num_tiles * args.splits;
     const int k_steps = (K + kBK - 1) / kBK;
     const int split_steps = (k_steps + args.splits - 1) / args.splits;
-    constexpr int kGroup = 16;
+    constexpr int kGroup = kPair ? 8 : 16;  // row tiles of a raster group: they share B's panels in L2
     // Work item `t`: a tile and its share [k0, k1) of the K stages.
     auto item = [&](int t, int& mb, int& nb, int& split, int& k0, int& k1) {
         split = t / num_tiles;
@@ -436,13 +596,15 @@ __global__ void __launch_bounds__(320, 1)
 
     if (warp == 0) {
         if (lane == 0) {
+            // ---------------- producer ----------------
             int stage = 0;
             uint32_t phase = 0;
             uint32_t issued[kStages] = {0};
             bool alive = true;
-            for (int t = blockIdx.x; t < num_items && alive; t += gridDim.x) {
+            for (int t = worker; t < num_items && alive; t += workers) {
                 int mb, nb, split, k0, k1;
                 item(t, mb, nb, split, k0, k1);
+                const int a0 = mb * C::kTileM + rank * kBM, b0 = nb * kBN + rank * C::kBRows;
                 for (int c0 = k0; c0 < k1 && alive; c0 = chunk_end(c0, k1))
                     for (int term = 0; term < args.terms && alive; ++term) {
                         // plane pairs, the small products first: (hi, lo), (lo, hi), (hi, hi)
@@ -453,48 +615,56 @@ __global__ void __launch_bounds__(320, 1)
                         const int c1 = chunk_end(c0, k1);
                         for (int ks = c0; ks < c1; ++ks) {
                             if (!ptx::mbar_wait(bar_empty + 8 * stage, phase ^ 1)) { alive = false; break; }
-                            const uint32_t full = bar_full + 8 * stage;
+                            const uint32_t own = bar_full + 8 * stage;
+                            const uint32_t full = kPair ? mapa(own, 0) : own;
                             const uint32_t sa = sbase + stage * C::kStageBytes;
                             const uint32_t sb = sa + C::kABytes;
-                            ptx::mbar_arrive_expect_tx(full, C::kStageBytes);
+                            // the first CTA's barrier counts both CTAs' bytes
+                            if (rank == 0) ptx::mbar_arrive_expect_tx(own, (kPair ? 2 : 1) * C::kStageBytes);
                             if (kAMn) {
 #pragma unroll
                                 for (int g = 0; g < kBM / 64; ++g)
-                                    ptx::tma_load_2d(sa + g * 8192, &tmap_a,
-                                                     (mb * (kBM / 64) + g) * args.pa.x_block + xa, ya + ks * kBK, full);
+                                    tma_load<kPair>(sa + g * 8192, &tmap_a, (a0 / 64 + g) * args.pa.x_block + xa,
+                                                    ya + ks * kBK, full);
                             } else {
-                                ptx::tma_load_2d(sa, &tmap_a, ks * args.pa.x_block + xa, ya + mb * kBM, full);
+                                tma_load<kPair>(sa, &tmap_a, ks * args.pa.x_block + xa, ya + a0, full);
                             }
                             if (kBMn) {
 #pragma unroll
-                                for (int g = 0; g < BN / 64; ++g)
-                                    ptx::tma_load_2d(sb + g * 8192, &tmap_b,
-                                                     (nb * (BN / 64) + g) * args.pb.x_block + xb, yb + ks * kBK, full);
+                                for (int g = 0; g < C::kBRows / 64; ++g)
+                                    tma_load<kPair>(sb + g * 8192, &tmap_b, (b0 / 64 + g) * args.pb.x_block + xb,
+                                                    yb + ks * kBK, full);
                             } else {
-                                ptx::tma_load_2d(sb, &tmap_b, ks * args.pb.x_block + xb, yb + nb * BN, full);
+                                tma_load<kPair>(sb, &tmap_b, ks * args.pb.x_block + xb, yb + b0, full);
                             }
                             issued[stage] += 1;
                             if (++stage == kStages) { stage = 0; phase ^= 1; }
                         }
                     }
             }
+            // Let every copy land, and every MMA's release of a stage arrive,
+            // before this CTA (and the pair) can exit.
             for (int s = 0; s < kStages; ++s)
-                if (issued[s] > 0) ptx::mbar_wait(bar_full + 8 * s, (issued[s] - 1) & 1);
+                if (issued[s] > 0) {
+                    if (rank == 0) ptx::mbar_wait(bar_full + 8 * s, (issued[s] - 1) & 1);
+                    if (alive) ptx::mbar_wait(bar_empty + 8 * s, (issued[s] - 1) & 1);
+                }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            const uint32_t idesc = idesc_f16(kBf16, kAMn, kBMn, kBM, BN);
+        if (lane == 0 && rank == 0) {
+            // ---------------- MMA issuer ----------------
+            const uint32_t idesc = idesc_f16(kBf16, kAMn, kBMn, C::kTileM, kBN);
             int stage = 0;
             uint32_t phase = 0, it = 0;
             bool alive = true;
-            for (int t = blockIdx.x; t < num_items && alive; t += gridDim.x) {
+            for (int t = worker; t < num_items && alive; t += workers) {
                 int mb, nb, split, k0, k1;
                 item(t, mb, nb, split, k0, k1);
                 for (int c0 = k0; c0 < k1; c0 = chunk_end(c0, k1), ++it) {
                     const uint32_t buf = it & 1;
                     if (!ptx::mbar_wait(bar_tmem_empty + 8 * buf, ((it >> 1) & 1) ^ 1)) { alive = false; break; }
                     ptx::tc_fence_after();
-                    const uint32_t acc = tmem + buf * BN;
+                    const uint32_t acc = tmem + buf * kBN;
                     const int steps = (chunk_end(c0, k1) - c0) * args.terms;
                     for (int ks = 0; ks < steps; ++ks) {
                         if (!ptx::mbar_wait(bar_full + 8 * stage, phase)) { alive = false; break; }
@@ -510,24 +680,29 @@ __global__ void __launch_bounds__(320, 1)
                                                      : ptx::smem_desc(sa + 32 * j, 0, 1024, ptx::kLayoutSwizzle128);
                             const uint64_t bd = kBMn ? ptx::smem_desc(sb + 2048 * j, 8192, 1024, ptx::kLayoutSwizzle128)
                                                      : ptx::smem_desc(sb + 32 * j, 0, 1024, ptx::kLayoutSwizzle128);
-                            mma_f16(acc, ad, bd, idesc, (ks > 0 || j > 0) ? 1u : 0u);
+                            mma_f16<kPair>(acc, ad, bd, idesc, (ks > 0 || j > 0) ? 1u : 0u);
                         }
-                        ptx::tc_commit(bar_empty + 8 * stage);
+                        commit<kPair>(bar_empty + 8 * stage);
                         if (++stage == kStages) { stage = 0; phase ^= 1; }
                     }
                     if (!alive) break;
-                    ptx::tc_commit(bar_tmem_full + 8 * buf);
+                    commit<kPair>(bar_tmem_full + 8 * buf);
                 }
             }
-            ptx::tc_commit(bar_drain);
+            // every MMA is done before TMEM is released
+            commit<kPair>(bar_drain);
             ptx::mbar_wait(bar_drain, 0);
         }
     } else {
-        constexpr int kCols = BN / 2;     // columns of this warp: half of the tile
+        // ---------------- epilogue ----------------
+        constexpr int kCols = kBN / 2;  // columns of this warp: half of the tile
         constexpr int kParts = kCols / 32;
         const int quarter = warp & 3;
         const int half = (warp - 2) >> 2;
-        const int row_in_tile = quarter * 32 + lane;
+        WarpRows wr;
+        wr.box = smem + C::kOffOut + (warp - 2) * 4096;
+        wr.lane = lane;
+        wr.M = M;
         // inverse of the operands' power-of-two scales
         float inv = 1.0f;
         if (args.scale_a >= 0) inv *= pow2i(-scale_exponent(args.state->amax[args.scale_a]));
@@ -535,85 +710,105 @@ __global__ void __launch_bounds__(320, 1)
         const float k2 = args.logit_scale * kLog2e * inv;
         const float gscale = kEpi == kEpiGrad && !kBf16 ? pow2i(scale_exponent(args.state->amax[2])) : 1.0f;
         const float out_scale = kEpi == kEpiOut ? inv * args.state->grad_scale : 1.0f;
+        OutPlan plan;
+        plan.vec = kEpi == kEpiOut && args.dst_col == 1 && args.dst_row * (args.dst_f32 ? 4 : 2) % 16 == 0 &&
+                   (reinterpret_cast<uintptr_t>(args.dst) & 15) == 0;
+        auto release = [&](uint32_t buf) {
+            ptx::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                if (kPair) arrive_cluster(mapa(bar_tmem_empty + 8 * buf, 0));
+                else ptx::mbar_arrive(bar_tmem_empty + 8 * buf);
+            }
+        };
         uint32_t it = 0;
         bool alive = true;
-        for (int t = blockIdx.x; t < num_items && alive; t += gridDim.x) {
+        for (int t = worker; t < num_items && alive; t += workers) {
             int mb, nb, split, k0, k1;
             item(t, mb, nb, split, k0, k1);
-            const int64_t m = int64_t(mb) * kBM + row_in_tile;
-            const bool row_in = m < M;
-            const int64_t ncol0 = int64_t(nb) * BN + half * kCols;
+            wr.m0 = int64_t(mb) * C::kTileM + rank * kBM + quarter * 32;
+            const int64_t m = wr.m0 + lane;
+            wr.row_in = m < M;
+            const int64_t ncol0 = int64_t(nb) * kBN + half * kCols;
             EntryCursor cur;
             float lse2 = 0.0f, coef = 0.0f;
-            if (kEpi != kEpiOut) cur.begin(args, m, row_in, args.v0 + ncol0);
-            if (kEpi == kEpiGrad && row_in) {
+            int dst_row = 0;
+            if (kEpi != kEpiOut) cur.begin(args, m, wr.row_in, args.v0 + ncol0);
+            if (kEpi == kEpiGrad && wr.row_in) {
                 lse2 = args.lse2[m];
                 coef = args.coef[m] * gscale;
             }
-            // one 32-column part of the finished accumulator
-            auto part = [&](int c, float (&r)[32]) {
-                const int64_t n0 = ncol0 + c * 32;
-                const int ncols = (int)max(int64_t(0), min(int64_t(32), int64_t(args.N) - n0));
-                if (kEpi == kEpiGrad) {
-                    if (n0 < (int64_t(args.N) + 63) / 64 * 64)
-                        grad_part<kBf16>(args, cur, m, n0, ncols, row_in, k2, lse2, coef, r);
-                } else if (kEpi == kEpiOut) {
-                    if (row_in && ncols) out_part(args, split, m, n0, ncols, out_scale, r);
-                }
-            };
+            if (kEpi == kEpiOut && wr.row_in) dst_row = args.row_map ? args.row_map[m] : int(m);
+            const uint32_t lanes = uint32_t(quarter * 32) << 16;
+            // a pair's second half may lie past the rows that the workspace holds
+            const bool rows_in = kEpi == kEpiOut || wr.m0 < (args.M + kBM - 1) / kBM * kBM;
             if (kChunked) {
-                float sum[kParts][32];
+                float sum[kParts / 2][2][32];
 #pragma unroll
                 for (int c = 0; c < kParts; ++c)
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) sum[c][j] = 0.0f;
+                    for (int j = 0; j < 32; ++j) sum[c / 2][c % 2][j] = 0.0f;
                 for (int c0 = k0; c0 < k1; c0 = chunk_end(c0, k1), ++it) {
                     const uint32_t buf = it & 1;
-                    if (!ptx::mbar_wait(bar_tmem_full + 8 * buf, (it >> 1) & 1)) { alive = false; break; }
-                    __syncwarp();
+                    if (!__all_sync(0xffffffffu, ptx::mbar_wait(bar_tmem_full + 8 * buf, (it >> 1) & 1))) {
+                        alive = false;
+                        break;
+                    }
                     ptx::tc_fence_after();
-                    const uint32_t acc = tmem + buf * BN + half * kCols + (uint32_t(quarter * 32) << 16);
+                    const uint32_t acc = tmem + buf * kBN + half * kCols + lanes;
 #pragma unroll
                     for (int c = 0; c < 2 * kParts; ++c) {
                         uint32_t u[16];
                         tmem_ld_32x32b_x16(acc + c * 16, u);
                         ptx::tmem_ld_wait();
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) sum[c / 2][c % 2 * 16 + j] += __uint_as_float(u[j]);
+                        for (int j = 0; j < 16; ++j) sum[c / 4][c / 2 % 2][c % 2 * 16 + j] += __uint_as_float(u[j]);
                     }
-                    ptx::tc_fence_before();
-                    ptx::mbar_arrive(bar_tmem_empty + 8 * buf);
+                    release(buf);
                 }
                 if (!alive) break;
+                if (!rows_in) continue;
                 if (kEpi == kEpiLse) {
-                    const float4 st = lse_tile<kBf16, kParts>(args, cur, m, ncol0, row_in, k2, sum);
+                    const float4 st = lse_tile<kBf16, kParts / 2>(args, wr, cur, ncol0, k2, sum);
                     args.partial[(args.v0 + ncol0) / kCols * args.rows_pad + m] = st;
+                } else if (kEpi == kEpiGrad) {
+#pragma unroll
+                    for (int b = 0; b < kParts / 2; ++b)
+                        if (ncol0 + b * 64 < args.N)
+                            grad_block<kBf16>(args, wr, cur, ncol0 + b * 64, k2, lse2, coef, sum[b]);
                 } else {
 #pragma unroll
-                    for (int c = 0; c < kParts; ++c) part(c, sum[c]);
+                    for (int b = 0; b < kParts / 2; ++b)
+                        out_block<true>(args, wr, plan, split, ncol0 + b * 64, out_scale, sum[b], dst_row);
                 }
             } else {
                 const uint32_t buf = it & 1;
                 const bool any = k0 < k1;  // an empty share has no accumulator: zeros
                 if (any) {
-                    if (!ptx::mbar_wait(bar_tmem_full + 8 * buf, (it >> 1) & 1)) break;
+                    if (!__all_sync(0xffffffffu, ptx::mbar_wait(bar_tmem_full + 8 * buf, (it >> 1) & 1))) break;
                     ptx::tc_fence_after();
                 }
-                const uint32_t acc = tmem + buf * BN + half * kCols + (uint32_t(quarter * 32) << 16);
+                const uint32_t acc = tmem + buf * kBN + half * kCols + lanes;
 #pragma unroll 1
-                for (int c = 0; c < kParts; ++c) {
-                    __syncwarp();
-                    uint32_t u[32];
-                    float r[32];
-                    ptx::tmem_ld_32x32b_x32(acc + c * 32, u);
-                    ptx::tmem_ld_wait();
+                for (int b = 0; b < kParts / 2; ++b) {
+                    float r[2][32];
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) r[j] = any ? __uint_as_float(u[j]) : 0.0f;
-                    part(c, r);
+                    for (int c = 0; c < 2; ++c) {
+                        uint32_t u[32];
+                        ptx::tmem_ld_32x32b_x32(acc + b * 64 + c * 32, u);
+                        ptx::tmem_ld_wait();
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) r[c][j] = any ? __uint_as_float(u[j]) : 0.0f;
+                    }
+                    const int64_t n0 = ncol0 + b * 64;
+                    if (kEpi == kEpiGrad) {
+                        if (rows_in && n0 < args.N) grad_block<kBf16>(args, wr, cur, n0, k2, lse2, coef, r);
+                    } else {
+                        out_block<false>(args, wr, plan, split, n0, out_scale, r, dst_row);
+                    }
                 }
                 if (any) {
-                    ptx::tc_fence_before();
-                    ptx::mbar_arrive(bar_tmem_empty + 8 * buf);
+                    release(buf);
                     ++it;
                 }
             }
@@ -621,8 +816,14 @@ __global__ void __launch_bounds__(320, 1)
     }
     ptx::tc_fence_before();
     __syncthreads();
+    if (kPair) {
+        // the MMA thread's last commit arrives in the second CTA too: not after it has left
+        if (rank == 1 && threadIdx.x == 0) ptx::mbar_wait(bar_drain, 0);
+        __syncwarp();
+        cluster_sync();
+    }
     ptx::tc_fence_after();
-    if (warp == 1) ptx::tmem_dealloc(tmem, C::kTmemCols);
+    if (warp == 1) tmem_dealloc<kPair>(tmem, C::kTmemCols);
 }
 
 }  // namespace head

@@ -515,26 +515,6 @@ struct Operand {
     Plane plane;
 };
 
-// Parts of the K walk of a contraction whose tiles alone do not fill the SMs:
-// the smallest estimate of waves x (stages + a tile's fixed cost) plus the
-// traffic of writing and adding the parts.  A stage of 128 x 256 x 64 takes
-// 0.27 us, a tile's fill and drain about 2 us, the adding launch 3 us.
-int choose_splits(int64_t M, int64_t N, int64_t K, int terms, int sms) {
-    const int64_t tiles = ((M + kBM - 1) / kBM) * ((N + 255) / 256), steps = (K + kBK - 1) / kBK;
-    int best = 1;
-    double best_us = 1e30;
-    for (int s = 1; s <= 64 && (s == 1 || steps / s >= 4); ++s) {
-        const int64_t waves = (tiles * s + sms - 1) / sms, share = (steps + s - 1) / s;
-        double us = double(waves) * (double(share * terms) * 0.27 + 2.0);
-        if (s > 1) us += 3.0 + double(s) * double(M) * double(N) * 8.0 / 6.0e6;
-        if (us < best_us * 0.97) {
-            best_us = us;
-            best = s;
-        }
-    }
-    return best;
-}
-
 int device_sms() {
     static int sms[64] = {};
     int dev = 0;
@@ -544,30 +524,77 @@ int device_sms() {
     return sms[dev];
 }
 
-template <bool kBf16, bool kAMn, bool kBMn, int kEpi>
-int gemm(const Operand& a, const Operand& b, GemmArgs args, cudaStream_t stream) {
-    constexpr int BN = 256, kStages = 4;
-    using Cf = Cfg<BN, kStages>;
-    const int64_t tiles = int64_t((args.M + kBM - 1) / kBM) * ((args.N + BN - 1) / BN);
-    if (tiles == 0) return SW_OK;
+// How a contraction is spread over the SMs: tiles of one CTA or of a pair, and
+// parts of the K walk where the tiles alone do not fill the SMs.  The smallest
+// estimate of waves x (stages + a tile's fixed cost), and for parts the traffic
+// of writing and adding them: a stage of 128 x 256 x 64 on one SM (or of
+// 256 x 256 x 64 on two) takes 0.27 us, a tile's fill and drain about 2 us, the
+// adding launch 3 us.
+struct Spread {
+    bool pair;
+    int splits;
+};
+Spread choose_spread(int64_t M, int64_t N, int64_t K, int terms, bool may_split) {
+    const int sms = device_sms();
+    const int64_t steps = (K + kBK - 1) / kBK, cols = (N + kBN - 1) / kBN;
+    Spread best{false, 1};
+    double best_us = 1e30;
+    for (int pair = 1; pair >= 0; --pair) {
+        const int64_t tiles = (M + (pair ? 2 * kBM : kBM) - 1) / (pair ? 2 * kBM : kBM) * cols;
+        const int64_t workers = pair ? sms / 2 : sms;
+        for (int s = 1; s <= (may_split ? 64 : 1) && (s == 1 || steps / s >= 4); ++s) {
+            const int64_t waves = (tiles * s + workers - 1) / workers, share = (steps + s - 1) / s;
+            double us = double(waves) * (double(share * terms) * 0.27 + 2.0);
+            if (s > 1) us += 3.0 + double(s) * double(M) * double(N) * 8.0 / 6.0e6;
+            if (us < best_us * 0.97) {
+                best_us = us;
+                best = Spread{pair != 0, s};
+            }
+        }
+    }
+    return best;
+}
+
+template <bool kPair, bool kBf16, bool kAMn, bool kBMn, int kEpi>
+int launch_gemm(const Operand& a, const Operand& b, const GemmArgs& args, cudaStream_t stream) {
+    using Cf = Cfg<kPair>;
+    const int64_t items = int64_t((args.M + Cf::kTileM - 1) / Cf::kTileM) * ((args.N + kBN - 1) / kBN) * args.splits;
+    if (items == 0) return SW_OK;
     CUtensorMap ma, mb;
     int rc = make_map(&ma, a.ptr, a.rows, a.cols, a.ld, kAMn ? kBK : kBM);
     if (rc != SW_OK) return rc;
-    rc = make_map(&mb, b.ptr, b.rows, b.cols, b.ld, kBMn ? kBK : BN);
+    rc = make_map(&mb, b.ptr, b.rows, b.cols, b.ld, kBMn ? kBK : Cf::kBRows);
     if (rc != SW_OK) return rc;
+    auto kernel = head_gemm_kernel<kPair, kBf16, kAMn, kBMn, kEpi>;
+    SW_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cf::kSmemBytes),
+                "linear head smem");
+    constexpr int kCtas = kPair ? 2 : 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(kCtas * (unsigned)std::min<int64_t>(items, device_sms() / kCtas));
+    cfg.blockDim = dim3(Cf::kThreads);
+    cfg.dynamicSmemBytes = Cf::kSmemBytes;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = kCtas;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = kPair ? 2 : 1;
+    SW_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, ma, mb, args), "linear head contraction");
+    return SW_OK;
+}
+
+template <bool kBf16, bool kAMn, bool kBMn, int kEpi>
+int gemm(const Operand& a, const Operand& b, GemmArgs args, const Spread& spread, cudaStream_t stream) {
     args.terms = kBf16 ? 1 : 3;
     args.pa = a.plane;
     args.pb = b.plane;
-    if (args.splits < 1) args.splits = 1;
-    constexpr bool kChunked = !kBf16 || kEpi == kEpiLse;
-    auto kernel = head_gemm_kernel<BN, kStages, kBf16, kAMn, kBMn, kEpi, kChunked>;
-    SW_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cf::kSmemBytes),
-                "linear head smem");
-    const int64_t items = tiles * args.splits;
-    SW_CUDA_TRY(launch_pdl(kernel, dim3((unsigned)std::min<int64_t>(items, device_sms())), dim3(Cf::kThreads),
-                           Cf::kSmemBytes, stream, ma, mb, args),
-                "linear head contraction");
-    return SW_OK;
+    args.splits = spread.splits;
+    return spread.pair ? launch_gemm<true, kBf16, kAMn, kBMn, kEpi>(a, b, args, stream)
+                       : launch_gemm<false, kBf16, kAMn, kBMn, kEpi>(a, b, args, stream);
 }
 
 struct Bump {
@@ -633,7 +660,7 @@ struct Shape {
     // time.  Packed weights are laid out `piece` columns at a time too.
     bool keep;
     int64_t rows, piece;
-    int dh_splits, dw_splits;
+    Spread dh, dw;
     bool dh_sums, dw_sums;   // fp32 running sums are needed
     int64_t ld_acc;
 };
@@ -657,8 +684,8 @@ Layout lay_out(Bump& b, const Call& c, const Shape& s) {
     l.hc = b.take<uint16_t>(s.planes * s.rows_pad * s.ld_h);
     if (c.loss) l.partial = b.take<float4>(s.half_tiles * s.rows_pad);
     if (s.keep) l.ent_s = b.take<float>(s.rows_pad * K);
-    if (s.dh_sums) l.dh_accum = b.take<float>(s.dh_splits * s.T * s.ld_acc);
-    if (s.dw_sums) l.dw_accum = b.take<float>(s.dw_splits * (s.keep ? s.V : s.piece) * s.ld_acc);
+    if (s.dh_sums) l.dh_accum = b.take<float>(s.dh.splits * s.T * s.ld_acc);
+    if (s.dw_sums) l.dw_accum = b.take<float>(s.dw.splits * (s.keep ? s.V : s.piece) * s.ld_acc);
     if (s.pack_w) l.wp = b.take<uint16_t>(s.planes * round_up(s.piece, kBK) * s.ld_w);
     if (s.grads) l.grad = b.take<uint16_t>(s.planes * s.rows * round_up(s.piece, 64));
     return l;
@@ -668,7 +695,7 @@ template <bool kF32>
 int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
     const sw_linear_head& p = *c.plan;
     constexpr bool kBf16 = !kF32;
-    const int esize = kF32 ? 4 : 2;
+    const int esize = kF32 ? 4 : 2, terms = kF32 ? 3 : 1;
     const unsigned row_blocks = (unsigned)((s.rows_pad + 31) / 32);
     SW_CUDA_TRY(cudaMemsetAsync(l.state, 0, sizeof(HeadState), stream), "linear head state");
     if (!c.targets)
@@ -812,21 +839,20 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
             a.count_is = kCountM;
             a.scale_a = kF32 ? 2 : -1;
             a.scale_b = kF32 ? 1 : -1;
-            a.splits = s.dh_splits;
             a.accum = s.dh_sums ? l.dh_accum + r0 * s.ld_acc : nullptr;
             a.slot = s.T * s.ld_acc;
             a.first = first_v;
-            a.last = last_v && s.dh_splits == 1;
+            a.last = last_v && s.dh.splits == 1;
             a.dst = c.dh;
             a.dst_row = p.dh_row;
             a.dst_col = p.dh_col;
             a.row_map = l.row_map + r0;
-            int rc = gemm<kBf16, false, true, kEpiOut>(gr, w, a, stream);
+            int rc = gemm<kBf16, false, true, kEpiOut>(gr, w, a, s.dh, stream);
             if (rc != SW_OK) return rc;
-            if (last_v && s.dh_splits > 1) {
+            if (last_v && s.dh.splits > 1) {
                 sa.accum = a.accum;
                 sa.slot = a.slot;
-                sa.splits = s.dh_splits;
+                sa.splits = s.dh.splits;
                 sa.rows = n;
                 sa.by_count = 1;
                 sa.row_map = a.row_map;
@@ -844,21 +870,20 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
             a.count_is = kCountK;
             a.scale_a = kF32 ? 2 : -1;
             a.scale_b = kF32 ? 0 : -1;
-            a.splits = s.dw_splits;
             a.accum = s.dw_sums ? l.dw_accum : nullptr;
             a.slot = (s.keep ? s.V : s.piece) * s.ld_acc;
             a.first = first_r;
-            a.last = last_r && s.dw_splits == 1;
+            a.last = last_r && s.dw.splits == 1;
             a.row_map = nullptr;
             a.dst = static_cast<uint8_t*>(c.dw) + v0 * p.dw_row * esize;
             a.dst_row = p.dw_row;
             a.dst_col = p.dw_col;
-            int rc = gemm<kBf16, true, true, kEpiOut>(gr, states(r0, round_up(std::max<int64_t>(n, 1), kBM)), a, stream);
+            int rc = gemm<kBf16, true, true, kEpiOut>(gr, states(r0, round_up(std::max<int64_t>(n, 1), kBM)), a, s.dw, stream);
             if (rc != SW_OK) return rc;
-            if (last_r && s.dw_splits > 1) {
+            if (last_r && s.dw.splits > 1) {
                 sa.accum = a.accum;
                 sa.slot = a.slot;
-                sa.splits = s.dw_splits;
+                sa.splits = s.dw.splits;
                 sa.rows = nv;
                 sa.by_count = 0;
                 sa.row_map = nullptr;
@@ -891,7 +916,9 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
             GemmArgs a = logits(r0, n, 0, s.V);
             a.keep = 1;
             a.ent_s = l.ent_s + r0 * g.ent_k;
-            if ((rc = gemm<kBf16, false, false, kEpiLse>(states(r0, round_up(std::max<int64_t>(n, 1), kBM)), w, a, stream)) != SW_OK) return rc;
+            rc = gemm<kBf16, false, false, kEpiLse>(states(r0, round_up(std::max<int64_t>(n, 1), kBM)), w, a,
+                                                    choose_spread(n, s.V, s.D, terms, false), stream);
+            if (rc != SW_OK) return rc;
             if ((rc = merge(r0, n)) != SW_OK) return rc;
             ScaleArgs sc;
             memset(&sc, 0, sizeof(sc));
@@ -923,7 +950,8 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
             const int64_t n = std::min(step, s.V - v0);
             Operand w;
             if ((rc = weights(v0, n, &w)) != SW_OK) return rc;
-            rc = gemm<kBf16, false, false, kEpiLse>(states(0, s.rows_pad), w, logits(0, s.T, v0, n), stream);
+            rc = gemm<kBf16, false, false, kEpiLse>(states(0, s.rows_pad), w, logits(0, s.T, v0, n),
+                                                    choose_spread(s.T, n, s.D, terms, false), stream);
             if (rc != SW_OK) return rc;
         }
         if ((rc = merge(0, s.T)) != SW_OK) return rc;
@@ -934,7 +962,8 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
         const int64_t n = std::min(s.piece, s.V - v0);
         Operand w;
         if ((rc = weights(v0, n, &w)) != SW_OK) return rc;
-        rc = gemm<kBf16, false, false, kEpiGrad>(states(0, s.rows_pad), w, logits(0, s.T, v0, n), stream);
+        rc = gemm<kBf16, false, false, kEpiGrad>(states(0, s.rows_pad), w, logits(0, s.T, v0, n),
+                                                 choose_spread(s.T, n, s.D, terms, false), stream);
         if (rc != SW_OK) return rc;
         if ((rc = gradients(0, s.T, v0, n, w, v0 == 0, v0 + n == s.V, true, true)) != SW_OK) return rc;
     }
@@ -1014,7 +1043,7 @@ int check_and_run(const char* name, Call& c, void* stream_ptr) {
     const int64_t budget = p->workspace_limit > 0 ? p->workspace_limit : kDefaultWorkspace;
     const int64_t packed = s.pack_w ? s.planes * round_up(V, kBK) * s.ld_w * 2 : 0;
     const int64_t grad_row = s.planes * round_up(V, 256) * 2;
-    const int terms = s.f32 ? 3 : 1, sms = device_sms();
+    const int terms = s.f32 ? 3 : 1;
     // One call for the loss and the gradients keeps the logits' exponentials
     // of as many rows as the workspace limit allows (6 T V D operations and one
     // more pass over them); from a kept lse, or where not even 1024 rows (or
@@ -1035,10 +1064,11 @@ int check_and_run(const char* name, Call& c, void* stream_ptr) {
         const int64_t per_column = (grads ? s.planes * s.rows_pad * 2 : 0) + (s.pack_w ? s.planes * s.ld_w * 2 : 0);
         if (per_column > 0) s.piece = std::min(s.piece, std::max<int64_t>(budget / per_column / 256 * 256, 256));
     }
-    s.dh_splits = c.dh ? choose_splits(std::min(s.rows, T), D, std::min(s.piece, V), terms, sms) : 1;
-    s.dw_splits = c.dw ? choose_splits(std::min(s.piece, V), D, std::min(s.rows, T), terms, sms) : 1;
-    s.dh_sums = c.dh && (s.dh_splits > 1 || s.piece < V);
-    s.dw_sums = c.dw && (s.dw_splits > 1 || s.rows < T);
+    s.dh = s.dw = Spread{false, 1};
+    if (c.dh) s.dh = choose_spread(std::min(s.rows, T), D, std::min(s.piece, V), terms, true);
+    if (c.dw) s.dw = choose_spread(std::min(s.piece, V), D, std::min(s.rows, T), terms, true);
+    s.dh_sums = c.dh && (s.dh.splits > 1 || s.piece < V);
+    s.dw_sums = c.dw && (s.dw.splits > 1 || s.rows < T);
 
     Bump measure{nullptr, 0};
     lay_out(measure, c, s);
