@@ -55,7 +55,8 @@ struct HeadState {
     int bad;                 // a target outside the vocabulary was seen
     uint32_t amax[3];        // largest finite |h|, |w|, |row factor| as float bits (Float32 only)
     float grad_scale;        // common factor of every row's gradient, applied to dh and dw in fp32
-    int pad[2];
+    int dh_splits;           // parts of the K walk of dh, chosen for the rows that count
+    int pad;
 };
 
 // Power-of-two multiplier that brings values of magnitude `amax` just under
@@ -87,11 +88,13 @@ struct GemmArgs {
     int row0;                // first compact row of this launch (the count starts there)
     int terms;               // plane pairs walked: 1, or 3 for Float32
     Plane pa, pb;            // where each operand's lo plane and 64-element blocks lie
-    int splits;              // parts of the K walk, each with its own slot of `accum`
+    int splits;              // parts of the K walk, each with its own rows of the sums (0: state->dh_splits)
+    int tile_n;              // columns of a tile: kBN, or fewer for logits of one CTA (a multiple of 16)
     int scale_a, scale_b;    // indexes into HeadState::amax of the operands' scales (-1: none)
     // logits epilogues
     float logit_scale;
     int64_t v0;              // first vocabulary column of this piece
+    int half0;               // its first row of `partial`
     const int* ent_idx;      // [rows][ent_k] target columns, ascending
     const float* ent_p;      // their probabilities (null: 1)
     const uint16_t* offs;    // [tile][rows_pad] first entry of each kEntryTile columns (null: one entry a row)
@@ -102,12 +105,12 @@ struct GemmArgs {
     int keep;                // kEpiLse: write exp2(logit - half tile's max) where the logits' gradient will be
     const float* lse2;       // kEpiGrad: per compact row
     const float* coef;
-    uint16_t* grad;          // [rows_pad][ld_grad]; Float32: every 64 columns as 64 hi then 64 lo values
-    int64_t ld_grad;         // 16-bit elements
-    // kEpiOut
-    float* accum;            // fp32 running sums [splits][M][ld_accum] (null: none)
-    int64_t ld_accum, slot;
-    int first, last;         // first: nothing to add yet; last: write dst
+    // kEpiOut.  sums: the result goes to fp32 running sums through the output
+    // map, part p of row m at row p * rounded(M) + m (where there is one part
+    // and `direct`, to dst after all).
+    int sums, direct;
+    int first;               // nothing to add yet
+    int tma;                 // dst is written through the output map too
     void* dst;
     int dst_f32;
     int64_t dst_row, dst_col;
@@ -122,9 +125,10 @@ struct Cfg {
     static constexpr int kABytes = kBM * kBK * 2;
     static constexpr int kBBytes = kBRows * kBK * 2;
     static constexpr int kStageBytes = kABytes + kBBytes;
-    static constexpr int kStages = kPair ? 6 : 4;
-    static constexpr int kOffOut = kStages * kStageBytes;  // 4 KiB per epilogue warp
-    static constexpr int kOffBar = kOffOut + 8 * 4096;
+    static constexpr int kStages = kPair ? 5 : 4;
+    static constexpr int kBoxes = kPair ? 2 : 1;           // 4 KiB staging boxes per epilogue warp
+    static constexpr int kOffOut = kStages * kStageBytes;
+    static constexpr int kOffBar = kOffOut + 8 * kBoxes * 4096;
     static constexpr int kNumBars = 2 * kStages + 5;
     static constexpr int kOffSlot = kOffBar + kNumBars * 8;
     static constexpr int kSmemBytes = kOffSlot + 16 + 1024;
@@ -195,6 +199,14 @@ __device__ __forceinline__ void tma_load(uint32_t dst, const void* tmap, int32_t
         ptx::tma_load_2d(dst, tmap, x, y, bar);
 }
 
+// Adds a box of shared memory to Float32 values in global memory.
+__device__ __forceinline__ void tma_add_2d(const void* tmap, int32_t x, int32_t y, uint32_t src) {
+    asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                     reinterpret_cast<uint64_t>(tmap)),
+                 "r"(x), "r"(y), "r"(src)
+                 : "memory");
+}
+
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
@@ -240,18 +252,23 @@ struct EntryCursor {
     const float* p;
     int e, end;
     int next;  // column of entry e, INT_MAX past the end
+    int64_t limit;  // first column that is another tile's
 
-    __device__ __forceinline__ void load() { next = e < end ? idx[e] : INT_MAX; }
-    __device__ __forceinline__ void begin(const GemmArgs& a, int64_t row, bool row_in, int64_t col0) {
+    __device__ __forceinline__ void load() {
+        next = e < end ? idx[e] : INT_MAX;
+        if (next >= limit) next = INT_MAX;
+    }
+    __device__ __forceinline__ void begin(const GemmArgs& a, int64_t row, bool row_in, int64_t col0, int cols) {
         e = 0;
         end = 0;
+        limit = col0 + cols;
         idx = a.ent_idx + row * a.ent_k;
         p = a.ent_p ? a.ent_p + row * a.ent_k : nullptr;
         if (row_in) {
             if (a.offs) {
                 const int64_t tile = col0 / kEntryTile;
                 e = a.offs[tile * a.rows_pad + row];
-                end = a.offs[(tile + 1) * a.rows_pad + row];
+                end = a.offs[((col0 + cols - 1) / kEntryTile + 1) * a.rows_pad + row];
             } else {
                 end = 1;
             }
@@ -307,31 +324,49 @@ __device__ __forceinline__ void transpose_rows(uint8_t* box, int lane, const uin
 }
 
 // What an epilogue warp knows about its 32 rows of a tile.
+template <int kBoxes>
 struct WarpRows {
-    uint8_t* box;   // its 4 KiB of shared memory
+    uint8_t* box;   // its staging boxes of 4 KiB
+    uint32_t next;  // the one to use next
     int lane;
     int64_t m0;     // first row; lane holds row m0 + lane
     int64_t M;      // rows that exist
     bool row_in;
-};
 
-// 128 bytes of each of the warp's rows of the logits' gradient (all rows of a
-// tile are written: the ones that do not exist as zeros).
-__device__ __forceinline__ void put_grad(const GemmArgs& args, const WarpRows& wr, int64_t element, uint32_t (&w)[32]) {
-    uint16_t* base = args.grad + wr.m0 * args.ld_grad + element;
-    transpose_rows(wr.box, wr.lane, w, [&](int row, int unit, const uint4& v) {
-        reinterpret_cast<uint4*>(base + row * args.ld_grad)[unit] = v;
-    });
-}
+    __device__ __forceinline__ uint8_t* take() {
+        uint8_t* b = box + next * 4096;
+        next = kBoxes > 1 ? next ^ 1 : 0;
+        return b;
+    }
+    // 32 rows x 128 bytes, a row per lane in registers, through a staging box
+    // (16-byte units swizzled by row % 8, as the map says) to element x, row y
+    // of the output map: stored, or added.  What lies outside the map is clipped.
+    __device__ __forceinline__ void store(const void* tmap, const uint32_t (&w)[32], int x, int y, bool add) {
+        uint8_t* b = take();
+        if (lane == 0) ptx::bulk_wait_group_read<kBoxes - 1>();  // an earlier store has read this box
+        __syncwarp();
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            *reinterpret_cast<uint4*>(b + lane * 128 + (u ^ (lane & 7)) * 16) =
+                make_uint4(w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
+        ptx::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+            if (add) tma_add_2d(tmap, x, y, ptx::smem_addr(b));
+            else ptx::tma_store_2d(tmap, x, y, ptx::smem_addr(b));
+            ptx::bulk_commit_group();
+        }
+    }
+};
 
 // Softmax statistics of a row over the half tile in registers, in base-2
 // units: ref = max k2 z, sum of exp2(k2 z - ref), target term sum p z.  With
 // `keep` the exponentials are stored too, for the gradient: as f16 times 2^15
 // (11 bits down to 2^-29 of the half tile's largest; the later rounding to
 // bf16 is the one that counts) or, for Float32, as they are.
-template <bool kBf16, int kBlocks>
-__device__ __forceinline__ float4 lse_tile(const GemmArgs& args, const WarpRows& wr, EntryCursor& cur, int64_t n0,
-                                           float k2, float (&r)[kBlocks][2][32]) {
+template <bool kBf16, int kBlocks, class Rows>
+__device__ __forceinline__ float4 lse_tile(const GemmArgs& args, const void* tmap_c, Rows& wr, EntryCursor& cur, int64_t n0,
+                                           int64_t n_end, float k2, float (&r)[kBlocks][2][32]) {
     const int64_t m = wr.m0 + wr.lane;
     float dot = 0.0f, top = -INFINITY;
 #pragma unroll
@@ -346,7 +381,7 @@ __device__ __forceinline__ float4 lse_tile(const GemmArgs& args, const WarpRows&
                 if (args.ent_s) args.ent_s[m * args.ent_k + cur.e] = v * k2;
             }
         });
-        const int ncols = (int)min(int64_t(32), int64_t(args.N) - (n0 + c * 32));
+        const int ncols = (int)min(int64_t(32), n_end - (n0 + c * 32));
         if (ncols < 32) {
 #pragma unroll
             for (int j = 0; j < 32; ++j)
@@ -371,7 +406,7 @@ __device__ __forceinline__ float4 lse_tile(const GemmArgs& args, const WarpRows&
         const float up = !wr.row_in ? 0.0f : kBf16 ? 32768.0f : 1.0f;
 #pragma unroll
         for (int b = 0; b < kBlocks; ++b) {
-            if (n0 + b * 64 >= args.N) break;  // (blocks of 64 columns are written whole)
+            if (n0 + b * 64 >= n_end) break;  // (blocks of 64 columns are written whole)
             if (kBf16) {
                 uint32_t w[32];
 #pragma unroll
@@ -379,14 +414,14 @@ __device__ __forceinline__ float4 lse_tile(const GemmArgs& args, const WarpRows&
                     const float (&x)[32] = r[b][j / 16];
                     w[j] = pack2<false>(x[2 * (j % 16)] * up, x[2 * (j % 16) + 1] * up);
                 }
-                put_grad(args, wr, n0 + b * 64, w);
+                wr.store(tmap_c, w, int(n0) + b * 64, int(wr.m0), false);
             } else {
 #pragma unroll
                 for (int c = 2 * b; c < 2 * b + 2; ++c) {
                     uint32_t w[32];
 #pragma unroll
                     for (int j = 0; j < 32; ++j) w[j] = wr.row_in ? __float_as_uint(r[c / 2][c % 2][j]) : 0u;
-                    put_grad(args, wr, 2 * (n0 + c * 32), w);
+                    wr.store(tmap_c, w, 2 * (int(n0) + c * 32), int(wr.m0), false);
                 }
             }
         }
@@ -396,8 +431,8 @@ __device__ __forceinline__ float4 lse_tile(const GemmArgs& args, const WarpRows&
 
 // Gradient with respect to 64 logits of a row: softmax minus target in fp32,
 // rounded once to the type the next contractions read.
-template <bool kBf16>
-__device__ __forceinline__ void grad_block(const GemmArgs& args, const WarpRows& wr, EntryCursor& cur, int64_t n0,
+template <bool kBf16, class Rows>
+__device__ __forceinline__ void grad_block(const GemmArgs& args, const void* tmap_c, Rows& wr, EntryCursor& cur, int64_t n0,
                                            float k2, float lse2, float coef, float (&r)[2][32]) {
     uint32_t hi[32];
 #pragma unroll
@@ -415,7 +450,7 @@ __device__ __forceinline__ void grad_block(const GemmArgs& args, const WarpRows&
 #pragma unroll
         for (int j = 0; j < 16; ++j) hi[c * 16 + j] = pack2<kBf16>(r[c][2 * j], r[c][2 * j + 1]);
     }
-    put_grad(args, wr, kBf16 ? n0 : 2 * n0, hi);
+    wr.store(tmap_c, hi, kBf16 ? int(n0) : 2 * int(n0), int(wr.m0), false);
     if (!kBf16) {
         uint32_t lo[32];
 #pragma unroll
@@ -425,50 +460,60 @@ __device__ __forceinline__ void grad_block(const GemmArgs& args, const WarpRows&
                 const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi[c * 16 + j]));
                 lo[c * 16 + j] = pack2<false>(r[c][2 * j] - h.x, r[c][2 * j + 1] - h.y);
             }
-        put_grad(args, wr, 2 * n0 + 64, lo);
+        wr.store(tmap_c, lo, 2 * int(n0) + 64, int(wr.m0), false);
     }
 }
 
-// Where out_block writes, as far as a launch fixes it.
-struct OutPlan {
-    bool vec;  // whole 16-byte units: unit column stride, aligned rows
-};
-
-// 32 Float32 columns (or, for a bf16 result that is not summed, 64 columns) of
-// the warp's rows: added to the running fp32 sum, and the last time written in
-// the result's type.
-template <bool kWide>
-__device__ __forceinline__ void out_words(const GemmArgs& args, const WarpRows& wr, const OutPlan& plan, int split,
-                                          int64_t n0, const uint32_t (&w)[32], int dst_row_of_lane) {
-    constexpr int kUnit = kWide ? 8 : 4;  // columns of 16 bytes
-    if (n0 >= args.N) return;
-    transpose_rows(wr.box, wr.lane, w, [&](int row, int unit, uint4 v) {
-        const int dst_row = __shfl_sync(0xffffffffu, dst_row_of_lane, row);
-        const int64_t m = wr.m0 + row, n = n0 + unit * kUnit;
-        const int ncols = (int)min(int64_t(kUnit), int64_t(args.N) - n);
-        if (m >= wr.M || ncols <= 0) return;
-        if (!kWide && args.accum) {
-            // (rows of the running sums are whole groups of four)
-            float4* a = reinterpret_cast<float4*>(args.accum + split * args.slot + m * args.ld_accum + n);
-            float4 x = make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z),
-                                   __uint_as_float(v.w));
-            if (!args.first) {
-                const float4 o = *a;
-                x.x += o.x;
-                x.y += o.y;
-                x.z += o.z;
-                x.w += o.w;
+// 64 columns of the warp's rows of a result, in registers as two parts of 32:
+// through the output map (running sums, or a dst that it describes), or row by
+// row where rows are scattered or not aligned.
+template <bool kF32, class Rows>
+__device__ __forceinline__ void out_block(const GemmArgs& args, const void* tmap_c, Rows& wr, bool sums, int sum_row,
+                                          bool vec, int64_t n0, float scale, float (&r)[2][32], int dst_row_of_lane) {
+    uint32_t w[32];
+    if (kF32 || sums) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const int64_t n1 = n0 + c * 32;
+            if (n1 >= args.N) break;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) w[j] = __float_as_uint(r[c][j] * scale);
+            if (sums || args.tma) {
+                wr.store(tmap_c, w, int(n1), sums ? sum_row : int(wr.m0), sums && !args.first);
+                continue;
             }
-            if (!args.last) {
-                *a = x;
-                return;
-            }
-            v = make_uint4(__float_as_uint(x.x), __float_as_uint(x.y), __float_as_uint(x.z), __float_as_uint(x.w));
+            transpose_rows(wr.box, wr.lane, w, [&](int row, int unit, uint4 v) {
+                const int dst_row = __shfl_sync(0xffffffffu, dst_row_of_lane, row);
+                const int64_t n = n1 + unit * 4;
+                const int ncols = (int)min(int64_t(4), int64_t(args.N) - n);
+                if (wr.m0 + row >= wr.M || ncols <= 0) return;
+                float* d = static_cast<float*>(args.dst) + int64_t(dst_row) * args.dst_row + n * args.dst_col;
+                if (vec && ncols == 4) {
+                    *reinterpret_cast<uint4*>(d) = v;
+                } else {
+                    const uint32_t q[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (j < ncols) d[j * args.dst_col] = __uint_as_float(q[j]);
+                }
+            });
         }
-        const int64_t at = int64_t(dst_row) * args.dst_row + n * args.dst_col;
-        if (kWide) {
-            uint16_t* d = static_cast<uint16_t*>(args.dst) + at;
-            if (plan.vec && ncols == 8) {
+    } else {
+        if (n0 >= args.N) return;
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+            w[j] = pack2<true>(r[j / 16][2 * (j % 16)] * scale, r[j / 16][2 * (j % 16) + 1] * scale);
+        if (args.tma) {
+            wr.store(tmap_c, w, int(n0), int(wr.m0), false);
+            return;
+        }
+        transpose_rows(wr.box, wr.lane, w, [&](int row, int unit, uint4 v) {
+            const int dst_row = __shfl_sync(0xffffffffu, dst_row_of_lane, row);
+            const int64_t n = n0 + unit * 8;
+            const int ncols = (int)min(int64_t(8), int64_t(args.N) - n);
+            if (wr.m0 + row >= wr.M || ncols <= 0) return;
+            uint16_t* d = static_cast<uint16_t*>(args.dst) + int64_t(dst_row) * args.dst_row + n * args.dst_col;
+            if (vec && ncols == 8) {
                 *reinterpret_cast<uint4*>(d) = v;
             } else {
                 const uint32_t q[4] = {v.x, v.y, v.z, v.w};
@@ -476,56 +521,16 @@ __device__ __forceinline__ void out_words(const GemmArgs& args, const WarpRows& 
                 for (int j = 0; j < 8; ++j)
                     if (j < ncols) d[j * args.dst_col] = uint16_t(q[j / 2] >> (j % 2 * 16));
             }
-        } else if (args.dst_f32) {
-            float* d = static_cast<float*>(args.dst) + at;
-            if (plan.vec && ncols == 4) {
-                *reinterpret_cast<uint4*>(d) = v;
-            } else {
-                const uint32_t q[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (j < ncols) d[j * args.dst_col] = __uint_as_float(q[j]);
-            }
-        } else {
-            __nv_bfloat16* d = static_cast<__nv_bfloat16*>(args.dst) + at;
-            const float q[4] = {__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z),
-                                __uint_as_float(v.w)};
-            if (plan.vec && ncols == 4) {
-                *reinterpret_cast<uint2*>(d) = make_uint2(pack2<true>(q[0], q[1]), pack2<true>(q[2], q[3]));
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (j < ncols) d[j * args.dst_col] = __float2bfloat16_rn(q[j]);
-            }
-        }
-    });
-}
-
-// 64 columns of the warp's rows, in registers as two parts of 32.
-template <bool kF32>
-__device__ __forceinline__ void out_block(const GemmArgs& args, const WarpRows& wr, const OutPlan& plan, int split,
-                                          int64_t n0, float scale, float (&r)[2][32], int dst_row_of_lane) {
-    uint32_t w[32];
-    if (kF32 || args.accum) {
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) w[j] = __float_as_uint(r[c][j] * scale);
-            out_words<false>(args, wr, plan, split, n0 + c * 32, w, dst_row_of_lane);
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-            w[j] = pack2<true>(r[j / 16][2 * (j % 16)] * scale, r[j / 16][2 * (j % 16) + 1] * scale);
-        out_words<true>(args, wr, plan, split, n0, w, dst_row_of_lane);
+        });
     }
 }
 
 template <bool kPair, bool kBf16, bool kAMn, bool kBMn, int kEpi>
 __global__ void __launch_bounds__(320, 1)
     head_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
-                     const GemmArgs args) {
+                     const __grid_constant__ CUtensorMap tmap_c, const GemmArgs args) {
     using C = Cfg<kPair>;
+    constexpr bool kNarrow = !kPair && kEpi == kEpiLse;  // tiles may have fewer than kBN columns
     constexpr bool kChunked = !kBf16 || kEpi == kEpiLse;
     // K stages between two register sums: 512 elements; 1024 in bf16, whose logits need 1e-6
     constexpr int kChunkSteps = kBf16 ? 16 : 8;
@@ -558,6 +563,7 @@ __global__ void __launch_bounds__(320, 1)
         ptx::fence_barrier_init();
         ptx::prefetch_tmap(&tmap_a);
         ptx::prefetch_tmap(&tmap_b);
+        if (kEpi == kEpiGrad || (kEpi == kEpiLse ? args.keep : args.sums | args.tma)) ptx::prefetch_tmap(&tmap_c);
     }
     if (warp == 1) tmem_alloc<kPair>(ptx::smem_addr(tmem_slot), C::kTmemCols);
     ptx::tc_fence_before();
@@ -572,11 +578,13 @@ __global__ void __launch_bounds__(320, 1)
     const int M = args.count_is == kCountM ? min(args.M, count) : args.M;
     const int K = args.count_is == kCountK ? min(args.K, count) : args.K;
     const int num_m = (M + C::kTileM - 1) / C::kTileM;
-    const int num_n = (args.N + kBN - 1) / kBN;
+    const int tile_n = kNarrow ? args.tile_n : kBN;
+    const int num_n = (args.N + tile_n - 1) / tile_n;
     const int num_tiles = num_m * num_n;
-    const int num_items = num_tiles * args.splits;
+    const int splits = args.splits > 0 ? args.splits : args.state->dh_splits;
+    const int num_items = num_tiles * splits;
     const int k_steps = (K + kBK - 1) / kBK;
-    const int split_steps = (k_steps + args.splits - 1) / args.splits;
+    const int split_steps = (k_steps + splits - 1) / splits;
     constexpr int kGroup = kPair ? 8 : 16;  // row tiles of a raster group: they share B's panels in L2
     // Work item `t`: a tile and its share [k0, k1) of the K stages.
     auto item = [&](int t, int& mb, int& nb, int& split, int& k0, int& k1) {
@@ -604,7 +612,8 @@ __global__ void __launch_bounds__(320, 1)
             for (int t = worker; t < num_items && alive; t += workers) {
                 int mb, nb, split, k0, k1;
                 item(t, mb, nb, split, k0, k1);
-                const int a0 = mb * C::kTileM + rank * kBM, b0 = nb * kBN + rank * C::kBRows;
+                const int a0 = mb * C::kTileM + rank * kBM, b0 = nb * tile_n + rank * C::kBRows;
+                const uint32_t bytes = kNarrow ? C::kABytes + tile_n * kBK * 2 : (kPair ? 2 : 1) * C::kStageBytes;
                 for (int c0 = k0; c0 < k1 && alive; c0 = chunk_end(c0, k1))
                     for (int term = 0; term < args.terms && alive; ++term) {
                         // plane pairs, the small products first: (hi, lo), (lo, hi), (hi, hi)
@@ -620,7 +629,7 @@ __global__ void __launch_bounds__(320, 1)
                             const uint32_t sa = sbase + stage * C::kStageBytes;
                             const uint32_t sb = sa + C::kABytes;
                             // the first CTA's barrier counts both CTAs' bytes
-                            if (rank == 0) ptx::mbar_arrive_expect_tx(own, (kPair ? 2 : 1) * C::kStageBytes);
+                            if (rank == 0) ptx::mbar_arrive_expect_tx(own, bytes);
                             if (kAMn) {
 #pragma unroll
                                 for (int g = 0; g < kBM / 64; ++g)
@@ -653,7 +662,7 @@ __global__ void __launch_bounds__(320, 1)
     } else if (warp == 1) {
         if (lane == 0 && rank == 0) {
             // ---------------- MMA issuer ----------------
-            const uint32_t idesc = idesc_f16(kBf16, kAMn, kBMn, C::kTileM, kBN);
+            const uint32_t idesc = idesc_f16(kBf16, kAMn, kBMn, C::kTileM, tile_n);
             int stage = 0;
             uint32_t phase = 0, it = 0;
             bool alive = true;
@@ -699,8 +708,9 @@ __global__ void __launch_bounds__(320, 1)
         constexpr int kParts = kCols / 32;
         const int quarter = warp & 3;
         const int half = (warp - 2) >> 2;
-        WarpRows wr;
-        wr.box = smem + C::kOffOut + (warp - 2) * 4096;
+        WarpRows<C::kBoxes> wr;
+        wr.box = smem + C::kOffOut + (warp - 2) * C::kBoxes * 4096;
+        wr.next = 0;
         wr.lane = lane;
         wr.M = M;
         // inverse of the operands' power-of-two scales
@@ -710,9 +720,10 @@ __global__ void __launch_bounds__(320, 1)
         const float k2 = args.logit_scale * kLog2e * inv;
         const float gscale = kEpi == kEpiGrad && !kBf16 ? pow2i(scale_exponent(args.state->amax[2])) : 1.0f;
         const float out_scale = kEpi == kEpiOut ? inv * args.state->grad_scale : 1.0f;
-        OutPlan plan;
-        plan.vec = kEpi == kEpiOut && args.dst_col == 1 && args.dst_row * (args.dst_f32 ? 4 : 2) % 16 == 0 &&
-                   (reinterpret_cast<uintptr_t>(args.dst) & 15) == 0;
+        // whole 16-byte units can be written at dst
+        const bool vec = kEpi == kEpiOut && args.dst_col == 1 && args.dst_row * (args.dst_f32 ? 4 : 2) % 16 == 0 &&
+                         (reinterpret_cast<uintptr_t>(args.dst) & 15) == 0;
+        const bool sums = args.sums && !(args.direct && splits == 1);
         auto release = [&](uint32_t buf) {
             ptx::tc_fence_before();
             __syncwarp();
@@ -729,16 +740,23 @@ __global__ void __launch_bounds__(320, 1)
             wr.m0 = int64_t(mb) * C::kTileM + rank * kBM + quarter * 32;
             const int64_t m = wr.m0 + lane;
             wr.row_in = m < M;
-            const int64_t ncol0 = int64_t(nb) * kBN + half * kCols;
+            const int64_t ncol0 = int64_t(nb) * tile_n + half * kCols;
+            const int64_t n_end = min(int64_t(args.N), int64_t(nb + 1) * tile_n);
+            // what the row needs beside its accumulator: read after the register
+            // sums, which take most of the registers, or while the MMAs run
             EntryCursor cur;
             float lse2 = 0.0f, coef = 0.0f;
             int dst_row = 0;
-            if (kEpi != kEpiOut) cur.begin(args, m, wr.row_in, args.v0 + ncol0);
-            if (kEpi == kEpiGrad && wr.row_in) {
-                lse2 = args.lse2[m];
-                coef = args.coef[m] * gscale;
-            }
-            if (kEpi == kEpiOut && wr.row_in) dst_row = args.row_map ? args.row_map[m] : int(m);
+            auto row_values = [&]() {
+                if (kEpi != kEpiOut)
+                    cur.begin(args, m, wr.row_in && ncol0 < n_end, args.v0 + ncol0, int(n_end - ncol0));
+                if (kEpi == kEpiGrad && wr.row_in) {
+                    lse2 = args.lse2[m];
+                    coef = args.coef[m] * gscale;
+                }
+                if (kEpi == kEpiOut && wr.row_in) dst_row = args.row_map ? args.row_map[m] : int(m);
+            };
+            const int sum_row = split * num_m * C::kTileM + int(wr.m0);
             const uint32_t lanes = uint32_t(quarter * 32) << 16;
             // a pair's second half may lie past the rows that the workspace holds
             const bool rows_in = kEpi == kEpiOut || wr.m0 < (args.M + kBM - 1) / kBM * kBM;
@@ -768,20 +786,23 @@ __global__ void __launch_bounds__(320, 1)
                 }
                 if (!alive) break;
                 if (!rows_in) continue;
+                row_values();
                 if (kEpi == kEpiLse) {
-                    const float4 st = lse_tile<kBf16, kParts / 2>(args, wr, cur, ncol0, k2, sum);
-                    args.partial[(args.v0 + ncol0) / kCols * args.rows_pad + m] = st;
+                    const float4 st = lse_tile<kBf16, kParts / 2>(args, &tmap_c, wr, cur, ncol0, n_end, k2, sum);
+                    args.partial[(int64_t(args.half0) + nb * 2 + half) * args.rows_pad + m] = st;
                 } else if (kEpi == kEpiGrad) {
 #pragma unroll
                     for (int b = 0; b < kParts / 2; ++b)
                         if (ncol0 + b * 64 < args.N)
-                            grad_block<kBf16>(args, wr, cur, ncol0 + b * 64, k2, lse2, coef, sum[b]);
+                            grad_block<kBf16>(args, &tmap_c, wr, cur, ncol0 + b * 64, k2, lse2, coef, sum[b]);
                 } else {
 #pragma unroll
                     for (int b = 0; b < kParts / 2; ++b)
-                        out_block<true>(args, wr, plan, split, ncol0 + b * 64, out_scale, sum[b], dst_row);
+                        out_block<true>(args, &tmap_c, wr, sums, sum_row, vec, ncol0 + b * 64, out_scale, sum[b],
+                                        dst_row);
                 }
             } else {
+                row_values();
                 const uint32_t buf = it & 1;
                 const bool any = k0 < k1;  // an empty share has no accumulator: zeros
                 if (any) {
@@ -802,9 +823,9 @@ __global__ void __launch_bounds__(320, 1)
                     }
                     const int64_t n0 = ncol0 + b * 64;
                     if (kEpi == kEpiGrad) {
-                        if (rows_in && n0 < args.N) grad_block<kBf16>(args, wr, cur, n0, k2, lse2, coef, r);
+                        if (rows_in && n0 < args.N) grad_block<kBf16>(args, &tmap_c, wr, cur, n0, k2, lse2, coef, r);
                     } else {
-                        out_block<false>(args, wr, plan, split, n0, out_scale, r, dst_row);
+                        out_block<false>(args, &tmap_c, wr, sums, sum_row, vec, n0, out_scale, r, dst_row);
                     }
                 }
                 if (any) {
@@ -813,6 +834,7 @@ __global__ void __launch_bounds__(320, 1)
                 }
             }
         }
+        if (lane == 0) ptx::bulk_wait_group0();  // this warp's stores are done
     }
     ptx::tc_fence_before();
     __syncthreads();

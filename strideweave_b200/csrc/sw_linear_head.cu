@@ -66,6 +66,21 @@ __global__ void teacher_flags_kernel(const int* index, const float* logits, int6
     if (lane == 0) flags[t] = any;
 }
 
+// Estimated microseconds of a contraction whose K walk is cut into s parts:
+// waves x (stages + a tile's fixed cost), and the traffic of writing and adding
+// the parts.  A stage of 128 x 256 x 64 on one SM (or of 256 x 256 x 64 on two)
+// takes 0.27 us, a tile's fill and drain about 2 us, the adding launch 3 us.
+constexpr int kMaxSplits = 64;
+__host__ __device__ inline float spread_cost(int64_t tiles, int64_t elements, int64_t K, int terms, int workers,
+                                             int s) {
+    const int64_t steps = (K + kBK - 1) / kBK;
+    if (s > 1 && (steps < 4 * s || tiles * s > 2 * workers)) return 1e30f;
+    const int64_t waves = (tiles * s + workers - 1) / workers, share = (steps + s - 1) / s;
+    float us = float(waves) * (float(share * terms) * 0.27f + 2.0f);
+    if (s > 1) us += 3.0f + float(s) * float(elements) * (8.0f / 6.0e6f);
+    return us;
+}
+
 struct RowsArgs {
     const int* targets;      // cross entropy, or null
     int ignore_index;
@@ -80,56 +95,83 @@ struct RowsArgs {
     float* coef;
     float* lse2;
     HeadState* state;
+    int64_t dh_rows, dh_cols, dh_k;  // the contraction of dh: rows of a launch at most, dim, columns of a piece
+    int dh_tile_m, dh_workers, terms;
 };
 
-// One CTA ranks the rows: row_map[0, count) are the rows that count, in order,
-// row_map[count, T) the others.  Then the factor of each compact row's gradient.
+// One CTA ranks the rows, four per thread and pass: row_map[0, count) are the
+// rows that count, in order, row_map[count, T) the others.
 __global__ void __launch_bounds__(1024) rows_kernel(const RowsArgs a) {
     __shared__ int warp_n[32];
     __shared__ int total;
+    __shared__ float cost[kMaxSplits];
     pdl_enter();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     int kept = 0, bad = 0;
-    for (int64_t base = 0; base < a.T; base += 1024) {
-        const int64_t t = base + tid;
-        bool keep = false;
-        int y = 0;
-        if (t < a.T) {
+    uint32_t top = 0;
+    for (int64_t base = 0; base < a.T; base += 4096) {
+        const int64_t t0 = base + tid * 4;
+        int y[4];
+        uint32_t keep = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            y[j] = 0;
+            if (t0 + j >= a.T) continue;
             if (a.targets) {
-                y = a.targets[t];
-                keep = y != a.ignore_index;
-                if (keep && (y < 0 || y >= a.V)) {
-                    keep = false;
-                    bad = 1;
+                y[j] = a.targets[t0 + j];
+                if (y[j] != a.ignore_index) {
+                    if (y[j] >= 0 && y[j] < a.V) keep |= 1u << j;
+                    else bad = 1;
                 }
-            } else {
-                keep = a.flags[t] != 0;
+            } else if (a.flags[t0 + j]) {
+                keep |= 1u << j;
             }
         }
-        const uint32_t votes = __ballot_sync(0xffffffffu, keep);
-        if (lane == 0) warp_n[warp] = __popc(votes);
+        int n = __popc(keep);
+        for (int o = 1; o < 32; o <<= 1) {
+            const int up = __shfl_up_sync(0xffffffffu, n, o);
+            if (lane >= o) n += up;
+        }
+        if (lane == 31) warp_n[warp] = n;
         __syncthreads();
         if (warp == 0) {
-            int n = warp_n[lane];
+            int w = warp_n[lane];
             for (int o = 1; o < 32; o <<= 1) {
-                const int up = __shfl_up_sync(0xffffffffu, n, o);
-                if (lane >= o) n += up;
+                const int up = __shfl_up_sync(0xffffffffu, w, o);
+                if (lane >= o) w += up;
             }
-            warp_n[lane] = n;
-            if (lane == 31) total = n;
+            warp_n[lane] = w;
+            if (lane == 31) total = w;
         }
         __syncthreads();
-        const int before = kept + (warp ? warp_n[warp - 1] : 0) + __popc(votes & ((1u << lane) - 1));
-        if (t < a.T) {
-            if (keep) {
+        int before = kept + (warp ? warp_n[warp - 1] : 0) + n - __popc(keep);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int64_t t = t0 + j;
+            if (t >= a.T) continue;
+            if (keep >> j & 1) {
                 a.row_map[before] = int(t);
-                if (a.targets) a.ent_idx[before] = y;
+                if (a.targets) a.ent_idx[before] = y[j];
+                if (a.coef) {
+                    const float g = a.mean || !a.upstream ? 1.0f : a.upstream[t];
+                    a.coef[before] = g;
+                    if (isfinite(g)) top = max(top, __float_as_uint(fabsf(g)));
+                }
+                if (a.lse) a.lse2[before] = a.lse[t] * kLog2e;
+                ++before;
             } else {
                 a.row_map[a.T - 1 - (t - before)] = int(t);
             }
         }
         kept += total;
         __syncthreads();
+    }
+    if (a.coef && top) atomicMax(&a.state->amax[2], top);
+    // the K walk's parts for dh, over the rows that turned out to count
+    if (tid < kMaxSplits) {
+        const int64_t rows = min(int64_t(kept), a.dh_rows);
+        const int64_t tiles = (rows + a.dh_tile_m - 1) / a.dh_tile_m * ((a.dh_cols + kBN - 1) / kBN);
+        cost[tid] = spread_cost(tiles, rows * a.dh_cols, a.dh_k, a.terms, a.dh_workers, tid + 1);
     }
     bad = __syncthreads_or(bad);
     if (tid == 0) {
@@ -139,20 +181,13 @@ __global__ void __launch_bounds__(1024) rows_kernel(const RowsArgs a) {
         // what every row's gradient is multiplied by stays out of the 16-bit
         // logits' gradient: a target's -1 is exact there, where the common
         // factor would round it the same way in every row
-        a.state->grad_scale = a.factor * (a.mean ? (a.upstream ? a.upstream[0] : 1.0f) / float(max(kept, 1)) : 1.0f);
+        a.state->grad_scale =
+            a.factor * (a.mean ? (a.upstream ? a.upstream[0] : 1.0f) / float(max(kept, 1)) : 1.0f);
+        int best = 0;
+        for (int s = 1; s < kMaxSplits; ++s)
+            if (cost[s] < cost[best] * 0.97f) best = s;
+        a.state->dh_splits = best + 1;
     }
-    __syncthreads();  // row_map is read back by other threads of this CTA
-    uint32_t top = 0;
-    for (int i = tid; i < kept; i += 1024) {
-        const int t = a.row_map[i];
-        if (a.coef) {
-            const float g = a.mean || !a.upstream ? 1.0f : a.upstream[t];
-            a.coef[i] = g;
-            if (isfinite(g)) top = max(top, __float_as_uint(fabsf(g)));
-        }
-        if (a.lse) a.lse2[i] = a.lse[t] * kLog2e;
-    }
-    if (a.coef && top) atomicMax(&a.state->amax[2], top);
 }
 
 // A warp per compact row: its teacher's probabilities and its entries in
@@ -219,23 +254,82 @@ __global__ void teacher_sort_kernel(const int* index, const float* logits, int K
     }
 }
 
-// Largest finite magnitude of a matrix (the rows of row_map when it is given).
-__global__ void amax_kernel(const float* x, int64_t rows, int64_t cols, int64_t sr, int64_t sc, const int* row_map,
-                            const HeadState* count_from, uint32_t* out) {
+// Largest finite magnitude of a matrix (of the rows of row_map when it is
+// given): a warp per row, or per column where columns are contiguous; `vec`:
+// rows are whole aligned groups of four.
+__global__ void __launch_bounds__(256) amax_kernel(const float* x, int64_t rows, int64_t cols, int64_t sr, int64_t sc,
+                                                   int vec, const int* row_map, const HeadState* count_from,
+                                                   uint32_t* out) {
     pdl_enter();
     if (count_from) rows = count_from->count;
-    const int64_t n = rows * cols;
-    uint32_t top = 0;
     const bool by_rows = sr == 1 && sc != 1;  // walk the unit stride fastest
-    for (int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; i < n; i += int64_t(gridDim.x) * blockDim.x) {
-        int64_t r = by_rows ? i % rows : i / cols;
-        const int64_t c = by_rows ? i / rows : i % cols;
-        if (row_map) r = row_map[r];
-        const float v = fabsf(x[r * sr + c * sc]);
+    const int64_t outer = by_rows ? cols : rows, inner = by_rows ? rows : cols;
+    const int64_t so = by_rows ? sc : sr, si = by_rows ? sr : sc;
+    const int lane = threadIdx.x & 31;
+    const int64_t warps = int64_t(gridDim.x) * 8;
+    uint32_t top = 0;
+    auto take = [&](float v) {
+        v = fabsf(v);
         if (v <= 3.402823466e38f) top = max(top, __float_as_uint(v));
+    };
+    for (int64_t o = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5); o < outer; o += warps) {
+        const float* p = x + (by_rows ? o : row_map ? int64_t(row_map[o]) : o) * so;
+        if (vec) {
+#pragma unroll 4
+            for (int64_t i = lane * 4; i < inner; i += 128) {
+                const float4 v = *reinterpret_cast<const float4*>(p + i);
+                take(v.x);
+                take(v.y);
+                take(v.z);
+                take(v.w);
+            }
+        } else {
+#pragma unroll 4
+            for (int64_t i = lane; i < inner; i += 32) take(p[(by_rows && row_map ? int64_t(row_map[i]) : i) * si]);
+        }
     }
     for (int o = 16; o; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if ((threadIdx.x & 31) == 0 && top) atomicMax(out, top);
+    if (lane == 0 && top) atomicMax(out, top);
+}
+
+// pack_kernel for rows that are whole aligned 16-byte units (8 columns at a
+// time, coalesced): a gather of bf16 rows, or the split of Float32 rows.
+template <bool kF32>
+__global__ void __launch_bounds__(256) pack_rows_kernel(const void* src, int64_t rows, int64_t cols, int64_t sr,
+                                                        const int* row_map, const HeadState* state, int use_count,
+                                                        int scale_of, uint16_t* dst, int64_t ld, int64_t rows_pad) {
+    pdl_enter();
+    const int64_t valid = use_count ? min(rows, int64_t(state->count)) : rows;
+    const float scale = kF32 ? pow2i(scale_exponent(state->amax[scale_of])) : 1.0f;
+    const int64_t units = cols / 8;  // ld == cols here
+    const int64_t stride = int64_t(gridDim.x) * 256;
+#pragma unroll 2
+    for (int64_t u = int64_t(blockIdx.x) * 256 + threadIdx.x; u < rows_pad * units; u += stride) {
+        const int64_t r = u / units, c = (u - r * units) * 8;
+        uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
+        if (r < valid) {
+            const int64_t at = (row_map ? int64_t(row_map[r]) : r) * sr + c;
+            if (kF32) {
+                const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(src) + at);
+                const float4 a = p[0], b = p[1];
+                const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+                uint32_t h[4], l[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float x = v[2 * j] * scale, y = v[2 * j + 1] * scale;
+                    const __half2 q = __floats2half2_rn(x, y);
+                    h[j] = *reinterpret_cast<const uint32_t*>(&q);
+                    l[j] = pack2<false>(x - __low2float(q), y - __high2float(q));
+                }
+                hi = make_uint4(h[0], h[1], h[2], h[3]);
+                lo = make_uint4(l[0], l[1], l[2], l[3]);
+            } else {
+                hi = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(src) + at);
+            }
+        }
+        *reinterpret_cast<uint4*>(dst + r * ld + c) = hi;
+        if (kF32) *reinterpret_cast<uint4*>(dst + (rows_pad + r) * ld + c) = lo;
+    }
 }
 
 // Gathers rows into the contraction's operand: [rows_pad][ld] 16-bit, a copy
@@ -366,6 +460,7 @@ struct ScaleArgs {
     uint16_t* grad;
     int64_t ld_grad, V;
     const float4* partial;
+    int tile_n;              // columns of a tile; its halves start at 0 and 128
     int rows_pad, row0;
     const HeadState* state;
     const float* lse2;
@@ -377,7 +472,7 @@ struct ScaleArgs {
 };
 template <bool kF32>
 __global__ void __launch_bounds__(256) scale_kernel(const ScaleArgs a) {
-    __shared__ float factor[kScaleCols / 128];
+    __shared__ float factor[kScaleCols / 64];
     pdl_enter();
     const int64_t i = blockIdx.x;
     if (i >= a.state->count - a.row0) return;
@@ -385,11 +480,11 @@ __global__ void __launch_bounds__(256) scale_kernel(const ScaleArgs a) {
     const int64_t c1 = min(c0 + kScaleCols, a.V);
     const float lse2 = a.lse2[i];
     const float coef = a.coef[i] * (kF32 ? pow2i(scale_exponent(a.state->amax[2])) : 1.0f);
-    const int halves = int((c1 - c0 + 127) / 128);
-    for (int t = threadIdx.x; t < halves; t += 256) {
-        const float ref = a.partial[(c0 / 128 + t) * a.rows_pad + i].x;
+    for (int64_t b = c0 + threadIdx.x * 64; b < c1; b += 256 * 64) {  // tiles are whole 64-column blocks
+        const int64_t tile = b / a.tile_n, half = tile * 2 + (b - tile * a.tile_n >= 128);
+        const float ref = a.partial[half * a.rows_pad + i].x;
         // (a half tile of nothing but -inf stored zeros)
-        factor[t] = ref == -INFINITY ? 0.0f : ex2(ref - lse2) * coef * (kF32 ? 1.0f : 1.0f / 32768.0f);
+        factor[(b - c0) / 64] = ref == -INFINITY ? 0.0f : ex2(ref - lse2) * coef * (kF32 ? 1.0f : 1.0f / 32768.0f);
     }
     __syncthreads();
     uint16_t* row = a.grad + i * a.ld_grad;
@@ -397,7 +492,7 @@ __global__ void __launch_bounds__(256) scale_kernel(const ScaleArgs a) {
         const int lane = threadIdx.x & 31;
         for (int64_t b = c0 + (threadIdx.x >> 5) * 64; b < c1; b += 8 * 64) {
             float2 v = reinterpret_cast<const float2*>(row + 2 * b)[lane];
-            const float f = factor[(b - c0) / 128];
+            const float f = factor[(b - c0) / 64];
             v.x = b + 2 * lane < a.V ? v.x * f : 0.0f;
             v.y = b + 2 * lane + 1 < a.V ? v.y * f : 0.0f;
             const __half2 hi = __floats2half2_rn(v.x, v.y);
@@ -410,7 +505,7 @@ __global__ void __launch_bounds__(256) scale_kernel(const ScaleArgs a) {
     } else {
         for (int64_t c = c0 + threadIdx.x * 8; c < c1; c += 256 * 8) {
             uint4 v = *reinterpret_cast<const uint4*>(row + c);
-            const float f = factor[(c - c0) / 128];
+            const float f = factor[(c - c0) / 64];
             uint32_t* w = reinterpret_cast<uint32_t*>(&v);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -439,11 +534,12 @@ __global__ void __launch_bounds__(256) scale_kernel(const ScaleArgs a) {
     }
 }
 
-// Result rows from the K walk's parts, added in order.
+// Result rows from the fp32 sums of the K walk's parts, added in order.
 struct SlotsArgs {
-    const float* accum;
-    int64_t ld_accum, slot;
-    int splits;
+    const float* sums;       // part p of row m at row p round_up(M, tile_m) + m
+    int64_t ld;
+    int splits, tile_m;      // splits 0: state->dh_splits
+    int direct;              // one part was written to dst already
     int64_t rows, cols;
     const HeadState* state;
     int by_count, row0;
@@ -454,14 +550,18 @@ struct SlotsArgs {
 template <bool kF32>
 __global__ void __launch_bounds__(256) sum_slots_kernel(const SlotsArgs a) {
     pdl_enter();
+    const int splits = a.splits > 0 ? a.splits : a.state->dh_splits;
+    if (a.direct && splits == 1) return;
     const int64_t rows = a.by_count ? min(a.rows, int64_t(max(a.state->count - a.row0, 0))) : a.rows;
+    const int64_t slot = (rows + a.tile_m - 1) / a.tile_m * a.tile_m * a.ld;
     const int64_t per_row = (a.cols + 3) / 4;
     for (int64_t u = int64_t(blockIdx.x) * 256 + threadIdx.x; u < rows * per_row; u += int64_t(gridDim.x) * 256) {
         const int64_t m = u / per_row, c = (u - m * per_row) * 4;
-        const float* p = a.accum + m * a.ld_accum + c;  // ld_accum is whole groups of four
+        const float* p = a.sums + m * a.ld + c;  // ld is whole groups of four
         float4 s = *reinterpret_cast<const float4*>(p);
-        for (int k = 1; k < a.splits; ++k) {
-            const float4 v = *reinterpret_cast<const float4*>(p + k * a.slot);
+#pragma unroll 4
+        for (int k = 1; k < splits; ++k) {
+            const float4 v = *reinterpret_cast<const float4*>(p + k * slot);
             s.x += v.x;
             s.y += v.y;
             s.z += v.z;
@@ -515,6 +615,8 @@ struct Operand {
     Plane plane;
 };
 
+int64_t round_up(int64_t x, int64_t q) { return (x + q - 1) / q * q; }
+
 int device_sms() {
     static int sms[64] = {};
     int dev = 0;
@@ -525,28 +627,21 @@ int device_sms() {
 }
 
 // How a contraction is spread over the SMs: tiles of one CTA or of a pair, and
-// parts of the K walk where the tiles alone do not fill the SMs.  The smallest
-// estimate of waves x (stages + a tile's fixed cost), and for parts the traffic
-// of writing and adding them: a stage of 128 x 256 x 64 on one SM (or of
-// 256 x 256 x 64 on two) takes 0.27 us, a tile's fill and drain about 2 us, the
-// adding launch 3 us.
+// parts of the K walk.
 struct Spread {
     bool pair;
     int splits;
 };
 Spread choose_spread(int64_t M, int64_t N, int64_t K, int terms, bool may_split) {
     const int sms = device_sms();
-    const int64_t steps = (K + kBK - 1) / kBK, cols = (N + kBN - 1) / kBN;
     Spread best{false, 1};
-    double best_us = 1e30;
+    float best_us = 1e30f;
     for (int pair = 1; pair >= 0; --pair) {
-        const int64_t tiles = (M + (pair ? 2 * kBM : kBM) - 1) / (pair ? 2 * kBM : kBM) * cols;
-        const int64_t workers = pair ? sms / 2 : sms;
-        for (int s = 1; s <= (may_split ? 64 : 1) && (s == 1 || steps / s >= 4); ++s) {
-            const int64_t waves = (tiles * s + workers - 1) / workers, share = (steps + s - 1) / s;
-            double us = double(waves) * (double(share * terms) * 0.27 + 2.0);
-            if (s > 1) us += 3.0 + double(s) * double(M) * double(N) * 8.0 / 6.0e6;
-            if (us < best_us * 0.97) {
+        const int tile_m = pair ? 2 * kBM : kBM, workers = pair ? sms / 2 : sms;
+        const int64_t tiles = (M + tile_m - 1) / tile_m * ((N + kBN - 1) / kBN);
+        for (int s = 1; s <= (may_split ? kMaxSplits : 1); ++s) {
+            const float us = spread_cost(tiles, M * N, K, terms, workers, s);
+            if (us < best_us * 0.97f) {
                 best_us = us;
                 best = Spread{pair != 0, s};
             }
@@ -555,16 +650,50 @@ Spread choose_spread(int64_t M, int64_t N, int64_t K, int terms, bool may_split)
     return best;
 }
 
+// Rows of fp32 sums that `splits` of any row count up to M may take: one part
+// of all M, or parts of at most two tiles per worker.
+int64_t sum_rows(int64_t M, int64_t N, bool pair) {
+    const int tile_m = pair ? 2 * kBM : kBM, workers = pair ? device_sms() / 2 : device_sms();
+    const int64_t cols = (N + kBN - 1) / kBN;
+    return std::max(round_up(M, tile_m), (2 * int64_t(workers) / cols + 1) * tile_m);
+}
+
+// Where a contraction writes through its output map: 16-bit or Float32 values,
+// in boxes of 128 bytes x 32 rows.
+struct Target {
+    const void* ptr;         // null: no map
+    int64_t rows, cols, ld;  // elements
+    bool f32;
+};
+
+int make_target_map(CUtensorMap* map, const Target& t) {
+    auto fn = tensor_map_encoder();
+    if (!fn) return fail(SW_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+    cuuint64_t dims[2] = {(cuuint64_t)t.cols, (cuuint64_t)t.rows};
+    cuuint64_t strides[1] = {(cuuint64_t)(t.ld * (t.f32 ? 4 : 2))};
+    cuuint32_t box[2] = {t.f32 ? 32u : 64u, 32};
+    cuuint32_t estr[2] = {1, 1};
+    CUresult r = fn(map, t.f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2,
+                    const_cast<void*>(t.ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(SW_ERR_CUDA, "cuTensorMapEncodeTiled (linear head result) failed (%d)", (int)r);
+    return SW_OK;
+}
+
 template <bool kPair, bool kBf16, bool kAMn, bool kBMn, int kEpi>
-int launch_gemm(const Operand& a, const Operand& b, const GemmArgs& args, cudaStream_t stream) {
+int launch_gemm(const Operand& a, const Operand& b, const Target& c, const GemmArgs& args, cudaStream_t stream) {
     using Cf = Cfg<kPair>;
-    const int64_t items = int64_t((args.M + Cf::kTileM - 1) / Cf::kTileM) * ((args.N + kBN - 1) / kBN) * args.splits;
+    const int max_splits = args.splits > 0 ? args.splits : kMaxSplits;
+    const int64_t items =
+        int64_t((args.M + Cf::kTileM - 1) / Cf::kTileM) * ((args.N + args.tile_n - 1) / args.tile_n) * max_splits;
     if (items == 0) return SW_OK;
-    CUtensorMap ma, mb;
+    CUtensorMap ma, mb, mc;
     int rc = make_map(&ma, a.ptr, a.rows, a.cols, a.ld, kAMn ? kBK : kBM);
     if (rc != SW_OK) return rc;
-    rc = make_map(&mb, b.ptr, b.rows, b.cols, b.ld, kBMn ? kBK : Cf::kBRows);
+    rc = make_map(&mb, b.ptr, b.rows, b.cols, b.ld, kBMn ? kBK : kPair ? Cf::kBRows : args.tile_n);
     if (rc != SW_OK) return rc;
+    memset(&mc, 0, sizeof(mc));
+    if (c.ptr && (rc = make_target_map(&mc, c)) != SW_OK) return rc;
     auto kernel = head_gemm_kernel<kPair, kBf16, kAMn, kBMn, kEpi>;
     SW_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cf::kSmemBytes),
                 "linear head smem");
@@ -583,18 +712,19 @@ int launch_gemm(const Operand& a, const Operand& b, const GemmArgs& args, cudaSt
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = kPair ? 2 : 1;
-    SW_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, ma, mb, args), "linear head contraction");
+    SW_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, ma, mb, mc, args), "linear head contraction");
     return SW_OK;
 }
 
 template <bool kBf16, bool kAMn, bool kBMn, int kEpi>
-int gemm(const Operand& a, const Operand& b, GemmArgs args, const Spread& spread, cudaStream_t stream) {
+int gemm(const Operand& a, const Operand& b, const Target& c, GemmArgs args, bool pair, cudaStream_t stream) {
     args.terms = kBf16 ? 1 : 3;
     args.pa = a.plane;
     args.pb = b.plane;
-    args.splits = spread.splits;
-    return spread.pair ? launch_gemm<true, kBf16, kAMn, kBMn, kEpi>(a, b, args, stream)
-                       : launch_gemm<false, kBf16, kAMn, kBMn, kEpi>(a, b, args, stream);
+    if (kEpi != kEpiOut) args.splits = 1;
+    if (kEpi != kEpiLse || pair) args.tile_n = kBN;
+    return pair ? launch_gemm<true, kBf16, kAMn, kBMn, kEpi>(a, b, c, args, stream)
+                : launch_gemm<false, kBf16, kAMn, kBMn, kEpi>(a, b, c, args, stream);
 }
 
 struct Bump {
@@ -608,8 +738,6 @@ struct Bump {
         return p;
     }
 };
-
-int64_t round_up(int64_t x, int64_t q) { return (x + q - 1) / q * q; }
 
 struct Call {
     const sw_linear_head* plan;
@@ -643,8 +771,8 @@ struct Layout {
     float* ent_s;
     uint16_t* hc;
     float4* partial;
-    float* dh_accum;
-    float* dw_accum;
+    float* dh_sums;
+    float* dw_sums;
     uint16_t* wp;
     uint16_t* grad;
 };
@@ -660,9 +788,12 @@ struct Shape {
     // time.  Packed weights are laid out `piece` columns at a time too.
     bool keep;
     int64_t rows, piece;
-    Spread dh, dw;
-    bool dh_sums, dw_sums;   // fp32 running sums are needed
-    int64_t ld_acc;
+    int tile_n;              // columns of a logits tile
+    bool logits_pair, dh_pair;
+    Spread dw;
+    // rows of fp32 sums of each gradient (0: it is written at once); dh's parts
+    // are chosen on the device, for the rows that count
+    int64_t dh_sum_rows, dw_sum_rows, ld_acc;
 };
 
 Layout lay_out(Bump& b, const Call& c, const Shape& s) {
@@ -684,8 +815,8 @@ Layout lay_out(Bump& b, const Call& c, const Shape& s) {
     l.hc = b.take<uint16_t>(s.planes * s.rows_pad * s.ld_h);
     if (c.loss) l.partial = b.take<float4>(s.half_tiles * s.rows_pad);
     if (s.keep) l.ent_s = b.take<float>(s.rows_pad * K);
-    if (s.dh_sums) l.dh_accum = b.take<float>(s.dh.splits * s.T * s.ld_acc);
-    if (s.dw_sums) l.dw_accum = b.take<float>(s.dw.splits * (s.keep ? s.V : s.piece) * s.ld_acc);
+    if (s.dh_sum_rows) l.dh_sums = b.take<float>(s.dh_sum_rows * s.ld_acc);
+    if (s.dw_sum_rows) l.dw_sums = b.take<float>(s.dw_sum_rows * s.ld_acc);
     if (s.pack_w) l.wp = b.take<uint16_t>(s.planes * round_up(s.piece, kBK) * s.ld_w);
     if (s.grads) l.grad = b.take<uint16_t>(s.planes * s.rows * round_up(s.piece, 64));
     return l;
@@ -696,7 +827,6 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
     const sw_linear_head& p = *c.plan;
     constexpr bool kBf16 = !kF32;
     const int esize = kF32 ? 4 : 2, terms = kF32 ? 3 : 1;
-    const unsigned row_blocks = (unsigned)((s.rows_pad + 31) / 32);
     SW_CUDA_TRY(cudaMemsetAsync(l.state, 0, sizeof(HeadState), stream), "linear head state");
     if (!c.targets)
         SW_CUDA_TRY(launch_pdl(teacher_flags_kernel, dim3((unsigned)std::max<int64_t>((s.T + 7) / 8, 1)), dim3(256), 0, stream,
@@ -718,6 +848,12 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
     ra.coef = s.grads ? l.coef : nullptr;
     ra.lse2 = l.lse2;
     ra.state = l.state;
+    ra.dh_rows = s.rows;
+    ra.dh_cols = s.D;
+    ra.dh_k = std::min(s.piece, s.V);
+    ra.dh_tile_m = s.dh_pair ? 2 * kBM : kBM;
+    ra.dh_workers = s.dh_pair ? device_sms() / 2 : device_sms();
+    ra.terms = terms;
     SW_CUDA_TRY(launch_pdl(rows_kernel, dim3(1), dim3(1024), 0, stream, ra), "linear head rows");
     if (!c.targets)
         SW_CUDA_TRY(launch_pdl(teacher_sort_kernel, dim3((unsigned)std::max<int64_t>((s.T + 3) / 4, 1)), dim3(128), 0, stream,
@@ -725,17 +861,42 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
                                (int)s.rows_pad, (int)((s.V + kEntryTile - 1) / kEntryTile), l.ent_idx, l.ent_p,
                                l.entropy, l.offs),
                     "teacher entries");
+    // rows of `cols` elements that the vector kernels can read
+    auto whole_rows = [&](const void* x, int64_t cols, int64_t sr, int64_t sc) {
+        return sc == 1 && cols % 8 == 0 && sr * esize % 16 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+    };
+    const unsigned fill = (unsigned)(8 * device_sms());
+    auto amax = [&](const void* x, int64_t rows, int64_t sr, int64_t sc, const int* map, const HeadState* count,
+                    uint32_t* out) -> int {
+        SW_CUDA_TRY(launch_pdl(amax_kernel, dim3(std::min<unsigned>(fill, (unsigned)((std::max(rows, s.D) + 7) / 8))),
+                               dim3(256), 0, stream, (const float*)x, rows, s.D, sr, sc,
+                               (int)whole_rows(x, s.D, sr, sc), map, count, out),
+                    "linear head scale");
+        return SW_OK;
+    };
+    auto pack = [&](const void* x, int64_t rows, int64_t sr, int64_t sc, const int* map, int use_count, int scale_of,
+                    uint16_t* dst, int64_t rows_pad) -> int {
+        if (whole_rows(x, s.D, sr, sc)) {
+            const int64_t units = rows_pad * (s.D / 8);
+            SW_CUDA_TRY(launch_pdl(pack_rows_kernel<kF32>, dim3((unsigned)std::min<int64_t>((units + 255) / 256, fill)),
+                                   dim3(256), 0, stream, x, rows, s.D, sr, map, l.state, use_count, scale_of, dst,
+                                   s.ld_h, rows_pad),
+                        "linear head operand");
+        } else {
+            SW_CUDA_TRY(launch_pdl(pack_kernel<kF32>,
+                                   dim3((unsigned)((rows_pad + 31) / 32), (unsigned)((s.ld_h + 31) / 32)), dim3(256), 0,
+                                   stream, x, rows, s.D, sr, sc, map, l.state, use_count, scale_of, dst, s.ld_h,
+                                   rows_pad),
+                        "linear head operand");
+        }
+        return SW_OK;
+    };
+    int rc;
     if (kF32) {
-        SW_CUDA_TRY(launch_pdl(amax_kernel, dim3(592), dim3(256), 0, stream, (const float*)c.h, s.T, s.D, p.h_row,
-                               p.h_col, l.row_map, l.state, &l.state->amax[0]),
-                    "linear head scale");
-        SW_CUDA_TRY(launch_pdl(amax_kernel, dim3(592), dim3(256), 0, stream, (const float*)c.w, s.V, s.D, p.w_row,
-                               p.w_col, (const int*)nullptr, (const HeadState*)nullptr, &l.state->amax[1]),
-                    "linear head scale");
+        if ((rc = amax(c.h, s.T, p.h_row, p.h_col, l.row_map, l.state, &l.state->amax[0])) != SW_OK) return rc;
+        if ((rc = amax(c.w, s.V, p.w_row, p.w_col, nullptr, nullptr, &l.state->amax[1])) != SW_OK) return rc;
     }
-    SW_CUDA_TRY(launch_pdl(pack_kernel<kF32>, dim3(row_blocks, (unsigned)((s.ld_h + 31) / 32)), dim3(256), 0, stream,
-                           c.h, s.T, s.D, p.h_row, p.h_col, l.row_map, l.state, 1, 0, l.hc, s.ld_h, s.rows_pad),
-                "linear head states");
+    if ((rc = pack(c.h, s.T, p.h_row, p.h_col, l.row_map, 1, 0, l.hc, s.rows_pad)) != SW_OK) return rc;
     const Plane dense{kBK, 0, 0};
     // rows [r0, r0 + n) of the gathered states
     auto states = [&](int64_t r0, int64_t n) {
@@ -750,8 +911,8 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
     g.ent_p = l.ent_p;
     g.ent_k = c.targets ? 1 : c.top_k;
     g.rows_pad = (int)s.rows_pad;
-    g.ld_grad = ld_grad;
-    g.ld_accum = s.ld_acc;
+    g.tile_n = s.tile_n;
+    const Target grad_out{l.grad, s.rows, ld_grad, ld_grad, false}, none{nullptr, 0, 0, 0, false};
 
     // the weights of columns [v0, v0 + n): in place, or packed into the workspace
     int64_t packed = -1;
@@ -763,12 +924,10 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
         }
         // zero rows up to whole K stages: a tail of G's zeros must not meet the next plane
         const int64_t rows = round_up(n, kBK);
-        if (packed != v0)
-            SW_CUDA_TRY(launch_pdl(pack_kernel<kF32>,
-                                   dim3((unsigned)((rows + 31) / 32), (unsigned)((s.ld_w + 31) / 32)), dim3(256), 0,
-                                   stream, (const void*)at, n, s.D, p.w_row, p.w_col, (const int*)nullptr, l.state, 0, 1,
-                                   l.wp, s.ld_w, rows),
-                        "linear head weights");
+        if (packed != v0) {
+            const int rc = pack(at, n, p.w_row, p.w_col, nullptr, 0, 1, l.wp, rows);
+            if (rc != SW_OK) return rc;
+        }
         packed = v0;
         *out = Operand{l.wp, s.planes * rows, s.D, s.ld_w, Plane{kBK, 0, (int)rows}};
         return SW_OK;
@@ -784,13 +943,13 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
         a.scale_a = kF32 ? 0 : -1;
         a.scale_b = kF32 ? 1 : -1;
         a.v0 = v0;
+        a.half0 = (int)(v0 / kBN * 2);
         a.ent_idx = l.ent_idx + r0 * g.ent_k;
         a.ent_p = l.ent_p ? l.ent_p + r0 * g.ent_k : nullptr;
         a.offs = l.offs ? l.offs + r0 : nullptr;
         a.partial = l.partial + r0;
         a.lse2 = l.lse2 + r0;
         a.coef = l.coef + r0;
-        a.grad = l.grad;
         return a;
     };
     auto merge = [&](int64_t r0, int64_t n) -> int {
@@ -827,11 +986,10 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
         a.dst_f32 = kF32;
         SlotsArgs sa;
         memset(&sa, 0, sizeof(sa));
-        sa.ld_accum = s.ld_acc;
+        sa.ld = s.ld_acc;
         sa.cols = s.D;
         sa.state = l.state;
         sa.row0 = (int)r0;
-        const unsigned slot_ctas = (unsigned)(8 * device_sms());
         if (c.dh && n > 0) {
             a.M = (int)n;
             a.N = (int)s.D;
@@ -839,28 +997,29 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
             a.count_is = kCountM;
             a.scale_a = kF32 ? 2 : -1;
             a.scale_b = kF32 ? 1 : -1;
-            a.accum = s.dh_sums ? l.dh_accum + r0 * s.ld_acc : nullptr;
-            a.slot = s.T * s.ld_acc;
+            a.splits = s.dh_sum_rows ? 0 : 1;
+            a.sums = s.dh_sum_rows > 0;
+            a.direct = first_v && last_v;
             a.first = first_v;
-            a.last = last_v && s.dh.splits == 1;
             a.dst = c.dh;
             a.dst_row = p.dh_row;
             a.dst_col = p.dh_col;
             a.row_map = l.row_map + r0;
-            int rc = gemm<kBf16, false, true, kEpiOut>(gr, w, a, s.dh, stream);
+            const Target out{l.dh_sums, s.dh_sum_rows, s.ld_acc, s.ld_acc, true};
+            int rc = gemm<kBf16, false, true, kEpiOut>(gr, w, s.dh_sum_rows ? out : none, a, s.dh_pair, stream);
             if (rc != SW_OK) return rc;
-            if (last_v && s.dh.splits > 1) {
-                sa.accum = a.accum;
-                sa.slot = a.slot;
-                sa.splits = s.dh.splits;
+            if (last_v && s.dh_sum_rows) {
+                sa.sums = l.dh_sums;
+                sa.splits = 0;
+                sa.tile_m = s.dh_pair ? 2 * kBM : kBM;
+                sa.direct = a.direct;
                 sa.rows = n;
                 sa.by_count = 1;
                 sa.row_map = a.row_map;
                 sa.dst = c.dh;
                 sa.dst_row = p.dh_row;
                 sa.dst_col = p.dh_col;
-                SW_CUDA_TRY(launch_pdl(sum_slots_kernel<kF32>, dim3(slot_ctas), dim3(256), 0, stream, sa),
-                            "linear head dh");
+                SW_CUDA_TRY(launch_pdl(sum_slots_kernel<kF32>, dim3(fill), dim3(256), 0, stream, sa), "linear head dh");
             }
         }
         if (c.dw) {
@@ -870,28 +1029,33 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
             a.count_is = kCountK;
             a.scale_a = kF32 ? 2 : -1;
             a.scale_b = kF32 ? 0 : -1;
-            a.accum = s.dw_sums ? l.dw_accum : nullptr;
-            a.slot = (s.keep ? s.V : s.piece) * s.ld_acc;
+            a.splits = s.dw.splits;
+            a.sums = s.dw_sum_rows > 0;
+            a.direct = 0;
             a.first = first_r;
-            a.last = last_r && s.dw.splits == 1;
             a.row_map = nullptr;
             a.dst = static_cast<uint8_t*>(c.dw) + v0 * p.dw_row * esize;
             a.dst_row = p.dw_row;
             a.dst_col = p.dw_col;
-            int rc = gemm<kBf16, true, true, kEpiOut>(gr, states(r0, round_up(std::max<int64_t>(n, 1), kBM)), a, s.dw, stream);
+            // (a map whose rows end inside 16 bytes would write the rest of them)
+            a.tma = !a.sums && p.dw_col == 1 && p.dw_row * esize % 16 == 0 && s.D * esize % 16 == 0 &&
+                    p.dw_row >= s.D && (reinterpret_cast<uintptr_t>(a.dst) & 15) == 0;
+            const Target sums{l.dw_sums, s.dw_sum_rows, s.ld_acc, s.ld_acc, true}, dst{a.dst, nv, s.D, p.dw_row, kF32};
+            int rc = gemm<kBf16, true, true, kEpiOut>(gr, states(r0, round_up(std::max<int64_t>(n, 1), kBM)),
+                                                      a.sums ? sums : a.tma ? dst : none, a, s.dw.pair, stream);
             if (rc != SW_OK) return rc;
-            if (last_r && s.dw.splits > 1) {
-                sa.accum = a.accum;
-                sa.slot = a.slot;
+            if (last_r && a.sums) {
+                sa.sums = l.dw_sums;
                 sa.splits = s.dw.splits;
+                sa.tile_m = s.dw.pair ? 2 * kBM : kBM;
+                sa.direct = 0;
                 sa.rows = nv;
                 sa.by_count = 0;
                 sa.row_map = nullptr;
                 sa.dst = a.dst;
                 sa.dst_row = p.dw_row;
                 sa.dst_col = p.dw_col;
-                SW_CUDA_TRY(launch_pdl(sum_slots_kernel<kF32>, dim3(slot_ctas), dim3(256), 0, stream, sa),
-                            "linear head dw");
+                SW_CUDA_TRY(launch_pdl(sum_slots_kernel<kF32>, dim3(fill), dim3(256), 0, stream, sa), "linear head dw");
             }
         }
         return SW_OK;
@@ -907,7 +1071,6 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
                                c.dh, (int)kF32, s.T, s.D, p.dh_row, p.dh_col, l.row_map, l.state),
                     "linear head ignored rows");
 
-    int rc;
     if (s.keep) {
         Operand w;
         if ((rc = weights(0, s.V, &w)) != SW_OK) return rc;
@@ -916,8 +1079,8 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
             GemmArgs a = logits(r0, n, 0, s.V);
             a.keep = 1;
             a.ent_s = l.ent_s + r0 * g.ent_k;
-            rc = gemm<kBf16, false, false, kEpiLse>(states(r0, round_up(std::max<int64_t>(n, 1), kBM)), w, a,
-                                                    choose_spread(n, s.V, s.D, terms, false), stream);
+            rc = gemm<kBf16, false, false, kEpiLse>(states(r0, round_up(std::max<int64_t>(n, 1), kBM)), w, grad_out, a,
+                                                    s.logits_pair, stream);
             if (rc != SW_OK) return rc;
             if ((rc = merge(r0, n)) != SW_OK) return rc;
             ScaleArgs sc;
@@ -926,6 +1089,7 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
             sc.ld_grad = ld_grad;
             sc.V = s.V;
             sc.partial = a.partial;
+            sc.tile_n = s.tile_n;
             sc.rows_pad = (int)s.rows_pad;
             sc.row0 = (int)r0;
             sc.state = l.state;
@@ -950,8 +1114,8 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
             const int64_t n = std::min(step, s.V - v0);
             Operand w;
             if ((rc = weights(v0, n, &w)) != SW_OK) return rc;
-            rc = gemm<kBf16, false, false, kEpiLse>(states(0, s.rows_pad), w, logits(0, s.T, v0, n),
-                                                    choose_spread(s.T, n, s.D, terms, false), stream);
+            rc = gemm<kBf16, false, false, kEpiLse>(states(0, s.rows_pad), w, none, logits(0, s.T, v0, n), s.logits_pair,
+                                                    stream);
             if (rc != SW_OK) return rc;
         }
         if ((rc = merge(0, s.T)) != SW_OK) return rc;
@@ -962,8 +1126,8 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
         const int64_t n = std::min(s.piece, s.V - v0);
         Operand w;
         if ((rc = weights(v0, n, &w)) != SW_OK) return rc;
-        rc = gemm<kBf16, false, false, kEpiGrad>(states(0, s.rows_pad), w, logits(0, s.T, v0, n),
-                                                 choose_spread(s.T, n, s.D, terms, false), stream);
+        rc = gemm<kBf16, false, false, kEpiGrad>(states(0, s.rows_pad), w, grad_out, logits(0, s.T, v0, n),
+                                                 s.logits_pair, stream);
         if (rc != SW_OK) return rc;
         if ((rc = gradients(0, s.T, v0, n, w, v0 == 0, v0 + n == s.V, true, true)) != SW_OK) return rc;
     }
@@ -1035,7 +1199,6 @@ int check_and_run(const char* name, Call& c, void* stream_ptr) {
     s.rows_pad = std::max<int64_t>(round_up(T, kBM), kBM);
     s.ld_h = s.ld_w = round_up(D, 8);
     s.grads = grads;
-    s.half_tiles = (V + 255) / 256 * 2;
     s.ld_acc = round_up(D, 4);
     // weights are read in place when TMA can: bf16, unit stride, 16-byte rows
     s.pack_w = s.f32 || p->w_col != 1 || p->w_row % 8 != 0 || p->w_row < D ||
@@ -1064,11 +1227,38 @@ int check_and_run(const char* name, Call& c, void* stream_ptr) {
         const int64_t per_column = (grads ? s.planes * s.rows_pad * 2 : 0) + (s.pack_w ? s.planes * s.ld_w * 2 : 0);
         if (per_column > 0) s.piece = std::min(s.piece, std::max<int64_t>(budget / per_column / 256 * 256, 256));
     }
-    s.dh = s.dw = Spread{false, 1};
-    if (c.dh) s.dh = choose_spread(std::min(s.rows, T), D, std::min(s.piece, V), terms, true);
-    if (c.dw) s.dw = choose_spread(std::min(s.piece, V), D, std::min(s.rows, T), terms, true);
-    s.dh_sums = c.dh && (s.dh.splits > 1 || s.piece < V);
-    s.dw_sums = c.dw && (s.dw.splits > 1 || s.rows < T);
+    s.logits_pair = choose_spread(std::min(s.rows, T), std::min(s.piece, V), D, terms, false).pair;
+    s.tile_n = kBN;
+    if (!s.logits_pair && c.loss && (s.piece >= V || !s.pack_w)) {
+        // few rows: a tile as narrow as fills the last wave (whole 64-column
+        // blocks where the exponentials are kept, else whole MMA widths)
+        const int q = s.keep ? 64 : 16, sms = device_sms();
+        const int64_t row_tiles = (T + kBM - 1) / kBM;
+        int64_t best = INT64_MAX;
+        for (int t = kBN; t >= 128; t -= q) {
+            const int64_t tiles = row_tiles * ((V + t - 1) / t), cost = (tiles + sms - 1) / sms * (t + 16);
+            if (cost < best) {
+                best = cost;
+                s.tile_n = t;
+            }
+        }
+    }
+    s.half_tiles = (V + s.tile_n - 1) / s.tile_n * 2;
+    s.dh_pair = false;
+    s.dw = Spread{false, 1};
+    s.dh_sum_rows = s.dw_sum_rows = 0;
+    if (c.dh && T > 0) {
+        const int64_t n = std::min(s.rows, T), nv = std::min(s.piece, V);
+        s.dh_pair = choose_spread(n, D, nv, terms, true).pair;
+        const int workers = s.dh_pair ? device_sms() / 2 : device_sms();
+        // (fewer than two tiles of columns per worker: some row count may split)
+        if (s.piece < V || 4 * ((D + kBN - 1) / kBN) <= 4 * workers) s.dh_sum_rows = sum_rows(n, D, s.dh_pair);
+    }
+    if (c.dw) {
+        const int64_t n = std::min(s.rows, T), nv = std::min(s.piece, V);
+        s.dw = choose_spread(nv, D, n, terms, true);
+        if (s.dw.splits > 1 || s.rows < T) s.dw_sum_rows = s.dw.splits * round_up(nv, s.dw.pair ? 2 * kBM : kBM);
+    }
 
     Bump measure{nullptr, 0};
     lay_out(measure, c, s);
