@@ -105,16 +105,10 @@ struct GemmArgs {
     int keep;                // kEpiLse: write exp2(logit - half tile's max) where the logits' gradient will be
     const float* lse2;       // kEpiGrad: per compact row
     const float* coef;
-    // kEpiOut.  sums: the result goes to fp32 running sums through the output
-    // map, part p of row m at row p * rounded(M) + m (where there is one part
-    // and `direct`, to dst after all).
-    int sums, direct;
+    // kEpiOut, through the output map: the result in its type, or fp32 running
+    // sums, part p of row m at row p round_up(M, tile) + m
+    int sums;
     int first;               // nothing to add yet
-    int tma;                 // dst is written through the output map too
-    void* dst;
-    int dst_f32;
-    int64_t dst_row, dst_col;
-    const int* row_map;      // destination row of each row (null: itself)
 };
 
 template <bool kPair>
@@ -244,51 +238,89 @@ __device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)
         : "r"(taddr));
 }
 
-// The target entries of one row inside a tile: a cursor over its ascending
-// list.  Rows are spread over a warp's lanes, and `take` runs for every entry
-// inside the 32 columns that the warp holds in registers.
+// Loads 32 consecutive Float32 TMEM columns of this warp's 32 lanes.
+__device__ __forceinline__ void tmem_ld_f32_x32(uint32_t taddr, float (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]),
+          "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]),
+          "=f"(r[16]), "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]),
+          "=f"(r[24]), "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
+        : "r"(taddr));
+}
+
+// The target entries of one row inside a half tile, a row per lane.  fetch()
+// copies them into the warp's staging box while the MMAs run (the lists are
+// ascending, in L2; walking them there would wait for L2 at every entry);
+// walk() then runs `take` for every entry inside 32 columns held in registers.
 struct EntryCursor {
+    static constexpr int kHeld = 16;  // entries of a row that the box holds; more are read from the list
     const int* idx;
     const float* p;
-    int e, end;
-    int next;  // column of entry e, INT_MAX past the end
-    int64_t limit;  // first column that is another tile's
+    uint2* box;     // [kHeld][32 lanes]
+    int first, n;   // the row's entries first .. first + n - 1 lie in the half tile
+    int i;          // the next one
+    int next;       // its column, INT_MAX past the end
+    float prob;     // and probability
 
-    __device__ __forceinline__ void load() {
-        next = e < end ? idx[e] : INT_MAX;
-        if (next >= limit) next = INT_MAX;
-    }
-    __device__ __forceinline__ void begin(const GemmArgs& a, int64_t row, bool row_in, int64_t col0, int cols) {
-        e = 0;
-        end = 0;
-        limit = col0 + cols;
+    __device__ __forceinline__ void fetch(const GemmArgs& a, uint8_t* warp_box, int lane, int64_t row, bool row_in,
+                                          int col0, int cols) {
         idx = a.ent_idx + row * a.ent_k;
         p = a.ent_p ? a.ent_p + row * a.ent_k : nullptr;
-        if (row_in) {
-            if (a.offs) {
-                const int64_t tile = col0 / kEntryTile;
-                e = a.offs[tile * a.rows_pad + row];
-                end = a.offs[((col0 + cols - 1) / kEntryTile + 1) * a.rows_pad + row];
-            } else {
-                end = 1;
-            }
+        box = reinterpret_cast<uint2*>(warp_box) + lane;
+        first = n = 0;
+        if (!row_in || cols <= 0) return;
+        int e = 0, end = 1;
+        if (a.offs) {
+            e = a.offs[int64_t(col0 / kEntryTile) * a.rows_pad + row];
+            end = a.offs[int64_t((col0 + cols - 1) / kEntryTile + 1) * a.rows_pad + row];
         }
-        load();
-        while (next < col0) {
-            ++e;
-            load();
+        for (; e < end; e += 4) {
+            int c[4];
+            float q[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const bool in = e + j < end;
+                c[j] = in ? idx[e + j] : INT_MAX;
+                q[j] = in && p ? p[e + j] : 1.0f;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (c[j] >= col0 && c[j] < col0 + cols) {
+                    if (n == 0) first = e + j;
+                    if (n < kHeld) box[n * 32] = make_uint2(uint32_t(c[j]), __float_as_uint(q[j]));
+                    ++n;
+                }
         }
     }
+    __device__ __forceinline__ void load() {
+        next = INT_MAX;
+        prob = 0.0f;
+        if (i < n) {
+            if (i < kHeld) {
+                const uint2 v = box[i * 32];
+                next = int(v.x);
+                prob = __uint_as_float(v.y);
+            } else {
+                next = idx[first + i];
+                prob = p ? p[first + i] : 1.0f;
+            }
+        }
+    }
+    __device__ __forceinline__ void begin() {
+        i = 0;
+        load();
+    }
     template <class F>
-    __device__ __forceinline__ void walk(int64_t chunk0, F&& take) {
-        int64_t rel = int64_t(next) - chunk0;
-        while (__any_sync(0xffffffffu, rel < 32)) {
-            const bool mine = rel < 32;
-            take(mine ? int(rel) : -1, mine ? (p ? p[e] : 1.0f) : 0.0f);
+    __device__ __forceinline__ void walk(int chunk0, F&& take) {
+        while (__any_sync(0xffffffffu, next < chunk0 + 32)) {
+            const bool mine = next < chunk0 + 32;
+            take(mine ? next - chunk0 : -1, prob);
             if (mine) {
-                ++e;
+                ++i;
                 load();
-                rel = int64_t(next) - chunk0;
             }
         }
     }
@@ -304,57 +336,70 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     return *reinterpret_cast<uint32_t*>(&v);
 }
 
-// Hands 32 rows x 128 bytes, a row per lane in registers, to `emit(row, unit,
-// 16 bytes)` so that eight lanes hold one row's 128 bytes: through the warp's
-// 4 KiB of shared memory, 16-byte units swizzled by row % 8 (conflict-free both
-// ways).
-template <class F>
-__device__ __forceinline__ void transpose_rows(uint8_t* box, int lane, const uint32_t (&w)[32], F&& emit) {
-    __syncwarp();
-#pragma unroll
-    for (int u = 0; u < 8; ++u)
-        *reinterpret_cast<uint4*>(box + lane * 128 + (u ^ (lane & 7)) * 16) =
-            make_uint4(w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int row = i * 4 + (lane >> 3), unit = lane & 7;
-        emit(row, unit, *reinterpret_cast<const uint4*>(box + row * 128 + (unit ^ (row & 7)) * 16));
-    }
-}
-
 // What an epilogue warp knows about its 32 rows of a tile.
 template <int kBoxes>
 struct WarpRows {
     uint8_t* box;   // its staging boxes of 4 KiB
-    uint32_t next;  // the one to use next
     int lane;
     int64_t m0;     // first row; lane holds row m0 + lane
     int64_t M;      // rows that exist
     bool row_in;
 
-    __device__ __forceinline__ uint8_t* take() {
-        uint8_t* b = box + next * 4096;
-        next = kBoxes > 1 ? next ^ 1 : 0;
-        return b;
-    }
-    // 32 rows x 128 bytes, a row per lane in registers, through a staging box
-    // (16-byte units swizzled by row % 8, as the map says) to element x, row y
-    // of the output map: stored, or added.  What lies outside the map is clipped.
-    __device__ __forceinline__ void store(const void* tmap, const uint32_t (&w)[32], int x, int y, bool add) {
-        uint8_t* b = take();
-        if (lane == 0) ptx::bulk_wait_group_read<kBoxes - 1>();  // an earlier store has read this box
+    // Stores of 32 rows x 128 bytes through the output map: begin() waits until
+    // the staging boxes are free, stage() writes a box, a row per lane in
+    // registers (16-byte units swizzled by row % 8, as the map says), and
+    // send() hands the boxes to TMA, at elements x0 (and x1) of row y: stored,
+    // or added.  What lies outside the map is clipped.  (The proxy fence costs
+    // about 1000 cycles: one for all boxes.)
+    __device__ __forceinline__ void begin() {
+        if (lane == 0) ptx::bulk_wait_group_read0();
         __syncwarp();
+    }
+    __device__ __forceinline__ void stage(int slot, const uint32_t (&w)[32]) {
+        uint8_t* b = box + slot * 4096 + lane * 128;
 #pragma unroll
         for (int u = 0; u < 8; ++u)
-            *reinterpret_cast<uint4*>(b + lane * 128 + (u ^ (lane & 7)) * 16) =
+            *reinterpret_cast<uint4*>(b + (u ^ (lane & 7)) * 16) =
                 make_uint4(w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
+    }
+    __device__ __forceinline__ void send(const void* tmap, int boxes, int x0, int x1, int y, bool add) {
         ptx::fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
-            if (add) tma_add_2d(tmap, x, y, ptx::smem_addr(b));
-            else ptx::tma_store_2d(tmap, x, y, ptx::smem_addr(b));
+            const uint32_t b = ptx::smem_addr(box);
+            if (add) {
+                tma_add_2d(tmap, x0, y, b);
+                if (boxes > 1) tma_add_2d(tmap, x1, y, b + 4096);
+            } else {
+                ptx::tma_store_2d(tmap, x0, y, b);
+                if (boxes > 1) ptx::tma_store_2d(tmap, x1, y, b + 4096);
+            }
             ptx::bulk_commit_group();
+        }
+    }
+    // The same for two rows' worth of boxes at elements x0 and x1, `second`:
+    // whether the second one exists.
+    template <class F>
+    __device__ __forceinline__ void send_two(const void* tmap, F&& words, bool second, int x0, int x1, int y,
+                                             bool add) {
+        uint32_t w[32];
+        begin();
+        words(0, w);
+        stage(0, w);
+        if (kBoxes > 1) {
+            if (second) {
+                words(1, w);
+                stage(1, w);
+            }
+            send(tmap, second ? 2 : 1, x0, x1, y, add);
+        } else {
+            send(tmap, 1, x0, 0, y, add);
+            if (second) {
+                begin();
+                words(1, w);
+                stage(0, w);
+                send(tmap, 1, x1, 0, y, add);
+            }
         }
     }
 };
@@ -371,14 +416,14 @@ __device__ __forceinline__ float4 lse_tile(const GemmArgs& args, const void* tma
     float dot = 0.0f, top = -INFINITY;
 #pragma unroll
     for (int c = 0; c < 2 * kBlocks; ++c) {
-        cur.walk(args.v0 + n0 + c * 32, [&](int rel, float p) {
+        cur.walk(int(args.v0 + n0) + c * 32, [&](int rel, float p) {
             float v = 0.0f;
 #pragma unroll
             for (int j = 0; j < 32; ++j)
                 if (j == rel) v = r[c / 2][c % 2][j];
             if (rel >= 0) {
                 dot += p * v;
-                if (args.ent_s) args.ent_s[m * args.ent_k + cur.e] = v * k2;
+                if (args.ent_s) args.ent_s[m * args.ent_k + cur.first + cur.i] = v * k2;
             }
         });
         const int ncols = (int)min(int64_t(32), n_end - (n0 + c * 32));
@@ -402,126 +447,119 @@ __device__ __forceinline__ float4 lse_tile(const GemmArgs& args, const void* tma
             sum += r[c / 2][c % 2][j];
         }
     }
-    if (args.keep) {
+    if (args.keep && n0 < n_end) {  // (blocks of 64 columns are written whole)
         const float up = !wr.row_in ? 0.0f : kBf16 ? 32768.0f : 1.0f;
+        if (kBf16) {
+            wr.send_two(
+                tmap_c,
+                [&](int b, uint32_t (&w)[32]) {
 #pragma unroll
-        for (int b = 0; b < kBlocks; ++b) {
-            if (n0 + b * 64 >= n_end) break;  // (blocks of 64 columns are written whole)
-            if (kBf16) {
-                uint32_t w[32];
+                    for (int j = 0; j < 32; ++j) {
+                        const float (&x)[32] = r[b][j / 16];
+                        w[j] = pack2<false>(x[2 * (j % 16)] * up, x[2 * (j % 16) + 1] * up);
+                    }
+                },
+                n0 + 64 < n_end, int(n0), int(n0) + 64, int(wr.m0), false);
+        } else {
 #pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                    const float (&x)[32] = r[b][j / 16];
-                    w[j] = pack2<false>(x[2 * (j % 16)] * up, x[2 * (j % 16) + 1] * up);
-                }
-                wr.store(tmap_c, w, int(n0) + b * 64, int(wr.m0), false);
-            } else {
+            for (int b = 0; b < kBlocks; ++b)
+                if (n0 + b * 64 < n_end)
+                    wr.send_two(
+                        tmap_c,
+                        [&](int c, uint32_t (&w)[32]) {
 #pragma unroll
-                for (int c = 2 * b; c < 2 * b + 2; ++c) {
-                    uint32_t w[32];
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) w[j] = wr.row_in ? __float_as_uint(r[c / 2][c % 2][j]) : 0u;
-                    wr.store(tmap_c, w, 2 * (int(n0) + c * 32), int(wr.m0), false);
-                }
-            }
+                            for (int j = 0; j < 32; ++j) w[j] = wr.row_in ? __float_as_uint(r[b][c][j]) : 0u;
+                        },
+                        true, 2 * (int(n0) + b * 64), 2 * (int(n0) + b * 64 + 32), int(wr.m0), false);
         }
     }
     return make_float4(ref, sum, dot * k2, 0.0f);
 }
 
-// Gradient with respect to 64 logits of a row: softmax minus target in fp32,
-// rounded once to the type the next contractions read.
+// Gradient with respect to the logits of a half tile's row: softmax minus
+// target in fp32, rounded once to the type the next contractions read.
 template <bool kBf16, class Rows>
-__device__ __forceinline__ void grad_block(const GemmArgs& args, const void* tmap_c, Rows& wr, EntryCursor& cur, int64_t n0,
-                                           float k2, float lse2, float coef, float (&r)[2][32]) {
-    uint32_t hi[32];
+__device__ __forceinline__ void grad_tile(const GemmArgs& args, const void* tmap_c, Rows& wr, EntryCursor& cur,
+                                          int64_t n0, float k2, float lse2, float coef, float (&r)[2][2][32]) {
+    if (n0 >= args.N) return;
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
+    for (int c = 0; c < 4; ++c) {
+        float (&x)[32] = r[c / 2][c % 2];
         const int ncols = (int)min(int64_t(32), int64_t(args.N) - (n0 + c * 32));
 #pragma unroll
-        for (int j = 0; j < 32; ++j) r[c][j] = ex2(fmaf(r[c][j], k2, -lse2));
-        cur.walk(args.v0 + n0 + c * 32, [&](int rel, float p) {
+        for (int j = 0; j < 32; ++j) x[j] = ex2(fmaf(x[j], k2, -lse2));
+        cur.walk(int(args.v0 + n0) + c * 32, [&](int rel, float p) {
 #pragma unroll
             for (int j = 0; j < 32; ++j)
-                if (j == rel) r[c][j] -= p;
+                if (j == rel) x[j] -= p;
         });
 #pragma unroll
-        for (int j = 0; j < 32; ++j) r[c][j] = wr.row_in && j < ncols ? r[c][j] * coef : 0.0f;
+        for (int j = 0; j < 32; ++j) x[j] *= coef;  // (0 in a row that does not exist)
+        if (ncols < 32) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) hi[c * 16 + j] = pack2<kBf16>(r[c][2 * j], r[c][2 * j + 1]);
+            for (int j = 0; j < 32; ++j)
+                if (j >= ncols) x[j] = 0.0f;
+        }
     }
-    wr.store(tmap_c, hi, kBf16 ? int(n0) : 2 * int(n0), int(wr.m0), false);
-    if (!kBf16) {
-        uint32_t lo[32];
+    if (kBf16) {
+        wr.send_two(
+            tmap_c,
+            [&](int b, uint32_t (&w)[32]) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
+                for (int j = 0; j < 32; ++j) w[j] = pack2<true>(r[b][j / 16][2 * (j % 16)], r[b][j / 16][2 * (j % 16) + 1]);
+            },
+            n0 + 64 < args.N, int(n0), int(n0) + 64, int(wr.m0), false);
+    } else {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi[c * 16 + j]));
-                lo[c * 16 + j] = pack2<false>(r[c][2 * j] - h.x, r[c][2 * j + 1] - h.y);
-            }
-        wr.store(tmap_c, lo, 2 * int(n0) + 64, int(wr.m0), false);
+        for (int b = 0; b < 2; ++b)
+            if (n0 + b * 64 < args.N)
+                wr.send_two(
+                    tmap_c,
+                    [&](int plane, uint32_t (&w)[32]) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            float& x = r[b][j / 16][2 * (j % 16)];
+                            float& y = r[b][j / 16][2 * (j % 16) + 1];
+                            const __half2 h = __floats2half2_rn(x, y);
+                            w[j] = *reinterpret_cast<const uint32_t*>(&h);
+                            if (plane == 0) {  // what the hi values leave
+                                x -= __low2float(h);
+                                y -= __high2float(h);
+                            }
+                        }
+                    },
+                    true, 2 * (int(n0) + b * 64), 2 * (int(n0) + b * 64) + 64, int(wr.m0), false);
     }
 }
 
-// 64 columns of the warp's rows of a result, in registers as two parts of 32:
-// through the output map (running sums, or a dst that it describes), or row by
-// row where rows are scattered or not aligned.
+// A half tile of a result, through the output map: into fp32 running sums (row
+// y of the map is this part's row) or in the result's type.
 template <bool kF32, class Rows>
-__device__ __forceinline__ void out_block(const GemmArgs& args, const void* tmap_c, Rows& wr, bool sums, int sum_row,
-                                          bool vec, int64_t n0, float scale, float (&r)[2][32], int dst_row_of_lane) {
-    uint32_t w[32];
-    if (kF32 || sums) {
+__device__ __forceinline__ void out_tile(const GemmArgs& args, const void* tmap_c, Rows& wr, int y, int64_t n0,
+                                         float scale, float (&r)[2][2][32]) {
+    if (n0 >= args.N) return;
+    if (kF32 || args.sums) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            const int64_t n1 = n0 + c * 32;
-            if (n1 >= args.N) break;
+        for (int b = 0; b < 2; ++b) {
+            const int x = int(n0) + b * 64;
+            if (x < args.N)
+                wr.send_two(
+                    tmap_c,
+                    [&](int c, uint32_t (&w)[32]) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) w[j] = __float_as_uint(r[c][j] * scale);
-            if (sums || args.tma) {
-                wr.store(tmap_c, w, int(n1), sums ? sum_row : int(wr.m0), sums && !args.first);
-                continue;
-            }
-            transpose_rows(wr.box, wr.lane, w, [&](int row, int unit, uint4 v) {
-                const int dst_row = __shfl_sync(0xffffffffu, dst_row_of_lane, row);
-                const int64_t n = n1 + unit * 4;
-                const int ncols = (int)min(int64_t(4), int64_t(args.N) - n);
-                if (wr.m0 + row >= wr.M || ncols <= 0) return;
-                float* d = static_cast<float*>(args.dst) + int64_t(dst_row) * args.dst_row + n * args.dst_col;
-                if (vec && ncols == 4) {
-                    *reinterpret_cast<uint4*>(d) = v;
-                } else {
-                    const uint32_t q[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (j < ncols) d[j * args.dst_col] = __uint_as_float(q[j]);
-                }
-            });
+                        for (int j = 0; j < 32; ++j) w[j] = __float_as_uint(r[b][c][j] * scale);
+                    },
+                    x + 32 < args.N, x, x + 32, y, args.sums && !args.first);
         }
     } else {
-        if (n0 >= args.N) return;
+        wr.send_two(
+            tmap_c,
+            [&](int b, uint32_t (&w)[32]) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j)
-            w[j] = pack2<true>(r[j / 16][2 * (j % 16)] * scale, r[j / 16][2 * (j % 16) + 1] * scale);
-        if (args.tma) {
-            wr.store(tmap_c, w, int(n0), int(wr.m0), false);
-            return;
-        }
-        transpose_rows(wr.box, wr.lane, w, [&](int row, int unit, uint4 v) {
-            const int dst_row = __shfl_sync(0xffffffffu, dst_row_of_lane, row);
-            const int64_t n = n0 + unit * 8;
-            const int ncols = (int)min(int64_t(8), int64_t(args.N) - n);
-            if (wr.m0 + row >= wr.M || ncols <= 0) return;
-            uint16_t* d = static_cast<uint16_t*>(args.dst) + int64_t(dst_row) * args.dst_row + n * args.dst_col;
-            if (vec && ncols == 8) {
-                *reinterpret_cast<uint4*>(d) = v;
-            } else {
-                const uint32_t q[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (j < ncols) d[j * args.dst_col] = uint16_t(q[j / 2] >> (j % 2 * 16));
-            }
-        });
+                for (int j = 0; j < 32; ++j)
+                    w[j] = pack2<true>(r[b][j / 16][2 * (j % 16)] * scale, r[b][j / 16][2 * (j % 16) + 1] * scale);
+            },
+            n0 + 64 < args.N, int(n0), int(n0) + 64, y, false);
     }
 }
 
@@ -563,7 +601,7 @@ __global__ void __launch_bounds__(320, 1)
         ptx::fence_barrier_init();
         ptx::prefetch_tmap(&tmap_a);
         ptx::prefetch_tmap(&tmap_b);
-        if (kEpi == kEpiGrad || (kEpi == kEpiLse ? args.keep : args.sums | args.tma)) ptx::prefetch_tmap(&tmap_c);
+        if (kEpi == kEpiGrad || kEpi == kEpiOut || args.keep) ptx::prefetch_tmap(&tmap_c);
     }
     if (warp == 1) tmem_alloc<kPair>(ptx::smem_addr(tmem_slot), C::kTmemCols);
     ptx::tc_fence_before();
@@ -705,12 +743,10 @@ __global__ void __launch_bounds__(320, 1)
     } else {
         // ---------------- epilogue ----------------
         constexpr int kCols = kBN / 2;  // columns of this warp: half of the tile
-        constexpr int kParts = kCols / 32;
         const int quarter = warp & 3;
         const int half = (warp - 2) >> 2;
         WarpRows<C::kBoxes> wr;
         wr.box = smem + C::kOffOut + (warp - 2) * C::kBoxes * 4096;
-        wr.next = 0;
         wr.lane = lane;
         wr.M = M;
         // inverse of the operands' power-of-two scales
@@ -720,10 +756,6 @@ __global__ void __launch_bounds__(320, 1)
         const float k2 = args.logit_scale * kLog2e * inv;
         const float gscale = kEpi == kEpiGrad && !kBf16 ? pow2i(scale_exponent(args.state->amax[2])) : 1.0f;
         const float out_scale = kEpi == kEpiOut ? inv * args.state->grad_scale : 1.0f;
-        // whole 16-byte units can be written at dst
-        const bool vec = kEpi == kEpiOut && args.dst_col == 1 && args.dst_row * (args.dst_f32 ? 4 : 2) % 16 == 0 &&
-                         (reinterpret_cast<uintptr_t>(args.dst) & 15) == 0;
-        const bool sums = args.sums && !(args.direct && splits == 1);
         auto release = [&](uint32_t buf) {
             ptx::tc_fence_before();
             __syncwarp();
@@ -742,96 +774,64 @@ __global__ void __launch_bounds__(320, 1)
             wr.row_in = m < M;
             const int64_t ncol0 = int64_t(nb) * tile_n + half * kCols;
             const int64_t n_end = min(int64_t(args.N), int64_t(nb + 1) * tile_n);
-            // what the row needs beside its accumulator: read after the register
-            // sums, which take most of the registers, or while the MMAs run
-            EntryCursor cur;
-            float lse2 = 0.0f, coef = 0.0f;
-            int dst_row = 0;
-            auto row_values = [&]() {
-                if (kEpi != kEpiOut)
-                    cur.begin(args, m, wr.row_in && ncol0 < n_end, args.v0 + ncol0, int(n_end - ncol0));
-                if (kEpi == kEpiGrad && wr.row_in) {
-                    lse2 = args.lse2[m];
-                    coef = args.coef[m] * gscale;
-                }
-                if (kEpi == kEpiOut && wr.row_in) dst_row = args.row_map ? args.row_map[m] : int(m);
-            };
-            const int sum_row = split * num_m * C::kTileM + int(wr.m0);
-            const uint32_t lanes = uint32_t(quarter * 32) << 16;
             // a pair's second half may lie past the rows that the workspace holds
             const bool rows_in = kEpi == kEpiOut || wr.m0 < (args.M + kBM - 1) / kBM * kBM;
-            if (kChunked) {
-                float sum[kParts / 2][2][32];
+            // what the row needs beside its accumulator, while the MMAs run
+            EntryCursor cur;
+            float lse2 = 0.0f, coef = 0.0f;
+            if (kEpi != kEpiOut) {
+                wr.begin();  // the entries go where the stores' boxes are
+                cur.fetch(args, wr.box, lane, m, wr.row_in, int(args.v0 + ncol0), int(n_end - ncol0));
+            }
+            if (kEpi == kEpiGrad && wr.row_in) {
+                lse2 = args.lse2[m];
+                coef = args.coef[m] * gscale;
+            }
+            const uint32_t lanes = uint32_t(quarter * 32) << 16;
+            // The half tile's row in registers: the accumulator is free again
+            // before any of the work on it.  (An empty share of K: zeros.)
+            float r[2][2][32];
+            if (k0 >= k1) {
 #pragma unroll
-                for (int c = 0; c < kParts; ++c)
+                for (int c = 0; c < 4; ++c)
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) sum[c / 2][c % 2][j] = 0.0f;
-                for (int c0 = k0; c0 < k1; c0 = chunk_end(c0, k1), ++it) {
-                    const uint32_t buf = it & 1;
-                    if (!__all_sync(0xffffffffu, ptx::mbar_wait(bar_tmem_full + 8 * buf, (it >> 1) & 1))) {
-                        alive = false;
-                        break;
-                    }
-                    ptx::tc_fence_after();
-                    const uint32_t acc = tmem + buf * kBN + half * kCols + lanes;
+                    for (int j = 0; j < 32; ++j) r[c / 2][c % 2][j] = 0.0f;
+            }
+            for (int c0 = k0; c0 < k1; c0 = chunk_end(c0, k1), ++it) {
+                const uint32_t buf = it & 1;
+                if (!__all_sync(0xffffffffu, ptx::mbar_wait(bar_tmem_full + 8 * buf, (it >> 1) & 1))) {
+                    alive = false;
+                    break;
+                }
+                ptx::tc_fence_after();
+                const uint32_t acc = tmem + buf * kBN + half * kCols + lanes;
+                if (c0 == k0) {
 #pragma unroll
-                    for (int c = 0; c < 2 * kParts; ++c) {
+                    for (int c = 0; c < 4; ++c) tmem_ld_f32_x32(acc + c * 32, r[c / 2][c % 2]);
+                    ptx::tmem_ld_wait();
+                } else if (kChunked) {
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) {
                         uint32_t u[16];
                         tmem_ld_32x32b_x16(acc + c * 16, u);
                         ptx::tmem_ld_wait();
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) sum[c / 4][c / 2 % 2][c % 2 * 16 + j] += __uint_as_float(u[j]);
+                        for (int j = 0; j < 16; ++j) r[c / 4][c / 2 % 2][c % 2 * 16 + j] += __uint_as_float(u[j]);
                     }
-                    release(buf);
                 }
-                if (!alive) break;
-                if (!rows_in) continue;
-                row_values();
-                if (kEpi == kEpiLse) {
-                    const float4 st = lse_tile<kBf16, kParts / 2>(args, &tmap_c, wr, cur, ncol0, n_end, k2, sum);
-                    args.partial[(int64_t(args.half0) + nb * 2 + half) * args.rows_pad + m] = st;
-                } else if (kEpi == kEpiGrad) {
-#pragma unroll
-                    for (int b = 0; b < kParts / 2; ++b)
-                        if (ncol0 + b * 64 < args.N)
-                            grad_block<kBf16>(args, &tmap_c, wr, cur, ncol0 + b * 64, k2, lse2, coef, sum[b]);
-                } else {
-#pragma unroll
-                    for (int b = 0; b < kParts / 2; ++b)
-                        out_block<true>(args, &tmap_c, wr, sums, sum_row, vec, ncol0 + b * 64, out_scale, sum[b],
-                                        dst_row);
-                }
+                release(buf);
+            }
+            if (!alive) break;
+            if (!rows_in) continue;
+            if (kEpi != kEpiOut) cur.begin();
+            if (kEpi == kEpiLse) {
+                const float4 st = lse_tile<kBf16, 2>(args, &tmap_c, wr, cur, ncol0, n_end, k2, r);
+                args.partial[(int64_t(args.half0) + nb * 2 + half) * args.rows_pad + m] = st;
+            } else if (kEpi == kEpiGrad) {
+                grad_tile<kBf16>(args, &tmap_c, wr, cur, ncol0, k2, lse2, coef, r);
             } else {
-                row_values();
-                const uint32_t buf = it & 1;
-                const bool any = k0 < k1;  // an empty share has no accumulator: zeros
-                if (any) {
-                    if (!__all_sync(0xffffffffu, ptx::mbar_wait(bar_tmem_full + 8 * buf, (it >> 1) & 1))) break;
-                    ptx::tc_fence_after();
-                }
-                const uint32_t acc = tmem + buf * kBN + half * kCols + lanes;
-#pragma unroll 1
-                for (int b = 0; b < kParts / 2; ++b) {
-                    float r[2][32];
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        uint32_t u[32];
-                        ptx::tmem_ld_32x32b_x32(acc + b * 64 + c * 32, u);
-                        ptx::tmem_ld_wait();
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) r[c][j] = any ? __uint_as_float(u[j]) : 0.0f;
-                    }
-                    const int64_t n0 = ncol0 + b * 64;
-                    if (kEpi == kEpiGrad) {
-                        if (rows_in && n0 < args.N) grad_block<kBf16>(args, &tmap_c, wr, cur, n0, k2, lse2, coef, r);
-                    } else {
-                        out_block<false>(args, &tmap_c, wr, sums, sum_row, vec, n0, out_scale, r, dst_row);
-                    }
-                }
-                if (any) {
-                    release(buf);
-                    ++it;
-                }
+                out_tile<!kBf16>(args, &tmap_c, wr, (args.sums ? split * num_m * C::kTileM : 0) + int(wr.m0), ncol0,
+                                 out_scale, r);
             }
         }
         if (lane == 0) ptx::bulk_wait_group0();  // this warp's stores are done

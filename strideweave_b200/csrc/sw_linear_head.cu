@@ -534,57 +534,54 @@ __global__ void __launch_bounds__(256) scale_kernel(const ScaleArgs a) {
     }
 }
 
-// Result rows from the fp32 sums of the K walk's parts, added in order.
+// Result rows from the fp32 sums of the K walk's parts, added in order, to
+// their places; with by_count, zeros in the rows that do not count.
 struct SlotsArgs {
     const float* sums;       // part p of row m at row p round_up(M, tile_m) + m
     int64_t ld;
     int splits, tile_m;      // splits 0: state->dh_splits
-    int direct;              // one part was written to dst already
     int64_t rows, cols;
     const HeadState* state;
     int by_count, row0;
     const int* row_map;
     void* dst;
     int64_t dst_row, dst_col;
+    int vec;                 // dst rows are contiguous and aligned to four elements
 };
 template <bool kF32>
 __global__ void __launch_bounds__(256) sum_slots_kernel(const SlotsArgs a) {
     pdl_enter();
     const int splits = a.splits > 0 ? a.splits : a.state->dh_splits;
-    if (a.direct && splits == 1) return;
-    const int64_t rows = a.by_count ? min(a.rows, int64_t(max(a.state->count - a.row0, 0))) : a.rows;
-    const int64_t slot = (rows + a.tile_m - 1) / a.tile_m * a.tile_m * a.ld;
+    const int64_t summed = a.by_count ? min(a.rows, int64_t(max(a.state->count - a.row0, 0))) : a.rows;
+    const int64_t slot = (summed + a.tile_m - 1) / a.tile_m * a.tile_m * a.ld;
     const int64_t per_row = (a.cols + 3) / 4;
-    for (int64_t u = int64_t(blockIdx.x) * 256 + threadIdx.x; u < rows * per_row; u += int64_t(gridDim.x) * 256) {
+    for (int64_t u = int64_t(blockIdx.x) * 256 + threadIdx.x; u < a.rows * per_row; u += int64_t(gridDim.x) * 256) {
         const int64_t m = u / per_row, c = (u - m * per_row) * 4;
         const float* p = a.sums + m * a.ld + c;  // ld is whole groups of four
-        float4 s = *reinterpret_cast<const float4*>(p);
+        float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (m < summed) {
+            s = *reinterpret_cast<const float4*>(p);
 #pragma unroll 4
-        for (int k = 1; k < splits; ++k) {
-            const float4 v = *reinterpret_cast<const float4*>(p + k * slot);
-            s.x += v.x;
-            s.y += v.y;
-            s.z += v.z;
-            s.w += v.w;
+            for (int k = 1; k < splits; ++k) {
+                const float4 v = *reinterpret_cast<const float4*>(p + k * slot);
+                s.x += v.x;
+                s.y += v.y;
+                s.z += v.z;
+                s.w += v.w;
+            }
         }
         const int64_t at = (a.row_map ? int64_t(a.row_map[m]) : m) * a.dst_row + c * a.dst_col;
         const float r[4] = {s.x, s.y, s.z, s.w};
+        if (a.vec && c + 4 <= a.cols) {
+            if (kF32) *reinterpret_cast<float4*>(static_cast<float*>(a.dst) + at) = s;
+            else
+                *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.dst) + at) =
+                    make_uint2(pack2<true>(s.x, s.y), pack2<true>(s.z, s.w));
+            continue;
+        }
         for (int j = 0; j < 4 && c + j < a.cols; ++j) {
             if (kF32) static_cast<float*>(a.dst)[at + j * a.dst_col] = r[j];
             else static_cast<__nv_bfloat16*>(a.dst)[at + j * a.dst_col] = __float2bfloat16_rn(r[j]);
-        }
-    }
-}
-
-// Zeroes the gradient of the rows that do not count.
-__global__ void zero_rows_kernel(void* dst, int f32, int64_t T, int64_t D, int64_t sr, int64_t sc, const int* row_map,
-                                 const HeadState* state) {
-    pdl_enter();
-    for (int64_t i = state->count + blockIdx.x; i < T; i += gridDim.x) {
-        const int64_t at = int64_t(row_map[i]) * sr;
-        for (int64_t d = threadIdx.x; d < D; d += blockDim.x) {
-            if (f32) static_cast<float*>(dst)[at + d * sc] = 0.0f;
-            else static_cast<uint16_t*>(dst)[at + d * sc] = 0;
         }
     }
 }
@@ -791,8 +788,8 @@ struct Shape {
     int tile_n;              // columns of a logits tile
     bool logits_pair, dh_pair;
     Spread dw;
-    // rows of fp32 sums of each gradient (0: it is written at once); dh's parts
-    // are chosen on the device, for the rows that count
+    // rows of fp32 sums of each gradient (0: it is written at once); dh's rows
+    // are always put in place from sums, whose parts are chosen on the device
     int64_t dh_sum_rows, dw_sum_rows, ld_acc;
 };
 
@@ -983,13 +980,30 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
         const Operand gr{l.grad, s.rows, kF32 ? 2 * round_up(nv, 64) : nv, ld_grad, gp};
         GemmArgs a = g;
         a.row0 = (int)r0;
-        a.dst_f32 = kF32;
-        SlotsArgs sa;
-        memset(&sa, 0, sizeof(sa));
-        sa.ld = s.ld_acc;
-        sa.cols = s.D;
-        sa.state = l.state;
-        sa.row0 = (int)r0;
+        auto finish = [&](float* sums, int splits, bool pair, int64_t rows, bool by_count, const int* row_map,
+                          void* dst, int64_t dst_row, int64_t dst_col) -> int {
+            SlotsArgs sa;
+            memset(&sa, 0, sizeof(sa));
+            sa.sums = sums;
+            sa.ld = s.ld_acc;
+            sa.splits = splits;
+            sa.tile_m = pair ? 2 * kBM : kBM;
+            sa.rows = rows;
+            sa.cols = s.D;
+            sa.state = l.state;
+            sa.by_count = by_count;
+            sa.row0 = (int)r0;
+            sa.row_map = row_map;
+            sa.dst = dst;
+            sa.dst_row = dst_row;
+            sa.dst_col = dst_col;
+            sa.vec = dst_col == 1 && dst_row % 4 == 0 && (reinterpret_cast<uintptr_t>(dst) & (4 * esize - 1)) == 0;
+            const int64_t units = rows * (s.ld_acc / 4);
+            SW_CUDA_TRY(launch_pdl(sum_slots_kernel<kF32>, dim3((unsigned)std::min<int64_t>((units + 255) / 256, fill)),
+                                   dim3(256), 0, stream, sa),
+                        "linear head sums");
+            return SW_OK;
+        };
         if (c.dh && n > 0) {
             a.M = (int)n;
             a.N = (int)s.D;
@@ -997,32 +1011,17 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
             a.count_is = kCountM;
             a.scale_a = kF32 ? 2 : -1;
             a.scale_b = kF32 ? 1 : -1;
-            a.splits = s.dh_sum_rows ? 0 : 1;
-            a.sums = s.dh_sum_rows > 0;
-            a.direct = first_v && last_v;
+            a.splits = 0;
+            a.sums = 1;
             a.first = first_v;
-            a.dst = c.dh;
-            a.dst_row = p.dh_row;
-            a.dst_col = p.dh_col;
-            a.row_map = l.row_map + r0;
             const Target out{l.dh_sums, s.dh_sum_rows, s.ld_acc, s.ld_acc, true};
-            int rc = gemm<kBf16, false, true, kEpiOut>(gr, w, s.dh_sum_rows ? out : none, a, s.dh_pair, stream);
+            int rc = gemm<kBf16, false, true, kEpiOut>(gr, w, out, a, s.dh_pair, stream);
+            if (rc == SW_OK && last_v)
+                rc = finish(l.dh_sums, 0, s.dh_pair, n, true, l.row_map + r0, c.dh, p.dh_row, p.dh_col);
             if (rc != SW_OK) return rc;
-            if (last_v && s.dh_sum_rows) {
-                sa.sums = l.dh_sums;
-                sa.splits = 0;
-                sa.tile_m = s.dh_pair ? 2 * kBM : kBM;
-                sa.direct = a.direct;
-                sa.rows = n;
-                sa.by_count = 1;
-                sa.row_map = a.row_map;
-                sa.dst = c.dh;
-                sa.dst_row = p.dh_row;
-                sa.dst_col = p.dh_col;
-                SW_CUDA_TRY(launch_pdl(sum_slots_kernel<kF32>, dim3(fill), dim3(256), 0, stream, sa), "linear head dh");
-            }
         }
         if (c.dw) {
+            uint8_t* dst = static_cast<uint8_t*>(c.dw) + v0 * p.dw_row * esize;
             a.M = (int)nv;
             a.N = (int)s.D;
             a.K = (int)n;
@@ -1031,32 +1030,14 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
             a.scale_b = kF32 ? 0 : -1;
             a.splits = s.dw.splits;
             a.sums = s.dw_sum_rows > 0;
-            a.direct = 0;
             a.first = first_r;
-            a.row_map = nullptr;
-            a.dst = static_cast<uint8_t*>(c.dw) + v0 * p.dw_row * esize;
-            a.dst_row = p.dw_row;
-            a.dst_col = p.dw_col;
-            // (a map whose rows end inside 16 bytes would write the rest of them)
-            a.tma = !a.sums && p.dw_col == 1 && p.dw_row * esize % 16 == 0 && s.D * esize % 16 == 0 &&
-                    p.dw_row >= s.D && (reinterpret_cast<uintptr_t>(a.dst) & 15) == 0;
-            const Target sums{l.dw_sums, s.dw_sum_rows, s.ld_acc, s.ld_acc, true}, dst{a.dst, nv, s.D, p.dw_row, kF32};
-            int rc = gemm<kBf16, true, true, kEpiOut>(gr, states(r0, round_up(std::max<int64_t>(n, 1), kBM)),
-                                                      a.sums ? sums : a.tma ? dst : none, a, s.dw.pair, stream);
+            const Target out = a.sums ? Target{l.dw_sums, s.dw_sum_rows, s.ld_acc, s.ld_acc, true}
+                                      : Target{dst, nv, s.D, p.dw_row, kF32};
+            int rc = gemm<kBf16, true, true, kEpiOut>(gr, states(r0, round_up(std::max<int64_t>(n, 1), kBM)), out, a,
+                                                      s.dw.pair, stream);
+            if (rc == SW_OK && a.sums && last_r)
+                rc = finish(l.dw_sums, s.dw.splits, s.dw.pair, nv, false, nullptr, dst, p.dw_row, p.dw_col);
             if (rc != SW_OK) return rc;
-            if (last_r && a.sums) {
-                sa.sums = l.dw_sums;
-                sa.splits = s.dw.splits;
-                sa.tile_m = s.dw.pair ? 2 * kBM : kBM;
-                sa.direct = 0;
-                sa.rows = nv;
-                sa.by_count = 0;
-                sa.row_map = nullptr;
-                sa.dst = a.dst;
-                sa.dst_row = p.dw_row;
-                sa.dst_col = p.dw_col;
-                SW_CUDA_TRY(launch_pdl(sum_slots_kernel<kF32>, dim3(fill), dim3(256), 0, stream, sa), "linear head dw");
-            }
         }
         return SW_OK;
     };
@@ -1066,11 +1047,6 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
                         "linear head mean loss");
         return SW_OK;
     };
-    if (c.dh && s.T > 0)
-        SW_CUDA_TRY(launch_pdl(zero_rows_kernel, dim3((unsigned)std::min<int64_t>(s.T, 1184)), dim3(256), 0, stream,
-                               c.dh, (int)kF32, s.T, s.D, p.dh_row, p.dh_col, l.row_map, l.state),
-                    "linear head ignored rows");
-
     if (s.keep) {
         Operand w;
         if ((rc = weights(0, s.V, &w)) != SW_OK) return rc;
@@ -1250,14 +1226,17 @@ int check_and_run(const char* name, Call& c, void* stream_ptr) {
     if (c.dh && T > 0) {
         const int64_t n = std::min(s.rows, T), nv = std::min(s.piece, V);
         s.dh_pair = choose_spread(n, D, nv, terms, true).pair;
-        const int workers = s.dh_pair ? device_sms() / 2 : device_sms();
-        // (fewer than two tiles of columns per worker: some row count may split)
-        if (s.piece < V || 4 * ((D + kBN - 1) / kBN) <= 4 * workers) s.dh_sum_rows = sum_rows(n, D, s.dh_pair);
+        s.dh_sum_rows = sum_rows(n, D, s.dh_pair);
     }
     if (c.dw) {
         const int64_t n = std::min(s.rows, T), nv = std::min(s.piece, V);
         s.dw = choose_spread(nv, D, n, terms, true);
-        if (s.dw.splits > 1 || s.rows < T) s.dw_sum_rows = s.dw.splits * round_up(nv, s.dw.pair ? 2 * kBM : kBM);
+        // written at once through TMA where that can describe dw (rows that end
+        // inside 16 bytes would be written past their end)
+        const int64_t es = s.f32 ? 4 : 2;
+        const bool direct = p->dw_col == 1 && p->dw_row * es % 16 == 0 && D * es % 16 == 0 && p->dw_row >= D &&
+                            (reinterpret_cast<uintptr_t>(c.dw) & 15) == 0;
+        if (!direct || s.dw.splits > 1 || s.rows < T) s.dw_sum_rows = s.dw.splits * round_up(nv, s.dw.pair ? 2 * kBM : kBM);
     }
 
     Bump measure{nullptr, 0};
