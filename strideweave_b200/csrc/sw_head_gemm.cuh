@@ -9,10 +9,17 @@
 //             rounded once to the operand type
 //   kEpiOut   the product itself: a gradient of the states or of the weights
 //
-// A persistent CTA (kPair false) walks 128 x 256 tiles, or a pair of CTAs on
-// neighbouring SMs (kPair) walks 256 x 256 tiles with tcgen05 cta_group::2: each
-// CTA holds its 128 rows of A and half of B in shared memory and its 128 rows
-// of the accumulator in TMEM, so a stage moves 32 KiB per SM instead of 48.
+// Tile shapes (kShape), on persistent CTAs:
+//   kSingle  128 x 256 on one CTA;
+//   kPair2   256 x 256 on a pair of CTAs on neighbouring SMs, tcgen05
+//            cta_group::2: each CTA holds its 128 rows of A and half of B in
+//            shared memory and its rows of the accumulator in TMEM, so a K
+//            stage moves 32 KiB per SM instead of 48;
+//   kTall    512 x 256 on a pair: two accumulators of 256 x 256 that share B, a
+//            stage of 48 KiB per SM for twice the work.  Nothing is left of TMEM
+//            for a second tile, so about 3000 cycles of a tile's epilogue are not
+//            hidden; in exchange a quarter fewer bytes come from L2, which under
+//            the power limit buys clock.
 // Warp 0 feeds a ring of 64-deep K stages by TMA (128-byte swizzle), one thread
 // of warp 1 (of the pair's first CTA) issues the MMAs, warps 2-9 drain one of
 // two TMEM accumulators while the other is being filled: warp w reads TMEM
@@ -43,11 +50,52 @@ constexpr int kBM = 128;
 constexpr int kBK = 64;                 // K elements of a stage: one 128-byte swizzle row
 constexpr int kBN = 256;
 constexpr int kEntryTile = 256;         // columns per entry of the target offset table
+// With at most this many rows that count, one bf16 rounding of a dominant entry
+// of the logits' gradient would show in a result (nothing averages it out), and
+// three quarters of a tile's rows are idle: rows 64 .. 127 then hold what the
+// rounding of rows 0 .. 63 left, against the same states.
+constexpr int kFewRows = 64;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
 enum { kEpiLse = 0, kEpiGrad = 1, kEpiOut = 2 };
-enum { kCountNone = 0, kCountM = 1, kCountK = 2 };
+enum { kCountM, kCountK };
+
+// How the tiles of a contraction are walked: groups of row tiles (which share
+// B's panels in L2), column tiles inside, row tiles innermost; the workers take
+// whole waves of tiles, and the tiles of the last, partial wave are cut into
+// `parts` shares of the K walk, each with its own rows of the fp32 sums: part 0
+// at the row itself, part p > 0 of rows from `row_f` on behind all rows.
+// Groups of 2048 rows: 512 / 1024 / 2048 / 4096 / 8192, an 8192 x 131072 x 4096
+// step under the power cap: 25.3 / 25.4 / 24.5 / 24.3 / 25.9 ms, 4096 x 32000 x
+// 4096: 2.94 / 2.88 / 2.81 / 2.82 / 2.91.
+struct Walk {
+    int num_m, num_n, tile_m, group, parts, whole, row_f;
+
+    __host__ __device__ Walk(int M, int cols_tiles, int rows_per_tile, int workers, int parts_)
+        : num_m((M + rows_per_tile - 1) / rows_per_tile), num_n(cols_tiles), tile_m(rows_per_tile),
+          group(2048 / rows_per_tile), parts(parts_) {
+        const int tiles = num_m * num_n;
+        whole = parts > 1 ? tiles / workers * workers : tiles;
+        row_f = whole / (group * num_n) * group * tile_m;
+    }
+    __host__ __device__ int items() const { return whole + (num_m * num_n - whole) * parts; }
+    __host__ __device__ int tile_of(int mb, int nb) const {
+        const int first = mb / group * group;
+        return first * num_n + nb * min_(num_m - first, group) + (mb - first);
+    }
+    __host__ __device__ void coords(int tile, int& mb, int& nb) const {
+        const int per_group = group * num_n, first = tile / per_group * group;
+        const int rows = min_(num_m - first, group), r = tile - first * num_n;
+        nb = r / rows;
+        mb = first + r - nb * rows;
+    }
+    // Row of the sums that holds row m of part p.
+    __host__ __device__ int sum_row(int p, int m) const {
+        return p == 0 ? m : num_m * tile_m + (p - 1) * (num_m * tile_m - row_f) + (m - row_f);
+    }
+    __host__ __device__ static int min_(int a, int b) { return a < b ? a : b; }
+};
 
 // What the preparation kernels leave for the contractions.
 struct HeadState {
@@ -57,6 +105,13 @@ struct HeadState {
     float grad_scale;        // common factor of every row's gradient, applied to dh and dw in fp32
     int dh_splits;           // parts of the K walk of dh, chosen for the rows that count
     int pad;
+
+    // Rows that count from row0 on, and whether they have remainder rows (bf16).
+    __device__ __forceinline__ int rows(int row0) const { return max(count - row0, 0); }
+    __device__ __forceinline__ bool few(int row0) const { return count <= kFewRows && rows(row0) > 0; }
+    __device__ __forceinline__ int rows_and_rest(int row0, bool bf16) const {
+        return bf16 && few(row0) ? kFewRows + rows(row0) : rows(row0);
+    }
 };
 
 // Power-of-two multiplier that brings values of magnitude `amax` just under
@@ -88,7 +143,7 @@ struct GemmArgs {
     int row0;                // first compact row of this launch (the count starts there)
     int terms;               // plane pairs walked: 1, or 3 for Float32
     Plane pa, pb;            // where each operand's lo plane and 64-element blocks lie
-    int splits;              // parts of the K walk, each with its own rows of the sums (0: state->dh_splits)
+    int splits;              // parts of the last wave's tiles (0: state->dh_splits)
     int tile_n;              // columns of a tile: kBN, or fewer for logits of one CTA (a multiple of 16)
     int scale_a, scale_b;    // indexes into HeadState::amax of the operands' scales (-1: none)
     // logits epilogues
@@ -111,16 +166,22 @@ struct GemmArgs {
     int first;               // nothing to add yet
 };
 
-template <bool kPair>
+enum { kSingle = 0, kPair2 = 1, kTall = 2 };
+__host__ __device__ constexpr int shape_rows(int shape) { return kBM << shape; }
+
+template <int kShape>
 struct Cfg {
+    static constexpr bool kPair = kShape != kSingle;
+    static constexpr int kAccs = kShape == kTall ? 2 : 1;  // accumulators of one tile
     static constexpr int kThreads = 64 + 256;
-    static constexpr int kTileM = kPair ? 2 * kBM : kBM;
+    static constexpr int kTileM = shape_rows(kShape);
+    static constexpr int kAccRows = kPair ? 2 * kBM : kBM; // rows of one accumulator over the CTAs
     static constexpr int kBRows = kPair ? kBN / 2 : kBN;  // rows of B that one CTA holds
-    static constexpr int kABytes = kBM * kBK * 2;
+    static constexpr int kABytes = kAccs * kBM * kBK * 2;
     static constexpr int kBBytes = kBRows * kBK * 2;
     static constexpr int kStageBytes = kABytes + kBBytes;
-    static constexpr int kStages = kPair ? 5 : 4;
-    static constexpr int kBoxes = kPair ? 2 : 1;           // 4 KiB staging boxes per epilogue warp
+    static constexpr int kStages = kShape == kPair2 ? 5 : 4;
+    static constexpr int kBoxes = kShape == kPair2 ? 2 : 1;           // 4 KiB staging boxes per epilogue warp
     static constexpr int kOffOut = kStages * kStageBytes;
     static constexpr int kOffBar = kOffOut + 8 * kBoxes * 4096;
     static constexpr int kNumBars = 2 * kStages + 5;
@@ -377,30 +438,24 @@ struct WarpRows {
             ptx::bulk_commit_group();
         }
     }
-    // The same for two rows' worth of boxes at elements x0 and x1, `second`:
-    // whether the second one exists.
+    // The same for two boxes, word(b, j) of box b, at elements x0 and x1;
+    // `second`: whether the second one exists.
     template <class F>
-    __device__ __forceinline__ void send_two(const void* tmap, F&& words, bool second, int x0, int x1, int y,
-                                             bool add) {
+    __device__ __forceinline__ void send_two(const void* tmap, F&& word, bool second, int x0, int x1, int y, bool add) {
         uint32_t w[32];
         begin();
-        words(0, w);
+#pragma unroll
+        for (int j = 0; j < 32; ++j) w[j] = word(0, j);
         stage(0, w);
-        if (kBoxes > 1) {
-            if (second) {
-                words(1, w);
-                stage(1, w);
-            }
-            send(tmap, second ? 2 : 1, x0, x1, y, add);
-        } else {
-            send(tmap, 1, x0, 0, y, add);
-            if (second) {
-                begin();
-                words(1, w);
-                stage(0, w);
-                send(tmap, 1, x1, 0, y, add);
-            }
+        if (kBoxes == 1) send(tmap, 1, x0, 0, y, add);
+        if (second) {
+            if (kBoxes == 1) begin();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) w[j] = word(1, j);
+            stage(kBoxes - 1, w);
         }
+        if (kBoxes > 1) send(tmap, second ? 2 : 1, x0, x1, y, add);
+        else if (second) send(tmap, 1, x1, 0, y, add);
     }
 };
 
@@ -452,12 +507,9 @@ __device__ __forceinline__ float4 lse_tile(const GemmArgs& args, const void* tma
         if (kBf16) {
             wr.send_two(
                 tmap_c,
-                [&](int b, uint32_t (&w)[32]) {
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        const float (&x)[32] = r[b][j / 16];
-                        w[j] = pack2<false>(x[2 * (j % 16)] * up, x[2 * (j % 16) + 1] * up);
-                    }
+                [&](int b, int j) {
+                    const float (&x)[32] = r[b][j / 16];
+                    return pack2<false>(x[2 * (j % 16)] * up, x[2 * (j % 16) + 1] * up);
                 },
                 n0 + 64 < n_end, int(n0), int(n0) + 64, int(wr.m0), false);
         } else {
@@ -465,12 +517,8 @@ __device__ __forceinline__ float4 lse_tile(const GemmArgs& args, const void* tma
             for (int b = 0; b < kBlocks; ++b)
                 if (n0 + b * 64 < n_end)
                     wr.send_two(
-                        tmap_c,
-                        [&](int c, uint32_t (&w)[32]) {
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) w[j] = wr.row_in ? __float_as_uint(r[b][c][j]) : 0u;
-                        },
-                        true, 2 * (int(n0) + b * 64), 2 * (int(n0) + b * 64 + 32), int(wr.m0), false);
+                        tmap_c, [&](int c, int j) { return wr.row_in ? __float_as_uint(r[b][c][j]) : 0u; }, true,
+                        2 * (int(n0) + b * 64), 2 * (int(n0) + b * 64 + 32), int(wr.m0), false);
         }
     }
     return make_float4(ref, sum, dot * k2, 0.0f);
@@ -478,10 +526,10 @@ __device__ __forceinline__ float4 lse_tile(const GemmArgs& args, const void* tma
 
 // Gradient with respect to the logits of a half tile's row: softmax minus
 // target in fp32, rounded once to the type the next contractions read.
-template <bool kBf16, class Rows>
+template <bool kBf16, bool kFew, class Rows>
 __device__ __forceinline__ void grad_tile(const GemmArgs& args, const void* tmap_c, Rows& wr, EntryCursor& cur,
                                           int64_t n0, float k2, float lse2, float coef, float (&r)[2][2][32]) {
-    if (n0 >= args.N) return;
+    if (n0 >= args.N || (kFew && wr.m0 >= kFewRows)) return;  // (the remainders' rows are written below)
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
         float (&x)[32] = r[c / 2][c % 2];
@@ -504,29 +552,37 @@ __device__ __forceinline__ void grad_tile(const GemmArgs& args, const void* tmap
     if (kBf16) {
         wr.send_two(
             tmap_c,
-            [&](int b, uint32_t (&w)[32]) {
-#pragma unroll
-                for (int j = 0; j < 32; ++j) w[j] = pack2<true>(r[b][j / 16][2 * (j % 16)], r[b][j / 16][2 * (j % 16) + 1]);
+            [&](int b, int j) {
+                float& x = r[b][j / 16][2 * (j % 16)];
+                float& y = r[b][j / 16][2 * (j % 16) + 1];
+                const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+                if (kFew) {  // what the rounding leaves
+                    x -= __low2float(h);
+                    y -= __high2float(h);
+                }
+                return *reinterpret_cast<const uint32_t*>(&h);
             },
             n0 + 64 < args.N, int(n0), int(n0) + 64, int(wr.m0), false);
+        if (kFew)
+            wr.send_two(
+                tmap_c,
+                [&](int b, int j) { return pack2<true>(r[b][j / 16][2 * (j % 16)], r[b][j / 16][2 * (j % 16) + 1]); },
+                n0 + 64 < args.N, int(n0), int(n0) + 64, int(wr.m0) + kFewRows, false);
     } else {
 #pragma unroll
         for (int b = 0; b < 2; ++b)
             if (n0 + b * 64 < args.N)
                 wr.send_two(
                     tmap_c,
-                    [&](int plane, uint32_t (&w)[32]) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            float& x = r[b][j / 16][2 * (j % 16)];
-                            float& y = r[b][j / 16][2 * (j % 16) + 1];
-                            const __half2 h = __floats2half2_rn(x, y);
-                            w[j] = *reinterpret_cast<const uint32_t*>(&h);
-                            if (plane == 0) {  // what the hi values leave
-                                x -= __low2float(h);
-                                y -= __high2float(h);
-                            }
+                    [&](int plane, int j) {
+                        float& x = r[b][j / 16][2 * (j % 16)];
+                        float& y = r[b][j / 16][2 * (j % 16) + 1];
+                        const __half2 h = __floats2half2_rn(x, y);
+                        if (plane == 0) {  // what the hi values leave
+                            x -= __low2float(h);
+                            y -= __high2float(h);
                         }
+                        return *reinterpret_cast<const uint32_t*>(&h);
                     },
                     true, 2 * (int(n0) + b * 64), 2 * (int(n0) + b * 64) + 64, int(wr.m0), false);
     }
@@ -545,31 +601,28 @@ __device__ __forceinline__ void out_tile(const GemmArgs& args, const void* tmap_
             if (x < args.N)
                 wr.send_two(
                     tmap_c,
-                    [&](int c, uint32_t (&w)[32]) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) w[j] = __float_as_uint(r[b][c][j] * scale);
-                    },
+                    [&](int c, int j) { return __float_as_uint(r[b][c][j] * scale); },
                     x + 32 < args.N, x, x + 32, y, args.sums && !args.first);
         }
     } else {
         wr.send_two(
             tmap_c,
-            [&](int b, uint32_t (&w)[32]) {
-#pragma unroll
-                for (int j = 0; j < 32; ++j)
-                    w[j] = pack2<true>(r[b][j / 16][2 * (j % 16)] * scale, r[b][j / 16][2 * (j % 16) + 1] * scale);
+            [&](int b, int j) {
+                return pack2<true>(r[b][j / 16][2 * (j % 16)] * scale, r[b][j / 16][2 * (j % 16) + 1] * scale);
             },
             n0 + 64 < args.N, int(n0), int(n0) + 64, y, false);
     }
 }
 
-template <bool kPair, bool kBf16, bool kAMn, bool kBMn, int kEpi>
+template <int kShape, bool kBf16, bool kAMn, bool kBMn, int kEpi>
 __global__ void __launch_bounds__(320, 1)
     head_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                      const __grid_constant__ CUtensorMap tmap_c, const GemmArgs args) {
-    using C = Cfg<kPair>;
+    using C = Cfg<kShape>;
+    constexpr bool kPair = C::kPair;
     constexpr bool kNarrow = !kPair && kEpi == kEpiLse;  // tiles may have fewer than kBN columns
     constexpr bool kChunked = !kBf16 || kEpi == kEpiLse;
+    static_assert(C::kAccs == 1 || !kChunked, "the tall tile has no accumulator to alternate with");
     // K stages between two register sums: 512 elements; 1024 in bf16, whose logits need 1e-6
     constexpr int kChunkSteps = kBf16 ? 16 : 8;
     constexpr int kStages = C::kStages;
@@ -612,31 +665,32 @@ __global__ void __launch_bounds__(320, 1)
     const uint32_t tmem = *tmem_slot;
     pdl_enter();
 
-    const int count = args.count_is == kCountNone ? 0 : max(args.state->count - args.row0, 0);
-    const int M = args.count_is == kCountM ? min(args.M, count) : args.M;
-    const int K = args.count_is == kCountK ? min(args.K, count) : args.K;
-    const int num_m = (M + C::kTileM - 1) / C::kTileM;
+    // rows that count, and for the gradients of few rows their remainders
+    const bool few = kBf16 && kEpi != kEpiLse && args.state->few(args.row0);
+    int rows = args.state->rows(args.row0);
+    if (!few) rows = min(rows, args.count_is == kCountM ? args.M : args.K);
+    else if (kEpi == kEpiOut) rows += kFewRows;
+    const int M = args.count_is == kCountM ? rows : args.M;
+    const int K = args.count_is == kCountK ? rows : args.K;
     const int tile_n = kNarrow ? args.tile_n : kBN;
-    const int num_n = (args.N + tile_n - 1) / tile_n;
-    const int num_tiles = num_m * num_n;
-    const int splits = args.splits > 0 ? args.splits : args.state->dh_splits;
-    const int num_items = num_tiles * splits;
+    const Walk walk(M, (args.N + tile_n - 1) / tile_n, C::kTileM, workers,
+                    args.splits > 0 ? args.splits : args.state->dh_splits);
+    const int num_items = walk.items();
     const int k_steps = (K + kBK - 1) / kBK;
-    const int split_steps = (k_steps + splits - 1) / splits;
-    constexpr int kGroup = kPair ? 8 : 16;  // row tiles of a raster group: they share B's panels in L2
+    const int part_steps = (k_steps + walk.parts - 1) / walk.parts;
     // Work item `t`: a tile and its share [k0, k1) of the K stages.
-    auto item = [&](int t, int& mb, int& nb, int& split, int& k0, int& k1) {
-        split = t / num_tiles;
-        t -= split * num_tiles;
-        k0 = min(split * split_steps, k_steps);
-        k1 = min(k0 + split_steps, k_steps);
-        const int per_group = kGroup * num_n;
-        const int g = t / per_group;
-        const int first = g * kGroup;
-        const int gsize = min(num_m - first, kGroup);
-        const int r = t % per_group;
-        mb = first + r % gsize;
-        nb = r / gsize;
+    auto item = [&](int t, int& mb, int& nb, int& part, int& k0, int& k1) {
+        part = 0;
+        k0 = 0;
+        k1 = k_steps;
+        if (t >= walk.whole && walk.parts > 1) {
+            const int tile = walk.whole + (t - walk.whole) / walk.parts;
+            part = (t - walk.whole) % walk.parts;
+            k0 = min(part * part_steps, k_steps);
+            k1 = min(k0 + part_steps, k_steps);
+            t = tile;
+        }
+        walk.coords(t, mb, nb);
     };
     auto chunk_end = [&](int k0, int k1) { return kChunked ? min(k0 + kChunkSteps, k1) : k1; };
 
@@ -668,13 +722,18 @@ __global__ void __launch_bounds__(320, 1)
                             const uint32_t sb = sa + C::kABytes;
                             // the first CTA's barrier counts both CTAs' bytes
                             if (rank == 0) ptx::mbar_arrive_expect_tx(own, bytes);
-                            if (kAMn) {
 #pragma unroll
-                                for (int g = 0; g < kBM / 64; ++g)
-                                    tma_load<kPair>(sa + g * 8192, &tmap_a, (a0 / 64 + g) * args.pa.x_block + xa,
-                                                    ya + ks * kBK, full);
-                            } else {
-                                tma_load<kPair>(sa, &tmap_a, ks * args.pa.x_block + xa, ya + a0, full);
+                            for (int h = 0; h < C::kAccs; ++h) {
+                                const uint32_t sah = sa + h * (kBM * kBK * 2);
+                                const int ah = a0 + h * C::kAccRows;
+                                if (kAMn) {
+#pragma unroll
+                                    for (int g = 0; g < kBM / 64; ++g)
+                                        tma_load<kPair>(sah + g * 8192, &tmap_a, (ah / 64 + g) * args.pa.x_block + xa,
+                                                        ya + ks * kBK, full);
+                                } else {
+                                    tma_load<kPair>(sah, &tmap_a, ks * args.pa.x_block + xa, ya + ah, full);
+                                }
                             }
                             if (kBMn) {
 #pragma unroll
@@ -700,40 +759,51 @@ __global__ void __launch_bounds__(320, 1)
     } else if (warp == 1) {
         if (lane == 0 && rank == 0) {
             // ---------------- MMA issuer ----------------
-            const uint32_t idesc = idesc_f16(kBf16, kAMn, kBMn, C::kTileM, tile_n);
+            const uint32_t idesc = idesc_f16(kBf16, kAMn, kBMn, C::kAccRows, tile_n);
             int stage = 0;
             uint32_t phase = 0, it = 0;
             bool alive = true;
             for (int t = worker; t < num_items && alive; t += workers) {
                 int mb, nb, split, k0, k1;
                 item(t, mb, nb, split, k0, k1);
-                for (int c0 = k0; c0 < k1; c0 = chunk_end(c0, k1), ++it) {
-                    const uint32_t buf = it & 1;
-                    if (!ptx::mbar_wait(bar_tmem_empty + 8 * buf, ((it >> 1) & 1) ^ 1)) { alive = false; break; }
-                    ptx::tc_fence_after();
-                    const uint32_t acc = tmem + buf * kBN;
+                for (int c0 = k0; c0 < k1 && alive; c0 = chunk_end(c0, k1), ++it) {
+                    // one tile alternates between the two accumulators, a tall one fills both
+                    const uint32_t buf0 = C::kAccs == 1 ? it & 1 : 0, drained = (C::kAccs == 1 ? it >> 1 : it) & 1;
                     const int steps = (chunk_end(c0, k1) - c0) * args.terms;
-                    for (int ks = 0; ks < steps; ++ks) {
+                    for (int ks = 0; ks < steps && alive; ++ks) {
                         if (!ptx::mbar_wait(bar_full + 8 * stage, phase)) { alive = false; break; }
                         ptx::tc_fence_after();
-                        const uint32_t sa = sbase + stage * C::kStageBytes;
-                        const uint32_t sb = sa + C::kABytes;
 #pragma unroll
-                        for (int j = 0; j < kBK / 16; ++j) {
-                            // K-major: 16 elements of K are 32 bytes of the swizzled row, 8-row groups 1024
-                            // bytes apart.  MN-major: 16 rows of K are 2048 bytes, 64-element blocks of the
-                            // other mode 8192 bytes apart, 8-row groups of K 1024.
-                            const uint64_t ad = kAMn ? ptx::smem_desc(sa + 2048 * j, 8192, 1024, ptx::kLayoutSwizzle128)
-                                                     : ptx::smem_desc(sa + 32 * j, 0, 1024, ptx::kLayoutSwizzle128);
-                            const uint64_t bd = kBMn ? ptx::smem_desc(sb + 2048 * j, 8192, 1024, ptx::kLayoutSwizzle128)
-                                                     : ptx::smem_desc(sb + 32 * j, 0, 1024, ptx::kLayoutSwizzle128);
-                            mma_f16<kPair>(acc, ad, bd, idesc, (ks > 0 || j > 0) ? 1u : 0u);
+                        for (int h = 0; h < C::kAccs; ++h) {
+                            const uint32_t buf = buf0 + h;
+                            if (ks == 0) {
+                                if (!ptx::mbar_wait(bar_tmem_empty + 8 * buf, drained ^ 1)) { alive = false; break; }
+                                ptx::tc_fence_after();
+                            }
+                            const uint32_t acc = tmem + buf * kBN;
+                            const uint32_t sa = sbase + stage * C::kStageBytes + h * (kBM * kBK * 2);
+                            const uint32_t sb = sbase + stage * C::kStageBytes + C::kABytes;
+#pragma unroll
+                            for (int j = 0; j < kBK / 16; ++j) {
+                                // K-major: 16 elements of K are 32 bytes of the swizzled row, 8-row groups 1024
+                                // bytes apart.  MN-major: 16 rows of K are 2048 bytes, 64-element blocks of the
+                                // other mode 8192 bytes apart, 8-row groups of K 1024.
+                                const uint64_t ad =
+                                    kAMn ? ptx::smem_desc(sa + 2048 * j, 8192, 1024, ptx::kLayoutSwizzle128)
+                                         : ptx::smem_desc(sa + 32 * j, 0, 1024, ptx::kLayoutSwizzle128);
+                                const uint64_t bd =
+                                    kBMn ? ptx::smem_desc(sb + 2048 * j, 8192, 1024, ptx::kLayoutSwizzle128)
+                                         : ptx::smem_desc(sb + 32 * j, 0, 1024, ptx::kLayoutSwizzle128);
+                                mma_f16<kPair>(acc, ad, bd, idesc, (ks > 0 || j > 0) ? 1u : 0u);
+                            }
+                            if (C::kAccs > 1 && ks + 1 == steps) commit<kPair>(bar_tmem_full + 8 * buf);
                         }
+                        if (!alive) break;
                         commit<kPair>(bar_empty + 8 * stage);
                         if (++stage == kStages) { stage = 0; phase ^= 1; }
                     }
                     if (!alive) break;
-                    commit<kPair>(bar_tmem_full + 8 * buf);
+                    if (C::kAccs == 1) commit<kPair>(bar_tmem_full + 8 * buf0);
                 }
             }
             // every MMA is done before TMEM is released
@@ -769,69 +839,74 @@ __global__ void __launch_bounds__(320, 1)
         for (int t = worker; t < num_items && alive; t += workers) {
             int mb, nb, split, k0, k1;
             item(t, mb, nb, split, k0, k1);
-            wr.m0 = int64_t(mb) * C::kTileM + rank * kBM + quarter * 32;
-            const int64_t m = wr.m0 + lane;
-            wr.row_in = m < M;
-            const int64_t ncol0 = int64_t(nb) * tile_n + half * kCols;
-            const int64_t n_end = min(int64_t(args.N), int64_t(nb + 1) * tile_n);
-            // a pair's second half may lie past the rows that the workspace holds
-            const bool rows_in = kEpi == kEpiOut || wr.m0 < (args.M + kBM - 1) / kBM * kBM;
-            // what the row needs beside its accumulator, while the MMAs run
-            EntryCursor cur;
-            float lse2 = 0.0f, coef = 0.0f;
-            if (kEpi != kEpiOut) {
-                wr.begin();  // the entries go where the stores' boxes are
-                cur.fetch(args, wr.box, lane, m, wr.row_in, int(args.v0 + ncol0), int(n_end - ncol0));
-            }
-            if (kEpi == kEpiGrad && wr.row_in) {
-                lse2 = args.lse2[m];
-                coef = args.coef[m] * gscale;
-            }
-            const uint32_t lanes = uint32_t(quarter * 32) << 16;
-            // The half tile's row in registers: the accumulator is free again
-            // before any of the work on it.  (An empty share of K: zeros.)
-            float r[2][2][32];
-            if (k0 >= k1) {
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) r[c / 2][c % 2][j] = 0.0f;
-            }
-            for (int c0 = k0; c0 < k1; c0 = chunk_end(c0, k1), ++it) {
-                const uint32_t buf = it & 1;
-                if (!__all_sync(0xffffffffu, ptx::mbar_wait(bar_tmem_full + 8 * buf, (it >> 1) & 1))) {
-                    alive = false;
-                    break;
+#pragma unroll 1
+            for (int h = 0; h < C::kAccs && alive; ++h) {
+    wr.m0 = int64_t(mb) * C::kTileM + h * C::kAccRows + rank * kBM + quarter * 32;
+                const int64_t m = wr.m0 + lane;
+                wr.row_in = m < M;
+                const int64_t ncol0 = int64_t(nb) * tile_n + half * kCols;
+                const int64_t n_end = min(int64_t(args.N), int64_t(nb + 1) * tile_n);
+                // a pair's second half may lie past the rows that the workspace holds
+                const bool rows_in = kEpi == kEpiOut || wr.m0 < (args.M + kBM - 1) / kBM * kBM;
+                // what the row needs beside its accumulator, while the MMAs run
+                EntryCursor cur;
+                float lse2 = 0.0f, coef = 0.0f;
+                if (kEpi != kEpiOut) {
+                    wr.begin();  // the entries go where the stores' boxes are
+                    cur.fetch(args, wr.box, lane, m, wr.row_in, int(args.v0 + ncol0), int(n_end - ncol0));
                 }
-                ptx::tc_fence_after();
-                const uint32_t acc = tmem + buf * kBN + half * kCols + lanes;
-                if (c0 == k0) {
+                if (kEpi == kEpiGrad && wr.row_in) {
+                    lse2 = args.lse2[m];
+                    coef = args.coef[m] * gscale;
+                }
+                const uint32_t lanes = uint32_t(quarter * 32) << 16;
+                // The half tile's row in registers: the accumulator is free again
+                // before any of the work on it.  (An empty share of K: zeros.)
+                float r[2][2][32];
+                if (k0 >= k1) {
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) tmem_ld_f32_x32(acc + c * 32, r[c / 2][c % 2]);
-                    ptx::tmem_ld_wait();
-                } else if (kChunked) {
+                    for (int c = 0; c < 4; ++c)
 #pragma unroll
-                    for (int c = 0; c < 8; ++c) {
-                        uint32_t u[16];
-                        tmem_ld_32x32b_x16(acc + c * 16, u);
-                        ptx::tmem_ld_wait();
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) r[c / 4][c / 2 % 2][c % 2 * 16 + j] += __uint_as_float(u[j]);
+                        for (int j = 0; j < 32; ++j) r[c / 2][c % 2][j] = 0.0f;
+                }
+                for (int c0 = k0; c0 < k1; c0 = chunk_end(c0, k1)) {
+                    const uint32_t buf = C::kAccs == 1 ? it & 1 : h, filled = (C::kAccs == 1 ? it >> 1 : it) & 1;
+                    if (!__all_sync(0xffffffffu, ptx::mbar_wait(bar_tmem_full + 8 * buf, filled))) {
+                        alive = false;
+                        break;
                     }
+                    ptx::tc_fence_after();
+                    const uint32_t acc = tmem + buf * kBN + half * kCols + lanes;
+                    if (c0 == k0) {
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) tmem_ld_f32_x32(acc + c * 32, r[c / 2][c % 2]);
+                        ptx::tmem_ld_wait();
+                    } else if (kChunked) {
+#pragma unroll
+                        for (int c = 0; c < 8; ++c) {
+                            uint32_t u[16];
+                            tmem_ld_32x32b_x16(acc + c * 16, u);
+                            ptx::tmem_ld_wait();
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) r[c / 4][c / 2 % 2][c % 2 * 16 + j] += __uint_as_float(u[j]);
+                        }
+                    }
+                    release(buf);
+                    if (h + 1 == C::kAccs) ++it;
                 }
-                release(buf);
-            }
-            if (!alive) break;
-            if (!rows_in) continue;
-            if (kEpi != kEpiOut) cur.begin();
-            if (kEpi == kEpiLse) {
-                const float4 st = lse_tile<kBf16, 2>(args, &tmap_c, wr, cur, ncol0, n_end, k2, r);
-                args.partial[(int64_t(args.half0) + nb * 2 + half) * args.rows_pad + m] = st;
-            } else if (kEpi == kEpiGrad) {
-                grad_tile<kBf16>(args, &tmap_c, wr, cur, ncol0, k2, lse2, coef, r);
-            } else {
-                out_tile<!kBf16>(args, &tmap_c, wr, (args.sums ? split * num_m * C::kTileM : 0) + int(wr.m0), ncol0,
-                                 out_scale, r);
+                if (!alive) break;
+                if (!rows_in) continue;
+                if (kEpi != kEpiOut) cur.begin();
+                if (kEpi == kEpiLse) {
+                    const float4 st = lse_tile<kBf16, 2>(args, &tmap_c, wr, cur, ncol0, n_end, k2, r);
+                    args.partial[(int64_t(args.half0) + nb * 2 + half) * args.rows_pad + m] = st;
+                } else if (kEpi == kEpiGrad) {
+                    if (few) grad_tile<kBf16, kBf16>(args, &tmap_c, wr, cur, ncol0, k2, lse2, coef, r);
+                    else grad_tile<kBf16, false>(args, &tmap_c, wr, cur, ncol0, k2, lse2, coef, r);
+                } else {
+                    out_tile<!kBf16>(args, &tmap_c, wr, args.sums ? walk.sum_row(split, int(wr.m0)) : int(wr.m0), ncol0,
+                                     out_scale, r);
+                }
             }
         }
         if (lane == 0) ptx::bulk_wait_group0();  // this warp's stores are done

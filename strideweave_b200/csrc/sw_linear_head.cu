@@ -66,18 +66,24 @@ __global__ void teacher_flags_kernel(const int* index, const float* logits, int6
     if (lane == 0) flags[t] = any;
 }
 
-// Estimated microseconds of a contraction whose K walk is cut into s parts:
-// waves x (stages + a tile's fixed cost), and the traffic of writing and adding
-// the parts.  A stage of 128 x 256 x 64 on one SM (or of 256 x 256 x 64 on two)
-// takes 0.27 us, a tile's fill and drain about 2 us, the adding launch 3 us.
-constexpr int kMaxSplits = 64;
-__host__ __device__ inline float spread_cost(int64_t tiles, int64_t elements, int64_t K, int terms, int workers,
-                                             int s) {
-    const int64_t steps = (K + kBK - 1) / kBK;
-    if (s > 1 && (steps < 4 * s || tiles * s > 2 * workers)) return 1e30f;
-    const int64_t waves = (tiles * s + workers - 1) / workers, share = (steps + s - 1) / s;
-    float us = float(waves) * (float(share * terms) * 0.27f + 2.0f);
-    if (s > 1) us += 3.0f + float(s) * float(elements) * (8.0f / 6.0e6f);
+// Estimated microseconds of a contraction in tiles of a shape, the tiles of its
+// last, partial wave cut into s parts of the K walk: waves x (stages + a tile's
+// cost that nothing hides), and the traffic of writing and adding the parts.  A
+// K stage takes 0.27 us (kSingle: 128 x 256 on one SM, kPair2: 256 x 256 on two)
+// or 0.52 (kTall), a tile's fill and drain 2 us (kTall: 5), an adding launch 3.
+constexpr int kMaxParts = 64;       // where the tiles do not fill one wave
+constexpr int kMaxTailParts = 4;    // of the tiles after whole waves
+__host__ __device__ inline int shape_workers(int shape, int sms) { return shape == kSingle ? sms : sms / 2; }
+__host__ __device__ inline float spread_cost(int64_t M, int64_t N, int64_t K, int terms, int shape, int sms, int s) {
+    const int workers = shape_workers(shape, sms), steps = int((K + kBK - 1) / kBK);
+    const int64_t tiles = ((M + shape_rows(shape) - 1) >> (7 + shape)) * ((N + kBN - 1) / kBN);
+    const int whole = int(tiles / workers), rest = int(tiles - int64_t(whole) * workers);
+    if (s > 1 && (steps < 4 * s || rest == 0 || (whole ? s > kMaxTailParts : rest * s > 2 * workers))) return 1e30f;
+    const float stage = float(terms) * (shape == kTall ? 0.52f : 0.27f), fixed = shape == kTall ? 5.0f : 2.0f;
+    const int share = (steps + s - 1) / s;
+    float us = float(whole) * (float(steps) * stage + fixed) +
+               float((rest * s + workers - 1) / workers) * (float(share) * stage + fixed);
+    if (s > 1) us += 3.0f + float(rest) * float(s) * float(shape_rows(shape) * kBN) * (8.0f / 6.0e6f);
     return us;
 }
 
@@ -96,7 +102,7 @@ struct RowsArgs {
     float* lse2;
     HeadState* state;
     int64_t dh_rows, dh_cols, dh_k;  // the contraction of dh: rows of a launch at most, dim, columns of a piece
-    int dh_tile_m, dh_workers, terms;
+    int dh_shape, sms, terms;
 };
 
 // One CTA ranks the rows, four per thread and pass: row_map[0, count) are the
@@ -104,7 +110,7 @@ struct RowsArgs {
 __global__ void __launch_bounds__(1024) rows_kernel(const RowsArgs a) {
     __shared__ int warp_n[32];
     __shared__ int total;
-    __shared__ float cost[kMaxSplits];
+    __shared__ float cost[kMaxParts];
     pdl_enter();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     int kept = 0, bad = 0;
@@ -168,10 +174,9 @@ __global__ void __launch_bounds__(1024) rows_kernel(const RowsArgs a) {
     }
     if (a.coef && top) atomicMax(&a.state->amax[2], top);
     // the K walk's parts for dh, over the rows that turned out to count
-    if (tid < kMaxSplits) {
+    if (tid < kMaxParts) {
         const int64_t rows = min(int64_t(kept), a.dh_rows);
-        const int64_t tiles = (rows + a.dh_tile_m - 1) / a.dh_tile_m * ((a.dh_cols + kBN - 1) / kBN);
-        cost[tid] = spread_cost(tiles, rows * a.dh_cols, a.dh_k, a.terms, a.dh_workers, tid + 1);
+        cost[tid] = spread_cost(rows, a.dh_cols, a.dh_k, a.terms, a.dh_shape, a.sms, tid + 1);
     }
     bad = __syncthreads_or(bad);
     if (tid == 0) {
@@ -184,7 +189,7 @@ __global__ void __launch_bounds__(1024) rows_kernel(const RowsArgs a) {
         a.state->grad_scale =
             a.factor * (a.mean ? (a.upstream ? a.upstream[0] : 1.0f) / float(max(kept, 1)) : 1.0f);
         int best = 0;
-        for (int s = 1; s < kMaxSplits; ++s)
+        for (int s = 1; s < kMaxParts; ++s)
             if (cost[s] < cost[best] * 0.97f) best = s;
         a.state->dh_splits = best + 1;
     }
@@ -300,15 +305,17 @@ __global__ void __launch_bounds__(256) pack_rows_kernel(const void* src, int64_t
                                                         int scale_of, uint16_t* dst, int64_t ld, int64_t rows_pad) {
     pdl_enter();
     const int64_t valid = use_count ? min(rows, int64_t(state->count)) : rows;
+    const bool twice = !kF32 && use_count && state->few(0);  // the rows again for their gradients' remainders
     const float scale = kF32 ? pow2i(scale_exponent(state->amax[scale_of])) : 1.0f;
     const int64_t units = cols / 8;  // ld == cols here
     const int64_t stride = int64_t(gridDim.x) * 256;
 #pragma unroll 2
     for (int64_t u = int64_t(blockIdx.x) * 256 + threadIdx.x; u < rows_pad * units; u += stride) {
         const int64_t r = u / units, c = (u - r * units) * 8;
+        const int64_t from = twice && r >= kFewRows ? r - kFewRows : r;
         uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
-        if (r < valid) {
-            const int64_t at = (row_map ? int64_t(row_map[r]) : r) * sr + c;
+        if (from < valid) {
+            const int64_t at = (row_map ? int64_t(row_map[from]) : from) * sr + c;
             if (kF32) {
                 const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(src) + at);
                 const float4 a = p[0], b = p[1];
@@ -342,12 +349,15 @@ __global__ void pack_kernel(const void* src, int64_t rows, int64_t cols, int64_t
     __shared__ float tile[32][33];
     pdl_enter();
     const int64_t valid = use_count ? min(rows, int64_t(state->count)) : rows;
+    const bool twice = !kF32 && use_count && state->few(0);  // the rows again for their gradients' remainders
     const float scale = kF32 ? pow2i(scale_exponent(state->amax[scale_of])) : 1.0f;
     const int64_t r0 = int64_t(blockIdx.x) * 32, c0 = int64_t(blockIdx.y) * 32;
     const bool by_rows = sr == 1 && sc != 1;
     const int x = threadIdx.x & 31, y0 = threadIdx.x >> 5;
     for (int y = y0; y < 32; y += 8) {
-        const int64_t r = r0 + (by_rows ? x : y), c = c0 + (by_rows ? y : x);
+        int64_t r = r0 + (by_rows ? x : y);
+        const int64_t c = c0 + (by_rows ? y : x);
+        if (twice && r >= kFewRows) r -= kFewRows;
         float v = 0.0f;
         if (r < valid && c < cols) {
             const int64_t at = (row_map ? int64_t(row_map[r]) : r) * sr + c * sc;
@@ -474,7 +484,9 @@ template <bool kF32>
 __global__ void __launch_bounds__(256) scale_kernel(const ScaleArgs a) {
     __shared__ float factor[kScaleCols / 64];
     pdl_enter();
-    const int64_t i = blockIdx.x;
+    // the last rows first: they are the ones the contraction left in L2, and the
+    // next one starts with the first
+    const int64_t i = int64_t(gridDim.x) - 1 - blockIdx.x;
     if (i >= a.state->count - a.row0) return;
     const int64_t c0 = int64_t(blockIdx.y) * kScaleCols;
     const int64_t c1 = min(c0 + kScaleCols, a.V);
@@ -488,6 +500,8 @@ __global__ void __launch_bounds__(256) scale_kernel(const ScaleArgs a) {
     }
     __syncthreads();
     uint16_t* row = a.grad + i * a.ld_grad;
+    const bool few = !kF32 && a.state->few(a.row0);
+    uint16_t* rest = row + kFewRows * a.ld_grad;
     if (kF32) {
         const int lane = threadIdx.x & 31;
         for (int64_t b = c0 + (threadIdx.x >> 5) * 64; b < c1; b += 8 * 64) {
@@ -504,15 +518,21 @@ __global__ void __launch_bounds__(256) scale_kernel(const ScaleArgs a) {
         }
     } else {
         for (int64_t c = c0 + threadIdx.x * 8; c < c1; c += 256 * 8) {
-            uint4 v = *reinterpret_cast<const uint4*>(row + c);
+            const uint4 v = *reinterpret_cast<const uint4*>(row + c);
             const float f = factor[(c - c0) / 64];
-            uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+            const uint32_t e[4] = {v.x, v.y, v.z, v.w};
+            uint32_t hi[4], lo[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float2 e = __half22float2(*reinterpret_cast<__half2*>(&w[j]));
-                w[j] = pack2<true>(e.x * f, e.y * f);
+                float2 g = __half22float2(*reinterpret_cast<const __half2*>(&e[j]));
+                g.x *= f;
+                g.y *= f;
+                const __nv_bfloat162 h = __floats2bfloat162_rn(g.x, g.y);
+                hi[j] = *reinterpret_cast<const uint32_t*>(&h);
+                lo[j] = pack2<true>(g.x - __low2float(h), g.y - __high2float(h));
             }
-            *reinterpret_cast<uint4*>(row + c) = v;
+            *reinterpret_cast<uint4*>(row + c) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            if (few) *reinterpret_cast<uint4*>(rest + c) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }
     }
     __syncthreads();  // the entries overwrite what the loop above wrote
@@ -529,7 +549,9 @@ __global__ void __launch_bounds__(256) scale_kernel(const ScaleArgs a) {
             d[0] = __half_as_ushort(hi);
             d[64] = __half_as_ushort(__float2half_rn(g - __half2float(hi)));
         } else {
-            row[col] = __bfloat16_as_ushort(__float2bfloat16_rn(g));
+            const __nv_bfloat16 hi = __float2bfloat16_rn(g);
+            row[col] = __bfloat16_as_ushort(hi);
+            if (few) rest[col] = __bfloat16_as_ushort(__float2bfloat16_rn(g - __bfloat162float(hi)));
         }
     }
 }
@@ -537,9 +559,9 @@ __global__ void __launch_bounds__(256) scale_kernel(const ScaleArgs a) {
 // Result rows from the fp32 sums of the K walk's parts, added in order, to
 // their places; with by_count, zeros in the rows that do not count.
 struct SlotsArgs {
-    const float* sums;       // part p of row m at row p round_up(M, tile_m) + m
+    const float* sums;       // rows as Walk places them
     int64_t ld;
-    int splits, tile_m;      // splits 0: state->dh_splits
+    int splits, tile_m, workers;  // splits 0: state->dh_splits
     int64_t rows, cols;
     const HeadState* state;
     int by_count, row0;
@@ -552,22 +574,27 @@ template <bool kF32>
 __global__ void __launch_bounds__(256) sum_slots_kernel(const SlotsArgs a) {
     pdl_enter();
     const int splits = a.splits > 0 ? a.splits : a.state->dh_splits;
-    const int64_t summed = a.by_count ? min(a.rows, int64_t(max(a.state->count - a.row0, 0))) : a.rows;
-    const int64_t slot = (summed + a.tile_m - 1) / a.tile_m * a.tile_m * a.ld;
+    const int64_t summed = a.by_count ? min(a.rows, int64_t(a.state->rows(a.row0))) : a.rows;
+    const bool few = !kF32 && a.by_count && a.state->few(a.row0);  // their remainders are further rows
+    const Walk walk(few ? a.state->rows_and_rest(a.row0, true) : int(summed), int((a.cols + kBN - 1) / kBN), a.tile_m, a.workers, splits);
     const int64_t per_row = (a.cols + 3) / 4;
     for (int64_t u = int64_t(blockIdx.x) * 256 + threadIdx.x; u < a.rows * per_row; u += int64_t(gridDim.x) * 256) {
         const int64_t m = u / per_row, c = (u - m * per_row) * 4;
-        const float* p = a.sums + m * a.ld + c;  // ld is whole groups of four
+        const float* p = a.sums + c;  // ld is whole groups of four
         float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if (m < summed) {
-            s = *reinterpret_cast<const float4*>(p);
+            const int tile = walk.tile_of(int(m) / a.tile_m, int(c) / kBN);
+            const int parts = tile < walk.whole ? 1 : splits;
+            for (int rest = 0; rest <= (few ? kFewRows : 0); rest += kFewRows) {
 #pragma unroll 4
-            for (int k = 1; k < splits; ++k) {
-                const float4 v = *reinterpret_cast<const float4*>(p + k * slot);
-                s.x += v.x;
-                s.y += v.y;
-                s.z += v.z;
-                s.w += v.w;
+                for (int k = 0; k < parts; ++k) {
+                    const float4 v =
+                        *reinterpret_cast<const float4*>(p + int64_t(walk.sum_row(k, int(m) + rest)) * a.ld);
+                    s.x += v.x;
+                    s.y += v.y;
+                    s.z += v.z;
+                    s.w += v.w;
+                }
             }
         }
         const int64_t at = (a.row_map ? int64_t(a.row_map[m]) : m) * a.dst_row + c * a.dst_col;
@@ -623,36 +650,38 @@ int device_sms() {
     return sms[dev];
 }
 
-// How a contraction is spread over the SMs: tiles of one CTA or of a pair, and
-// parts of the K walk.
+// How a contraction is spread over the SMs: the tile shape and the parts of the
+// K walk.
 struct Spread {
-    bool pair;
+    int shape;
     int splits;
 };
-Spread choose_spread(int64_t M, int64_t N, int64_t K, int terms, bool may_split) {
-    const int sms = device_sms();
-    Spread best{false, 1};
+// `sum_us`: what it costs more to go through fp32 sums when nothing else asks
+// for them.
+Spread choose_spread(int64_t M, int64_t N, int64_t K, int terms, int tallest, bool may_split, float sum_us = 0.0f) {
+    Spread best{kSingle, 1};
     float best_us = 1e30f;
-    for (int pair = 1; pair >= 0; --pair) {
-        const int tile_m = pair ? 2 * kBM : kBM, workers = pair ? sms / 2 : sms;
-        const int64_t tiles = (M + tile_m - 1) / tile_m * ((N + kBN - 1) / kBN);
-        for (int s = 1; s <= (may_split ? kMaxSplits : 1); ++s) {
-            const float us = spread_cost(tiles, M * N, K, terms, workers, s);
+    for (int shape = tallest; shape >= kSingle; --shape)
+        for (int s = 1; s <= (may_split ? kMaxParts : 1); ++s) {
+            const float us = spread_cost(M, N, K, terms, shape, device_sms(), s) + (s > 1 ? sum_us : 0.0f);
             if (us < best_us * 0.97f) {
                 best_us = us;
-                best = Spread{pair != 0, s};
+                best = Spread{shape, s};
             }
         }
-    }
     return best;
 }
 
-// Rows of fp32 sums that `splits` of any row count up to M may take: one part
-// of all M, or parts of at most two tiles per worker.
-int64_t sum_rows(int64_t M, int64_t N, bool pair) {
-    const int tile_m = pair ? 2 * kBM : kBM, workers = pair ? device_sms() / 2 : device_sms();
-    const int64_t cols = (N + kBN - 1) / kBN;
-    return std::max(round_up(M, tile_m), (2 * int64_t(workers) / cols + 1) * tile_m);
+// Rows of fp32 sums that the parts of any row count up to M may take: all rows,
+// and those of the parts past the first, of at most two tiles per worker where
+// the tiles do not fill a wave, else of the row groups that the last wave
+// reaches.
+int64_t sum_rows(int64_t M, int64_t N, int shape) {
+    const int64_t cols = (N + kBN - 1) / kBN, tile_m = shape_rows(shape), all = round_up(M, tile_m);
+    const int64_t workers = shape_workers(shape, device_sms()), group = 2048 / tile_m;
+    const int64_t few = (2 * workers / cols + 1) * tile_m;
+    const int64_t tail = std::min(all, (workers / (group * cols) + 2) * group * tile_m) * (kMaxTailParts - 1);
+    return all + std::max(few, tail);
 }
 
 // Where a contraction writes through its output map: 16-bit or Float32 values,
@@ -677,13 +706,12 @@ int make_target_map(CUtensorMap* map, const Target& t) {
     return SW_OK;
 }
 
-template <bool kPair, bool kBf16, bool kAMn, bool kBMn, int kEpi>
+template <int kShape, bool kBf16, bool kAMn, bool kBMn, int kEpi>
 int launch_gemm(const Operand& a, const Operand& b, const Target& c, const GemmArgs& args, cudaStream_t stream) {
-    using Cf = Cfg<kPair>;
-    const int max_splits = args.splits > 0 ? args.splits : kMaxSplits;
-    const int64_t items =
-        int64_t((args.M + Cf::kTileM - 1) / Cf::kTileM) * ((args.N + args.tile_n - 1) / args.tile_n) * max_splits;
-    if (items == 0) return SW_OK;
+    using Cf = Cfg<kShape>;
+    constexpr bool kPair = Cf::kPair;
+    const int64_t tiles = int64_t((args.M + Cf::kTileM - 1) / Cf::kTileM) * ((args.N + args.tile_n - 1) / args.tile_n);
+    if (tiles == 0) return SW_OK;
     CUtensorMap ma, mb, mc;
     int rc = make_map(&ma, a.ptr, a.rows, a.cols, a.ld, kAMn ? kBK : kBM);
     if (rc != SW_OK) return rc;
@@ -691,12 +719,12 @@ int launch_gemm(const Operand& a, const Operand& b, const Target& c, const GemmA
     if (rc != SW_OK) return rc;
     memset(&mc, 0, sizeof(mc));
     if (c.ptr && (rc = make_target_map(&mc, c)) != SW_OK) return rc;
-    auto kernel = head_gemm_kernel<kPair, kBf16, kAMn, kBMn, kEpi>;
+    auto kernel = head_gemm_kernel<kShape, kBf16, kAMn, kBMn, kEpi>;
     SW_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cf::kSmemBytes),
                 "linear head smem");
     constexpr int kCtas = kPair ? 2 : 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(kCtas * (unsigned)std::min<int64_t>(items, device_sms() / kCtas));
+    cfg.gridDim = dim3(kCtas * (unsigned)(args.splits == 1 ? std::min<int64_t>(tiles, device_sms() / kCtas) : device_sms() / kCtas));
     cfg.blockDim = dim3(Cf::kThreads);
     cfg.dynamicSmemBytes = Cf::kSmemBytes;
     cfg.stream = stream;
@@ -714,14 +742,19 @@ int launch_gemm(const Operand& a, const Operand& b, const Target& c, const GemmA
 }
 
 template <bool kBf16, bool kAMn, bool kBMn, int kEpi>
-int gemm(const Operand& a, const Operand& b, const Target& c, GemmArgs args, bool pair, cudaStream_t stream) {
+int gemm(const Operand& a, const Operand& b, const Target& c, GemmArgs args, int shape, cudaStream_t stream) {
     args.terms = kBf16 ? 1 : 3;
     args.pa = a.plane;
     args.pb = b.plane;
     if (kEpi != kEpiOut) args.splits = 1;
-    if (kEpi != kEpiLse || pair) args.tile_n = kBN;
-    return pair ? launch_gemm<true, kBf16, kAMn, kBMn, kEpi>(a, b, c, args, stream)
-                : launch_gemm<false, kBf16, kAMn, kBMn, kEpi>(a, b, c, args, stream);
+    if (kEpi != kEpiLse || shape != kSingle) args.tile_n = kBN;
+    if (shape == kSingle) return launch_gemm<kSingle, kBf16, kAMn, kBMn, kEpi>(a, b, c, args, stream);
+    // results summed in registers (Float32, and the statistics) have no tall tile,
+    // and the logits' gradient has too much to do after a tile (4096 x 32000, dim
+    // 1024 / 2048 / 4096: 242 / 395 / 719 us against 201 / 362 / 695)
+    constexpr int kTallest = kBf16 && kEpi == kEpiOut ? kTall : kPair2;
+    return shape == kTall ? launch_gemm<kTallest, kBf16, kAMn, kBMn, kEpi>(a, b, c, args, stream)
+                          : launch_gemm<kPair2, kBf16, kAMn, kBMn, kEpi>(a, b, c, args, stream);
 }
 
 struct Bump {
@@ -786,7 +819,7 @@ struct Shape {
     bool keep;
     int64_t rows, piece;
     int tile_n;              // columns of a logits tile
-    bool logits_pair, dh_pair;
+    int logits_shape, dh_shape;
     Spread dw;
     // rows of fp32 sums of each gradient (0: it is written at once); dh's rows
     // are always put in place from sums, whose parts are chosen on the device
@@ -848,8 +881,8 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
     ra.dh_rows = s.rows;
     ra.dh_cols = s.D;
     ra.dh_k = std::min(s.piece, s.V);
-    ra.dh_tile_m = s.dh_pair ? 2 * kBM : kBM;
-    ra.dh_workers = s.dh_pair ? device_sms() / 2 : device_sms();
+    ra.dh_shape = s.dh_shape;
+    ra.sms = device_sms();
     ra.terms = terms;
     SW_CUDA_TRY(launch_pdl(rows_kernel, dim3(1), dim3(1024), 0, stream, ra), "linear head rows");
     if (!c.targets)
@@ -980,14 +1013,15 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
         const Operand gr{l.grad, s.rows, kF32 ? 2 * round_up(nv, 64) : nv, ld_grad, gp};
         GemmArgs a = g;
         a.row0 = (int)r0;
-        auto finish = [&](float* sums, int splits, bool pair, int64_t rows, bool by_count, const int* row_map,
+        auto finish = [&](float* sums, int splits, int shape, int64_t rows, bool by_count, const int* row_map,
                           void* dst, int64_t dst_row, int64_t dst_col) -> int {
             SlotsArgs sa;
             memset(&sa, 0, sizeof(sa));
             sa.sums = sums;
             sa.ld = s.ld_acc;
             sa.splits = splits;
-            sa.tile_m = pair ? 2 * kBM : kBM;
+            sa.tile_m = shape_rows(shape);
+            sa.workers = shape_workers(shape, device_sms());
             sa.rows = rows;
             sa.cols = s.D;
             sa.state = l.state;
@@ -1015,9 +1049,9 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
             a.sums = 1;
             a.first = first_v;
             const Target out{l.dh_sums, s.dh_sum_rows, s.ld_acc, s.ld_acc, true};
-            int rc = gemm<kBf16, false, true, kEpiOut>(gr, w, out, a, s.dh_pair, stream);
+            int rc = gemm<kBf16, false, true, kEpiOut>(gr, w, out, a, s.dh_shape, stream);
             if (rc == SW_OK && last_v)
-                rc = finish(l.dh_sums, 0, s.dh_pair, n, true, l.row_map + r0, c.dh, p.dh_row, p.dh_col);
+                rc = finish(l.dh_sums, 0, s.dh_shape, n, true, l.row_map + r0, c.dh, p.dh_row, p.dh_col);
             if (rc != SW_OK) return rc;
         }
         if (c.dw) {
@@ -1034,9 +1068,9 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
             const Target out = a.sums ? Target{l.dw_sums, s.dw_sum_rows, s.ld_acc, s.ld_acc, true}
                                       : Target{dst, nv, s.D, p.dw_row, kF32};
             int rc = gemm<kBf16, true, true, kEpiOut>(gr, states(r0, round_up(std::max<int64_t>(n, 1), kBM)), out, a,
-                                                      s.dw.pair, stream);
+                                                      s.dw.shape, stream);
             if (rc == SW_OK && a.sums && last_r)
-                rc = finish(l.dw_sums, s.dw.splits, s.dw.pair, nv, false, nullptr, dst, p.dw_row, p.dw_col);
+                rc = finish(l.dw_sums, s.dw.splits, s.dw.shape, nv, false, nullptr, dst, p.dw_row, p.dw_col);
             if (rc != SW_OK) return rc;
         }
         return SW_OK;
@@ -1056,7 +1090,7 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
             a.keep = 1;
             a.ent_s = l.ent_s + r0 * g.ent_k;
             rc = gemm<kBf16, false, false, kEpiLse>(states(r0, round_up(std::max<int64_t>(n, 1), kBM)), w, grad_out, a,
-                                                    s.logits_pair, stream);
+                                                    s.logits_shape, stream);
             if (rc != SW_OK) return rc;
             if ((rc = merge(r0, n)) != SW_OK) return rc;
             ScaleArgs sc;
@@ -1090,7 +1124,7 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
             const int64_t n = std::min(step, s.V - v0);
             Operand w;
             if ((rc = weights(v0, n, &w)) != SW_OK) return rc;
-            rc = gemm<kBf16, false, false, kEpiLse>(states(0, s.rows_pad), w, none, logits(0, s.T, v0, n), s.logits_pair,
+            rc = gemm<kBf16, false, false, kEpiLse>(states(0, s.rows_pad), w, none, logits(0, s.T, v0, n), s.logits_shape,
                                                     stream);
             if (rc != SW_OK) return rc;
         }
@@ -1103,7 +1137,7 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
         Operand w;
         if ((rc = weights(v0, n, &w)) != SW_OK) return rc;
         rc = gemm<kBf16, false, false, kEpiGrad>(states(0, s.rows_pad), w, grad_out, logits(0, s.T, v0, n),
-                                                 s.logits_pair, stream);
+                                                 s.logits_shape, stream);
         if (rc != SW_OK) return rc;
         if ((rc = gradients(0, s.T, v0, n, w, v0 == 0, v0 + n == s.V, true, true)) != SW_OK) return rc;
     }
@@ -1203,9 +1237,10 @@ int check_and_run(const char* name, Call& c, void* stream_ptr) {
         const int64_t per_column = (grads ? s.planes * s.rows_pad * 2 : 0) + (s.pack_w ? s.planes * s.ld_w * 2 : 0);
         if (per_column > 0) s.piece = std::min(s.piece, std::max<int64_t>(budget / per_column / 256 * 256, 256));
     }
-    s.logits_pair = choose_spread(std::min(s.rows, T), std::min(s.piece, V), D, terms, false).pair;
+    const int tallest = s.f32 ? kPair2 : kTall;
+    s.logits_shape = choose_spread(std::min(s.rows, T), std::min(s.piece, V), D, terms, kPair2, false).shape;
     s.tile_n = kBN;
-    if (!s.logits_pair && c.loss && (s.piece >= V || !s.pack_w)) {
+    if (s.logits_shape == kSingle && c.loss && (s.piece >= V || !s.pack_w)) {
         // few rows: a tile as narrow as fills the last wave (whole 64-column
         // blocks where the exponentials are kept, else whole MMA widths)
         const int q = s.keep ? 64 : 16, sms = device_sms();
@@ -1220,23 +1255,24 @@ int check_and_run(const char* name, Call& c, void* stream_ptr) {
         }
     }
     s.half_tiles = (V + s.tile_n - 1) / s.tile_n * 2;
-    s.dh_pair = false;
-    s.dw = Spread{false, 1};
+    s.dh_shape = kSingle;
+    s.dw = Spread{kSingle, 1};
     s.dh_sum_rows = s.dw_sum_rows = 0;
     if (c.dh && T > 0) {
         const int64_t n = std::min(s.rows, T), nv = std::min(s.piece, V);
-        s.dh_pair = choose_spread(n, D, nv, terms, true).pair;
-        s.dh_sum_rows = sum_rows(n, D, s.dh_pair);
+        s.dh_shape = choose_spread(n, D, nv, terms, tallest, true).shape;
+        s.dh_sum_rows = sum_rows(n, D, s.dh_shape);
     }
     if (c.dw) {
         const int64_t n = std::min(s.rows, T), nv = std::min(s.piece, V);
-        s.dw = choose_spread(nv, D, n, terms, true);
         // written at once through TMA where that can describe dw (rows that end
         // inside 16 bytes would be written past their end)
         const int64_t es = s.f32 ? 4 : 2;
         const bool direct = p->dw_col == 1 && p->dw_row * es % 16 == 0 && D * es % 16 == 0 && p->dw_row >= D &&
-                            (reinterpret_cast<uintptr_t>(c.dw) & 15) == 0;
-        if (!direct || s.dw.splits > 1 || s.rows < T) s.dw_sum_rows = s.dw.splits * round_up(nv, s.dw.pair ? 2 * kBM : kBM);
+                            (reinterpret_cast<uintptr_t>(c.dw) & 15) == 0 && s.rows >= T;
+        s.dw = choose_spread(nv, D, n, terms, tallest, true,
+                             direct ? float(nv) * float(D) * float(8 + es) / 6.0e6f : 0.0f);
+        if (!direct || s.dw.splits > 1) s.dw_sum_rows = sum_rows(nv, D, s.dw.shape);
     }
 
     Bump measure{nullptr, 0};
