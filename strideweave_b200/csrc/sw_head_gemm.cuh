@@ -97,14 +97,14 @@ struct Walk {
     __host__ __device__ static int min_(int a, int b) { return a < b ? a : b; }
 };
 
-// What the preparation kernels leave for the contractions.
+// What the preparation kernel leaves for the others.
 struct HeadState {
     int count;               // rows that count (compact rows)
     int bad;                 // a target outside the vocabulary was seen
     uint32_t amax[3];        // largest finite |h|, |w|, |row factor| as float bits (Float32 only)
     float grad_scale;        // common factor of every row's gradient, applied to dh and dw in fp32
     int dh_splits;           // parts of the K walk of dh, chosen for the rows that count
-    int pad;
+    int done;                // rows whose loss is written
 
     // Rows that count from row0 on, and whether they have remainder rows (bf16).
     __device__ __forceinline__ int rows(int row0) const { return max(count - row0, 0); }
@@ -144,18 +144,17 @@ struct GemmArgs {
     int terms;               // plane pairs walked: 1, or 3 for Float32
     Plane pa, pb;            // where each operand's lo plane and 64-element blocks lie
     int splits;              // parts of the last wave's tiles (0: state->dh_splits)
-    int tile_n;              // columns of a tile: kBN, or fewer for logits of one CTA (a multiple of 16)
     int scale_a, scale_b;    // indexes into HeadState::amax of the operands' scales (-1: none)
     // logits epilogues
     float logit_scale;
     int64_t v0;              // first vocabulary column of this piece
-    int half0;               // its first row of `partial`
     const int* ent_idx;      // [rows][ent_k] target columns, ascending
     const float* ent_p;      // their probabilities (null: 1)
     const uint16_t* offs;    // [tile][rows_pad] first entry of each kEntryTile columns (null: one entry a row)
     int ent_k;
     int rows_pad;
-    float4* partial;         // kEpiLse: [half tile][rows_pad] (max, sum, target term, -) in base-2 units
+    float4* partial;         // kEpiLse: [rows_pad][half_tiles] (max, sum, target term, -) in base-2 units
+    int half_tiles;          // 128-column halves of the vocabulary's tiles
     float* ent_s;            // kEpiLse: base-2 logit of every target entry (null: not kept)
     int keep;                // kEpiLse: write exp2(logit - half tile's max) where the logits' gradient will be
     const float* lse2;       // kEpiGrad: per compact row
@@ -620,7 +619,6 @@ __global__ void __launch_bounds__(320, 1)
                      const __grid_constant__ CUtensorMap tmap_c, const GemmArgs args) {
     using C = Cfg<kShape>;
     constexpr bool kPair = C::kPair;
-    constexpr bool kNarrow = !kPair && kEpi == kEpiLse;  // tiles may have fewer than kBN columns
     constexpr bool kChunked = !kBf16 || kEpi == kEpiLse;
     static_assert(C::kAccs == 1 || !kChunked, "the tall tile has no accumulator to alternate with");
     // K stages between two register sums: 512 elements; 1024 in bf16, whose logits need 1e-6
@@ -672,8 +670,7 @@ __global__ void __launch_bounds__(320, 1)
     else if (kEpi == kEpiOut) rows += kFewRows;
     const int M = args.count_is == kCountM ? rows : args.M;
     const int K = args.count_is == kCountK ? rows : args.K;
-    const int tile_n = kNarrow ? args.tile_n : kBN;
-    const Walk walk(M, (args.N + tile_n - 1) / tile_n, C::kTileM, workers,
+    const Walk walk(M, (args.N + kBN - 1) / kBN, C::kTileM, workers,
                     args.splits > 0 ? args.splits : args.state->dh_splits);
     const int num_items = walk.items();
     const int k_steps = (K + kBK - 1) / kBK;
@@ -704,8 +701,8 @@ __global__ void __launch_bounds__(320, 1)
             for (int t = worker; t < num_items && alive; t += workers) {
                 int mb, nb, split, k0, k1;
                 item(t, mb, nb, split, k0, k1);
-                const int a0 = mb * C::kTileM + rank * kBM, b0 = nb * tile_n + rank * C::kBRows;
-                const uint32_t bytes = kNarrow ? C::kABytes + tile_n * kBK * 2 : (kPair ? 2 : 1) * C::kStageBytes;
+                const int a0 = mb * C::kTileM + rank * kBM, b0 = nb * kBN + rank * C::kBRows;
+                constexpr uint32_t bytes = (kPair ? 2 : 1) * C::kStageBytes;
                 for (int c0 = k0; c0 < k1 && alive; c0 = chunk_end(c0, k1))
                     for (int term = 0; term < args.terms && alive; ++term) {
                         // plane pairs, the small products first: (hi, lo), (lo, hi), (hi, hi)
@@ -759,7 +756,7 @@ __global__ void __launch_bounds__(320, 1)
     } else if (warp == 1) {
         if (lane == 0 && rank == 0) {
             // ---------------- MMA issuer ----------------
-            const uint32_t idesc = idesc_f16(kBf16, kAMn, kBMn, C::kAccRows, tile_n);
+            const uint32_t idesc = idesc_f16(kBf16, kAMn, kBMn, C::kAccRows, kBN);
             int stage = 0;
             uint32_t phase = 0, it = 0;
             bool alive = true;
@@ -844,8 +841,8 @@ __global__ void __launch_bounds__(320, 1)
     wr.m0 = int64_t(mb) * C::kTileM + h * C::kAccRows + rank * kBM + quarter * 32;
                 const int64_t m = wr.m0 + lane;
                 wr.row_in = m < M;
-                const int64_t ncol0 = int64_t(nb) * tile_n + half * kCols;
-                const int64_t n_end = min(int64_t(args.N), int64_t(nb + 1) * tile_n);
+                const int64_t ncol0 = int64_t(nb) * kBN + half * kCols;
+                const int64_t n_end = min(int64_t(args.N), ncol0 + kCols);
                 // a pair's second half may lie past the rows that the workspace holds
                 const bool rows_in = kEpi == kEpiOut || wr.m0 < (args.M + kBM - 1) / kBM * kBM;
                 // what the row needs beside its accumulator, while the MMAs run
@@ -899,7 +896,7 @@ __global__ void __launch_bounds__(320, 1)
                 if (kEpi != kEpiOut) cur.begin();
                 if (kEpi == kEpiLse) {
                     const float4 st = lse_tile<kBf16, 2>(args, &tmap_c, wr, cur, ncol0, n_end, k2, r);
-                    args.partial[(int64_t(args.half0) + nb * 2 + half) * args.rows_pad + m] = st;
+                    args.partial[m * args.half_tiles + (args.v0 + ncol0) / kCols] = st;
                 } else if (kEpi == kEpiGrad) {
                     if (few) grad_tile<kBf16, kBf16>(args, &tmap_c, wr, cur, ncol0, k2, lse2, coef, r);
                     else grad_tile<kBf16, false>(args, &tmap_c, wr, cur, ncol0, k2, lse2, coef, r);

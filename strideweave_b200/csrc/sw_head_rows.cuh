@@ -1,0 +1,699 @@
+// sw_head_rows.cuh - what surrounds the contractions of the linear head's
+// losses (sw_linear_head.cu): the rows that count and their targets, the
+// operands' 16-bit planes, the loss from the tiles' statistics, the logits'
+// gradient from the kept exponentials, and the gradients' places.
+#pragma once
+
+#include "sw_head_gemm.cuh"
+
+namespace sw {
+namespace head {
+
+constexpr int kMaxTeacher = SW_MAX_TEACHER;
+
+__device__ __forceinline__ float warp_max(float v) {
+    for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+__device__ __forceinline__ float warp_sum(float v) {
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+__device__ __forceinline__ int warp_sum_int(int v) {
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+__device__ __forceinline__ bool entry_counts(int index, float logit, int64_t V) {
+    return index >= 0 && index < V && logit != -INFINITY;
+}
+
+// Estimated microseconds of a contraction in tiles of a shape, the tiles of its
+// last, partial wave cut into s parts of the K walk: waves x (stages + a tile's
+// cost that nothing hides), and the traffic of writing and adding the parts.  A
+// K stage takes 0.27 us (kSingle: 128 x 256 on one SM, kPair2: 256 x 256 on two)
+// or 0.52 (kTall), a tile's fill and drain 2 us (kTall: 5), an adding launch 3.
+constexpr int kMaxParts = 64;       // where the tiles do not fill one wave
+constexpr int kMaxTailParts = 4;    // of the tiles after whole waves
+__host__ __device__ inline int shape_workers(int shape, int sms) { return shape == kSingle ? sms : sms / 2; }
+__host__ __device__ inline float spread_cost(int64_t M, int64_t N, int64_t K, int terms, int shape, int sms, int s) {
+    const int workers = shape_workers(shape, sms), steps = int((K + kBK - 1) / kBK);
+    const int64_t tiles = ((M + shape_rows(shape) - 1) >> (7 + shape)) * ((N + kBN - 1) / kBN);
+    const int whole = int(tiles / workers), rest = int(tiles - int64_t(whole) * workers);
+    if (s > 1 && (steps < 4 * s || rest == 0 || (whole ? s > kMaxTailParts : rest * s > 2 * workers))) return 1e30f;
+    const float stage = float(terms) * (shape == kTall ? 0.52f : 0.27f), fixed = shape == kTall ? 5.0f : 2.0f;
+    const int share = (steps + s - 1) / s;
+    float us = float(whole) * (float(steps) * stage + fixed) +
+               float((rest * s + workers - 1) / workers) * (float(share) * stage + fixed);
+    if (s > 1) us += 3.0f + float(rest) * float(s) * float(shape_rows(shape) * kBN) * (8.0f / 6.0e6f);
+    return us;
+}
+
+// ---- preparation ---------------------------------------------------------------
+
+// flags[t] = 1 when the teacher's row has an entry (a warp per row).
+__device__ __forceinline__ bool teacher_row_counts(const int* index, const float* logits, int64_t t, int K, int64_t V,
+                                                   int lane) {
+    bool any = false;
+    for (int k = lane; k < K; k += 32) {
+        const int i = index[t * K + k];
+        if (i >= V) report_device_error(SW_ERR_INVALID);
+        any |= entry_counts(i, logits[t * K + k], V);
+    }
+    return __any_sync(0xffffffffu, any);
+}
+__global__ void __launch_bounds__(256) teacher_flags_kernel(const int* index, const float* logits, int64_t T, int K,
+                                                            int64_t V, uint8_t* flags) {
+    pdl_enter();
+    const int64_t t = int64_t(blockIdx.x) * 8 + threadIdx.x / 32;
+    if (t >= T) return;
+    const bool any = teacher_row_counts(index, logits, t, K, V, threadIdx.x & 31);
+    if ((threadIdx.x & 31) == 0) flags[t] = any;
+}
+
+struct PrepareArgs {
+    const int* targets;      // cross entropy, or null
+    int ignore_index;
+    const int* index;        // distillation
+    const float* logits;
+    const uint8_t* flags;    // null: every CTA looks at the teacher's rows itself
+    int top_k;
+    float inv_tau;
+    int64_t T, V;
+    int rows_pad, entry_tiles;
+    const float* upstream;   // null: 1
+    int mean;
+    float factor;            // c f
+    const float* lse;        // a kept lse to start from, or null
+    int* row_map;            // compact rows, then the rows that do not count
+    int* ent_idx;
+    float* ent_p;
+    float* entropy;
+    uint16_t* offs;
+    float* coef;             // null: no gradients
+    float* lse2;
+    HeadState* state;
+    // the contraction of dh: rows of a launch at most, dim, columns of a piece
+    int64_t dh_rows, dh_cols, dh_k;
+    int dh_shape, sms, terms;
+    // bf16 states, gathered here (null: Float32, split later by split_kernel)
+    const uint16_t* h;
+    int64_t D, sr, sc;
+    int vec;                 // rows are whole aligned 16-byte units
+    uint16_t* hc;
+    int64_t ld;
+};
+constexpr int kInlineFlags = 8192;  // teacher entries up to which every CTA looks at all of them
+
+// One teacher row, by a warp: its probabilities and its entries in ascending
+// column order, the sum of p log p, and the first entry of every kEntryTile
+// columns.
+__device__ __forceinline__ void sort_teacher_row(const PrepareArgs& a, int64_t t, int i, int lane, int* cols,
+                                                 int* sorted) {
+    const int K = a.top_k;
+    float top = -INFINITY;
+    int n = 0;
+    for (int k = lane; k < K; k += 32) {
+        const int col = a.index[t * K + k];
+        const float x = a.logits[t * K + k];
+        const bool ok = entry_counts(col, x, a.V);
+        cols[k] = ok ? col : INT_MAX;
+        if (ok) {
+            top = fmaxf(top, x * a.inv_tau);
+            ++n;
+        }
+    }
+    top = warp_max(top);
+    n = warp_sum_int(n);
+    __syncwarp();
+    float sum = 0.0f;
+    for (int k = lane; k < K; k += 32)
+        if (cols[k] != INT_MAX) sum += expf(a.logits[t * K + k] * a.inv_tau - top);
+    sum = warp_sum(sum);
+    const float log_sum = logf(sum);
+    float ent = 0.0f;
+    for (int k = lane; k < K; k += 32) {
+        const int col = cols[k];
+        int rank = 0;
+#pragma unroll 8
+        for (int j = 0; j < K; ++j) rank += (cols[j] < col) || (cols[j] == col && j < k);
+        float p = 0.0f;
+        if (col != INT_MAX) {
+            const float x = a.logits[t * K + k] * a.inv_tau - top;
+            p = expf(x) / sum;
+            if (p > 0.0f || p != p) ent += p * (x - log_sum);
+        }
+        sorted[rank] = col;
+        a.ent_idx[int64_t(i) * K + rank] = col;
+        a.ent_p[int64_t(i) * K + rank] = p;
+    }
+    ent = warp_sum(ent);
+    if (lane == 0) a.entropy[i] = ent;
+    __syncwarp();
+    for (int tile = lane; tile <= a.entry_tiles; tile += 32) {
+        const int64_t col0 = int64_t(tile) * kEntryTile;
+        int lo = 0, hi = n;  // entries [0, n) are the real ones
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (sorted[mid] < col0) lo = mid + 1;
+            else hi = mid;
+        }
+        a.offs[int64_t(tile) * a.rows_pad + i] = uint16_t(lo);
+    }
+}
+
+// kRows rows per CTA.  Each CTA counts the rows before its own and all rows
+// that count (T flags from L2: with 8 rows a CTA 33 MB in all at T = 8192), so
+// nothing waits for anything: row_map[0, count) are the rows that count, in
+// order, row_map[count, T) the others.  It then leaves what its rows need: the
+// target entries, the factor of their gradient, and in bf16 the states
+// themselves, gathered; the places of rows that do not count are zeros.
+template <int kRows>
+__global__ void __launch_bounds__(256) prepare_kernel(const PrepareArgs a) {
+    constexpr int kCols = 256;
+    __shared__ uint8_t s_flags[kInlineFlags];
+    __shared__ int s_before[8], s_total[8], s_bad[8];
+    __shared__ int s_dest[kRows];     // compact row, or the place of a row that does not count
+    __shared__ uint8_t s_keep[kRows];
+    __shared__ __align__(16) int s_sort[8][2 * kMaxTeacher];
+    __shared__ __align__(16) uint16_t s_tile[kRows][kCols + 8];
+    pdl_enter();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int64_t t0 = int64_t(blockIdx.x) * kRows;
+    const bool inline_flags = !a.targets && !a.flags;
+    if (inline_flags) {
+        for (int64_t t = warp; t < a.T; t += 8) {
+            const bool any = teacher_row_counts(a.index, a.logits, t, a.top_k, a.V, lane);
+            if (lane == 0) s_flags[t] = any;
+        }
+        __syncthreads();
+    }
+    int before = 0, total = 0, bad = 0;
+    auto counts = [&](int64_t t) {
+        if (!a.targets) return inline_flags ? s_flags[t] != 0 : a.flags[t] != 0;
+        const int y = a.targets[t];
+        if (y == a.ignore_index) return false;
+        const bool ok = y >= 0 && y < a.V;
+        if (!ok) bad = 1;
+        return ok;
+    };
+#pragma unroll 4
+    for (int64_t t = tid; t < a.T; t += 256) {
+        const int k = counts(t);
+        total += k;
+        if (t < t0) before += k;
+    }
+    before = warp_sum_int(before);
+    total = warp_sum_int(total);
+    bad = __any_sync(0xffffffffu, bad);
+    if (lane == 0) {
+        s_before[warp] = before;
+        s_total[warp] = total;
+        s_bad[warp] = bad;
+    }
+    __syncthreads();
+    before = total = bad = 0;
+    for (int w = 0; w < 8; ++w) {
+        before += s_before[w];
+        total += s_total[w];
+        bad |= s_bad[w];
+    }
+    if (warp == 0) {
+        const int64_t t = t0 + lane;
+        const bool mine = lane < kRows && t < a.T;
+        const bool keep = mine && counts(t);
+        const uint32_t votes = __ballot_sync(0xffffffffu, keep);
+        const int rank = before + __popc(votes & ((1u << lane) - 1));
+        if (lane < kRows) {
+            const int64_t dest = keep ? rank : mine ? a.T - 1 - (t - rank) : t;
+            s_dest[lane] = dest < a.rows_pad ? int(dest) : -1;
+            s_keep[lane] = keep;
+            if (mine) a.row_map[dest] = int(t);
+            if (keep) {
+                if (a.targets) a.ent_idx[rank] = a.targets[t];
+                if (a.coef) a.coef[rank] = a.mean || !a.upstream ? 1.0f : a.upstream[t];
+                if (a.lse) a.lse2[rank] = a.lse[t] * kLog2e;
+            }
+        }
+    }
+    __syncthreads();
+    if (blockIdx.x == 0) {
+        uint32_t top = 0;  // of the row factors (Float32 only)
+        if (a.coef && !a.h) {
+            for (int64_t t = tid; t < a.T; t += 256)
+                if (counts(t)) {
+                    const float g = a.mean || !a.upstream ? 1.0f : a.upstream[t];
+                    if (isfinite(g)) top = max(top, __float_as_uint(fabsf(g)));
+                }
+            top = __reduce_max_sync(0xffffffffu, top);
+            if (lane == 0) s_total[warp] = int(top);
+        }
+        __syncthreads();
+        if (warp == 0) {
+            // the K walk's parts for dh, over the rows that turned out to count:
+            // the fewest whose estimate is within 3% of the least
+            int splits = 1;
+            if (a.dh_cols) {
+                const int64_t rows = min(int64_t(total), a.dh_rows);
+                const float c0 = spread_cost(rows, a.dh_cols, a.dh_k, a.terms, a.dh_shape, a.sms, lane + 1);
+                const float c1 = spread_cost(rows, a.dh_cols, a.dh_k, a.terms, a.dh_shape, a.sms, lane + 33);
+                const float least = -warp_max(-fminf(c0, c1)) * 1.03f;
+                const uint32_t first = __ballot_sync(0xffffffffu, c0 <= least);
+                splits = first ? __ffs(first) : 32 + __ffs(__ballot_sync(0xffffffffu, c1 <= least));
+            }
+            if (lane == 0) {
+                if (a.coef && !a.h)
+                    for (int w = 0; w < 8; ++w) top = max(top, uint32_t(s_total[w]));
+                HeadState s;
+                s.count = total;
+                s.bad = bad;
+                s.amax[0] = s.amax[1] = 0;
+                s.amax[2] = top;
+                // what every row's gradient is multiplied by stays out of the
+                // 16-bit logits' gradient: a target's -1 is exact there, where
+                // the common factor would round it the same way in every row
+                s.grad_scale =
+                    a.factor * (a.mean ? (a.upstream && a.coef ? a.upstream[0] : 1.0f) / float(max(total, 1)) : 1.0f);
+                s.dh_splits = splits;
+                s.done = 0;
+                *a.state = s;
+                if (bad) report_device_error(SW_ERR_INVALID);
+            }
+        }
+    }
+    if (!a.targets)
+        for (int r = warp; r < kRows; r += 8)
+            if (s_keep[r]) sort_teacher_row(a, t0 + r, s_dest[r], lane, s_sort[warp], s_sort[warp] + kMaxTeacher);
+    if (!a.h) return;
+    // states: row r of this CTA to s_dest[r], and where few rows count again to
+    // the places that go with their gradients' remainders
+    const bool few = total <= kFewRows && total > 0;
+    auto put = [&](int r, int64_t c, const uint4& v) {
+        const int d = s_dest[r];
+        if (d < 0) return;
+        const uint4 zero = make_uint4(0, 0, 0, 0);
+        if (s_keep[r]) {
+            *reinterpret_cast<uint4*>(a.hc + d * a.ld + c) = v;
+            if (few) *reinterpret_cast<uint4*>(a.hc + (d + kFewRows) * a.ld + c) = v;
+        } else if (!few || d < kFewRows || d >= kFewRows + total) {
+            *reinterpret_cast<uint4*>(a.hc + d * a.ld + c) = zero;
+        }
+    };
+    if (a.vec) {
+        const int units = int(a.ld / 8);
+        for (int u = tid; u < kRows * units; u += 256) {
+            const int r = u / units, c = (u - r * units) * 8;
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (s_keep[r]) v = *reinterpret_cast<const uint4*>(a.h + (t0 + r) * a.sr + c);
+            put(r, c, v);
+        }
+        return;
+    }
+    const bool by_rows = a.sr == 1 && a.sc != 1;  // walk the unit stride fastest
+    for (int64_t c0 = 0; c0 < a.ld; c0 += kCols) {
+        for (int u = tid; u < kRows * kCols; u += 256) {
+            const int r = by_rows ? u % kRows : u / kCols, c = by_rows ? u / kRows : u % kCols;
+            s_tile[r][c] = s_keep[r] && c0 + c < a.D ? a.h[(t0 + r) * a.sr + (c0 + c) * a.sc] : uint16_t(0);
+        }
+        __syncthreads();
+        for (int u = tid; u < kRows * (kCols / 8); u += 256) {
+            const int r = u / (kCols / 8), c = u % (kCols / 8) * 8;
+            if (c0 + c < a.ld) put(r, c0 + c, *reinterpret_cast<const uint4*>(&s_tile[r][c]));
+        }
+        __syncthreads();
+    }
+}
+
+// ---- 16-bit planes of Float32 operands, and of bf16 weights TMA cannot read ------
+
+struct SplitJob {
+    const void* src;
+    int64_t rows, cols, sr, sc;
+    int vec;                 // rows are whole aligned 16-byte units (Float32: pairs of them)
+    const int* row_map;      // null: all rows; else the compact ones, as many as count
+    int scale_of;            // index of its magnitude in HeadState::amax
+    uint16_t* dst;
+    int64_t ld, rows_pad;
+    unsigned ctas;           // the first CTAs of the grid belong to the first job
+};
+
+// Largest finite magnitudes of one or two matrices: a warp per row, or per
+// column where columns are contiguous.
+__global__ void __launch_bounds__(256) amax_kernel(const SplitJob j0, const SplitJob j1, HeadState* state) {
+    pdl_enter();
+    const bool second = blockIdx.x >= j0.ctas;
+    const SplitJob& j = second ? j1 : j0;
+    const float* x = static_cast<const float*>(j.src);
+    const int64_t rows = j.row_map ? state->count : j.rows;
+    const bool by_rows = j.sr == 1 && j.sc != 1;  // walk the unit stride fastest
+    const int64_t outer = by_rows ? j.cols : rows, inner = by_rows ? rows : j.cols;
+    const int64_t so = by_rows ? j.sc : j.sr, si = by_rows ? j.sr : j.sc;
+    const int lane = threadIdx.x & 31;
+    const int64_t first = int64_t(blockIdx.x - (second ? j0.ctas : 0)) * 8 + (threadIdx.x >> 5);
+    uint32_t top = 0;
+    auto take = [&](float v) {
+        v = fabsf(v);
+        if (v <= 3.402823466e38f) top = max(top, __float_as_uint(v));
+    };
+    for (int64_t o = first; o < outer; o += int64_t(j.ctas) * 8) {
+        const float* p = x + (by_rows ? o : j.row_map ? int64_t(j.row_map[o]) : o) * so;
+        if (j.vec) {
+#pragma unroll 4
+            for (int64_t i = lane * 4; i < inner; i += 128) {
+                const float4 v = *reinterpret_cast<const float4*>(p + i);
+                take(v.x);
+                take(v.y);
+                take(v.z);
+                take(v.w);
+            }
+        } else {
+#pragma unroll 4
+            for (int64_t i = lane; i < inner; i += 32) take(p[(by_rows && j.row_map ? int64_t(j.row_map[i]) : i) * si]);
+        }
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (lane == 0 && top) atomicMax(&state->amax[j.scale_of], top);
+}
+
+// One or two matrices into operands [rows_pad][ld]: a copy of bf16 values, or
+// two f16 planes of a Float32 value times 2^q (hi rounded to nearest, lo the
+// rest).  Rows past the ones that count are zero.
+template <bool kF32>
+__global__ void __launch_bounds__(256) split_kernel(const SplitJob j0, const SplitJob j1, const HeadState* state) {
+    __shared__ float tile[32][33];
+    pdl_enter();
+    const bool second = blockIdx.x >= j0.ctas;
+    const SplitJob& j = second ? j1 : j0;
+    const int64_t cta = blockIdx.x - (second ? j0.ctas : 0);
+    const int64_t valid = j.row_map ? min(j.rows, int64_t(state->count)) : j.rows;
+    const float scale = kF32 ? pow2i(scale_exponent(state->amax[j.scale_of])) : 1.0f;
+    if (j.vec) {
+        const int64_t units = j.cols / 8;  // ld == cols here
+#pragma unroll 2
+        for (int64_t u = cta * 256 + threadIdx.x; u < j.rows_pad * units; u += int64_t(j.ctas) * 256) {
+            const int64_t r = u / units, c = (u - r * units) * 8;
+            uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
+            if (r < valid) {
+                const int64_t at = (j.row_map ? int64_t(j.row_map[r]) : r) * j.sr + c;
+                if (kF32) {
+                    const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(j.src) + at);
+                    const float4 a = p[0], b = p[1];
+                    const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+                    uint32_t h[4], l[4];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const float x = v[2 * q] * scale, y = v[2 * q + 1] * scale;
+                        const __half2 b2 = __floats2half2_rn(x, y);
+                        h[q] = *reinterpret_cast<const uint32_t*>(&b2);
+                        l[q] = pack2<false>(x - __low2float(b2), y - __high2float(b2));
+                    }
+                    hi = make_uint4(h[0], h[1], h[2], h[3]);
+                    lo = make_uint4(l[0], l[1], l[2], l[3]);
+                } else {
+                    hi = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(j.src) + at);
+                }
+            }
+            *reinterpret_cast<uint4*>(j.dst + r * j.ld + c) = hi;
+            if (kF32) *reinterpret_cast<uint4*>(j.dst + (j.rows_pad + r) * j.ld + c) = lo;
+        }
+        return;
+    }
+    // 32 x 32 tiles through shared memory, read along the unit stride
+    const bool by_rows = j.sr == 1 && j.sc != 1;
+    const int x = threadIdx.x & 31, y0 = threadIdx.x >> 5;
+    const int64_t tiles_c = (j.ld + 31) / 32, tiles = (j.rows_pad + 31) / 32 * tiles_c;
+    for (int64_t t = cta; t < tiles; t += j.ctas) {
+        const int64_t r0 = t / tiles_c * 32, c0 = t % tiles_c * 32;
+        for (int y = y0; y < 32; y += 8) {
+            const int64_t r = r0 + (by_rows ? x : y), c = c0 + (by_rows ? y : x);
+            float v = 0.0f;
+            if (r < valid && c < j.cols) {
+                const int64_t at = (j.row_map ? int64_t(j.row_map[r]) : r) * j.sr + c * j.sc;
+                v = kF32 ? static_cast<const float*>(j.src)[at]
+                         : __bfloat162float(static_cast<const __nv_bfloat16*>(j.src)[at]);
+            }
+            tile[by_rows ? x : y][by_rows ? y : x] = v;
+        }
+        __syncthreads();
+        for (int y = y0; y < 32; y += 8) {
+            const int64_t r = r0 + y, c = c0 + x;
+            if (r < j.rows_pad && c < j.ld) {
+                const float v = tile[y][x];
+                if (kF32) {
+                    const float s = v * scale;
+                    const __half hi = __float2half_rn(s);
+                    j.dst[r * j.ld + c] = __half_as_ushort(hi);
+                    j.dst[(j.rows_pad + r) * j.ld + c] = __half_as_ushort(__float2half_rn(s - __half2float(hi)));
+                } else {
+                    j.dst[r * j.ld + c] = __bfloat16_as_ushort(__float2bfloat16_rn(v));
+                }
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// ---- after the logits ------------------------------------------------------------
+
+struct LossArgs {
+    const float4* partial;   // [rows_pad][half_tiles]
+    int half_tiles;
+    int row0, rows;          // compact rows [row0, row0 + rows), a CTA each
+    int all_rows;            // CTAs over all launches that write a row's loss
+    HeadState* state;
+    const int* row_map;
+    const int* targets;
+    int ignore_index;
+    const float* entropy;    // distillation, or null
+    float factor;            // f
+    float* row_loss;         // compact
+    float* lse2;             // compact: for gradients that start from the logits again
+    float* loss;             // per row, or the mean; null: neither
+    int mean;
+    float* lse;              // per row, or null
+    // the logits' gradient from the kept exponentials (grad null: none)
+    uint16_t* grad;          // of row row0
+    int64_t ld_grad, V, seg; // seg: columns of a CTA
+    const float* coef;       // compact, as the entries
+    const int* ent_idx;
+    const float* ent_p;
+    const float* ent_s;
+    int ent_k;
+};
+
+// A row's statistics from its half tiles', its loss, and (grad) the gradient of
+// its logits: exp2(k2 z - ref) 2^(ref - lse2) is the softmax, in place of the
+// stored exponentials, and the target entries are written from their own
+// Float32 logits (where the softmax is near p, the stored 11 bits of it would
+// not be enough).  A thread takes 8 columns (bf16), a warp a block of 64
+// (Float32: hi and lo values replace the block they were computed from).  The
+// last row to be done adds up the mean, in a fixed order.
+template <bool kF32>
+__global__ void __launch_bounds__(256) loss_kernel(const LossArgs a) {
+    constexpr int kSub = 8192;
+    __shared__ float factor[kSub / 128];
+    __shared__ float s_ref[8], s_sum[8], s_dot[8];
+    __shared__ int s_last;
+    pdl_enter();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    // the last rows first: they are the ones the contraction left in L2, and the
+    // next one starts with the first
+    const int64_t i = int64_t(gridDim.x) - 1 - blockIdx.x;
+    const bool writes = blockIdx.y == 0;
+    const int count = a.state->rows(a.row0);
+    float lse2 = 0.0f;
+    if (i < count) {
+        const float4* part = a.partial + (a.row0 + i) * a.half_tiles;
+        float ref = -INFINITY, sum = 0.0f, dot = 0.0f;
+        auto add = [&](float r, float s, float d) {
+            const float next = fmaxf(ref, r), base = next == -INFINITY ? 0.0f : next;
+            sum = sum * ex2(ref - base) + s * ex2(r - base);
+            ref = next;
+            dot += d;
+        };
+#pragma unroll 4
+        for (int t = tid; t < a.half_tiles; t += 256) {
+            const float4 p = part[t];
+            add(p.x, p.y, p.z);
+        }
+        for (int o = 16; o; o >>= 1)
+            add(__shfl_xor_sync(0xffffffffu, ref, o), __shfl_xor_sync(0xffffffffu, sum, o),
+                __shfl_xor_sync(0xffffffffu, dot, o));
+        if (lane == 0) {
+            s_ref[warp] = ref;
+            s_sum[warp] = sum;
+            s_dot[warp] = dot;
+        }
+        __syncthreads();
+        ref = s_ref[0];
+        sum = s_sum[0];
+        dot = s_dot[0];
+        for (int w = 1; w < 8; ++w) add(s_ref[w], s_sum[w], s_dot[w]);
+        lse2 = ref + log2f(sum);
+        if (writes && tid == 0) {
+            const float v = a.factor * ((a.entropy ? a.entropy[a.row0 + i] : 0.0f) + (lse2 - dot) * kLn2);
+            const int64_t row = a.row_map[a.row0 + i];
+            a.row_loss[a.row0 + i] = v;
+            a.lse2[a.row0 + i] = lse2;
+            if (a.loss && !a.mean) a.loss[row] = v;
+            if (a.lse) a.lse[row] = lse2 * kLn2;
+        }
+    } else if (writes && tid == 0 && i < a.rows) {
+        const int64_t row = a.row_map[a.row0 + i];
+        float v = 0.0f;
+        if (a.targets && a.targets[row] != a.ignore_index) v = NAN;  // a target outside the vocabulary
+        if (a.loss && !a.mean) a.loss[row] = v;
+        if (a.lse) a.lse[row] = 0.0f;
+    }
+    if (writes && a.mean) {
+        if (tid == 0) {
+            __threadfence();
+            s_last = atomicAdd(&a.state->done, 1) == a.all_rows - 1;
+        }
+        __syncthreads();
+        if (s_last) {
+            __threadfence();
+            float s = 0.0f;
+            for (int r = tid; r < a.state->count; r += 256) s += __ldcg(a.row_loss + r);
+            s = warp_sum(s);
+            __syncthreads();
+            if (lane == 0) s_dot[warp] = s;
+            __syncthreads();
+            if (tid == 0) {
+                s = 0.0f;
+                for (int w = 0; w < 8; ++w) s += s_dot[w];
+                *a.loss = a.state->bad ? NAN : s / float(a.state->count);
+            }
+        }
+    }
+    if (!a.grad || i >= count) return;
+    const int64_t c_begin = int64_t(blockIdx.y) * a.seg, c_end = min(c_begin + a.seg, a.V);
+    const float coef = a.coef[a.row0 + i] * (kF32 ? pow2i(scale_exponent(a.state->amax[2])) : 1.0f);
+    uint16_t* row = a.grad + i * a.ld_grad;
+    const bool few = !kF32 && a.state->few(a.row0);
+    uint16_t* rest = row + kFewRows * a.ld_grad;
+    for (int64_t c0 = c_begin; c0 < c_end; c0 += kSub) {
+        const int64_t c1 = min(c0 + kSub, c_end);
+        __syncthreads();
+        for (int t = tid; t < int((c1 - c0 + 127) / 128); t += 256) {
+            const float ref = a.partial[(a.row0 + i) * a.half_tiles + c0 / 128 + t].x;
+            // (a half tile of nothing but -inf stored zeros)
+            factor[t] = ref == -INFINITY ? 0.0f : ex2(ref - lse2) * coef * (kF32 ? 1.0f : 1.0f / 32768.0f);
+        }
+        __syncthreads();
+        if (kF32) {
+#pragma unroll 2
+            for (int64_t b = c0 + warp * 64; b < c1; b += 8 * 64) {
+                float2 v = reinterpret_cast<const float2*>(row + 2 * b)[lane];
+                const float f = factor[(b - c0) / 128];
+                v.x = b + 2 * lane < a.V ? v.x * f : 0.0f;
+                v.y = b + 2 * lane + 1 < a.V ? v.y * f : 0.0f;
+                const __half2 hi = __floats2half2_rn(v.x, v.y);
+                const __half2 lo = __floats2half2_rn(v.x - __low2float(hi), v.y - __high2float(hi));
+                __syncwarp();
+                reinterpret_cast<__half2*>(row + 2 * b)[lane] = hi;
+                reinterpret_cast<__half2*>(row + 2 * b + 64)[lane] = lo;
+            }
+        } else {
+#pragma unroll 4
+            for (int64_t c = c0 + tid * 8; c < c1; c += 256 * 8) {
+                const uint4 v = *reinterpret_cast<const uint4*>(row + c);
+                const float f = factor[(c - c0) / 128];
+                const uint32_t e[4] = {v.x, v.y, v.z, v.w};
+                uint32_t hi[4], lo[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float2 g = __half22float2(*reinterpret_cast<const __half2*>(&e[j]));
+                    g.x *= f;
+                    g.y *= f;
+                    const __nv_bfloat162 h = __floats2bfloat162_rn(g.x, g.y);
+                    hi[j] = *reinterpret_cast<const uint32_t*>(&h);
+                    lo[j] = pack2<true>(g.x - __low2float(h), g.y - __high2float(h));
+                }
+                *reinterpret_cast<uint4*>(row + c) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                if (few) *reinterpret_cast<uint4*>(rest + c) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            }
+        }
+    }
+    __syncthreads();  // the entries overwrite what the loop above wrote
+    for (int k = tid; k < a.ent_k; k += 256) {
+        const int64_t at = (a.row0 + i) * a.ent_k + k;
+        const int col = a.ent_idx[at];
+        if (col < c_begin || col >= c_end || (k > 0 && a.ent_idx[at - 1] == col)) continue;
+        float p = a.ent_p ? a.ent_p[at] : 1.0f;
+        for (int j = 1; k + j < a.ent_k && a.ent_idx[at + j] == col; ++j) p += a.ent_p[at + j];
+        const float g = (ex2(a.ent_s[at] - lse2) - p) * coef;
+        if (kF32) {
+            uint16_t* d = row + (col & ~63) * int64_t(2) + (col & 63);
+            const __half hi = __float2half_rn(g);
+            d[0] = __half_as_ushort(hi);
+            d[64] = __half_as_ushort(__float2half_rn(g - __half2float(hi)));
+        } else {
+            const __nv_bfloat16 hi = __float2bfloat16_rn(g);
+            row[col] = __bfloat16_as_ushort(hi);
+            if (few) rest[col] = __bfloat16_as_ushort(__float2bfloat16_rn(g - __bfloat162float(hi)));
+        }
+    }
+}
+
+// ---- after the gradients' contractions ---------------------------------------------
+
+// Result rows from the fp32 sums of the K walk's parts, added in order, to
+// their places; with by_count, zeros in the rows that do not count.
+struct PlaceArgs {
+    const float* sums;       // rows as Walk places them
+    int64_t ld;
+    int splits, tile_m, workers;  // splits 0: state->dh_splits
+    int64_t rows, cols;
+    const HeadState* state;
+    int by_count, row0;
+    const int* row_map;
+    void* dst;
+    int64_t dst_row, dst_col;
+    int vec;                 // dst rows are contiguous and aligned to four elements
+};
+template <bool kF32>
+__global__ void __launch_bounds__(256) place_kernel(const PlaceArgs a) {
+    pdl_enter();
+    const int splits = a.splits > 0 ? a.splits : a.state->dh_splits;
+    const int64_t summed = a.by_count ? min(a.rows, int64_t(a.state->rows(a.row0))) : a.rows;
+    const bool few = !kF32 && a.by_count && a.state->few(a.row0);  // their remainders are further rows
+    const Walk walk(few ? kFewRows + int(summed) : int(summed), int((a.cols + kBN - 1) / kBN), a.tile_m, a.workers,
+                    splits);
+    const int64_t per_row = (a.cols + 3) / 4;
+    for (int64_t u = int64_t(blockIdx.x) * 256 + threadIdx.x; u < a.rows * per_row; u += int64_t(gridDim.x) * 256) {
+        const int64_t m = u / per_row, c = (u - m * per_row) * 4;
+        const float* p = a.sums + c;  // ld is whole groups of four
+        float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (m < summed) {
+            const int tile = walk.tile_of(int(m) / a.tile_m, int(c) / kBN);
+            const int parts = tile < walk.whole ? 1 : splits;
+            for (int rest = 0; rest <= (few ? kFewRows : 0); rest += kFewRows) {
+#pragma unroll 4
+                for (int k = 0; k < parts; ++k) {
+                    const float4 v =
+                        *reinterpret_cast<const float4*>(p + int64_t(walk.sum_row(k, int(m) + rest)) * a.ld);
+                    s.x += v.x;
+                    s.y += v.y;
+                    s.z += v.z;
+                    s.w += v.w;
+                }
+            }
+        }
+        const int64_t at = (a.row_map ? int64_t(a.row_map[m]) : m) * a.dst_row + c * a.dst_col;
+        const float r[4] = {s.x, s.y, s.z, s.w};
+        if (a.vec && c + 4 <= a.cols) {
+            if (kF32) *reinterpret_cast<float4*>(static_cast<float*>(a.dst) + at) = s;
+            else
+                *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.dst) + at) =
+                    make_uint2(pack2<true>(s.x, s.y), pack2<true>(s.z, s.w));
+            continue;
+        }
+        for (int j = 0; j < 4 && c + j < a.cols; ++j) {
+            if (kF32) static_cast<float*>(a.dst)[at + j * a.dst_col] = r[j];
+            else static_cast<__nv_bfloat16*>(a.dst)[at + j * a.dst_col] = __float2bfloat16_rn(r[j]);
+        }
+    }
+}
+
+}  // namespace head
+}  // namespace sw

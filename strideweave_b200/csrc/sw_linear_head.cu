@@ -24,7 +24,7 @@
 #include <cstring>
 
 #include "sw_common.cuh"
-#include "sw_head_gemm.cuh"
+#include "sw_head_rows.cuh"
 #include "sw_ptx.cuh"
 #include "sw_tma.cuh"
 
@@ -32,586 +32,9 @@ namespace sw {
 namespace head {
 namespace {
 
-constexpr int kMaxTeacher = SW_MAX_TEACHER;
+// What the pieces may take unless the plan says otherwise: the exponentials of
+// 16384 rows over a vocabulary of 131072.
 constexpr int64_t kDefaultWorkspace = int64_t(4) << 30;
-
-__device__ __forceinline__ float warp_max(float v) {
-    for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-    return v;
-}
-__device__ __forceinline__ float warp_sum(float v) {
-    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
-}
-__device__ __forceinline__ bool entry_counts(int index, float logit, int64_t V) {
-    return index >= 0 && index < V && logit != -INFINITY;
-}
-
-// ---- preparation ---------------------------------------------------------------
-
-// flags[t] = 1 when the teacher's row has an entry (a warp per row).
-__global__ void teacher_flags_kernel(const int* index, const float* logits, int64_t T, int K, int64_t V,
-                                     uint8_t* flags) {
-    pdl_enter();
-    const int64_t t = int64_t(blockIdx.x) * (blockDim.x / 32) + threadIdx.x / 32;
-    const int lane = threadIdx.x & 31;
-    if (t >= T) return;
-    bool any = false;
-    for (int k = lane; k < K; k += 32) {
-        const int i = index[t * K + k];
-        if (i >= V) report_device_error(SW_ERR_INVALID);
-        any |= entry_counts(i, logits[t * K + k], V);
-    }
-    any = __any_sync(0xffffffffu, any);
-    if (lane == 0) flags[t] = any;
-}
-
-// Estimated microseconds of a contraction in tiles of a shape, the tiles of its
-// last, partial wave cut into s parts of the K walk: waves x (stages + a tile's
-// cost that nothing hides), and the traffic of writing and adding the parts.  A
-// K stage takes 0.27 us (kSingle: 128 x 256 on one SM, kPair2: 256 x 256 on two)
-// or 0.52 (kTall), a tile's fill and drain 2 us (kTall: 5), an adding launch 3.
-constexpr int kMaxParts = 64;       // where the tiles do not fill one wave
-constexpr int kMaxTailParts = 4;    // of the tiles after whole waves
-__host__ __device__ inline int shape_workers(int shape, int sms) { return shape == kSingle ? sms : sms / 2; }
-__host__ __device__ inline float spread_cost(int64_t M, int64_t N, int64_t K, int terms, int shape, int sms, int s) {
-    const int workers = shape_workers(shape, sms), steps = int((K + kBK - 1) / kBK);
-    const int64_t tiles = ((M + shape_rows(shape) - 1) >> (7 + shape)) * ((N + kBN - 1) / kBN);
-    const int whole = int(tiles / workers), rest = int(tiles - int64_t(whole) * workers);
-    if (s > 1 && (steps < 4 * s || rest == 0 || (whole ? s > kMaxTailParts : rest * s > 2 * workers))) return 1e30f;
-    const float stage = float(terms) * (shape == kTall ? 0.52f : 0.27f), fixed = shape == kTall ? 5.0f : 2.0f;
-    const int share = (steps + s - 1) / s;
-    float us = float(whole) * (float(steps) * stage + fixed) +
-               float((rest * s + workers - 1) / workers) * (float(share) * stage + fixed);
-    if (s > 1) us += 3.0f + float(rest) * float(s) * float(shape_rows(shape) * kBN) * (8.0f / 6.0e6f);
-    return us;
-}
-
-struct RowsArgs {
-    const int* targets;      // cross entropy, or null
-    int ignore_index;
-    const uint8_t* flags;    // distillation
-    int64_t T, V;
-    const float* upstream;   // null: 1
-    int mean;
-    float factor;            // c f
-    const float* lse;        // a kept lse to start from, or null
-    int* row_map;            // compact rows, then the rows that do not count
-    int* ent_idx;            // cross entropy: the compact rows' targets
-    float* coef;
-    float* lse2;
-    HeadState* state;
-    int64_t dh_rows, dh_cols, dh_k;  // the contraction of dh: rows of a launch at most, dim, columns of a piece
-    int dh_shape, sms, terms;
-};
-
-// One CTA ranks the rows, four per thread and pass: row_map[0, count) are the
-// rows that count, in order, row_map[count, T) the others.
-__global__ void __launch_bounds__(1024) rows_kernel(const RowsArgs a) {
-    __shared__ int warp_n[32];
-    __shared__ int total;
-    __shared__ float cost[kMaxParts];
-    pdl_enter();
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    int kept = 0, bad = 0;
-    uint32_t top = 0;
-    for (int64_t base = 0; base < a.T; base += 4096) {
-        const int64_t t0 = base + tid * 4;
-        int y[4];
-        uint32_t keep = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            y[j] = 0;
-            if (t0 + j >= a.T) continue;
-            if (a.targets) {
-                y[j] = a.targets[t0 + j];
-                if (y[j] != a.ignore_index) {
-                    if (y[j] >= 0 && y[j] < a.V) keep |= 1u << j;
-                    else bad = 1;
-                }
-            } else if (a.flags[t0 + j]) {
-                keep |= 1u << j;
-            }
-        }
-        int n = __popc(keep);
-        for (int o = 1; o < 32; o <<= 1) {
-            const int up = __shfl_up_sync(0xffffffffu, n, o);
-            if (lane >= o) n += up;
-        }
-        if (lane == 31) warp_n[warp] = n;
-        __syncthreads();
-        if (warp == 0) {
-            int w = warp_n[lane];
-            for (int o = 1; o < 32; o <<= 1) {
-                const int up = __shfl_up_sync(0xffffffffu, w, o);
-                if (lane >= o) w += up;
-            }
-            warp_n[lane] = w;
-            if (lane == 31) total = w;
-        }
-        __syncthreads();
-        int before = kept + (warp ? warp_n[warp - 1] : 0) + n - __popc(keep);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int64_t t = t0 + j;
-            if (t >= a.T) continue;
-            if (keep >> j & 1) {
-                a.row_map[before] = int(t);
-                if (a.targets) a.ent_idx[before] = y[j];
-                if (a.coef) {
-                    const float g = a.mean || !a.upstream ? 1.0f : a.upstream[t];
-                    a.coef[before] = g;
-                    if (isfinite(g)) top = max(top, __float_as_uint(fabsf(g)));
-                }
-                if (a.lse) a.lse2[before] = a.lse[t] * kLog2e;
-                ++before;
-            } else {
-                a.row_map[a.T - 1 - (t - before)] = int(t);
-            }
-        }
-        kept += total;
-        __syncthreads();
-    }
-    if (a.coef && top) atomicMax(&a.state->amax[2], top);
-    // the K walk's parts for dh, over the rows that turned out to count
-    if (tid < kMaxParts) {
-        const int64_t rows = min(int64_t(kept), a.dh_rows);
-        cost[tid] = spread_cost(rows, a.dh_cols, a.dh_k, a.terms, a.dh_shape, a.sms, tid + 1);
-    }
-    bad = __syncthreads_or(bad);
-    if (tid == 0) {
-        a.state->count = kept;
-        a.state->bad = bad;
-        if (bad) report_device_error(SW_ERR_INVALID);
-        // what every row's gradient is multiplied by stays out of the 16-bit
-        // logits' gradient: a target's -1 is exact there, where the common
-        // factor would round it the same way in every row
-        a.state->grad_scale =
-            a.factor * (a.mean ? (a.upstream ? a.upstream[0] : 1.0f) / float(max(kept, 1)) : 1.0f);
-        int best = 0;
-        for (int s = 1; s < kMaxParts; ++s)
-            if (cost[s] < cost[best] * 0.97f) best = s;
-        a.state->dh_splits = best + 1;
-    }
-}
-
-// A warp per compact row: its teacher's probabilities and its entries in
-// ascending column order, the row's sum of p log p, and the first entry of
-// every kEntryTile columns.
-__global__ void teacher_sort_kernel(const int* index, const float* logits, int K, int64_t V, float inv_tau,
-                                    const int* row_map, const HeadState* state, int rows_pad, int tiles,
-                                    int* ent_idx, float* ent_p, float* entropy, uint16_t* offs) {
-    __shared__ int s_idx[4][kMaxTeacher];
-    __shared__ int s_sorted[4][kMaxTeacher];
-    pdl_enter();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int i = blockIdx.x * 4 + warp;
-    if (i >= state->count) return;
-    const int64_t t = row_map[i];
-    float top = -INFINITY;
-    for (int k = lane; k < K; k += 32) {
-        const int col = index[t * K + k];
-        const float x = logits[t * K + k];
-        const bool ok = entry_counts(col, x, V);
-        s_idx[warp][k] = ok ? col : INT_MAX;
-        if (ok) top = fmaxf(top, x * inv_tau);
-    }
-    top = warp_max(top);
-    __syncwarp();
-    float sum = 0.0f;
-    for (int k = lane; k < K; k += 32)
-        if (s_idx[warp][k] != INT_MAX) sum += expf(logits[t * K + k] * inv_tau - top);
-    sum = warp_sum(sum);
-    const float log_sum = logf(sum);
-    float ent = 0.0f;
-    int n = 0;
-    for (int k = lane; k < K; k += 32) {
-        const int col = s_idx[warp][k];
-        int rank = 0;
-        for (int j = 0; j < K; ++j) {
-            const int o = s_idx[warp][j];
-            rank += (o < col) || (o == col && j < k);
-        }
-        float p = 0.0f;
-        if (col != INT_MAX) {
-            const float x = logits[t * K + k] * inv_tau - top;
-            p = expf(x) / sum;
-            if (p > 0.0f || p != p) ent += p * (x - log_sum);
-            ++n;
-        }
-        s_sorted[warp][rank] = col;
-        ent_idx[int64_t(i) * K + rank] = col;
-        ent_p[int64_t(i) * K + rank] = p;
-    }
-    ent = warp_sum(ent);
-    if (lane == 0) entropy[i] = ent;
-    for (int o = 16; o; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-    __syncwarp();
-    for (int tile = lane; tile <= tiles; tile += 32) {
-        const int64_t col0 = int64_t(tile) * kEntryTile;
-        int lo = 0, hi = n;  // entries [0, n) are the real ones
-        while (lo < hi) {
-            const int mid = (lo + hi) >> 1;
-            if (s_sorted[warp][mid] < col0) lo = mid + 1;
-            else hi = mid;
-        }
-        offs[int64_t(tile) * rows_pad + i] = uint16_t(lo);
-    }
-}
-
-// Largest finite magnitude of a matrix (of the rows of row_map when it is
-// given): a warp per row, or per column where columns are contiguous; `vec`:
-// rows are whole aligned groups of four.
-__global__ void __launch_bounds__(256) amax_kernel(const float* x, int64_t rows, int64_t cols, int64_t sr, int64_t sc,
-                                                   int vec, const int* row_map, const HeadState* count_from,
-                                                   uint32_t* out) {
-    pdl_enter();
-    if (count_from) rows = count_from->count;
-    const bool by_rows = sr == 1 && sc != 1;  // walk the unit stride fastest
-    const int64_t outer = by_rows ? cols : rows, inner = by_rows ? rows : cols;
-    const int64_t so = by_rows ? sc : sr, si = by_rows ? sr : sc;
-    const int lane = threadIdx.x & 31;
-    const int64_t warps = int64_t(gridDim.x) * 8;
-    uint32_t top = 0;
-    auto take = [&](float v) {
-        v = fabsf(v);
-        if (v <= 3.402823466e38f) top = max(top, __float_as_uint(v));
-    };
-    for (int64_t o = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5); o < outer; o += warps) {
-        const float* p = x + (by_rows ? o : row_map ? int64_t(row_map[o]) : o) * so;
-        if (vec) {
-#pragma unroll 4
-            for (int64_t i = lane * 4; i < inner; i += 128) {
-                const float4 v = *reinterpret_cast<const float4*>(p + i);
-                take(v.x);
-                take(v.y);
-                take(v.z);
-                take(v.w);
-            }
-        } else {
-#pragma unroll 4
-            for (int64_t i = lane; i < inner; i += 32) take(p[(by_rows && row_map ? int64_t(row_map[i]) : i) * si]);
-        }
-    }
-    for (int o = 16; o; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (lane == 0 && top) atomicMax(out, top);
-}
-
-// pack_kernel for rows that are whole aligned 16-byte units (8 columns at a
-// time, coalesced): a gather of bf16 rows, or the split of Float32 rows.
-template <bool kF32>
-__global__ void __launch_bounds__(256) pack_rows_kernel(const void* src, int64_t rows, int64_t cols, int64_t sr,
-                                                        const int* row_map, const HeadState* state, int use_count,
-                                                        int scale_of, uint16_t* dst, int64_t ld, int64_t rows_pad) {
-    pdl_enter();
-    const int64_t valid = use_count ? min(rows, int64_t(state->count)) : rows;
-    const bool twice = !kF32 && use_count && state->few(0);  // the rows again for their gradients' remainders
-    const float scale = kF32 ? pow2i(scale_exponent(state->amax[scale_of])) : 1.0f;
-    const int64_t units = cols / 8;  // ld == cols here
-    const int64_t stride = int64_t(gridDim.x) * 256;
-#pragma unroll 2
-    for (int64_t u = int64_t(blockIdx.x) * 256 + threadIdx.x; u < rows_pad * units; u += stride) {
-        const int64_t r = u / units, c = (u - r * units) * 8;
-        const int64_t from = twice && r >= kFewRows ? r - kFewRows : r;
-        uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
-        if (from < valid) {
-            const int64_t at = (row_map ? int64_t(row_map[from]) : from) * sr + c;
-            if (kF32) {
-                const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(src) + at);
-                const float4 a = p[0], b = p[1];
-                const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-                uint32_t h[4], l[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float x = v[2 * j] * scale, y = v[2 * j + 1] * scale;
-                    const __half2 q = __floats2half2_rn(x, y);
-                    h[j] = *reinterpret_cast<const uint32_t*>(&q);
-                    l[j] = pack2<false>(x - __low2float(q), y - __high2float(q));
-                }
-                hi = make_uint4(h[0], h[1], h[2], h[3]);
-                lo = make_uint4(l[0], l[1], l[2], l[3]);
-            } else {
-                hi = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(src) + at);
-            }
-        }
-        *reinterpret_cast<uint4*>(dst + r * ld + c) = hi;
-        if (kF32) *reinterpret_cast<uint4*>(dst + (rows_pad + r) * ld + c) = lo;
-    }
-}
-
-// Gathers rows into the contraction's operand: [rows_pad][ld] 16-bit, a copy
-// of bf16 values, or two f16 planes of a Float32 value times 2^q (hi rounded
-// to nearest, lo the rest).  Rows past the ones that count are zero.
-template <bool kF32>
-__global__ void pack_kernel(const void* src, int64_t rows, int64_t cols, int64_t sr, int64_t sc, const int* row_map,
-                            const HeadState* state, int use_count, int scale_of, uint16_t* dst, int64_t ld,
-                            int64_t rows_pad) {
-    __shared__ float tile[32][33];
-    pdl_enter();
-    const int64_t valid = use_count ? min(rows, int64_t(state->count)) : rows;
-    const bool twice = !kF32 && use_count && state->few(0);  // the rows again for their gradients' remainders
-    const float scale = kF32 ? pow2i(scale_exponent(state->amax[scale_of])) : 1.0f;
-    const int64_t r0 = int64_t(blockIdx.x) * 32, c0 = int64_t(blockIdx.y) * 32;
-    const bool by_rows = sr == 1 && sc != 1;
-    const int x = threadIdx.x & 31, y0 = threadIdx.x >> 5;
-    for (int y = y0; y < 32; y += 8) {
-        int64_t r = r0 + (by_rows ? x : y);
-        const int64_t c = c0 + (by_rows ? y : x);
-        if (twice && r >= kFewRows) r -= kFewRows;
-        float v = 0.0f;
-        if (r < valid && c < cols) {
-            const int64_t at = (row_map ? int64_t(row_map[r]) : r) * sr + c * sc;
-            v = kF32 ? static_cast<const float*>(src)[at] : __bfloat162float(static_cast<const __nv_bfloat16*>(src)[at]);
-        }
-        tile[by_rows ? x : y][by_rows ? y : x] = v;
-    }
-    __syncthreads();
-    for (int y = y0; y < 32; y += 8) {
-        const int64_t r = r0 + y, c = c0 + x;
-        if (r >= rows_pad || c >= ld) continue;
-        const float v = tile[y][x];
-        if (kF32) {
-            const float s = v * scale;
-            const __half hi = __float2half_rn(s);
-            dst[r * ld + c] = __half_as_ushort(hi);
-            dst[(rows_pad + r) * ld + c] = __half_as_ushort(__float2half_rn(s - __half2float(hi)));
-        } else {
-            const __nv_bfloat16 b = __float2bfloat16_rn(v);
-            dst[r * ld + c] = __bfloat16_as_ushort(b);
-        }
-    }
-}
-
-// ---- after the forward ---------------------------------------------------------
-
-struct MergeArgs {
-    const float4* partial;
-    int tiles, rows_pad;
-    int64_t row0, T, V;      // compact rows [row0, T)
-    const HeadState* state;
-    const int* row_map;
-    const int* targets;
-    int ignore_index;
-    const float* entropy;    // distillation, or null
-    float factor;            // f
-    float* row_loss;         // compact
-    float* lse2;             // compact
-    float* loss;             // per row, or null
-    float* lse;              // per row, or null
-};
-
-// 32 rows x 8 slices of the tiles per CTA.
-__global__ void __launch_bounds__(256) merge_kernel(const MergeArgs a) {
-    __shared__ float4 part[8][32];
-    pdl_enter();
-    const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
-    const int64_t i = a.row0 + int64_t(blockIdx.x) * 32 + lane;
-    const int count = a.state->count;
-    float ref = -INFINITY, sum = 0.0f, dot = 0.0f;
-    if (i < count) {
-        for (int t = slice; t < a.tiles; t += 8) {
-            const float4 p = a.partial[int64_t(t) * a.rows_pad + i];
-            const float next = fmaxf(ref, p.x), base = next == -INFINITY ? 0.0f : next;
-            sum = sum * ex2(ref - base) + p.y * ex2(p.x - base);
-            ref = next;
-            dot += p.z;
-        }
-    }
-    part[slice][lane] = make_float4(ref, sum, dot, 0.0f);
-    __syncthreads();
-    if (slice || i >= a.T) return;
-    const int64_t row = a.row_map[i];
-    if (i >= count) {
-        float v = 0.0f;
-        if (a.targets && a.targets[row] != a.ignore_index) v = NAN;  // a target outside the vocabulary
-        if (a.loss) a.loss[row] = v;
-        if (a.lse) a.lse[row] = 0.0f;
-        return;
-    }
-    for (int s = 1; s < 8; ++s) {
-        const float4 p = part[s][lane];
-        const float next = fmaxf(ref, p.x), base = next == -INFINITY ? 0.0f : next;
-        sum = sum * ex2(ref - base) + p.y * ex2(p.x - base);
-        ref = next;
-        dot += p.z;
-    }
-    const float l2 = ref + log2f(sum);
-    const float v = a.factor * ((a.entropy ? a.entropy[i] : 0.0f) + (l2 - dot) * kLn2);
-    a.lse2[i] = l2;
-    a.row_loss[i] = v;
-    if (a.loss) a.loss[row] = v;
-    if (a.lse) a.lse[row] = l2 * kLn2;
-}
-
-// loss = mean of the compact rows' losses, summed in a fixed order.
-__global__ void __launch_bounds__(1024) mean_kernel(const float* row_loss, const HeadState* state, float* loss) {
-    __shared__ float part[32];
-    pdl_enter();
-    const int n = state->count;
-    float s = 0.0f;
-    for (int i = threadIdx.x; i < n; i += 1024) s += row_loss[i];
-    s = warp_sum(s);
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s;
-    __syncthreads();
-    if (threadIdx.x < 32) {
-        s = warp_sum(part[threadIdx.x]);
-        if (threadIdx.x == 0) *loss = state->bad ? NAN : s / float(n);
-    }
-}
-
-// The kept exponentials of the logits become their gradient, in place:
-// exp2(k2 z - ref) 2^(ref - lse2) is the softmax, and the target entries are
-// written from their own Float32 logits (where the softmax is near p, the
-// stored 11 bits of it would not be enough).  A CTA takes kScaleCols columns of
-// a row; a thread 8 columns (bf16), a half warp 32 columns (Float32: hi and lo
-// values replace the 64-column block they were computed from).
-constexpr int kScaleCols = 8192;
-struct ScaleArgs {
-    uint16_t* grad;
-    int64_t ld_grad, V;
-    const float4* partial;
-    int tile_n;              // columns of a tile; its halves start at 0 and 128
-    int rows_pad, row0;
-    const HeadState* state;
-    const float* lse2;
-    const float* coef;
-    const int* ent_idx;
-    const float* ent_p;
-    const float* ent_s;
-    int ent_k;
-};
-template <bool kF32>
-__global__ void __launch_bounds__(256) scale_kernel(const ScaleArgs a) {
-    __shared__ float factor[kScaleCols / 64];
-    pdl_enter();
-    // the last rows first: they are the ones the contraction left in L2, and the
-    // next one starts with the first
-    const int64_t i = int64_t(gridDim.x) - 1 - blockIdx.x;
-    if (i >= a.state->count - a.row0) return;
-    const int64_t c0 = int64_t(blockIdx.y) * kScaleCols;
-    const int64_t c1 = min(c0 + kScaleCols, a.V);
-    const float lse2 = a.lse2[i];
-    const float coef = a.coef[i] * (kF32 ? pow2i(scale_exponent(a.state->amax[2])) : 1.0f);
-    for (int64_t b = c0 + threadIdx.x * 64; b < c1; b += 256 * 64) {  // tiles are whole 64-column blocks
-        const int64_t tile = b / a.tile_n, half = tile * 2 + (b - tile * a.tile_n >= 128);
-        const float ref = a.partial[half * a.rows_pad + i].x;
-        // (a half tile of nothing but -inf stored zeros)
-        factor[(b - c0) / 64] = ref == -INFINITY ? 0.0f : ex2(ref - lse2) * coef * (kF32 ? 1.0f : 1.0f / 32768.0f);
-    }
-    __syncthreads();
-    uint16_t* row = a.grad + i * a.ld_grad;
-    const bool few = !kF32 && a.state->few(a.row0);
-    uint16_t* rest = row + kFewRows * a.ld_grad;
-    if (kF32) {
-        const int lane = threadIdx.x & 31;
-        for (int64_t b = c0 + (threadIdx.x >> 5) * 64; b < c1; b += 8 * 64) {
-            float2 v = reinterpret_cast<const float2*>(row + 2 * b)[lane];
-            const float f = factor[(b - c0) / 64];
-            v.x = b + 2 * lane < a.V ? v.x * f : 0.0f;
-            v.y = b + 2 * lane + 1 < a.V ? v.y * f : 0.0f;
-            const __half2 hi = __floats2half2_rn(v.x, v.y);
-            const __half2 lo = __floats2half2_rn(v.x - __low2float(hi), v.y - __high2float(hi));
-            __syncwarp();
-            reinterpret_cast<__half2*>(row + 2 * b)[lane] = hi;
-            reinterpret_cast<__half2*>(row + 2 * b + 64)[lane] = lo;
-            __syncwarp();
-        }
-    } else {
-        for (int64_t c = c0 + threadIdx.x * 8; c < c1; c += 256 * 8) {
-            const uint4 v = *reinterpret_cast<const uint4*>(row + c);
-            const float f = factor[(c - c0) / 64];
-            const uint32_t e[4] = {v.x, v.y, v.z, v.w};
-            uint32_t hi[4], lo[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                float2 g = __half22float2(*reinterpret_cast<const __half2*>(&e[j]));
-                g.x *= f;
-                g.y *= f;
-                const __nv_bfloat162 h = __floats2bfloat162_rn(g.x, g.y);
-                hi[j] = *reinterpret_cast<const uint32_t*>(&h);
-                lo[j] = pack2<true>(g.x - __low2float(h), g.y - __high2float(h));
-            }
-            *reinterpret_cast<uint4*>(row + c) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-            if (few) *reinterpret_cast<uint4*>(rest + c) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-        }
-    }
-    __syncthreads();  // the entries overwrite what the loop above wrote
-    for (int k = threadIdx.x; k < a.ent_k; k += 256) {
-        const int64_t at = i * a.ent_k + k;
-        const int col = a.ent_idx[at];
-        if (col < c0 || col >= c1 || (k > 0 && a.ent_idx[at - 1] == col)) continue;
-        float p = a.ent_p ? a.ent_p[at] : 1.0f;
-        for (int j = 1; k + j < a.ent_k && a.ent_idx[at + j] == col; ++j) p += a.ent_p[at + j];
-        const float g = (ex2(a.ent_s[at] - lse2) - p) * coef;
-        if (kF32) {
-            uint16_t* d = row + (col & ~63) * int64_t(2) + (col & 63);
-            const __half hi = __float2half_rn(g);
-            d[0] = __half_as_ushort(hi);
-            d[64] = __half_as_ushort(__float2half_rn(g - __half2float(hi)));
-        } else {
-            const __nv_bfloat16 hi = __float2bfloat16_rn(g);
-            row[col] = __bfloat16_as_ushort(hi);
-            if (few) rest[col] = __bfloat16_as_ushort(__float2bfloat16_rn(g - __bfloat162float(hi)));
-        }
-    }
-}
-
-// Result rows from the fp32 sums of the K walk's parts, added in order, to
-// their places; with by_count, zeros in the rows that do not count.
-struct SlotsArgs {
-    const float* sums;       // rows as Walk places them
-    int64_t ld;
-    int splits, tile_m, workers;  // splits 0: state->dh_splits
-    int64_t rows, cols;
-    const HeadState* state;
-    int by_count, row0;
-    const int* row_map;
-    void* dst;
-    int64_t dst_row, dst_col;
-    int vec;                 // dst rows are contiguous and aligned to four elements
-};
-template <bool kF32>
-__global__ void __launch_bounds__(256) sum_slots_kernel(const SlotsArgs a) {
-    pdl_enter();
-    const int splits = a.splits > 0 ? a.splits : a.state->dh_splits;
-    const int64_t summed = a.by_count ? min(a.rows, int64_t(a.state->rows(a.row0))) : a.rows;
-    const bool few = !kF32 && a.by_count && a.state->few(a.row0);  // their remainders are further rows
-    const Walk walk(few ? a.state->rows_and_rest(a.row0, true) : int(summed), int((a.cols + kBN - 1) / kBN), a.tile_m, a.workers, splits);
-    const int64_t per_row = (a.cols + 3) / 4;
-    for (int64_t u = int64_t(blockIdx.x) * 256 + threadIdx.x; u < a.rows * per_row; u += int64_t(gridDim.x) * 256) {
-        const int64_t m = u / per_row, c = (u - m * per_row) * 4;
-        const float* p = a.sums + c;  // ld is whole groups of four
-        float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (m < summed) {
-            const int tile = walk.tile_of(int(m) / a.tile_m, int(c) / kBN);
-            const int parts = tile < walk.whole ? 1 : splits;
-            for (int rest = 0; rest <= (few ? kFewRows : 0); rest += kFewRows) {
-#pragma unroll 4
-                for (int k = 0; k < parts; ++k) {
-                    const float4 v =
-                        *reinterpret_cast<const float4*>(p + int64_t(walk.sum_row(k, int(m) + rest)) * a.ld);
-                    s.x += v.x;
-                    s.y += v.y;
-                    s.z += v.z;
-                    s.w += v.w;
-                }
-            }
-        }
-        const int64_t at = (a.row_map ? int64_t(a.row_map[m]) : m) * a.dst_row + c * a.dst_col;
-        const float r[4] = {s.x, s.y, s.z, s.w};
-        if (a.vec && c + 4 <= a.cols) {
-            if (kF32) *reinterpret_cast<float4*>(static_cast<float*>(a.dst) + at) = s;
-            else
-                *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.dst) + at) =
-                    make_uint2(pack2<true>(s.x, s.y), pack2<true>(s.z, s.w));
-            continue;
-        }
-        for (int j = 0; j < 4 && c + j < a.cols; ++j) {
-            if (kF32) static_cast<float*>(a.dst)[at + j * a.dst_col] = r[j];
-            else static_cast<__nv_bfloat16*>(a.dst)[at + j * a.dst_col] = __float2bfloat16_rn(r[j]);
-        }
-    }
-}
 
 // ---- host ----------------------------------------------------------------------
 
@@ -710,18 +133,24 @@ template <int kShape, bool kBf16, bool kAMn, bool kBMn, int kEpi>
 int launch_gemm(const Operand& a, const Operand& b, const Target& c, const GemmArgs& args, cudaStream_t stream) {
     using Cf = Cfg<kShape>;
     constexpr bool kPair = Cf::kPair;
-    const int64_t tiles = int64_t((args.M + Cf::kTileM - 1) / Cf::kTileM) * ((args.N + args.tile_n - 1) / args.tile_n);
+    const int64_t tiles = int64_t((args.M + Cf::kTileM - 1) / Cf::kTileM) * ((args.N + kBN - 1) / kBN);
     if (tiles == 0) return SW_OK;
     CUtensorMap ma, mb, mc;
     int rc = make_map(&ma, a.ptr, a.rows, a.cols, a.ld, kAMn ? kBK : kBM);
     if (rc != SW_OK) return rc;
-    rc = make_map(&mb, b.ptr, b.rows, b.cols, b.ld, kBMn ? kBK : kPair ? Cf::kBRows : args.tile_n);
+    rc = make_map(&mb, b.ptr, b.rows, b.cols, b.ld, kBMn ? kBK : Cf::kBRows);
     if (rc != SW_OK) return rc;
     memset(&mc, 0, sizeof(mc));
     if (c.ptr && (rc = make_target_map(&mc, c)) != SW_OK) return rc;
     auto kernel = head_gemm_kernel<kShape, kBf16, kAMn, kBMn, kEpi>;
-    SW_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cf::kSmemBytes),
-                "linear head smem");
+    static bool configured[64] = {};  // per device: the attribute stays
+    int dev = 0;
+    SW_CUDA_TRY(cudaGetDevice(&dev), "cudaGetDevice");
+    if (dev < 0 || dev >= 64 || !configured[dev]) {
+        SW_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cf::kSmemBytes),
+                    "linear head smem");
+        if (dev >= 0 && dev < 64) configured[dev] = true;
+    }
     constexpr int kCtas = kPair ? 2 : 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(kCtas * (unsigned)(args.splits == 1 ? std::min<int64_t>(tiles, device_sms() / kCtas) : device_sms() / kCtas));
@@ -747,7 +176,6 @@ int gemm(const Operand& a, const Operand& b, const Target& c, GemmArgs args, int
     args.pa = a.plane;
     args.pb = b.plane;
     if (kEpi != kEpiOut) args.splits = 1;
-    if (kEpi != kEpiLse || shape != kSingle) args.tile_n = kBN;
     if (shape == kSingle) return launch_gemm<kSingle, kBf16, kAMn, kBMn, kEpi>(a, b, c, args, stream);
     // results summed in registers (Float32, and the statistics) have no tall tile,
     // and the logits' gradient has too much to do after a tile (4096 x 32000, dim
@@ -808,9 +236,9 @@ struct Layout {
 };
 
 struct Shape {
-    int64_t T, D, V, rows_pad, ld_h, ld_w;
-    int64_t half_tiles;      // 128-column pieces of the vocabulary, each with its statistics
-    bool f32, pack_w, grads;
+    int64_t T, D, V, rows_pad, ld_h;
+    int64_t half_tiles;      // 128-column halves of the vocabulary's tiles, each with its statistics
+    bool f32, pack_w, grads, flags;
     int planes;
     // Gradients: `keep`: the forward's exponentials of `rows` compact rows at a
     // time stay in the workspace and become the logits' gradient.  Otherwise
@@ -818,7 +246,6 @@ struct Shape {
     // time.  Packed weights are laid out `piece` columns at a time too.
     bool keep;
     int64_t rows, piece;
-    int tile_n;              // columns of a logits tile
     int logits_shape, dh_shape;
     Spread dw;
     // rows of fp32 sums of each gradient (0: it is written at once); dh's rows
@@ -834,7 +261,7 @@ Layout lay_out(Bump& b, const Call& c, const Shape& s) {
     l.row_map = b.take<int>(s.T);
     l.ent_idx = b.take<int>(s.rows_pad * K);
     if (!c.targets) {
-        l.flags = b.take<uint8_t>(s.T);
+        if (s.flags) l.flags = b.take<uint8_t>(s.T);
         l.ent_p = b.take<float>(s.rows_pad * K);
         l.entropy = b.take<float>(s.rows_pad);
         l.offs = b.take<uint16_t>(s.rows_pad * ((s.V + kEntryTile - 1) / kEntryTile + 1));
@@ -847,7 +274,7 @@ Layout lay_out(Bump& b, const Call& c, const Shape& s) {
     if (s.keep) l.ent_s = b.take<float>(s.rows_pad * K);
     if (s.dh_sum_rows) l.dh_sums = b.take<float>(s.dh_sum_rows * s.ld_acc);
     if (s.dw_sum_rows) l.dw_sums = b.take<float>(s.dw_sum_rows * s.ld_acc);
-    if (s.pack_w) l.wp = b.take<uint16_t>(s.planes * round_up(s.piece, kBK) * s.ld_w);
+    if (s.pack_w) l.wp = b.take<uint16_t>(s.planes * round_up(s.piece, kBK) * s.ld_h);
     if (s.grads) l.grad = b.take<uint16_t>(s.planes * s.rows * round_up(s.piece, 64));
     return l;
 }
@@ -856,77 +283,111 @@ template <bool kF32>
 int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
     const sw_linear_head& p = *c.plan;
     constexpr bool kBf16 = !kF32;
-    const int esize = kF32 ? 4 : 2, terms = kF32 ? 3 : 1;
-    SW_CUDA_TRY(cudaMemsetAsync(l.state, 0, sizeof(HeadState), stream), "linear head state");
-    if (!c.targets)
-        SW_CUDA_TRY(launch_pdl(teacher_flags_kernel, dim3((unsigned)std::max<int64_t>((s.T + 7) / 8, 1)), dim3(256), 0, stream,
+    const int esize = kF32 ? 4 : 2, terms = kF32 ? 3 : 1, sms = device_sms();
+    const unsigned fill = (unsigned)(8 * sms);
+    const int top_k = c.targets ? 1 : c.top_k;
+    // rows of dim elements that the vector kernels can read
+    auto whole_rows = [&](const void* x, int64_t sr, int64_t sc) {
+        return sc == 1 && s.D % 8 == 0 && sr * esize % 16 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+    };
+    if (s.flags)
+        SW_CUDA_TRY(launch_pdl(teacher_flags_kernel, dim3((unsigned)((s.T + 7) / 8)), dim3(256), 0, stream,
                                c.teacher_index, c.teacher_logits, s.T, c.top_k, s.V, l.flags),
                     "teacher rows");
-    RowsArgs ra;
-    memset(&ra, 0, sizeof(ra));
-    ra.targets = c.targets;
-    ra.ignore_index = c.ignore_index;
-    ra.flags = l.flags;
-    ra.T = s.T;
-    ra.V = s.V;
-    ra.upstream = c.upstream;
-    ra.mean = p.reduction == SW_HEAD_MEAN;
-    ra.factor = c.scale * c.factor;
-    ra.lse = c.loss ? nullptr : c.lse;
-    ra.row_map = l.row_map;
-    ra.ent_idx = l.ent_idx;
-    ra.coef = s.grads ? l.coef : nullptr;
-    ra.lse2 = l.lse2;
-    ra.state = l.state;
-    ra.dh_rows = s.rows;
-    ra.dh_cols = s.D;
-    ra.dh_k = std::min(s.piece, s.V);
-    ra.dh_shape = s.dh_shape;
-    ra.sms = device_sms();
-    ra.terms = terms;
-    SW_CUDA_TRY(launch_pdl(rows_kernel, dim3(1), dim3(1024), 0, stream, ra), "linear head rows");
-    if (!c.targets)
-        SW_CUDA_TRY(launch_pdl(teacher_sort_kernel, dim3((unsigned)std::max<int64_t>((s.T + 3) / 4, 1)), dim3(128), 0, stream,
-                               c.teacher_index, c.teacher_logits, c.top_k, s.V, c.scale, l.row_map, l.state,
-                               (int)s.rows_pad, (int)((s.V + kEntryTile - 1) / kEntryTile), l.ent_idx, l.ent_p,
-                               l.entropy, l.offs),
-                    "teacher entries");
-    // rows of `cols` elements that the vector kernels can read
-    auto whole_rows = [&](const void* x, int64_t cols, int64_t sr, int64_t sc) {
-        return sc == 1 && cols % 8 == 0 && sr * esize % 16 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+    PrepareArgs pa;
+    memset(&pa, 0, sizeof(pa));
+    pa.targets = c.targets;
+    pa.ignore_index = c.ignore_index;
+    pa.index = c.teacher_index;
+    pa.logits = c.teacher_logits;
+    pa.flags = l.flags;
+    pa.top_k = top_k;
+    pa.inv_tau = c.scale;
+    pa.T = s.T;
+    pa.V = s.V;
+    pa.rows_pad = (int)s.rows_pad;
+    pa.entry_tiles = (int)((s.V + kEntryTile - 1) / kEntryTile);
+    pa.upstream = c.upstream;
+    pa.mean = p.reduction == SW_HEAD_MEAN;
+    pa.factor = c.scale * c.factor;
+    pa.lse = c.loss ? nullptr : c.lse;
+    pa.row_map = l.row_map;
+    pa.ent_idx = l.ent_idx;
+    pa.ent_p = l.ent_p;
+    pa.entropy = l.entropy;
+    pa.offs = l.offs;
+    pa.coef = s.grads ? l.coef : nullptr;
+    pa.lse2 = l.lse2;
+    pa.state = l.state;
+    if (c.dh) {
+        pa.dh_rows = s.rows;
+        pa.dh_cols = s.D;
+        pa.dh_k = std::min(s.piece, s.V);
+    }
+    pa.dh_shape = s.dh_shape;
+    pa.sms = sms;
+    pa.terms = terms;
+    if (kBf16) {
+        pa.h = static_cast<const uint16_t*>(c.h);
+        pa.D = s.D;
+        pa.sr = p.h_row;
+        pa.sc = p.h_col;
+        pa.vec = whole_rows(c.h, p.h_row, p.h_col);
+        pa.hc = l.hc;
+        pa.ld = s.ld_h;
+        if (!pa.h) pa.h = l.hc;  // no rows: only zeros are written
+    }
+    // 8 rows a CTA for parallelism; 32 where every CTA's look at all T rows would show
+    if (s.T <= 16384)
+        SW_CUDA_TRY(launch_pdl(prepare_kernel<8>, dim3((unsigned)(s.rows_pad / 8)), dim3(256), 0, stream, pa),
+                    "linear head rows");
+    else
+        SW_CUDA_TRY(launch_pdl(prepare_kernel<32>, dim3((unsigned)(s.rows_pad / 32)), dim3(256), 0, stream, pa),
+                    "linear head rows");
+    auto job = [&](const void* x, int64_t rows, int64_t sr, int64_t sc, const int* map, int scale_of, uint16_t* dst,
+                   int64_t rows_pad) {
+        SplitJob j;
+        memset(&j, 0, sizeof(j));
+        j.src = x;
+        j.rows = rows;
+        j.cols = s.D;
+        j.sr = sr;
+        j.sc = sc;
+        j.vec = whole_rows(x, sr, sc);
+        j.row_map = map;
+        j.scale_of = scale_of;
+        j.dst = dst;
+        j.ld = s.ld_h;
+        j.rows_pad = rows_pad;
+        const int64_t units = j.vec ? rows_pad * (s.D / 8) / 256 : (rows_pad + 31) / 32 * ((s.ld_h + 31) / 32);
+        j.ctas = (unsigned)std::max<int64_t>(std::min<int64_t>(units, fill), 1);
+        return j;
     };
-    const unsigned fill = (unsigned)(8 * device_sms());
-    auto amax = [&](const void* x, int64_t rows, int64_t sr, int64_t sc, const int* map, const HeadState* count,
-                    uint32_t* out) -> int {
-        SW_CUDA_TRY(launch_pdl(amax_kernel, dim3(std::min<unsigned>(fill, (unsigned)((std::max(rows, s.D) + 7) / 8))),
-                               dim3(256), 0, stream, (const float*)x, rows, s.D, sr, sc,
-                               (int)whole_rows(x, s.D, sr, sc), map, count, out),
-                    "linear head scale");
-        return SW_OK;
-    };
-    auto pack = [&](const void* x, int64_t rows, int64_t sr, int64_t sc, const int* map, int use_count, int scale_of,
-                    uint16_t* dst, int64_t rows_pad) -> int {
-        if (whole_rows(x, s.D, sr, sc)) {
-            const int64_t units = rows_pad * (s.D / 8);
-            SW_CUDA_TRY(launch_pdl(pack_rows_kernel<kF32>, dim3((unsigned)std::min<int64_t>((units + 255) / 256, fill)),
-                                   dim3(256), 0, stream, x, rows, s.D, sr, map, l.state, use_count, scale_of, dst,
-                                   s.ld_h, rows_pad),
-                        "linear head operand");
-        } else {
-            SW_CUDA_TRY(launch_pdl(pack_kernel<kF32>,
-                                   dim3((unsigned)((rows_pad + 31) / 32), (unsigned)((s.ld_h + 31) / 32)), dim3(256), 0,
-                                   stream, x, rows, s.D, sr, sc, map, l.state, use_count, scale_of, dst, s.ld_h,
-                                   rows_pad),
-                        "linear head operand");
-        }
+    SplitJob none_job;
+    memset(&none_job, 0, sizeof(none_job));
+    auto split = [&](const SplitJob& j0, const SplitJob& j1) -> int {
+        SW_CUDA_TRY(launch_pdl(split_kernel<kF32>, dim3(j0.ctas + j1.ctas), dim3(256), 0, stream, j0, j1, l.state),
+                    "linear head operands");
         return SW_OK;
     };
     int rc;
+    // the weights of columns [v0, v0 + n): in place, or packed into the workspace,
+    // with zero rows up to whole K stages (a tail of G's zeros must not meet the
+    // next plane); the first piece together with the states
+    int64_t packed = -1;
+    auto weight_job = [&](int64_t v0, int64_t n) {
+        return job(static_cast<const uint8_t*>(c.w) + v0 * p.w_row * esize, n, p.w_row, p.w_col, nullptr, 1, l.wp,
+                   round_up(n, kBK));
+    };
     if (kF32) {
-        if ((rc = amax(c.h, s.T, p.h_row, p.h_col, l.row_map, l.state, &l.state->amax[0])) != SW_OK) return rc;
-        if ((rc = amax(c.w, s.V, p.w_row, p.w_col, nullptr, nullptr, &l.state->amax[1])) != SW_OK) return rc;
+        const SplitJob jh = job(c.h, s.T, p.h_row, p.h_col, l.row_map, 0, l.hc, s.rows_pad);
+        const int64_t n = std::min(s.piece, s.V);
+        SplitJob jw = weight_job(0, n), all = job(c.w, s.V, p.w_row, p.w_col, nullptr, 1, nullptr, s.V);
+        SW_CUDA_TRY(launch_pdl(amax_kernel, dim3(jh.ctas + all.ctas), dim3(256), 0, stream, jh, all, l.state),
+                    "linear head scales");
+        if ((rc = split(jh, jw)) != SW_OK) return rc;
+        packed = 0;
     }
-    if ((rc = pack(c.h, s.T, p.h_row, p.h_col, l.row_map, 1, 0, l.hc, s.rows_pad)) != SW_OK) return rc;
     const Plane dense{kBK, 0, 0};
     // rows [r0, r0 + n) of the gathered states
     auto states = [&](int64_t r0, int64_t n) {
@@ -939,27 +400,21 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
     g.state = l.state;
     g.logit_scale = c.scale;
     g.ent_p = l.ent_p;
-    g.ent_k = c.targets ? 1 : c.top_k;
+    g.ent_k = top_k;
+    g.half_tiles = (int)s.half_tiles;
     g.rows_pad = (int)s.rows_pad;
-    g.tile_n = s.tile_n;
     const Target grad_out{l.grad, s.rows, ld_grad, ld_grad, false}, none{nullptr, 0, 0, 0, false};
 
-    // the weights of columns [v0, v0 + n): in place, or packed into the workspace
-    int64_t packed = -1;
     auto weights = [&](int64_t v0, int64_t n, Operand* out) -> int {
-        const uint8_t* at = static_cast<const uint8_t*>(c.w) + v0 * p.w_row * esize;
         if (!s.pack_w) {
+            const uint8_t* at = static_cast<const uint8_t*>(c.w) + v0 * p.w_row * esize;
             *out = Operand{reinterpret_cast<const uint16_t*>(at), n, s.D, p.w_row, dense};
             return SW_OK;
         }
-        // zero rows up to whole K stages: a tail of G's zeros must not meet the next plane
         const int64_t rows = round_up(n, kBK);
-        if (packed != v0) {
-            const int rc = pack(at, n, p.w_row, p.w_col, nullptr, 0, 1, l.wp, rows);
-            if (rc != SW_OK) return rc;
-        }
+        if (packed != v0 && (rc = split(weight_job(v0, n), none_job)) != SW_OK) return rc;
         packed = v0;
-        *out = Operand{l.wp, s.planes * rows, s.D, s.ld_w, Plane{kBK, 0, (int)rows}};
+        *out = Operand{l.wp, s.planes * rows, s.D, s.ld_h, Plane{kBK, 0, (int)rows}};
         return SW_OK;
     };
     // logits of compact rows [r0, r0 + n) and columns [v0, v0 + nv)
@@ -973,36 +428,52 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
         a.scale_a = kF32 ? 0 : -1;
         a.scale_b = kF32 ? 1 : -1;
         a.v0 = v0;
-        a.half0 = (int)(v0 / kBN * 2);
         a.ent_idx = l.ent_idx + r0 * g.ent_k;
         a.ent_p = l.ent_p ? l.ent_p + r0 * g.ent_k : nullptr;
         a.offs = l.offs ? l.offs + r0 : nullptr;
-        a.partial = l.partial + r0;
+        a.partial = l.partial + r0 * s.half_tiles;
         a.lse2 = l.lse2 + r0;
         a.coef = l.coef + r0;
         return a;
     };
-    auto merge = [&](int64_t r0, int64_t n) -> int {
-        MergeArgs m;
-        memset(&m, 0, sizeof(m));
-        m.partial = l.partial;
-        m.tiles = (int)s.half_tiles;
-        m.rows_pad = (int)s.rows_pad;
-        m.row0 = r0;
-        m.T = std::min(s.T, r0 + n);
-        m.V = s.V;
-        m.state = l.state;
-        m.row_map = l.row_map;
-        m.targets = c.targets;
-        m.ignore_index = c.ignore_index;
-        m.entropy = l.entropy;
-        m.factor = c.factor;
-        m.row_loss = l.row_loss;
-        m.lse2 = l.lse2;
-        m.loss = p.reduction == SW_HEAD_MEAN ? nullptr : c.loss;
-        m.lse = c.lse;
-        SW_CUDA_TRY(launch_pdl(merge_kernel, dim3((unsigned)std::max<int64_t>((n + 31) / 32, 1)), dim3(256), 0, stream,
-                               m),
+    // the loss of compact rows [r0, r0 + n), and with `grad` their logits' gradient
+    auto losses = [&](int64_t r0, int64_t n, bool grad) -> int {
+        LossArgs a;
+        memset(&a, 0, sizeof(a));
+        a.partial = l.partial;
+        a.half_tiles = (int)s.half_tiles;
+        a.row0 = (int)r0;
+        a.rows = (int)n;
+        a.all_rows = (int)std::max<int64_t>(s.T, 1);
+        a.state = l.state;
+        a.row_map = l.row_map;
+        a.targets = c.targets;
+        a.ignore_index = c.ignore_index;
+        a.entropy = l.entropy;
+        a.factor = c.factor;
+        a.row_loss = l.row_loss;
+        a.lse2 = l.lse2;
+        a.loss = c.loss;
+        a.mean = p.reduction == SW_HEAD_MEAN;
+        a.lse = c.lse;
+        int64_t segs = 1;
+        if (grad) {
+            // a CTA takes a whole row, or where rows are few a part of one of at
+            // least 2048 columns
+            segs = std::max<int64_t>(1, std::min<int64_t>((s.V + 2047) / 2048, 4 * sms / std::max<int64_t>(n, 1)));
+            a.grad = l.grad;
+            a.ld_grad = ld_grad;
+            a.V = s.V;
+            a.seg = round_up((s.V + segs - 1) / segs, 512);
+            segs = (s.V + a.seg - 1) / a.seg;
+            a.coef = l.coef;
+            a.ent_idx = l.ent_idx;
+            a.ent_p = l.ent_p;
+            a.ent_s = l.ent_s;
+            a.ent_k = top_k;
+        }
+        SW_CUDA_TRY(launch_pdl(loss_kernel<kF32>, dim3((unsigned)std::max<int64_t>(n, 1), (unsigned)segs), dim3(256), 0,
+                               stream, a),
                     "linear head loss");
         return SW_OK;
     };
@@ -1015,7 +486,7 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
         a.row0 = (int)r0;
         auto finish = [&](float* sums, int splits, int shape, int64_t rows, bool by_count, const int* row_map,
                           void* dst, int64_t dst_row, int64_t dst_col) -> int {
-            SlotsArgs sa;
+            PlaceArgs sa;
             memset(&sa, 0, sizeof(sa));
             sa.sums = sums;
             sa.ld = s.ld_acc;
@@ -1033,7 +504,7 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
             sa.dst_col = dst_col;
             sa.vec = dst_col == 1 && dst_row % 4 == 0 && (reinterpret_cast<uintptr_t>(dst) & (4 * esize - 1)) == 0;
             const int64_t units = rows * (s.ld_acc / 4);
-            SW_CUDA_TRY(launch_pdl(sum_slots_kernel<kF32>, dim3((unsigned)std::min<int64_t>((units + 255) / 256, fill)),
+            SW_CUDA_TRY(launch_pdl(place_kernel<kF32>, dim3((unsigned)std::min<int64_t>((units + 255) / 256, fill)),
                                    dim3(256), 0, stream, sa),
                         "linear head sums");
             return SW_OK;
@@ -1075,12 +546,6 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
         }
         return SW_OK;
     };
-    auto mean = [&]() -> int {
-        if (c.loss && p.reduction == SW_HEAD_MEAN)
-            SW_CUDA_TRY(launch_pdl(mean_kernel, dim3(1), dim3(1024), 0, stream, l.row_loss, l.state, c.loss),
-                        "linear head mean loss");
-        return SW_OK;
-    };
     if (s.keep) {
         Operand w;
         if ((rc = weights(0, s.V, &w)) != SW_OK) return rc;
@@ -1092,31 +557,10 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
             rc = gemm<kBf16, false, false, kEpiLse>(states(r0, round_up(std::max<int64_t>(n, 1), kBM)), w, grad_out, a,
                                                     s.logits_shape, stream);
             if (rc != SW_OK) return rc;
-            if ((rc = merge(r0, n)) != SW_OK) return rc;
-            ScaleArgs sc;
-            memset(&sc, 0, sizeof(sc));
-            sc.grad = l.grad;
-            sc.ld_grad = ld_grad;
-            sc.V = s.V;
-            sc.partial = a.partial;
-            sc.tile_n = s.tile_n;
-            sc.rows_pad = (int)s.rows_pad;
-            sc.row0 = (int)r0;
-            sc.state = l.state;
-            sc.lse2 = a.lse2;
-            sc.coef = a.coef;
-            sc.ent_idx = a.ent_idx;
-            sc.ent_p = a.ent_p;
-            sc.ent_s = a.ent_s;
-            sc.ent_k = g.ent_k;
-            if (n > 0)
-                SW_CUDA_TRY(launch_pdl(scale_kernel<kF32>,
-                                       dim3((unsigned)n, (unsigned)((s.V + kScaleCols - 1) / kScaleCols)), dim3(256), 0,
-                                       stream, sc),
-                            "linear head logits' gradient");
+            if ((rc = losses(r0, n, true)) != SW_OK) return rc;
             if ((rc = gradients(r0, n, 0, s.V, w, true, true, r0 == 0, r0 + s.rows >= s.T)) != SW_OK) return rc;
         }
-        return mean();
+        return SW_OK;
     }
     if (c.loss) {
         const int64_t step = s.pack_w ? s.piece : s.V;
@@ -1128,8 +572,7 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
                                                     stream);
             if (rc != SW_OK) return rc;
         }
-        if ((rc = merge(0, s.T)) != SW_OK) return rc;
-        if ((rc = mean()) != SW_OK) return rc;
+        if ((rc = losses(0, s.T, false)) != SW_OK) return rc;
     }
     if (!s.grads) return SW_OK;
     for (int64_t v0 = 0; v0 < s.V; v0 += s.piece) {
@@ -1207,14 +650,15 @@ int check_and_run(const char* name, Call& c, void* stream_ptr) {
     s.f32 = p->dtype == SW_HEAD_F32;
     s.planes = s.f32 ? 2 : 1;
     s.rows_pad = std::max<int64_t>(round_up(T, kBM), kBM);
-    s.ld_h = s.ld_w = round_up(D, 8);
+    s.ld_h = round_up(D, 8);
+    s.flags = !c.targets && T * c.top_k > kInlineFlags;
     s.grads = grads;
     s.ld_acc = round_up(D, 4);
     // weights are read in place when TMA can: bf16, unit stride, 16-byte rows
     s.pack_w = s.f32 || p->w_col != 1 || p->w_row % 8 != 0 || p->w_row < D ||
                (reinterpret_cast<uintptr_t>(c.w) & 15) != 0;
     const int64_t budget = p->workspace_limit > 0 ? p->workspace_limit : kDefaultWorkspace;
-    const int64_t packed = s.pack_w ? s.planes * round_up(V, kBK) * s.ld_w * 2 : 0;
+    const int64_t packed = s.pack_w ? s.planes * round_up(V, kBK) * s.ld_h * 2 : 0;
     const int64_t grad_row = s.planes * round_up(V, 256) * 2;
     const int terms = s.f32 ? 3 : 1;
     // One call for the loss and the gradients keeps the logits' exponentials
@@ -1234,27 +678,12 @@ int check_and_run(const char* name, Call& c, void* stream_ptr) {
     s.piece = round_up(V, 256);
     if (!s.keep) {
         // as wide as the limit allows, in whole 256-column tiles
-        const int64_t per_column = (grads ? s.planes * s.rows_pad * 2 : 0) + (s.pack_w ? s.planes * s.ld_w * 2 : 0);
+        const int64_t per_column = (grads ? s.planes * s.rows_pad * 2 : 0) + (s.pack_w ? s.planes * s.ld_h * 2 : 0);
         if (per_column > 0) s.piece = std::min(s.piece, std::max<int64_t>(budget / per_column / 256 * 256, 256));
     }
     const int tallest = s.f32 ? kPair2 : kTall;
     s.logits_shape = choose_spread(std::min(s.rows, T), std::min(s.piece, V), D, terms, kPair2, false).shape;
-    s.tile_n = kBN;
-    if (s.logits_shape == kSingle && c.loss && (s.piece >= V || !s.pack_w)) {
-        // few rows: a tile as narrow as fills the last wave (whole 64-column
-        // blocks where the exponentials are kept, else whole MMA widths)
-        const int q = s.keep ? 64 : 16, sms = device_sms();
-        const int64_t row_tiles = (T + kBM - 1) / kBM;
-        int64_t best = INT64_MAX;
-        for (int t = kBN; t >= 128; t -= q) {
-            const int64_t tiles = row_tiles * ((V + t - 1) / t), cost = (tiles + sms - 1) / sms * (t + 16);
-            if (cost < best) {
-                best = cost;
-                s.tile_n = t;
-            }
-        }
-    }
-    s.half_tiles = (V + s.tile_n - 1) / s.tile_n * 2;
+    s.half_tiles = (V + kBN - 1) / kBN * 2;
     s.dh_shape = kSingle;
     s.dw = Spread{kSingle, 1};
     s.dh_sum_rows = s.dw_sum_rows = 0;
