@@ -31,7 +31,7 @@ __device__ __forceinline__ bool entry_counts(int index, float logit, int64_t V) 
 // last, partial wave cut into s parts of the K walk: waves x (stages + a tile's
 // cost that nothing hides), and the traffic of writing and adding the parts.  A
 // K stage takes 0.27 us (kSingle: 128 x 256 on one SM, kPair2: 256 x 256 on two)
-// or 0.52 (kTall), a tile's fill and drain 2 us (kTall: 5), an adding launch 3.
+// or 0.52 (kTall), a tile's fill and drain 2, 2.5 and 5 us, an adding launch 3.
 constexpr int kMaxParts = 64;       // where the tiles do not fill one wave
 constexpr int kMaxTailParts = 4;    // of the tiles after whole waves
 __host__ __device__ inline int shape_workers(int shape, int sms) { return shape == kSingle ? sms : sms / 2; }
@@ -40,7 +40,8 @@ __host__ __device__ inline float spread_cost(int64_t M, int64_t N, int64_t K, in
     const int64_t tiles = ((M + shape_rows(shape) - 1) >> (7 + shape)) * ((N + kBN - 1) / kBN);
     const int whole = int(tiles / workers), rest = int(tiles - int64_t(whole) * workers);
     if (s > 1 && (steps < 4 * s || rest == 0 || (whole ? s > kMaxTailParts : rest * s > 2 * workers))) return 1e30f;
-    const float stage = float(terms) * (shape == kTall ? 0.52f : 0.27f), fixed = shape == kTall ? 5.0f : 2.0f;
+    const float stage = float(terms) * (shape == kTall ? 0.52f : 0.27f);
+    const float fixed = shape == kTall ? 5.0f : shape == kPair2 ? 2.5f : 2.0f;
     const int share = (steps + s - 1) / s;
     float us = float(whole) * (float(steps) * stage + fixed) +
                float((rest * s + workers - 1) / workers) * (float(share) * stage + fixed);
@@ -181,9 +182,13 @@ __global__ void __launch_bounds__(256) prepare_kernel(const PrepareArgs a) {
     const int64_t t0 = int64_t(blockIdx.x) * kRows;
     const bool inline_flags = !a.targets && !a.flags;
     if (inline_flags) {
-        for (int64_t t = warp; t < a.T; t += 8) {
-            const bool any = teacher_row_counts(a.index, a.logits, t, a.top_k, a.V, lane);
-            if (lane == 0) s_flags[t] = any;
+        for (int t = tid; t < int(a.T); t += 256) s_flags[t] = 0;
+        __syncthreads();
+#pragma unroll 4
+        for (int e = tid; e < int(a.T) * a.top_k; e += 256) {
+            const int i = a.index[e];
+            if (i >= a.V) report_device_error(SW_ERR_INVALID);
+            if (entry_counts(i, a.logits[e], a.V)) s_flags[e / a.top_k] = 1;
         }
         __syncthreads();
     }
@@ -236,7 +241,7 @@ __global__ void __launch_bounds__(256) prepare_kernel(const PrepareArgs a) {
         }
     }
     __syncthreads();
-    if (blockIdx.x == 0) {
+    if (blockIdx.x == gridDim.x - 1) {  // (its rows are mostly padding)
         uint32_t top = 0;  // of the row factors (Float32 only)
         if (a.coef && !a.h) {
             for (int64_t t = tid; t < a.T; t += 256)
@@ -489,7 +494,7 @@ struct LossArgs {
 // last row to be done adds up the mean, in a fixed order.
 template <bool kF32>
 __global__ void __launch_bounds__(256) loss_kernel(const LossArgs a) {
-    constexpr int kSub = 8192;
+    constexpr int kSub = kF32 ? 2048 : 8192;  // columns of a batch: four loads a thread
     __shared__ float factor[kSub / 128];
     __shared__ float s_ref[8], s_sum[8], s_dot[8];
     __shared__ int s_last;
@@ -501,6 +506,26 @@ __global__ void __launch_bounds__(256) loss_kernel(const LossArgs a) {
     const bool writes = blockIdx.y == 0;
     const int count = a.state->rows(a.row0);
     float lse2 = 0.0f;
+    // the first 8192 columns' exponentials are on their way while the statistics
+    // are added up, and later each batch while the one before it is written
+    const int64_t c_begin = int64_t(blockIdx.y) * a.seg, c_end = min(c_begin + a.seg, a.V);
+    uint16_t* row = a.grad + i * a.ld_grad;
+    uint4 held[4];
+    auto fetch = [&](int64_t c0) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int64_t c = c0 + (kF32 ? 64 * warp + 512 * j : tid * 8 + 2048 * j);
+            if (c >= c_end) continue;
+            if (kF32) {
+                const float2 v = reinterpret_cast<const float2*>(row + 2 * c)[lane];
+                held[j].x = __float_as_uint(v.x);
+                held[j].y = __float_as_uint(v.y);
+            } else {
+                held[j] = *reinterpret_cast<const uint4*>(row + c);
+            }
+        }
+    };
+    if (a.grad && i < count) fetch(c_begin);
     if (i < count) {
         const float4* part = a.partial + (a.row0 + i) * a.half_tiles;
         float ref = -INFINITY, sum = 0.0f, dot = 0.0f;
@@ -566,9 +591,7 @@ __global__ void __launch_bounds__(256) loss_kernel(const LossArgs a) {
         }
     }
     if (!a.grad || i >= count) return;
-    const int64_t c_begin = int64_t(blockIdx.y) * a.seg, c_end = min(c_begin + a.seg, a.V);
     const float coef = a.coef[a.row0 + i] * (kF32 ? pow2i(scale_exponent(a.state->amax[2])) : 1.0f);
-    uint16_t* row = a.grad + i * a.ld_grad;
     const bool few = !kF32 && a.state->few(a.row0);
     uint16_t* rest = row + kFewRows * a.ld_grad;
     for (int64_t c0 = c_begin; c0 < c_end; c0 += kSub) {
@@ -580,34 +603,35 @@ __global__ void __launch_bounds__(256) loss_kernel(const LossArgs a) {
             factor[t] = ref == -INFINITY ? 0.0f : ex2(ref - lse2) * coef * (kF32 ? 1.0f : 1.0f / 32768.0f);
         }
         __syncthreads();
-        if (kF32) {
-#pragma unroll 2
-            for (int64_t b = c0 + warp * 64; b < c1; b += 8 * 64) {
-                float2 v = reinterpret_cast<const float2*>(row + 2 * b)[lane];
-                const float f = factor[(b - c0) / 128];
-                v.x = b + 2 * lane < a.V ? v.x * f : 0.0f;
-                v.y = b + 2 * lane + 1 < a.V ? v.y * f : 0.0f;
+        uint4 now[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) now[j] = held[j];
+        if (c1 < c_end) fetch(c1);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int64_t c = c0 + (kF32 ? 64 * warp + 512 * j : tid * 8 + 2048 * j);
+            if (c >= c1) continue;
+            const float f = factor[(c - c0) / 128];
+            if (kF32) {
+                float2 v = make_float2(__uint_as_float(now[j].x), __uint_as_float(now[j].y));
+                v.x = c + 2 * lane < a.V ? v.x * f : 0.0f;
+                v.y = c + 2 * lane + 1 < a.V ? v.y * f : 0.0f;
                 const __half2 hi = __floats2half2_rn(v.x, v.y);
                 const __half2 lo = __floats2half2_rn(v.x - __low2float(hi), v.y - __high2float(hi));
-                __syncwarp();
-                reinterpret_cast<__half2*>(row + 2 * b)[lane] = hi;
-                reinterpret_cast<__half2*>(row + 2 * b + 64)[lane] = lo;
-            }
-        } else {
-#pragma unroll 4
-            for (int64_t c = c0 + tid * 8; c < c1; c += 256 * 8) {
-                const uint4 v = *reinterpret_cast<const uint4*>(row + c);
-                const float f = factor[(c - c0) / 128];
-                const uint32_t e[4] = {v.x, v.y, v.z, v.w};
+                __syncwarp();  // (the whole block was read before any of it is replaced)
+                reinterpret_cast<__half2*>(row + 2 * c)[lane] = hi;
+                reinterpret_cast<__half2*>(row + 2 * c + 64)[lane] = lo;
+            } else {
+                const uint32_t e[4] = {now[j].x, now[j].y, now[j].z, now[j].w};
                 uint32_t hi[4], lo[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    float2 g = __half22float2(*reinterpret_cast<const __half2*>(&e[j]));
+                for (int q = 0; q < 4; ++q) {
+                    float2 g = __half22float2(*reinterpret_cast<const __half2*>(&e[q]));
                     g.x *= f;
                     g.y *= f;
                     const __nv_bfloat162 h = __floats2bfloat162_rn(g.x, g.y);
-                    hi[j] = *reinterpret_cast<const uint32_t*>(&h);
-                    lo[j] = pack2<true>(g.x - __low2float(h), g.y - __high2float(h));
+                    hi[q] = *reinterpret_cast<const uint32_t*>(&h);
+                    lo[q] = pack2<true>(g.x - __low2float(h), g.y - __high2float(h));
                 }
                 *reinterpret_cast<uint4*>(row + c) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
                 if (few) *reinterpret_cast<uint4*>(rest + c) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
@@ -659,16 +683,17 @@ __global__ void __launch_bounds__(256) place_kernel(const PlaceArgs a) {
     const bool few = !kF32 && a.by_count && a.state->few(a.row0);  // their remainders are further rows
     const Walk walk(few ? kFewRows + int(summed) : int(summed), int((a.cols + kBN - 1) / kBN), a.tile_m, a.workers,
                     splits);
-    const int64_t per_row = (a.cols + 3) / 4;
-    for (int64_t u = int64_t(blockIdx.x) * 256 + threadIdx.x; u < a.rows * per_row; u += int64_t(gridDim.x) * 256) {
-        const int64_t m = u / per_row, c = (u - m * per_row) * 4;
+    // a CTA takes 1024 columns of a row at a time
+    const int64_t spans = (a.cols + 1023) / 1024;
+    for (int64_t u = blockIdx.x; u < a.rows * spans; u += gridDim.x) {
+        const int64_t m = u / spans, c = (u - m * spans) * 1024 + threadIdx.x * 4;
+        if (c >= a.cols) continue;
         const float* p = a.sums + c;  // ld is whole groups of four
         float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if (m < summed) {
-            const int tile = walk.tile_of(int(m) / a.tile_m, int(c) / kBN);
-            const int parts = tile < walk.whole ? 1 : splits;
+            const int parts = walk.tile_of(int(m) / a.tile_m, int(c) / kBN) < walk.whole ? 1 : splits;
             for (int rest = 0; rest <= (few ? kFewRows : 0); rest += kFewRows) {
-#pragma unroll 4
+#pragma unroll 8
                 for (int k = 0; k < parts; ++k) {
                     const float4 v =
                         *reinterpret_cast<const float4*>(p + int64_t(walk.sum_row(k, int(m) + rest)) * a.ld);
@@ -680,7 +705,6 @@ __global__ void __launch_bounds__(256) place_kernel(const PlaceArgs a) {
             }
         }
         const int64_t at = (a.row_map ? int64_t(a.row_map[m]) : m) * a.dst_row + c * a.dst_col;
-        const float r[4] = {s.x, s.y, s.z, s.w};
         if (a.vec && c + 4 <= a.cols) {
             if (kF32) *reinterpret_cast<float4*>(static_cast<float*>(a.dst) + at) = s;
             else
@@ -688,6 +712,7 @@ __global__ void __launch_bounds__(256) place_kernel(const PlaceArgs a) {
                     make_uint2(pack2<true>(s.x, s.y), pack2<true>(s.z, s.w));
             continue;
         }
+        const float r[4] = {s.x, s.y, s.z, s.w};
         for (int j = 0; j < 4 && c + j < a.cols; ++j) {
             if (kF32) static_cast<float*>(a.dst)[at + j * a.dst_col] = r[j];
             else static_cast<__nv_bfloat16*>(a.dst)[at + j * a.dst_col] = __float2bfloat16_rn(r[j]);

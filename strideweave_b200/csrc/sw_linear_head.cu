@@ -503,8 +503,8 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
             sa.dst_row = dst_row;
             sa.dst_col = dst_col;
             sa.vec = dst_col == 1 && dst_row % 4 == 0 && (reinterpret_cast<uintptr_t>(dst) & (4 * esize - 1)) == 0;
-            const int64_t units = rows * (s.ld_acc / 4);
-            SW_CUDA_TRY(launch_pdl(place_kernel<kF32>, dim3((unsigned)std::min<int64_t>((units + 255) / 256, fill)),
+            const int64_t spans = rows * ((s.D + 1023) / 1024);
+            SW_CUDA_TRY(launch_pdl(place_kernel<kF32>, dim3((unsigned)std::min<int64_t>(spans, fill)),
                                    dim3(256), 0, stream, sa),
                         "linear head sums");
             return SW_OK;
