@@ -60,6 +60,7 @@ constexpr float kLn2 = 0.6931471805599453f;
 
 enum { kEpiLse = 0, kEpiGrad = 1, kEpiOut = 2 };
 enum { kCountM, kCountK };
+enum { kKMajor, kMnMajor, kBoth };       // A in memory; kBoth: of two contractions, each its own
 
 // How the tiles of a contraction are walked: groups of row tiles (which share
 // B's panels in L2), column tiles inside, row tiles innermost; the workers take
@@ -136,15 +137,32 @@ struct Plane {
     int x_block, x_plane, y_plane;
 };
 
-struct GemmArgs {
+// One contraction of a launch.
+struct Problem {
     int M, N, K;
     int count_is;            // which extent the device-side row count bounds
-    const HeadState* state;
-    int row0;                // first compact row of this launch (the count starts there)
-    int terms;               // plane pairs walked: 1, or 3 for Float32
+    int a_mn;                // A is MN-major in memory (gradients of the weights)
     Plane pa, pb;            // where each operand's lo plane and 64-element blocks lie
     int splits;              // parts of the last wave's tiles (0: state->dh_splits)
     int scale_a, scale_b;    // indexes into HeadState::amax of the operands' scales (-1: none)
+    // kEpiOut, through the output map: the result in its type, or fp32 running
+    // sums, with rows as Walk places them
+    int sums;
+    int first;               // nothing to add yet
+};
+
+// Tensor maps of the operands and of what is written, per contraction.
+struct alignas(64) Maps {
+    CUtensorMap a[2], b[2], c[2];
+};
+
+struct GemmArgs {
+    Problem p[2];            // two at once: the gradients of states and weights of few rows
+    int problems;
+    int alternate;           // every second worker takes the second one first
+    const HeadState* state;
+    int row0;                // first compact row of this launch (the count starts there)
+    int terms;               // plane pairs walked: 1, or 3 for Float32
     // logits epilogues
     float logit_scale;
     int64_t v0;              // first vocabulary column of this piece
@@ -159,10 +177,6 @@ struct GemmArgs {
     int keep;                // kEpiLse: write exp2(logit - half tile's max) where the logits' gradient will be
     const float* lse2;       // kEpiGrad: per compact row
     const float* coef;
-    // kEpiOut, through the output map: the result in its type, or fp32 running
-    // sums, part p of row m at row p round_up(M, tile) + m
-    int sums;
-    int first;               // nothing to add yet
 };
 
 enum { kSingle = 0, kPair2 = 1, kTall = 2 };
@@ -188,6 +202,58 @@ struct Cfg {
     static constexpr int kSmemBytes = kOffSlot + 16 + 1024;
     static constexpr int kTmemCols = 2 * kBN;
     static_assert(kSmemBytes <= 232448, "shared memory budget");
+};
+
+// Estimated microseconds of a K stage, and of a tile's fill and drain that
+// nothing hides: a stage takes 0.27 us (kSingle: 128 x 256 on one SM), 0.26 (kPair2:
+// 256 x 256 on two) or 0.52 (kTall).
+__host__ __device__ inline float stage_us(int shape, int terms) { return float(terms) * (shape == kTall ? 0.52f : shape == kPair2 ? 0.26f : 0.27f); }
+__host__ __device__ inline float fixed_us(int shape) { return shape == kTall ? 5.0f : shape == kPair2 ? 2.5f : 2.0f; }
+__host__ __device__ inline int shape_workers(int shape, int sms) { return shape == kSingle ? sms : sms / 2; }
+
+// A contraction of a launch as one worker sees it: its tiles and K stages, and
+// which work items are its own, item i: `pre` of them come before the workers'
+// common rounds (see below).
+struct Plan {
+    Walk walk;
+    int items, k_steps, part_steps;
+    int pre, pre_first, pre_stride, pool;
+
+    __device__ __forceinline__ Plan(int M, int N, int K, int tile_m, int workers, int parts)
+        : walk(M, (N + kBN - 1) / kBN, tile_m, workers, parts), items(walk.items()), k_steps((K + kBK - 1) / kBK),
+          part_steps((k_steps + parts - 1) / parts), pre(0), pre_first(0), pre_stride(0), pool(0) {}
+    // The contraction `before` left all workers but the first items % workers
+    // one item ahead: they take `gain` items of this one first, as many as last
+    // as long as one of the other's.
+    __device__ __forceinline__ void follow(const Plan& before, int worker, int workers, float stage, float fixed) {
+        const int rest = before.items % workers;
+        if (rest == 0) return;
+        const int gain = int((float(before.part_steps) * stage + fixed) / (float(part_steps) * stage + fixed) + 0.5f);
+        pre_stride = workers - rest;
+        pool = int(min(int64_t(items), int64_t(pre_stride) * gain));
+        pre_first = worker - rest;
+        if (pre_first >= 0 && pre_first < pool) pre = (pool - pre_first + pre_stride - 1) / pre_stride;
+    }
+    // Item i of a worker, or -1 after its last one.
+    __device__ __forceinline__ int nth(int i, int worker, int workers) const {
+        if (i < pre) return pre_first + i * pre_stride;
+        const int64_t t = int64_t(pool) + worker + int64_t(i - pre) * workers;
+        return t < items ? int(t) : -1;
+    }
+    // Item t: its tile and its share [k0, k1) of the K stages.
+    __device__ __forceinline__ void item(int t, int& mb, int& nb, int& part, int& k0, int& k1) const {
+        part = 0;
+        k0 = 0;
+        k1 = k_steps;
+        if (t >= walk.whole && walk.parts > 1) {
+            const int tile = walk.whole + (t - walk.whole) / walk.parts;
+            part = (t - walk.whole) % walk.parts;
+            k0 = min(part * part_steps, k_steps);
+            k1 = min(k0 + part_steps, k_steps);
+            t = tile;
+        }
+        walk.coords(t, mb, nb);
+    }
 };
 
 // D[tmem] (+)= A[smem] B[smem], 16-bit operands, fp32 accumulation.
@@ -402,7 +468,6 @@ struct WarpRows {
     uint8_t* box;   // its staging boxes of 4 KiB
     int lane;
     int64_t m0;     // first row; lane holds row m0 + lane
-    int64_t M;      // rows that exist
     bool row_in;
 
     // Stores of 32 rows x 128 bytes through the output map: begin() waits until
@@ -528,11 +593,11 @@ __device__ __forceinline__ float4 lse_tile(const GemmArgs& args, const void* tma
 template <bool kBf16, bool kFew, class Rows>
 __device__ __forceinline__ void grad_tile(const GemmArgs& args, const void* tmap_c, Rows& wr, EntryCursor& cur,
                                           int64_t n0, float k2, float lse2, float coef, float (&r)[2][2][32]) {
-    if (n0 >= args.N || (kFew && wr.m0 >= kFewRows)) return;  // (the remainders' rows are written below)
+    if (n0 >= args.p[0].N || (kFew && wr.m0 >= kFewRows)) return;  // (the remainders' rows are written below)
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
         float (&x)[32] = r[c / 2][c % 2];
-        const int ncols = (int)min(int64_t(32), int64_t(args.N) - (n0 + c * 32));
+        const int ncols = (int)min(int64_t(32), int64_t(args.p[0].N) - (n0 + c * 32));
 #pragma unroll
         for (int j = 0; j < 32; ++j) x[j] = ex2(fmaf(x[j], k2, -lse2));
         cur.walk(int(args.v0 + n0) + c * 32, [&](int rel, float p) {
@@ -561,16 +626,16 @@ __device__ __forceinline__ void grad_tile(const GemmArgs& args, const void* tmap
                 }
                 return *reinterpret_cast<const uint32_t*>(&h);
             },
-            n0 + 64 < args.N, int(n0), int(n0) + 64, int(wr.m0), false);
+            n0 + 64 < args.p[0].N, int(n0), int(n0) + 64, int(wr.m0), false);
         if (kFew)
             wr.send_two(
                 tmap_c,
                 [&](int b, int j) { return pack2<true>(r[b][j / 16][2 * (j % 16)], r[b][j / 16][2 * (j % 16) + 1]); },
-                n0 + 64 < args.N, int(n0), int(n0) + 64, int(wr.m0) + kFewRows, false);
+                n0 + 64 < args.p[0].N, int(n0), int(n0) + 64, int(wr.m0) + kFewRows, false);
     } else {
 #pragma unroll
         for (int b = 0; b < 2; ++b)
-            if (n0 + b * 64 < args.N)
+            if (n0 + b * 64 < args.p[0].N)
                 wr.send_two(
                     tmap_c,
                     [&](int plane, int j) {
@@ -590,7 +655,7 @@ __device__ __forceinline__ void grad_tile(const GemmArgs& args, const void* tmap
 // A half tile of a result, through the output map: into fp32 running sums (row
 // y of the map is this part's row) or in the result's type.
 template <bool kF32, class Rows>
-__device__ __forceinline__ void out_tile(const GemmArgs& args, const void* tmap_c, Rows& wr, int y, int64_t n0,
+__device__ __forceinline__ void out_tile(const Problem& args, const void* tmap_c, Rows& wr, int y, int64_t n0,
                                          float scale, float (&r)[2][2][32]) {
     if (n0 >= args.N) return;
     if (kF32 || args.sums) {
@@ -613,10 +678,12 @@ __device__ __forceinline__ void out_tile(const GemmArgs& args, const void* tmap_
     }
 }
 
-template <int kShape, bool kBf16, bool kAMn, bool kBMn, int kEpi>
+template <int kShape, bool kBf16, int kEpi, int kA>
 __global__ void __launch_bounds__(320, 1)
-    head_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
-                     const __grid_constant__ CUtensorMap tmap_c, const GemmArgs args) {
+    head_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmArgs args) {
+    constexpr bool kBMn = kEpi == kEpiOut;  // logits contract K-major operands
+    constexpr int kProblems = kA == kBoth ? 2 : 1;
+    auto mn_major = [](const Problem& p) { return kA == kBoth ? p.a_mn != 0 : kA == kMnMajor; };
     using C = Cfg<kShape>;
     constexpr bool kPair = C::kPair;
     constexpr bool kChunked = !kBf16 || kEpi == kEpiLse;
@@ -650,9 +717,11 @@ __global__ void __launch_bounds__(320, 1)
         }
         ptx::mbar_init(bar_drain, 1);
         ptx::fence_barrier_init();
-        ptx::prefetch_tmap(&tmap_a);
-        ptx::prefetch_tmap(&tmap_b);
-        if (kEpi == kEpiGrad || kEpi == kEpiOut || args.keep) ptx::prefetch_tmap(&tmap_c);
+        for (int q = 0; q < args.problems; ++q) {
+            ptx::prefetch_tmap(&maps.a[q]);
+            ptx::prefetch_tmap(&maps.b[q]);
+            if (kEpi == kEpiGrad || kEpi == kEpiOut || args.keep) ptx::prefetch_tmap(&maps.c[q]);
+        }
     }
     if (warp == 1) tmem_alloc<kPair>(ptx::smem_addr(tmem_slot), C::kTmemCols);
     ptx::tc_fence_before();
@@ -665,30 +734,22 @@ __global__ void __launch_bounds__(320, 1)
 
     // rows that count, and for the gradients of few rows their remainders
     const bool few = kBf16 && kEpi != kEpiLse && args.state->few(args.row0);
-    int rows = args.state->rows(args.row0);
-    if (!few) rows = min(rows, args.count_is == kCountM ? args.M : args.K);
-    else if (kEpi == kEpiOut) rows += kFewRows;
-    const int M = args.count_is == kCountM ? rows : args.M;
-    const int K = args.count_is == kCountK ? rows : args.K;
-    const Walk walk(M, (args.N + kBN - 1) / kBN, C::kTileM, workers,
-                    args.splits > 0 ? args.splits : args.state->dh_splits);
-    const int num_items = walk.items();
-    const int k_steps = (K + kBK - 1) / kBK;
-    const int part_steps = (k_steps + walk.parts - 1) / walk.parts;
-    // Work item `t`: a tile and its share [k0, k1) of the K stages.
-    auto item = [&](int t, int& mb, int& nb, int& part, int& k0, int& k1) {
-        part = 0;
-        k0 = 0;
-        k1 = k_steps;
-        if (t >= walk.whole && walk.parts > 1) {
-            const int tile = walk.whole + (t - walk.whole) / walk.parts;
-            part = (t - walk.whole) % walk.parts;
-            k0 = min(part * part_steps, k_steps);
-            k1 = min(k0 + part_steps, k_steps);
-            t = tile;
-        }
-        walk.coords(t, mb, nb);
+    auto plan_of = [&](const Problem& p) {
+        int rows = args.state->rows(args.row0);
+        if (!few) rows = min(rows, p.count_is == kCountM ? p.M : p.K);
+        else if (kEpi == kEpiOut) rows += kFewRows;
+        return Plan(p.count_is == kCountM ? rows : p.M, p.N, p.count_is == kCountK ? rows : p.K, C::kTileM, workers,
+                    p.splits > 0 ? p.splits : args.state->dh_splits);
     };
+    const Plan plan0 = plan_of(args.p[0]);
+    Plan plan1 = plan0;
+    if (kProblems > 1 && args.problems > 1) {
+        plan1 = plan_of(args.p[1]);
+        plan1.follow(plan0, worker, workers, stage_us(kShape, args.terms), fixed_us(kShape));
+    }
+    // Reading the weights for the one and writing the other is what a call of
+    // few rows does: half of the workers at a time do each.
+    const int flip = kProblems > 1 && args.problems > 1 && args.alternate && (worker & 1);
     auto chunk_end = [&](int k0, int k1) { return kChunked ? min(k0 + kChunkSteps, k1) : k1; };
 
     if (warp == 0) {
@@ -698,52 +759,60 @@ __global__ void __launch_bounds__(320, 1)
             uint32_t phase = 0;
             uint32_t issued[kStages] = {0};
             bool alive = true;
-            for (int t = worker; t < num_items && alive; t += workers) {
-                int mb, nb, split, k0, k1;
-                item(t, mb, nb, split, k0, k1);
-                const int a0 = mb * C::kTileM + rank * kBM, b0 = nb * kBN + rank * C::kBRows;
-                constexpr uint32_t bytes = (kPair ? 2 : 1) * C::kStageBytes;
-                for (int c0 = k0; c0 < k1 && alive; c0 = chunk_end(c0, k1))
-                    for (int term = 0; term < args.terms && alive; ++term) {
-                        // plane pairs, the small products first: (hi, lo), (lo, hi), (hi, hi)
-                        const int pa = args.terms == 3 && term == 1;
-                        const int pb = args.terms == 3 && term == 0;
-                        const int xa = pa * args.pa.x_plane, ya = pa * args.pa.y_plane;
-                        const int xb = pb * args.pb.x_plane, yb = pb * args.pb.y_plane;
-                        const int c1 = chunk_end(c0, k1);
-                        for (int ks = c0; ks < c1; ++ks) {
-                            if (!ptx::mbar_wait(bar_empty + 8 * stage, phase ^ 1)) { alive = false; break; }
-                            const uint32_t own = bar_full + 8 * stage;
-                            const uint32_t full = kPair ? mapa(own, 0) : own;
-                            const uint32_t sa = sbase + stage * C::kStageBytes;
-                            const uint32_t sb = sa + C::kABytes;
-                            // the first CTA's barrier counts both CTAs' bytes
-                            if (rank == 0) ptx::mbar_arrive_expect_tx(own, bytes);
+            for (int ph = 0; ph < (kProblems > 1 ? args.problems : 1) && alive; ++ph) {
+                const int q = kProblems > 1 ? ph ^ flip : 0;
+                const Plan plan = kProblems > 1 && q ? plan1 : plan0;
+                const Problem& p = args.p[q];
+                const CUtensorMap *ma = &maps.a[q], *mb_ = &maps.b[q];
+                const bool a_mn = mn_major(p);
+                for (int i = 0, t; alive && (t = plan.nth(i, worker, workers)) >= 0; ++i) {
+                    int mb, nb, split, k0, k1;
+                    plan.item(t, mb, nb, split, k0, k1);
+                    const int a0 = mb * C::kTileM + rank * kBM, b0 = nb * kBN + rank * C::kBRows;
+                    constexpr uint32_t bytes = (kPair ? 2 : 1) * C::kStageBytes;
+                    for (int c0 = k0; c0 < k1 && alive; c0 = chunk_end(c0, k1))
+                        for (int term = 0; term < args.terms && alive; ++term) {
+                            // plane pairs, the small products first: (hi, lo), (lo, hi), (hi, hi)
+                            const int pa = args.terms == 3 && term == 1;
+                            const int pb = args.terms == 3 && term == 0;
+                            const int xa = pa * p.pa.x_plane, ya = pa * p.pa.y_plane;
+                            const int xb = pb * p.pb.x_plane, yb = pb * p.pb.y_plane;
+                            const int c1 = chunk_end(c0, k1);
+                            for (int ks = c0; ks < c1; ++ks) {
+                                if (!ptx::mbar_wait(bar_empty + 8 * stage, phase ^ 1)) { alive = false; break; }
+                                const uint32_t own = bar_full + 8 * stage;
+                                const uint32_t full = kPair ? mapa(own, 0) : own;
+                                const uint32_t sa = sbase + stage * C::kStageBytes;
+                                const uint32_t sb = sa + C::kABytes;
+                                // the first CTA's barrier counts both CTAs' bytes
+                                if (rank == 0) ptx::mbar_arrive_expect_tx(own, bytes);
 #pragma unroll
-                            for (int h = 0; h < C::kAccs; ++h) {
-                                const uint32_t sah = sa + h * (kBM * kBK * 2);
-                                const int ah = a0 + h * C::kAccRows;
-                                if (kAMn) {
+                                for (int h = 0; h < C::kAccs; ++h) {
+                                    const uint32_t sah = sa + h * (kBM * kBK * 2);
+                                    const int ah = a0 + h * C::kAccRows;
+                                    // (an MN-major map's boxes are 64 x 64, a K-major one's 64 x 128)
+                                    if (a_mn) {
 #pragma unroll
-                                    for (int g = 0; g < kBM / 64; ++g)
-                                        tma_load<kPair>(sah + g * 8192, &tmap_a, (ah / 64 + g) * args.pa.x_block + xa,
-                                                        ya + ks * kBK, full);
-                                } else {
-                                    tma_load<kPair>(sah, &tmap_a, ks * args.pa.x_block + xa, ya + ah, full);
+                                        for (int g = 0; g < kBM / 64; ++g)
+                                            tma_load<kPair>(sah + g * 8192, ma, (ah / 64 + g) * p.pa.x_block + xa,
+                                                            ya + ks * kBK, full);
+                                    } else {
+                                        tma_load<kPair>(sah, ma, ks * p.pa.x_block + xa, ya + ah, full);
+                                    }
                                 }
-                            }
-                            if (kBMn) {
+                                if (kBMn) {
 #pragma unroll
-                                for (int g = 0; g < C::kBRows / 64; ++g)
-                                    tma_load<kPair>(sb + g * 8192, &tmap_b, (b0 / 64 + g) * args.pb.x_block + xb,
-                                                    yb + ks * kBK, full);
-                            } else {
-                                tma_load<kPair>(sb, &tmap_b, ks * args.pb.x_block + xb, yb + b0, full);
+                                    for (int g = 0; g < C::kBRows / 64; ++g)
+                                        tma_load<kPair>(sb + g * 8192, mb_, (b0 / 64 + g) * p.pb.x_block + xb,
+                                                        yb + ks * kBK, full);
+                                } else {
+                                    tma_load<kPair>(sb, mb_, ks * p.pb.x_block + xb, yb + b0, full);
+                                }
+                                issued[stage] += 1;
+                                if (++stage == kStages) { stage = 0; phase ^= 1; }
                             }
-                            issued[stage] += 1;
-                            if (++stage == kStages) { stage = 0; phase ^= 1; }
                         }
-                    }
+                }
             }
             // Let every copy land, and every MMA's release of a stage arrive,
             // before this CTA (and the pair) can exit.
@@ -756,13 +825,21 @@ __global__ void __launch_bounds__(320, 1)
     } else if (warp == 1) {
         if (lane == 0 && rank == 0) {
             // ---------------- MMA issuer ----------------
-            const uint32_t idesc = idesc_f16(kBf16, kAMn, kBMn, C::kAccRows, kBN);
             int stage = 0;
             uint32_t phase = 0, it = 0;
             bool alive = true;
-            for (int t = worker; t < num_items && alive; t += workers) {
+            for (int ph = 0; ph < (kProblems > 1 ? args.problems : 1) && alive; ++ph) {
+                const int q = kProblems > 1 ? ph ^ flip : 0;
+                const Plan plan = kProblems > 1 && q ? plan1 : plan0;
+                const bool a_mn = mn_major(args.p[q]);
+                const uint32_t idesc = idesc_f16(kBf16, a_mn, kBMn, C::kAccRows, kBN);
+                // K-major: 16 elements of K are 32 bytes of the swizzled row, 8-row groups 1024 bytes apart.
+                // MN-major: 16 rows of K are 2048 bytes, 64-element blocks of the other mode 8192 bytes
+                // apart, 8-row groups of K 1024.
+                const uint32_t a_step = a_mn ? 2048 : 32, a_block = a_mn ? 8192 : 0;
+                for (int i = 0, t; alive && (t = plan.nth(i, worker, workers)) >= 0; ++i) {
                 int mb, nb, split, k0, k1;
-                item(t, mb, nb, split, k0, k1);
+                plan.item(t, mb, nb, split, k0, k1);
                 for (int c0 = k0; c0 < k1 && alive; c0 = chunk_end(c0, k1), ++it) {
                     // one tile alternates between the two accumulators, a tall one fills both
                     const uint32_t buf0 = C::kAccs == 1 ? it & 1 : 0, drained = (C::kAccs == 1 ? it >> 1 : it) & 1;
@@ -782,15 +859,10 @@ __global__ void __launch_bounds__(320, 1)
                             const uint32_t sb = sbase + stage * C::kStageBytes + C::kABytes;
 #pragma unroll
                             for (int j = 0; j < kBK / 16; ++j) {
-                                // K-major: 16 elements of K are 32 bytes of the swizzled row, 8-row groups 1024
-                                // bytes apart.  MN-major: 16 rows of K are 2048 bytes, 64-element blocks of the
-                                // other mode 8192 bytes apart, 8-row groups of K 1024.
-                                const uint64_t ad =
-                                    kAMn ? ptx::smem_desc(sa + 2048 * j, 8192, 1024, ptx::kLayoutSwizzle128)
-                                         : ptx::smem_desc(sa + 32 * j, 0, 1024, ptx::kLayoutSwizzle128);
-                                const uint64_t bd =
-                                    kBMn ? ptx::smem_desc(sb + 2048 * j, 8192, 1024, ptx::kLayoutSwizzle128)
-                                         : ptx::smem_desc(sb + 32 * j, 0, 1024, ptx::kLayoutSwizzle128);
+                                const uint64_t ad = ptx::smem_desc(sa + a_step * j, a_block, 1024, ptx::kLayoutSwizzle128);
+                                const uint64_t bd = kBMn
+                                                        ? ptx::smem_desc(sb + 2048 * j, 8192, 1024, ptx::kLayoutSwizzle128)
+                                                        : ptx::smem_desc(sb + 32 * j, 0, 1024, ptx::kLayoutSwizzle128);
                                 mma_f16<kPair>(acc, ad, bd, idesc, (ks > 0 || j > 0) ? 1u : 0u);
                             }
                             if (C::kAccs > 1 && ks + 1 == steps) commit<kPair>(bar_tmem_full + 8 * buf);
@@ -802,6 +874,7 @@ __global__ void __launch_bounds__(320, 1)
                     if (!alive) break;
                     if (C::kAccs == 1) commit<kPair>(bar_tmem_full + 8 * buf0);
                 }
+            }
             }
             // every MMA is done before TMEM is released
             commit<kPair>(bar_drain);
@@ -815,14 +888,15 @@ __global__ void __launch_bounds__(320, 1)
         WarpRows<C::kBoxes> wr;
         wr.box = smem + C::kOffOut + (warp - 2) * C::kBoxes * 4096;
         wr.lane = lane;
-        wr.M = M;
         // inverse of the operands' power-of-two scales
-        float inv = 1.0f;
-        if (args.scale_a >= 0) inv *= pow2i(-scale_exponent(args.state->amax[args.scale_a]));
-        if (args.scale_b >= 0) inv *= pow2i(-scale_exponent(args.state->amax[args.scale_b]));
-        const float k2 = args.logit_scale * kLog2e * inv;
+        auto inverse = [&](const Problem& p) {
+            float inv = 1.0f;
+            if (p.scale_a >= 0) inv *= pow2i(-scale_exponent(args.state->amax[p.scale_a]));
+            if (p.scale_b >= 0) inv *= pow2i(-scale_exponent(args.state->amax[p.scale_b]));
+            return inv;
+        };
+        const float k2 = args.logit_scale * kLog2e * inverse(args.p[0]);
         const float gscale = kEpi == kEpiGrad && !kBf16 ? pow2i(scale_exponent(args.state->amax[2])) : 1.0f;
-        const float out_scale = kEpi == kEpiOut ? inv * args.state->grad_scale : 1.0f;
         auto release = [&](uint32_t buf) {
             ptx::tc_fence_before();
             __syncwarp();
@@ -833,18 +907,25 @@ __global__ void __launch_bounds__(320, 1)
         };
         uint32_t it = 0;
         bool alive = true;
-        for (int t = worker; t < num_items && alive; t += workers) {
+        for (int ph = 0; ph < (kProblems > 1 ? args.problems : 1) && alive; ++ph) {
+            const int q = kProblems > 1 ? ph ^ flip : 0;
+            const Plan plan = kProblems > 1 && q ? plan1 : plan0;
+            const Problem& p = args.p[q];
+            const void* tmap_c = &maps.c[q];
+            const int M = kEpi == kEpiOut ? 0 : min(args.state->rows(args.row0), few ? INT_MAX : p.M);
+            const float out_scale = kEpi == kEpiOut ? inverse(p) * args.state->grad_scale : 1.0f;
+            for (int i = 0, t; alive && (t = plan.nth(i, worker, workers)) >= 0; ++i) {
             int mb, nb, split, k0, k1;
-            item(t, mb, nb, split, k0, k1);
+            plan.item(t, mb, nb, split, k0, k1);
 #pragma unroll 1
             for (int h = 0; h < C::kAccs && alive; ++h) {
     wr.m0 = int64_t(mb) * C::kTileM + h * C::kAccRows + rank * kBM + quarter * 32;
                 const int64_t m = wr.m0 + lane;
                 wr.row_in = m < M;
                 const int64_t ncol0 = int64_t(nb) * kBN + half * kCols;
-                const int64_t n_end = min(int64_t(args.N), ncol0 + kCols);
+                const int64_t n_end = min(int64_t(p.N), ncol0 + kCols);
                 // a pair's second half may lie past the rows that the workspace holds
-                const bool rows_in = kEpi == kEpiOut || wr.m0 < (args.M + kBM - 1) / kBM * kBM;
+                const bool rows_in = kEpi == kEpiOut || wr.m0 < (p.M + kBM - 1) / kBM * kBM;
                 // what the row needs beside its accumulator, while the MMAs run
                 EntryCursor cur;
                 float lse2 = 0.0f, coef = 0.0f;
@@ -895,16 +976,17 @@ __global__ void __launch_bounds__(320, 1)
                 if (!rows_in) continue;
                 if (kEpi != kEpiOut) cur.begin();
                 if (kEpi == kEpiLse) {
-                    const float4 st = lse_tile<kBf16, 2>(args, &tmap_c, wr, cur, ncol0, n_end, k2, r);
+                    const float4 st = lse_tile<kBf16, 2>(args, tmap_c, wr, cur, ncol0, n_end, k2, r);
                     args.partial[m * args.half_tiles + (args.v0 + ncol0) / kCols] = st;
                 } else if (kEpi == kEpiGrad) {
-                    if (few) grad_tile<kBf16, kBf16>(args, &tmap_c, wr, cur, ncol0, k2, lse2, coef, r);
-                    else grad_tile<kBf16, false>(args, &tmap_c, wr, cur, ncol0, k2, lse2, coef, r);
+                    if (few) grad_tile<kBf16, kBf16>(args, tmap_c, wr, cur, ncol0, k2, lse2, coef, r);
+                    else grad_tile<kBf16, false>(args, tmap_c, wr, cur, ncol0, k2, lse2, coef, r);
                 } else {
-                    out_tile<!kBf16>(args, &tmap_c, wr, args.sums ? walk.sum_row(split, int(wr.m0)) : int(wr.m0), ncol0,
+                    out_tile<!kBf16>(p, tmap_c, wr, p.sums ? plan.walk.sum_row(split, int(wr.m0)) : int(wr.m0), ncol0,
                                      out_scale, r);
                 }
             }
+        }
         }
         if (lane == 0) ptx::bulk_wait_group0();  // this warp's stores are done
     }

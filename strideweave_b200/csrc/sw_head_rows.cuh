@@ -28,23 +28,22 @@ __device__ __forceinline__ bool entry_counts(int index, float logit, int64_t V) 
 }
 
 // Estimated microseconds of a contraction in tiles of a shape, the tiles of its
-// last, partial wave cut into s parts of the K walk: waves x (stages + a tile's
-// cost that nothing hides), and the traffic of writing and adding the parts.  A
-// K stage takes 0.27 us (kSingle: 128 x 256 on one SM, kPair2: 256 x 256 on two)
-// or 0.52 (kTall), a tile's fill and drain 2, 2.5 and 5 us, an adding launch 3.
+// last, partial wave cut into s parts of the K walk: waves x (stages + what a tile
+// hides nowhere), and the traffic of writing and adding the parts.
 constexpr int kMaxParts = 64;       // where the tiles do not fill one wave
 constexpr int kMaxTailParts = 4;    // of the tiles after whole waves
-__host__ __device__ inline int shape_workers(int shape, int sms) { return shape == kSingle ? sms : sms / 2; }
+__host__ __device__ inline int64_t tiles_of(int64_t M, int64_t N, int shape) {
+    return ((M + shape_rows(shape) - 1) >> (7 + shape)) * ((N + kBN - 1) / kBN);
+}
 __host__ __device__ inline float spread_cost(int64_t M, int64_t N, int64_t K, int terms, int shape, int sms, int s) {
     const int workers = shape_workers(shape, sms), steps = int((K + kBK - 1) / kBK);
-    const int64_t tiles = ((M + shape_rows(shape) - 1) >> (7 + shape)) * ((N + kBN - 1) / kBN);
+    const int64_t tiles = tiles_of(M, N, shape);
     const int whole = int(tiles / workers), rest = int(tiles - int64_t(whole) * workers);
     if (s > 1 && (steps < 4 * s || rest == 0 || (whole ? s > kMaxTailParts : rest * s > 2 * workers))) return 1e30f;
-    const float stage = float(terms) * (shape == kTall ? 0.52f : 0.27f);
-    const float fixed = shape == kTall ? 5.0f : shape == kPair2 ? 2.5f : 2.0f;
-    const int share = (steps + s - 1) / s;
-    float us = float(whole) * (float(steps) * stage + fixed) +
-               float((rest * s + workers - 1) / workers) * (float(share) * stage + fixed);
+    const float stage = stage_us(shape, terms), fixed = fixed_us(shape);
+    const float one = float(steps) * stage + fixed, part = float((steps + s - 1) / s) * stage + fixed;
+    const float waves = float(whole) * one + float((rest * s + workers - 1) / workers) * part;
+    float us = waves;
     if (s > 1) us += 3.0f + float(rest) * float(s) * float(shape_rows(shape) * kBN) * (8.0f / 6.0e6f);
     return us;
 }

@@ -73,25 +73,19 @@ int device_sms() {
     return sms[dev];
 }
 
-// How a contraction is spread over the SMs: the tile shape and the parts of the
-// K walk.
+// How a contraction is spread over the SMs: the parts of the K walk that suit a
+// tile shape, and the estimate.  `sum_us`: what it costs more to go through fp32
+// sums when nothing else asks for them.
 struct Spread {
-    int shape;
     int splits;
+    float us;
 };
-// `sum_us`: what it costs more to go through fp32 sums when nothing else asks
-// for them.
-Spread choose_spread(int64_t M, int64_t N, int64_t K, int terms, int tallest, bool may_split, float sum_us = 0.0f) {
-    Spread best{kSingle, 1};
-    float best_us = 1e30f;
-    for (int shape = tallest; shape >= kSingle; --shape)
-        for (int s = 1; s <= (may_split ? kMaxParts : 1); ++s) {
-            const float us = spread_cost(M, N, K, terms, shape, device_sms(), s) + (s > 1 ? sum_us : 0.0f);
-            if (us < best_us * 0.97f) {
-                best_us = us;
-                best = Spread{shape, s};
-            }
-        }
+Spread choose_parts(int64_t M, int64_t N, int64_t K, int terms, int shape, bool may_split, float sum_us = 0.0f) {
+    Spread best{1, 1e30f};
+    for (int s = 1; s <= (may_split ? kMaxParts : 1); ++s) {
+        const float us = spread_cost(M, N, K, terms, shape, device_sms(), s) + (s > 1 ? sum_us : 0.0f);
+        if (us < best.us * 0.97f) best = Spread{s, us};
+    }
     return best;
 }
 
@@ -129,20 +123,31 @@ int make_target_map(CUtensorMap* map, const Target& t) {
     return SW_OK;
 }
 
-template <int kShape, bool kBf16, bool kAMn, bool kBMn, int kEpi>
-int launch_gemm(const Operand& a, const Operand& b, const Target& c, const GemmArgs& args, cudaStream_t stream) {
+// The operands and the result of one contraction.
+struct Tensors {
+    Operand a, b;
+    Target c;
+};
+
+template <int kShape, bool kBf16, int kEpi, int kA>
+int launch_gemm(const Tensors* t, GemmArgs& args, cudaStream_t stream) {
     using Cf = Cfg<kShape>;
-    constexpr bool kPair = Cf::kPair;
-    const int64_t tiles = int64_t((args.M + Cf::kTileM - 1) / Cf::kTileM) * ((args.N + kBN - 1) / kBN);
-    if (tiles == 0) return SW_OK;
-    CUtensorMap ma, mb, mc;
-    int rc = make_map(&ma, a.ptr, a.rows, a.cols, a.ld, kAMn ? kBK : kBM);
-    if (rc != SW_OK) return rc;
-    rc = make_map(&mb, b.ptr, b.rows, b.cols, b.ld, kBMn ? kBK : Cf::kBRows);
-    if (rc != SW_OK) return rc;
-    memset(&mc, 0, sizeof(mc));
-    if (c.ptr && (rc = make_target_map(&mc, c)) != SW_OK) return rc;
-    auto kernel = head_gemm_kernel<kShape, kBf16, kAMn, kBMn, kEpi>;
+    Maps maps;
+    memset(&maps, 0, sizeof(maps));
+    for (int q = 0; q < args.problems; ++q) {
+        // boxes of K-major operands are 64 wide and as high as a CTA's share of
+        // the tile, of MN-major ones 64 x 64
+        Problem& p = args.p[q];
+        int rc = make_map(&maps.a[q], t[q].a.ptr, t[q].a.rows, t[q].a.cols, t[q].a.ld, p.a_mn ? kBK : kBM);
+        if (rc == SW_OK)
+            rc = make_map(&maps.b[q], t[q].b.ptr, t[q].b.rows, t[q].b.cols, t[q].b.ld,
+                          kEpi == kEpiOut ? kBK : Cf::kBRows);
+        if (rc == SW_OK && t[q].c.ptr) rc = make_target_map(&maps.c[q], t[q].c);
+        if (rc != SW_OK) return rc;
+        p.pa = t[q].a.plane;
+        p.pb = t[q].b.plane;
+    }
+    auto kernel = head_gemm_kernel<kShape, kBf16, kEpi, kA>;
     static bool configured[64] = {};  // per device: the attribute stays
     int dev = 0;
     SW_CUDA_TRY(cudaGetDevice(&dev), "cudaGetDevice");
@@ -151,9 +156,14 @@ int launch_gemm(const Operand& a, const Operand& b, const Target& c, const GemmA
                     "linear head smem");
         if (dev >= 0 && dev < 64) configured[dev] = true;
     }
-    constexpr int kCtas = kPair ? 2 : 1;
+    constexpr int kCtas = Cf::kPair ? 2 : 1;
+    // every SM, unless it is known here that there are fewer tiles
+    int64_t items = device_sms() / kCtas;
+    if (args.problems == 1 && args.p[0].splits == 1)
+        items = std::min<int64_t>(items, tiles_of(args.p[0].M, args.p[0].N, kShape));
+    if (items == 0) return SW_OK;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(kCtas * (unsigned)(args.splits == 1 ? std::min<int64_t>(tiles, device_sms() / kCtas) : device_sms() / kCtas));
+    cfg.gridDim = dim3(kCtas * (unsigned)items);
     cfg.blockDim = dim3(Cf::kThreads);
     cfg.dynamicSmemBytes = Cf::kSmemBytes;
     cfg.stream = stream;
@@ -165,24 +175,23 @@ int launch_gemm(const Operand& a, const Operand& b, const Target& c, const GemmA
     attr[1].val.clusterDim.y = 1;
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = kPair ? 2 : 1;
-    SW_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, ma, mb, mc, args), "linear head contraction");
+    cfg.numAttrs = Cf::kPair ? 2 : 1;
+    SW_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, maps, args), "linear head contraction");
     return SW_OK;
 }
 
-template <bool kBf16, bool kAMn, bool kBMn, int kEpi>
-int gemm(const Operand& a, const Operand& b, const Target& c, GemmArgs args, int shape, cudaStream_t stream) {
+// One contraction, or the gradients' two in one launch (kBoth, single CTAs' tiles).
+template <bool kBf16, int kEpi, int kA>
+int gemm(const Tensors* t, GemmArgs& args, int shape, cudaStream_t stream) {
     args.terms = kBf16 ? 1 : 3;
-    args.pa = a.plane;
-    args.pb = b.plane;
-    if (kEpi != kEpiOut) args.splits = 1;
-    if (shape == kSingle) return launch_gemm<kSingle, kBf16, kAMn, kBMn, kEpi>(a, b, c, args, stream);
+    if (kA == kBoth || shape == kSingle) return launch_gemm<kSingle, kBf16, kEpi, kA>(t, args, stream);
     // results summed in registers (Float32, and the statistics) have no tall tile,
     // and the logits' gradient has too much to do after a tile (4096 x 32000, dim
     // 1024 / 2048 / 4096: 242 / 395 / 719 us against 201 / 362 / 695)
-    constexpr int kTallest = kBf16 && kEpi == kEpiOut ? kTall : kPair2;
-    return shape == kTall ? launch_gemm<kTallest, kBf16, kAMn, kBMn, kEpi>(a, b, c, args, stream)
-                          : launch_gemm<kPair2, kBf16, kAMn, kBMn, kEpi>(a, b, c, args, stream);
+    constexpr int kMost = kA == kBoth ? kSingle : kBf16 && kEpi == kEpiOut ? kTall : kPair2;
+    constexpr int kMiddle = kA == kBoth ? kSingle : kPair2;
+    return shape == kTall ? launch_gemm<kMost, kBf16, kEpi, kA>(t, args, stream)
+                          : launch_gemm<kMiddle, kBf16, kEpi, kA>(t, args, stream);
 }
 
 struct Bump {
@@ -246,8 +255,10 @@ struct Shape {
     // time.  Packed weights are laid out `piece` columns at a time too.
     bool keep;
     int64_t rows, piece;
-    int logits_shape, dh_shape;
-    Spread dw;
+    // Few rows (one row tile): the gradients' contractions share a launch, which
+    // reads the weights while it writes their gradient.
+    bool together;
+    int logits_shape, dh_shape, dw_shape, dw_splits;
     // rows of fp32 sums of each gradient (0: it is written at once); dh's rows
     // are always put in place from sums, whose parts are chosen on the device
     int64_t dh_sum_rows, dw_sum_rows, ld_acc;
@@ -420,13 +431,15 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
     // logits of compact rows [r0, r0 + n) and columns [v0, v0 + nv)
     auto logits = [&](int64_t r0, int64_t n, int64_t v0, int64_t nv) {
         GemmArgs a = g;
-        a.M = (int)n;
-        a.N = (int)nv;
-        a.K = (int)s.D;
-        a.count_is = kCountM;
+        a.problems = 1;
+        a.p[0].M = (int)n;
+        a.p[0].N = (int)nv;
+        a.p[0].K = (int)s.D;
+        a.p[0].count_is = kCountM;
+        a.p[0].splits = 1;
+        a.p[0].scale_a = kF32 ? 0 : -1;
+        a.p[0].scale_b = kF32 ? 1 : -1;
         a.row0 = (int)r0;
-        a.scale_a = kF32 ? 0 : -1;
-        a.scale_b = kF32 ? 1 : -1;
         a.v0 = v0;
         a.ent_idx = l.ent_idx + r0 * g.ent_k;
         a.ent_p = l.ent_p ? l.ent_p + r0 * g.ent_k : nullptr;
@@ -492,7 +505,7 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
             sa.ld = s.ld_acc;
             sa.splits = splits;
             sa.tile_m = shape_rows(shape);
-            sa.workers = shape_workers(shape, device_sms());
+            sa.workers = shape_workers(shape, sms);
             sa.rows = rows;
             sa.cols = s.D;
             sa.state = l.state;
@@ -509,42 +522,59 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
                         "linear head sums");
             return SW_OK;
         };
+        Tensors t[2];
+        uint8_t* dw = c.dw ? static_cast<uint8_t*>(c.dw) + v0 * p.dw_row * esize : nullptr;
         if (c.dh && n > 0) {
-            a.M = (int)n;
-            a.N = (int)s.D;
-            a.K = (int)nv;
-            a.count_is = kCountM;
-            a.scale_a = kF32 ? 2 : -1;
-            a.scale_b = kF32 ? 1 : -1;
-            a.splits = 0;
-            a.sums = 1;
-            a.first = first_v;
-            const Target out{l.dh_sums, s.dh_sum_rows, s.ld_acc, s.ld_acc, true};
-            int rc = gemm<kBf16, false, true, kEpiOut>(gr, w, out, a, s.dh_shape, stream);
-            if (rc == SW_OK && last_v)
-                rc = finish(l.dh_sums, 0, s.dh_shape, n, true, l.row_map + r0, c.dh, p.dh_row, p.dh_col);
-            if (rc != SW_OK) return rc;
+            Problem& q = a.p[a.problems];
+            q.M = (int)n;
+            q.N = (int)s.D;
+            q.K = (int)nv;
+            q.count_is = kCountM;
+            q.scale_a = kF32 ? 2 : -1;
+            q.scale_b = kF32 ? 1 : -1;
+            q.splits = 0;
+            q.sums = 1;
+            q.first = first_v;
+            t[a.problems++] = Tensors{gr, w, Target{l.dh_sums, s.dh_sum_rows, s.ld_acc, s.ld_acc, true}};
         }
-        if (c.dw) {
-            uint8_t* dst = static_cast<uint8_t*>(c.dw) + v0 * p.dw_row * esize;
-            a.M = (int)nv;
-            a.N = (int)s.D;
-            a.K = (int)n;
-            a.count_is = kCountK;
-            a.scale_a = kF32 ? 2 : -1;
-            a.scale_b = kF32 ? 0 : -1;
-            a.splits = s.dw.splits;
-            a.sums = s.dw_sum_rows > 0;
-            a.first = first_r;
-            const Target out = a.sums ? Target{l.dw_sums, s.dw_sum_rows, s.ld_acc, s.ld_acc, true}
-                                      : Target{dst, nv, s.D, p.dw_row, kF32};
-            int rc = gemm<kBf16, true, true, kEpiOut>(gr, states(r0, round_up(std::max<int64_t>(n, 1), kBM)), out, a,
-                                                      s.dw.shape, stream);
-            if (rc == SW_OK && a.sums && last_r)
-                rc = finish(l.dw_sums, s.dw.splits, s.dw.shape, nv, false, nullptr, dst, p.dw_row, p.dw_col);
-            if (rc != SW_OK) return rc;
+        if (dw) {
+            Problem& q = a.p[a.problems];
+            q.M = (int)nv;
+            q.N = (int)s.D;
+            q.K = (int)n;
+            q.count_is = kCountK;
+            q.a_mn = 1;
+            q.scale_a = kF32 ? 2 : -1;
+            q.scale_b = kF32 ? 0 : -1;
+            q.splits = s.dw_splits;
+            q.sums = s.dw_sum_rows > 0;
+            q.first = first_r;
+            Target out{dw, nv, s.D, p.dw_row, kF32};
+            if (q.sums) out = Target{l.dw_sums, s.dw_sum_rows, s.ld_acc, s.ld_acc, true};
+            const Operand st = states(r0, round_up(std::max<int64_t>(n, 1), kBM));
+            t[a.problems++] = Tensors{gr, st, out};
         }
-        return SW_OK;
+        int rc = SW_OK;
+        if (a.problems == 2 && s.together) {
+            a.alternate = 1;
+            rc = gemm<kBf16, kEpiOut, kBoth>(t, a, kSingle, stream);
+        } else {
+            const bool two = a.problems == 2;
+            a.problems = 1;
+            if (c.dh && n > 0) rc = gemm<kBf16, kEpiOut, kKMajor>(t, a, s.dh_shape, stream);
+            if (rc == SW_OK && dw) {
+                if (two) {
+                    t[0] = t[1];
+                    a.p[0] = a.p[1];
+                }
+                rc = gemm<kBf16, kEpiOut, kMnMajor>(t, a, s.dw_shape, stream);
+            }
+        }
+        if (rc == SW_OK && c.dh && n > 0 && last_v)
+            rc = finish(l.dh_sums, 0, s.dh_shape, n, true, l.row_map + r0, c.dh, p.dh_row, p.dh_col);
+        if (rc == SW_OK && s.dw_sum_rows && last_r)
+            rc = finish(l.dw_sums, s.dw_splits, s.dw_shape, nv, false, nullptr, dw, p.dw_row, p.dw_col);
+        return rc;
     };
     if (s.keep) {
         Operand w;
@@ -554,9 +584,8 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
             GemmArgs a = logits(r0, n, 0, s.V);
             a.keep = 1;
             a.ent_s = l.ent_s + r0 * g.ent_k;
-            rc = gemm<kBf16, false, false, kEpiLse>(states(r0, round_up(std::max<int64_t>(n, 1), kBM)), w, grad_out, a,
-                                                    s.logits_shape, stream);
-            if (rc != SW_OK) return rc;
+            const Tensors t{states(r0, round_up(std::max<int64_t>(n, 1), kBM)), w, grad_out};
+            if ((rc = gemm<kBf16, kEpiLse, kKMajor>(&t, a, s.logits_shape, stream)) != SW_OK) return rc;
             if ((rc = losses(r0, n, true)) != SW_OK) return rc;
             if ((rc = gradients(r0, n, 0, s.V, w, true, true, r0 == 0, r0 + s.rows >= s.T)) != SW_OK) return rc;
         }
@@ -568,9 +597,9 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
             const int64_t n = std::min(step, s.V - v0);
             Operand w;
             if ((rc = weights(v0, n, &w)) != SW_OK) return rc;
-            rc = gemm<kBf16, false, false, kEpiLse>(states(0, s.rows_pad), w, none, logits(0, s.T, v0, n), s.logits_shape,
-                                                    stream);
-            if (rc != SW_OK) return rc;
+            GemmArgs a = logits(0, s.T, v0, n);
+            const Tensors t{states(0, s.rows_pad), w, none};
+            if ((rc = gemm<kBf16, kEpiLse, kKMajor>(&t, a, s.logits_shape, stream)) != SW_OK) return rc;
         }
         if ((rc = losses(0, s.T, false)) != SW_OK) return rc;
     }
@@ -579,9 +608,9 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
         const int64_t n = std::min(s.piece, s.V - v0);
         Operand w;
         if ((rc = weights(v0, n, &w)) != SW_OK) return rc;
-        rc = gemm<kBf16, false, false, kEpiGrad>(states(0, s.rows_pad), w, grad_out, logits(0, s.T, v0, n),
-                                                 s.logits_shape, stream);
-        if (rc != SW_OK) return rc;
+        GemmArgs a = logits(0, s.T, v0, n);
+        const Tensors t{states(0, s.rows_pad), w, grad_out};
+        if ((rc = gemm<kBf16, kEpiGrad, kKMajor>(&t, a, s.logits_shape, stream)) != SW_OK) return rc;
         if ((rc = gradients(0, s.T, v0, n, w, v0 == 0, v0 + n == s.V, true, true)) != SW_OK) return rc;
     }
     return SW_OK;
@@ -681,28 +710,36 @@ int check_and_run(const char* name, Call& c, void* stream_ptr) {
         const int64_t per_column = (grads ? s.planes * s.rows_pad * 2 : 0) + (s.pack_w ? s.planes * s.ld_h * 2 : 0);
         if (per_column > 0) s.piece = std::min(s.piece, std::max<int64_t>(budget / per_column / 256 * 256, 256));
     }
-    const int tallest = s.f32 ? kPair2 : kTall;
-    s.logits_shape = choose_spread(std::min(s.rows, T), std::min(s.piece, V), D, terms, kPair2, false).shape;
     s.half_tiles = (V + kBN - 1) / kBN * 2;
-    s.dh_shape = kSingle;
-    s.dw = Spread{kSingle, 1};
-    s.dh_sum_rows = s.dw_sum_rows = 0;
-    if (c.dh && T > 0) {
-        const int64_t n = std::min(s.rows, T), nv = std::min(s.piece, V);
-        s.dh_shape = choose_spread(n, D, nv, terms, tallest, true).shape;
-        s.dh_sum_rows = sum_rows(n, D, s.dh_shape);
+    const int64_t n = std::min(s.rows, T), nv = std::min(s.piece, V);
+    s.logits_shape = choose_parts(n, nv, D, terms, kSingle, false).us <
+                             0.97f * choose_parts(n, nv, D, terms, kPair2, false).us
+                         ? kSingle
+                         : kPair2;
+    // dw is written at once through TMA where that can describe it (rows that end
+    // inside 16 bytes would be written past their end).
+    const int64_t es = s.f32 ? 4 : 2;
+    const bool direct = p->dw_col == 1 && p->dw_row * es % 16 == 0 && D * es % 16 == 0 && p->dw_row >= D &&
+                        (reinterpret_cast<uintptr_t>(c.dw) & 15) == 0 && s.rows >= T;
+    const float sum_us = direct ? float(nv) * float(D) * float(8 + es) / 6.0e6f : 0.0f;
+    s.together = c.dh && c.dw && n <= kBM;
+    s.dh_shape = s.dw_shape = kSingle;
+    s.dw_splits = 1;
+    float dh_us = 1e30f, dw_us = 1e30f;
+    for (int shape = s.together ? kSingle : s.f32 ? kPair2 : kTall; grads && shape >= kSingle; --shape) {
+        const Spread dh = choose_parts(n, D, nv, terms, shape, true), dw = choose_parts(nv, D, n, terms, shape, true, sum_us);
+        if (dh.us < dh_us * 0.97f) {
+            dh_us = dh.us;
+            s.dh_shape = shape;
+        }
+        if (dw.us < dw_us * 0.97f) {
+            dw_us = dw.us;
+            s.dw_shape = shape;
+            s.dw_splits = dw.splits;
+        }
     }
-    if (c.dw) {
-        const int64_t n = std::min(s.rows, T), nv = std::min(s.piece, V);
-        // written at once through TMA where that can describe dw (rows that end
-        // inside 16 bytes would be written past their end)
-        const int64_t es = s.f32 ? 4 : 2;
-        const bool direct = p->dw_col == 1 && p->dw_row * es % 16 == 0 && D * es % 16 == 0 && p->dw_row >= D &&
-                            (reinterpret_cast<uintptr_t>(c.dw) & 15) == 0 && s.rows >= T;
-        s.dw = choose_spread(nv, D, n, terms, tallest, true,
-                             direct ? float(nv) * float(D) * float(8 + es) / 6.0e6f : 0.0f);
-        if (!direct || s.dw.splits > 1) s.dw_sum_rows = sum_rows(nv, D, s.dw.shape);
-    }
+    s.dh_sum_rows = c.dh && T > 0 ? sum_rows(n, D, s.dh_shape) : 0;
+    s.dw_sum_rows = c.dw && (!direct || s.dw_splits > 1) ? sum_rows(nv, D, s.dw_shape) : 0;
 
     Bump measure{nullptr, 0};
     lay_out(measure, c, s);
