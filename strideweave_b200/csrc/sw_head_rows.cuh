@@ -390,8 +390,10 @@ __global__ void __launch_bounds__(256) split_kernel(const SplitJob j0, const Spl
     const int64_t cta = blockIdx.x - (second ? j0.ctas : 0);
     const int64_t valid = j.row_map ? min(j.rows, int64_t(state->count)) : j.rows;
     const float scale = kF32 ? pow2i(scale_exponent(state->amax[j.scale_of])) : 1.0f;
-    if (j.vec) {
-        const int64_t units = j.cols / 8;  // ld == cols here
+    if (j.sc == 1) {
+        // a thread writes 8 columns; it reads them as vectors where rows are
+        // aligned, else one by one (neighbouring threads share the sectors)
+        const int64_t units = j.ld / 8;
 #pragma unroll 2
         for (int64_t u = cta * 256 + threadIdx.x; u < j.rows_pad * units; u += int64_t(j.ctas) * 256) {
             const int64_t r = u / units, c = (u - r * units) * 8;
@@ -399,9 +401,15 @@ __global__ void __launch_bounds__(256) split_kernel(const SplitJob j0, const Spl
             if (r < valid) {
                 const int64_t at = (j.row_map ? int64_t(j.row_map[r]) : r) * j.sr + c;
                 if (kF32) {
-                    const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(j.src) + at);
-                    const float4 a = p[0], b = p[1];
-                    const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+                    const float* p = static_cast<const float*>(j.src) + at;
+                    float v[8];
+                    if (j.vec) {
+                        const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+                        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+                    } else {
+#pragma unroll
+                        for (int q = 0; q < 8; ++q) v[q] = c + q < j.cols ? p[q] : 0.0f;
+                    }
                     uint32_t h[4], l[4];
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
@@ -413,7 +421,15 @@ __global__ void __launch_bounds__(256) split_kernel(const SplitJob j0, const Spl
                     hi = make_uint4(h[0], h[1], h[2], h[3]);
                     lo = make_uint4(l[0], l[1], l[2], l[3]);
                 } else {
-                    hi = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(j.src) + at);
+                    const uint16_t* p = static_cast<const uint16_t*>(j.src) + at;
+                    if (j.vec) {
+                        hi = *reinterpret_cast<const uint4*>(p);
+                    } else {
+                        uint32_t w[8];
+#pragma unroll
+                        for (int q = 0; q < 8; ++q) w[q] = c + q < j.cols ? p[q] : 0;
+                        hi = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
+                    }
                 }
             }
             *reinterpret_cast<uint4*>(j.dst + r * j.ld + c) = hi;
@@ -422,7 +438,7 @@ __global__ void __launch_bounds__(256) split_kernel(const SplitJob j0, const Spl
         return;
     }
     // 32 x 32 tiles through shared memory, read along the unit stride
-    const bool by_rows = j.sr == 1 && j.sc != 1;
+    const bool by_rows = j.sr == 1;
     const int x = threadIdx.x & 31, y0 = threadIdx.x >> 5;
     const int64_t tiles_c = (j.ld + 31) / 32, tiles = (j.rows_pad + 31) / 32 * tiles_c;
     for (int64_t t = cta; t < tiles; t += j.ctas) {
@@ -716,6 +732,48 @@ __global__ void __launch_bounds__(256) place_kernel(const PlaceArgs a) {
             if (kF32) static_cast<float*>(a.dst)[at + j * a.dst_col] = r[j];
             else static_cast<__nv_bfloat16*>(a.dst)[at + j * a.dst_col] = __float2bfloat16_rn(r[j]);
         }
+    }
+}
+
+// A result that TMA could not write where it belongs, from rows padded to whole
+// 16 bytes: dense destinations as aligned 16-byte vectors whatever their rows'
+// alignment (reads of neighbouring threads share sectors), others element by
+// element.
+template <class E>
+__global__ void __launch_bounds__(256) unpad_kernel(const E* src, int64_t ld, int64_t rows, int64_t cols, E* dst,
+                                                    int64_t dst_row, int64_t dst_col) {
+    pdl_enter();
+    constexpr int kPer = 16 / sizeof(E);
+    const int64_t n = rows * cols, step = int64_t(gridDim.x) * 256, first = int64_t(blockIdx.x) * 256 + threadIdx.x;
+    if (dst_col == 1 && (dst_row == cols || rows == 1)) {
+        const int64_t head = min(n, int64_t((16 - (reinterpret_cast<uintptr_t>(dst) & 15)) & 15) / int64_t(sizeof(E)));
+        const int64_t vectors = (n - head) / kPer;
+        for (int64_t v = first; v < vectors; v += step) {
+            const int64_t f = head + v * kPer;
+            int64_t r = f / cols, c = f - r * cols;
+            E e[kPer];
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) {
+                e[j] = src[r * ld + c];
+                if (++c == cols) {
+                    c = 0;
+                    ++r;
+                }
+            }
+            *reinterpret_cast<uint4*>(dst + f) = *reinterpret_cast<const uint4*>(e);
+        }
+        const int64_t tail = head + vectors * kPer;
+        for (int64_t f = first; f < n - (tail - head); f += step) {
+            const int64_t g = f < head ? f : tail + (f - head), r = g / cols;
+            dst[g] = src[r * ld + (g - r * cols)];
+        }
+        return;
+    }
+    const bool by_rows = dst_row == 1 && dst_col != 1;  // walk the unit stride fastest
+    const int64_t inner = by_rows ? rows : cols;
+    for (int64_t f = first; f < n; f += step) {
+        const int64_t o = f / inner, i = f - o * inner, r = by_rows ? i : o, c = by_rows ? o : i;
+        dst[r * dst_row + c * dst_col] = src[r * ld + c];
     }
 }
 

@@ -22,6 +22,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <type_traits>
 
 #include "sw_common.cuh"
 #include "sw_head_rows.cuh"
@@ -240,6 +241,7 @@ struct Layout {
     float4* partial;
     float* dh_sums;
     float* dw_sums;
+    void* dw_rows;
     uint16_t* wp;
     uint16_t* grad;
 };
@@ -262,6 +264,9 @@ struct Shape {
     // rows of fp32 sums of each gradient (0: it is written at once); dh's rows
     // are always put in place from sums, whose parts are chosen on the device
     int64_t dh_sum_rows, dw_sum_rows, ld_acc;
+    // dw goes to rows padded to 16 bytes first, in its own type (TMA cannot write
+    // it where it belongs)
+    bool dw_padded;
 };
 
 Layout lay_out(Bump& b, const Call& c, const Shape& s) {
@@ -285,6 +290,7 @@ Layout lay_out(Bump& b, const Call& c, const Shape& s) {
     if (s.keep) l.ent_s = b.take<float>(s.rows_pad * K);
     if (s.dh_sum_rows) l.dh_sums = b.take<float>(s.dh_sum_rows * s.ld_acc);
     if (s.dw_sum_rows) l.dw_sums = b.take<float>(s.dw_sum_rows * s.ld_acc);
+    if (s.dw_padded) l.dw_rows = b.take<uint8_t>(std::min(s.piece, s.V) * round_up(s.D * (s.f32 ? 4 : 2), 16));
     if (s.pack_w) l.wp = b.take<uint16_t>(s.planes * round_up(s.piece, kBK) * s.ld_h);
     if (s.grads) l.grad = b.take<uint16_t>(s.planes * s.rows * round_up(s.piece, 64));
     return l;
@@ -523,6 +529,7 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
             return SW_OK;
         };
         Tensors t[2];
+        const int64_t ld_rows = round_up(s.D * esize, 16) / esize;
         uint8_t* dw = c.dw ? static_cast<uint8_t*>(c.dw) + v0 * p.dw_row * esize : nullptr;
         if (c.dh && n > 0) {
             Problem& q = a.p[a.problems];
@@ -550,6 +557,8 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
             q.sums = s.dw_sum_rows > 0;
             q.first = first_r;
             Target out{dw, nv, s.D, p.dw_row, kF32};
+            // (a map whose rows end inside 16 bytes would be written past them: whole ones here)
+            if (s.dw_padded) out = Target{l.dw_rows, nv, ld_rows, ld_rows, kF32};
             if (q.sums) out = Target{l.dw_sums, s.dw_sum_rows, s.ld_acc, s.ld_acc, true};
             const Operand st = states(r0, round_up(std::max<int64_t>(n, 1), kBM));
             t[a.problems++] = Tensors{gr, st, out};
@@ -574,6 +583,13 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
             rc = finish(l.dh_sums, 0, s.dh_shape, n, true, l.row_map + r0, c.dh, p.dh_row, p.dh_col);
         if (rc == SW_OK && s.dw_sum_rows && last_r)
             rc = finish(l.dw_sums, s.dw_splits, s.dw_shape, nv, false, nullptr, dw, p.dw_row, p.dw_col);
+        if (rc == SW_OK && s.dw_padded) {
+            using E = typename std::conditional<kF32, float, uint16_t>::type;
+            SW_CUDA_TRY(launch_pdl(unpad_kernel<E>, dim3((unsigned)std::min<int64_t>((nv * s.D + 2047) / 2048, fill)),
+                                   dim3(256), 0, stream, static_cast<const E*>(l.dw_rows), ld_rows, nv, s.D,
+                                   reinterpret_cast<E*>(dw), p.dw_row, p.dw_col),
+                        "linear head dw");
+        }
         return rc;
     };
     if (s.keep) {
@@ -720,8 +736,9 @@ int check_and_run(const char* name, Call& c, void* stream_ptr) {
     // inside 16 bytes would be written past their end).
     const int64_t es = s.f32 ? 4 : 2;
     const bool direct = p->dw_col == 1 && p->dw_row * es % 16 == 0 && D * es % 16 == 0 && p->dw_row >= D &&
-                        (reinterpret_cast<uintptr_t>(c.dw) & 15) == 0 && s.rows >= T;
-    const float sum_us = direct ? float(nv) * float(D) * float(8 + es) / 6.0e6f : 0.0f;
+                        (reinterpret_cast<uintptr_t>(c.dw) & 15) == 0;
+    const bool one_part = s.rows >= T;  // nothing to add to what is written
+    const float sum_us = one_part ? float(nv) * float(D) * float(8 + es) / 6.0e6f : 0.0f;
     s.together = c.dh && c.dw && n <= kBM;
     s.dh_shape = s.dw_shape = kSingle;
     s.dw_splits = 1;
@@ -739,7 +756,8 @@ int check_and_run(const char* name, Call& c, void* stream_ptr) {
         }
     }
     s.dh_sum_rows = c.dh && T > 0 ? sum_rows(n, D, s.dh_shape) : 0;
-    s.dw_sum_rows = c.dw && (!direct || s.dw_splits > 1) ? sum_rows(nv, D, s.dw_shape) : 0;
+    s.dw_sum_rows = c.dw && (!one_part || s.dw_splits > 1) ? sum_rows(nv, D, s.dw_shape) : 0;
+    s.dw_padded = c.dw && !s.dw_sum_rows && !direct;
 
     Bump measure{nullptr, 0};
     lay_out(measure, c, s);
