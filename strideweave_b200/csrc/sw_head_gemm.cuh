@@ -750,6 +750,11 @@ __global__ void __launch_bounds__(320, 1)
     // Reading the weights for the one and writing the other is what a call of
     // few rows does: half of the workers at a time do each.
     const int flip = kProblems > 1 && args.problems > 1 && args.alternate && (worker & 1);
+    // Columns that the MMAs of column tile `nb` compute: whole 64s of what is left
+    // of a result (a dim of 64 or 320 would waste three quarters of a tile).
+    auto tile_cols = [&](const Problem& p, int nb) {
+        return kEpi == kEpiOut ? min(kBN, (p.N - nb * kBN + 63) / 64 * 64) : kBN;
+    };
     auto chunk_end = [&](int k0, int k1) { return kChunked ? min(k0 + kChunkSteps, k1) : k1; };
 
     if (warp == 0) {
@@ -768,8 +773,11 @@ __global__ void __launch_bounds__(320, 1)
                 for (int i = 0, t; alive && (t = plan.nth(i, worker, workers)) >= 0; ++i) {
                     int mb, nb, split, k0, k1;
                     plan.item(t, mb, nb, split, k0, k1);
-                    const int a0 = mb * C::kTileM + rank * kBM, b0 = nb * kBN + rank * C::kBRows;
-                    constexpr uint32_t bytes = (kPair ? 2 : 1) * C::kStageBytes;
+                    const int b_cols = tile_cols(p, nb) / (kPair ? 2 : 1);  // of this CTA
+                    const int boxes = (b_cols + 63) / 64;
+                    const int a0 = mb * C::kTileM + rank * kBM, b0 = nb * kBN + rank * b_cols;
+                    const uint32_t bytes =
+                        (kPair ? 2 : 1) * (C::kABytes + (kEpi == kEpiOut ? boxes * 8192 : C::kBBytes));
                     for (int c0 = k0; c0 < k1 && alive; c0 = chunk_end(c0, k1))
                         for (int term = 0; term < args.terms && alive; ++term) {
                             // plane pairs, the small products first: (hi, lo), (lo, hi), (hi, hi)
@@ -801,10 +809,9 @@ __global__ void __launch_bounds__(320, 1)
                                     }
                                 }
                                 if (kBMn) {
-#pragma unroll
-                                    for (int g = 0; g < C::kBRows / 64; ++g)
-                                        tma_load<kPair>(sb + g * 8192, mb_, (b0 / 64 + g) * p.pb.x_block + xb,
-                                                        yb + ks * kBK, full);
+                                    // (B's planes lie below each other: its columns are as in memory)
+                                    for (int g = 0; g < boxes; ++g)
+                                        tma_load<kPair>(sb + g * 8192, mb_, b0 + g * 64, yb + ks * kBK, full);
                                 } else {
                                     tma_load<kPair>(sb, mb_, ks * p.pb.x_block + xb, yb + b0, full);
                                 }
@@ -832,7 +839,6 @@ __global__ void __launch_bounds__(320, 1)
                 const int q = kProblems > 1 ? ph ^ flip : 0;
                 const Plan plan = kProblems > 1 && q ? plan1 : plan0;
                 const bool a_mn = mn_major(args.p[q]);
-                const uint32_t idesc = idesc_f16(kBf16, a_mn, kBMn, C::kAccRows, kBN);
                 // K-major: 16 elements of K are 32 bytes of the swizzled row, 8-row groups 1024 bytes apart.
                 // MN-major: 16 rows of K are 2048 bytes, 64-element blocks of the other mode 8192 bytes
                 // apart, 8-row groups of K 1024.
@@ -840,6 +846,7 @@ __global__ void __launch_bounds__(320, 1)
                 for (int i = 0, t; alive && (t = plan.nth(i, worker, workers)) >= 0; ++i) {
                 int mb, nb, split, k0, k1;
                 plan.item(t, mb, nb, split, k0, k1);
+                const uint32_t idesc = idesc_f16(kBf16, a_mn, kBMn, C::kAccRows, tile_cols(args.p[q], nb));
                 for (int c0 = k0; c0 < k1 && alive; c0 = chunk_end(c0, k1), ++it) {
                     // one tile alternates between the two accumulators, a tall one fills both
                     const uint32_t buf0 = C::kAccs == 1 ? it & 1 : 0, drained = (C::kAccs == 1 ? it >> 1 : it) & 1;

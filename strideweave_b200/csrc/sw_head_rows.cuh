@@ -40,7 +40,8 @@ __host__ __device__ inline float spread_cost(int64_t M, int64_t N, int64_t K, in
     const int64_t tiles = tiles_of(M, N, shape);
     const int whole = int(tiles / workers), rest = int(tiles - int64_t(whole) * workers);
     if (s > 1 && (steps < 4 * s || rest == 0 || (whole ? s > kMaxTailParts : rest * s > 2 * workers))) return 1e30f;
-    const float stage = stage_us(shape, terms), fixed = fixed_us(shape);
+    // (a narrow result's tiles compute what they need, but load all of A)
+    const float stage = stage_us(shape, terms) * (N <= kBN / 2 ? 0.5f : 1.0f), fixed = fixed_us(shape);
     const float one = float(steps) * stage + fixed, part = float((steps + s - 1) / s) * stage + fixed;
     const float waves = float(whole) * one + float((rest * s + workers - 1) / workers) * part;
     float us = waves;
