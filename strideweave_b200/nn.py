@@ -8,6 +8,11 @@ These mirror the reference's `strideweave.nn` pieces:
 - `MSELoss`: modules.py:129-200, mean of squared differences;
 - `SGD`: src/strideweave/nn/optim.py:17-100, p -= lr * p.grad.
 
+`LinearCrossEntropy` and `LinearDistillation` have no reference counterpart
+(its losses take whole predictions): losses of a linear head over a large
+vocabulary, against target words or a teacher's top logits, that never hold the
+logits.
+
 The autograd graph is still the reference's (`Tensor.backward`), but every
 node runs on the GPU:
 
@@ -18,6 +23,8 @@ node runs on the GPU:
   products.
 - `SGD.step` is one fused update kernel per parameter. The reference updates
   one element at a time through carrier indexing.
+- The linear head's losses contract states and weights on the tensor cores and
+  reduce each logits tile where it is (`sw_linear_xent`, `sw_linear_distill`).
 
 Elementwise operations work on a tensor's whole storage range. That needs a
 compact, injective layout, which the contraction results always have.
@@ -30,8 +37,9 @@ from typing import Any, Iterable
 import numpy as np
 
 from . import _native as N
-from ._host import DType, Layout, Operation, Shape, Stride, Tensor, require_capability, resolve_operation_plan
-from .layout_plan import canonical_layout
+from ._host import (BFloat16, DType, Layout, Operation, Shape, Stride, Tensor, require_capability,
+                    resolve_operation_plan)
+from .layout_plan import canonical_layout, mode_leaves, mode_size, single_stride
 
 
 def _compact(t: Any, name: str) -> tuple[int, int]:
@@ -122,6 +130,196 @@ def gelu(t: Tensor) -> Tensor:
 def mse_loss(pred: Tensor, target: Tensor) -> Tensor:
     return pred.carrier.dispatch_op("mse_loss").forward(pred, target)
 
+# ---- losses of a linear head ----------------------------------------------------------
+
+
+def _head_operand(t: Any, name: str) -> tuple[int, int, int, tuple[int, int], str]:
+    """(address, rows, columns, element strides, dtype name) of a Float32 or
+    BFloat16 CUDA matrix whose modes each walk memory with one stride."""
+    from .carrier import CUDA
+
+    if not isinstance(t, Tensor):
+        raise TypeError(f"{name} must be a Tensor")
+    t._require_single_subtensor("CUDA linear head loss")
+    if not isinstance(t.carrier, CUDA) or t.carrier.dtype() not in (DType.Float32, BFloat16):
+        raise TypeError(f"{name} must be a Float32 or BFloat16 tensor on a CUDA carrier")
+    if t.carrier.swizzle is not None:
+        raise NotImplementedError(f"{name}: swizzled carriers are not supported by the linear head's losses")
+    if len(t.layout) != 2:
+        raise ValueError(f"{name} must have a two-mode layout")
+    r, c = single_stride(mode_leaves(t.layout, 0)), single_stride(mode_leaves(t.layout, 1))
+    if r is None or c is None:
+        raise NotImplementedError(f"{name}: each mode must walk memory with a single stride")
+    size, dtype = (4, "Float32") if t.carrier.dtype() is DType.Float32 else (2, "BFloat16")
+    return t.carrier.data_ptr + size * t.offset, r[0], c[0], (r[1], c[1]), dtype
+
+
+def _head_vector(t: Any, name: str, dtype: Any, size: int) -> int:
+    """Address of a contiguous 32-bit CUDA tensor of `size` elements."""
+    from .carrier import CUDA
+
+    if not isinstance(t, Tensor):
+        raise TypeError(f"{name} must be a Tensor")
+    t._require_single_subtensor("CUDA linear head loss")
+    if not isinstance(t.carrier, CUDA) or t.carrier.dtype() is not dtype:
+        raise TypeError(f"{name} must be a tensor of dtype {dtype.name} on a CUDA carrier")
+    if t.carrier.swizzle is not None:
+        raise NotImplementedError(f"{name}: swizzled carriers are not supported by the linear head's losses")
+    if t.size() != size:
+        raise ValueError(f"{name} must have {size} elements (got {t.size()})")
+    expect = 1
+    for mode in reversed(range(len(t.layout))):  # row-major
+        walk = single_stride(mode_leaves(t.layout, mode))
+        if walk is None or (walk[0] > 1 and walk[1] != expect):
+            raise NotImplementedError(f"{name} must be contiguous, last mode fastest")
+        expect *= walk[0]
+    return t.carrier.data_ptr + 4 * t.offset
+
+
+class _LinearHeadLoss(Operation):
+    """What the two losses of a linear head share; see `linear_cross_entropy`."""
+
+    reduction = "mean"
+
+    def _run(self, x: Any, weight: Any, **kw: Any) -> None:
+        raise NotImplementedError
+
+    def _shape(self, x: Any, weight: Any) -> tuple[tuple, int]:
+        xp, T, D, xs, dtype = _head_operand(x, "x")
+        wp, V, D2, ws, dtype2 = _head_operand(weight, "weight")
+        if D != D2:
+            raise ValueError("Matmul inner dimensions must match")
+        if dtype != dtype2:
+            raise TypeError("x and weight must share their dtype")
+        return (dtype, xp, xs, wp, ws, T, V, D), T
+
+    def _outputs(self, x: Any, T: int) -> tuple[Tensor, Any]:
+        from .carrier import CUDA
+
+        dev = x.carrier.device
+        loss = (Tensor(CUDA(1, dtype=DType.Float32, empty=True, device=dev), 0, SCALAR) if self.reduction == "mean" else
+                Tensor(CUDA(T, dtype=DType.Float32, empty=True, device=dev), 0, Layout(Shape(T), Stride(1))))
+        return loss, CUDA(T, dtype=DType.Float32, empty=True, device=dev)
+
+    def _forward(self, x: Any, weight: Any) -> Tensor:
+        head, T = self._shape(x, weight)
+        loss, lse = self._outputs(x, T)
+        self._run(head, loss_ptr=_ptr(loss), lse_ptr=lse.data_ptr)
+        self.ctx["output_layout"] = loss.layout
+        self.ctx["lse"] = lse
+        return loss
+
+    def _gradients(self, x: Any, weight: Any) -> tuple[Tensor, Tensor, dict]:
+        """dx and dw, unwritten, in injective layouts of x and weight, and the
+        arguments that say where they are."""
+        from .carrier import CUDA
+        from .layout_plan import injective_layout_for
+
+        out, args = [], {}
+        for name, t in (("dh", x), ("dw", weight)):
+            layout = injective_layout_for(t.layout)
+            g = Tensor(CUDA(layout.cosize, dtype=t.carrier.dtype(), empty=True, device=t.carrier.device), 0, layout)
+            args[name + "_ptr"], _, _, args[name + "_strides"], _ = _head_operand(g, name)
+            out.append(g)
+        return out[0], out[1], args
+
+    def backward(self, gradient: Any) -> tuple[Any, Any]:
+        x, weight = self.inputs()
+        head, T = self._shape(x, weight)
+        up = _head_vector(gradient, "gradient", DType.Float32, 1 if self.reduction == "mean" else T)
+        dx, dw, where = self._gradients(x, weight)
+        self._run(head, lse_ptr=self.ctx["lse"].data_ptr, upstream_ptr=up, **where)
+        return dx, dw
+
+    def loss_and_gradients(self, x: Any, weight: Any) -> tuple[Tensor, Tensor, Tensor]:
+        head, T = self._shape(x, weight)
+        loss, lse = self._outputs(x, T)
+        dx, dw, where = self._gradients(x, weight)
+        self._run(head, loss_ptr=_ptr(loss), lse_ptr=lse.data_ptr, **where)
+        return loss, dx, dw
+
+
+class CudaLinearCrossEntropy(_LinearHeadLoss):
+    targets: Any = None
+    ignore_index = -100
+    logit_scale = 1.0
+
+    def _run(self, head: tuple, **kw: Any) -> None:
+        from . import kernels
+
+        kernels.linear_cross_entropy(*head, _head_vector(self.targets, "targets", DType.Int32, head[5]),
+                                     ignore_index=self.ignore_index, logit_scale=self.logit_scale,
+                                     reduction=self.reduction, **kw)
+
+
+class CudaLinearDistillation(_LinearHeadLoss):
+    index: Any = None
+    logits: Any = None
+    temperature = 1.0
+
+    def _run(self, head: tuple, **kw: Any) -> None:
+        from . import kernels
+
+        if not isinstance(self.index, Tensor) or len(self.index.layout) != 2:
+            raise ValueError("index must have a two-mode layout [tokens, entries]")
+        top_k = mode_size(self.index.layout, 1)
+        kernels.linear_distillation(*head, _head_vector(self.index, "index", DType.Int32, head[5] * top_k),
+                                    _head_vector(self.logits, "logits", DType.Float32, head[5] * top_k), top_k,
+                                    temperature=self.temperature, reduction=self.reduction, **kw)
+
+
+def _cross_entropy_operation(x: Tensor, targets: Tensor, ignore_index: int, logit_scale: float, reduction: str) -> Any:
+    op = x.carrier.dispatch_op("linear_cross_entropy")
+    op.targets, op.ignore_index, op.logit_scale, op.reduction = targets, ignore_index, logit_scale, reduction
+    return op
+
+
+def _distillation_operation(x: Tensor, index: Tensor, logits: Tensor, temperature: float, reduction: str) -> Any:
+    op = x.carrier.dispatch_op("linear_distillation")
+    op.index, op.logits, op.temperature, op.reduction = index, logits, temperature, reduction
+    return op
+
+
+def linear_cross_entropy(x: Tensor, weight: Tensor, targets: Tensor, *, ignore_index: int = -100,
+                         logit_scale: float = 1.0, reduction: str = "mean") -> Tensor:
+    """Softmax cross entropy of logit_scale * x . weight^T, x [T, D] and weight
+    [V, D] Float32 or BFloat16, against Int32 targets [T], without holding the
+    logits; differentiable in x and weight.  Rows whose target is ignore_index
+    do not count.  `reduction`: "mean" over the rows that count, or "none"."""
+    return _cross_entropy_operation(x, targets, ignore_index, logit_scale, reduction).forward(x, weight)
+
+
+def linear_distillation(x: Tensor, weight: Tensor, index: Tensor, logits: Tensor, *, temperature: float = 1.0,
+                        reduction: str = "mean") -> Tensor:
+    """temperature^2 KL(teacher || softmax(x . weight^T / temperature)), the
+    teacher given by its top logits of each row: Int32 columns `index` and
+    Float32 `logits`, both [T, K] row-major, a negative column marking an absent
+    entry; differentiable in x and weight, without holding the logits."""
+    return _distillation_operation(x, index, logits, temperature, reduction).forward(x, weight)
+
+
+def linear_cross_entropy_and_gradients(x: Tensor, weight: Tensor, targets: Tensor, *, ignore_index: int = -100,
+                                       logit_scale: float = 1.0, reduction: str = "mean"
+                                       ) -> tuple[Tensor, Tensor, Tensor]:
+    """(loss, dx, dw) of `linear_cross_entropy` with unit upstream gradient in
+    one call, which computes the logits once (an autograd forward and backward
+    computes them twice)."""
+    from strideweave import no_grad
+
+    with no_grad():
+        return _cross_entropy_operation(x, targets, ignore_index, logit_scale,
+                                        reduction).loss_and_gradients(x, weight)
+
+
+def linear_distillation_and_gradients(x: Tensor, weight: Tensor, index: Tensor, logits: Tensor, *,
+                                      temperature: float = 1.0, reduction: str = "mean"
+                                      ) -> tuple[Tensor, Tensor, Tensor]:
+    """(loss, dx, dw) of `linear_distillation`, as `linear_cross_entropy_and_gradients`."""
+    from strideweave import no_grad
+
+    with no_grad():
+        return _distillation_operation(x, index, logits, temperature, reduction).loss_and_gradients(x, weight)
+
 
 # ---- modules ------------------------------------------------------------------------
 
@@ -168,6 +366,27 @@ class GELU:
 class MSELoss:
     def __call__(self, pred: Tensor, target: Tensor) -> Tensor:
         return mse_loss(pred, target)
+
+
+class LinearCrossEntropy:
+    """Module form of `linear_cross_entropy`."""
+
+    def __init__(self, *, ignore_index: int = -100, logit_scale: float = 1.0, reduction: str = "mean") -> None:
+        self.ignore_index, self.logit_scale, self.reduction = ignore_index, logit_scale, reduction
+
+    def __call__(self, x: Tensor, weight: Tensor, targets: Tensor) -> Tensor:
+        return linear_cross_entropy(x, weight, targets, ignore_index=self.ignore_index, logit_scale=self.logit_scale,
+                                    reduction=self.reduction)
+
+
+class LinearDistillation:
+    """Module form of `linear_distillation`."""
+
+    def __init__(self, *, temperature: float = 1.0, reduction: str = "mean") -> None:
+        self.temperature, self.reduction = temperature, reduction
+
+    def __call__(self, x: Tensor, weight: Tensor, index: Tensor, logits: Tensor) -> Tensor:
+        return linear_distillation(x, weight, index, logits, temperature=self.temperature, reduction=self.reduction)
 
 
 class MLP:
@@ -528,7 +747,9 @@ class SGD:
             p.grad = None
 
 
-NN_OPERATIONS = {"gelu": CudaGelu, "mse_loss": CudaMSELoss}
+NN_OPERATIONS = {"gelu": CudaGelu, "mse_loss": CudaMSELoss, "linear_cross_entropy": CudaLinearCrossEntropy,
+                 "linear_distillation": CudaLinearDistillation}
 
-__all__ = ["CapturedTrainStep", "GELU", "MLP", "MSELoss", "MXLinear", "SGD", "gelu", "gelu_grad", "mse_loss",
-           "train_step"]
+__all__ = ["CapturedTrainStep", "GELU", "LinearCrossEntropy", "LinearDistillation", "MLP", "MSELoss", "MXLinear", "SGD",
+           "gelu", "gelu_grad", "linear_cross_entropy", "linear_cross_entropy_and_gradients", "linear_distillation",
+           "linear_distillation_and_gradients", "mse_loss", "train_step"]

@@ -482,3 +482,48 @@ def test_long_walks_keep_their_precision(dtype):
     h, w, y = states(T, V, D, dtype)
     up = torch.ones(1, device="cuda")
     check(call(h, w, targets=y, mean=True, up=up), reference(h, w, up, targets=y, mean=True), dtype, True)
+
+
+def test_the_example_learns():
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    root = Path(__file__).resolve().parent.parent
+    out = subprocess.run([sys.executable, str(root / "examples" / "train_head.py"), "--steps", "12", "--tokens", "200",
+                          "--vocab", "1000", "--dim", "64"], capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0, out.stdout + out.stderr
+
+
+def test_through_the_tensor_api():
+    """nn's losses on CUDA carrier tensors, autograd and the one-call form, against the raw entry points."""
+    sw = pytest.importorskip("strideweave")
+    import numpy as np
+    from strideweave import Layout, Shape, Stride, Tensor
+
+    from strideweave_b200 import CUDA, nn
+
+    rng = np.random.default_rng(0)
+    T, V, D = 40, 300, 48
+    h = rng.standard_normal((T, D)).astype(np.float32)
+    w = (rng.standard_normal((V, D)) * 0.2).astype(np.float32)
+    y = rng.integers(0, V, T).astype(np.int32)
+    y[3] = IGNORE
+
+    def matrix(a):
+        return Tensor(CUDA.from_numpy(a.ravel()), 0, Layout(Shape(list(a.shape)), Stride([a.shape[1], 1])))
+
+    x, weight = matrix(h), matrix(w)
+    targets = Tensor(CUDA.from_numpy(y), 0, Layout(Shape(T), Stride(1)))
+    loss, dx, dw = nn.linear_cross_entropy_and_gradients(x, weight, targets)
+    up = torch.ones(1, device="cuda")
+    want = call(torch.from_numpy(h).cuda(), torch.from_numpy(w).cuda(), targets=torch.from_numpy(y).cuda(), mean=True,
+                up=up)
+    assert loss.carrier.to_numpy()[0] == want["loss"].cpu().numpy()[0]
+    np.testing.assert_array_equal(dx.carrier.to_numpy(), want["dh"].cpu().numpy().ravel())
+    np.testing.assert_array_equal(dw.carrier.to_numpy(), want["dw"].cpu().numpy().ravel())
+    alone = nn.linear_cross_entropy(x, weight, targets)
+    assert alone.carrier.to_numpy()[0] == loss.carrier.to_numpy()[0]
+    with pytest.raises(ValueError, match="targets must have 40 elements"):
+        nn.linear_cross_entropy(x, weight, Tensor(CUDA.from_numpy(y[:5]), 0, Layout(Shape(5), Stride(1))))
+    assert sw is not None
