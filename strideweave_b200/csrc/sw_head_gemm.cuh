@@ -171,8 +171,9 @@ struct GemmArgs {
     const uint16_t* offs;    // [tile][rows_pad] first entry of each kEntryTile columns (null: one entry a row)
     int ent_k;
     int rows_pad;
-    float4* partial;         // kEpiLse: [rows_pad][half_tiles] (max, sum, target term, -) in base-2 units
-    int half_tiles;          // 128-column halves of the vocabulary's tiles
+    float4* partial;         // kEpiLse: [rows_pad][slots] (max, sum, target term, -) in base-2 units
+    int slots, slot_shift;   // a slot for each 1 << slot_shift columns: 128, or a narrow tile's 64
+    int tile_n;              // logits tiles of one CTA: 256 columns, or 128 or 64 where they spread over more SMs
     float* ent_s;            // kEpiLse: base-2 logit of every target entry (null: not kept)
     int keep;                // kEpiLse: write exp2(logit - half tile's max) where the logits' gradient will be
     const float* lse2;       // kEpiGrad: per compact row
@@ -219,8 +220,8 @@ struct Plan {
     int items, k_steps, part_steps;
     int pre, pre_first, pre_stride, pool;
 
-    __device__ __forceinline__ Plan(int M, int N, int K, int tile_m, int workers, int parts)
-        : walk(M, (N + kBN - 1) / kBN, tile_m, workers, parts), items(walk.items()), k_steps((K + kBK - 1) / kBK),
+    __device__ __forceinline__ Plan(int M, int N, int K, int tile_m, int tile_n, int workers, int parts)
+        : walk(M, (N + tile_n - 1) / tile_n, tile_m, workers, parts), items(walk.items()), k_steps((K + kBK - 1) / kBK),
           part_steps((k_steps + parts - 1) / parts), pre(0), pre_first(0), pre_stride(0), pool(0) {}
     // The contraction `before` left all workers but the first items % workers
     // one item ahead: they take `gain` items of this one first, as many as last
@@ -592,12 +593,13 @@ __device__ __forceinline__ float4 lse_tile(const GemmArgs& args, const void* tma
 // target in fp32, rounded once to the type the next contractions read.
 template <bool kBf16, bool kFew, class Rows>
 __device__ __forceinline__ void grad_tile(const GemmArgs& args, const void* tmap_c, Rows& wr, EntryCursor& cur,
-                                          int64_t n0, float k2, float lse2, float coef, float (&r)[2][2][32]) {
-    if (n0 >= args.p[0].N || (kFew && wr.m0 >= kFewRows)) return;  // (the remainders' rows are written below)
+                                          int64_t n0, int64_t n_end, float k2, float lse2, float coef,
+                                          float (&r)[2][2][32]) {
+    if (n0 >= n_end || (kFew && wr.m0 >= kFewRows)) return;  // (the remainders' rows are written below)
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
         float (&x)[32] = r[c / 2][c % 2];
-        const int ncols = (int)min(int64_t(32), int64_t(args.p[0].N) - (n0 + c * 32));
+        const int ncols = (int)min(int64_t(32), n_end - (n0 + c * 32));
 #pragma unroll
         for (int j = 0; j < 32; ++j) x[j] = ex2(fmaf(x[j], k2, -lse2));
         cur.walk(int(args.v0 + n0) + c * 32, [&](int rel, float p) {
@@ -626,16 +628,16 @@ __device__ __forceinline__ void grad_tile(const GemmArgs& args, const void* tmap
                 }
                 return *reinterpret_cast<const uint32_t*>(&h);
             },
-            n0 + 64 < args.p[0].N, int(n0), int(n0) + 64, int(wr.m0), false);
+            n0 + 64 < n_end, int(n0), int(n0) + 64, int(wr.m0), false);
         if (kFew)
             wr.send_two(
                 tmap_c,
                 [&](int b, int j) { return pack2<true>(r[b][j / 16][2 * (j % 16)], r[b][j / 16][2 * (j % 16) + 1]); },
-                n0 + 64 < args.p[0].N, int(n0), int(n0) + 64, int(wr.m0) + kFewRows, false);
+                n0 + 64 < n_end, int(n0), int(n0) + 64, int(wr.m0) + kFewRows, false);
     } else {
 #pragma unroll
         for (int b = 0; b < 2; ++b)
-            if (n0 + b * 64 < args.p[0].N)
+            if (n0 + b * 64 < n_end)
                 wr.send_two(
                     tmap_c,
                     [&](int plane, int j) {
@@ -732,13 +734,16 @@ __global__ void __launch_bounds__(320, 1)
     const uint32_t tmem = *tmem_slot;
     pdl_enter();
 
+    constexpr bool kNarrow = kShape == kSingle && kEpi != kEpiOut;  // tiles may be narrower
+    const int tile_n = kNarrow ? args.tile_n : kBN;
     // rows that count, and for the gradients of few rows their remainders
     const bool few = kBf16 && kEpi != kEpiLse && args.state->few(args.row0);
     auto plan_of = [&](const Problem& p) {
         int rows = args.state->rows(args.row0);
         if (!few) rows = min(rows, p.count_is == kCountM ? p.M : p.K);
         else if (kEpi == kEpiOut) rows += kFewRows;
-        return Plan(p.count_is == kCountM ? rows : p.M, p.N, p.count_is == kCountK ? rows : p.K, C::kTileM, workers,
+        return Plan(p.count_is == kCountM ? rows : p.M, p.N, p.count_is == kCountK ? rows : p.K, C::kTileM, tile_n,
+                    workers,
                     p.splits > 0 ? p.splits : args.state->dh_splits);
     };
     const Plan plan0 = plan_of(args.p[0]);
@@ -753,7 +758,7 @@ __global__ void __launch_bounds__(320, 1)
     // Columns that the MMAs of column tile `nb` compute: whole 64s of what is left
     // of a result (a dim of 64 or 320 would waste three quarters of a tile).
     auto tile_cols = [&](const Problem& p, int nb) {
-        return kEpi == kEpiOut ? min(kBN, (p.N - nb * kBN + 63) / 64 * 64) : kBN;
+        return kEpi == kEpiOut ? min(kBN, (p.N - nb * kBN + 63) / 64 * 64) : tile_n;
     };
     auto chunk_end = [&](int k0, int k1) { return kChunked ? min(k0 + kChunkSteps, k1) : k1; };
 
@@ -775,9 +780,9 @@ __global__ void __launch_bounds__(320, 1)
                     plan.item(t, mb, nb, split, k0, k1);
                     const int b_cols = tile_cols(p, nb) / (kPair ? 2 : 1);  // of this CTA
                     const int boxes = (b_cols + 63) / 64;
-                    const int a0 = mb * C::kTileM + rank * kBM, b0 = nb * kBN + rank * b_cols;
+                    const int a0 = mb * C::kTileM + rank * kBM, b0 = nb * tile_n + rank * b_cols;
                     const uint32_t bytes =
-                        (kPair ? 2 : 1) * (C::kABytes + (kEpi == kEpiOut ? boxes * 8192 : C::kBBytes));
+                        (kPair ? 2 : 1) * (C::kABytes + (kEpi == kEpiOut ? boxes * 64 : b_cols) * kBK * 2);
                     for (int c0 = k0; c0 < k1 && alive; c0 = chunk_end(c0, k1))
                         for (int term = 0; term < args.terms && alive; ++term) {
                             // plane pairs, the small products first: (hi, lo), (lo, hi), (hi, hi)
@@ -929,10 +934,12 @@ __global__ void __launch_bounds__(320, 1)
     wr.m0 = int64_t(mb) * C::kTileM + h * C::kAccRows + rank * kBM + quarter * 32;
                 const int64_t m = wr.m0 + lane;
                 wr.row_in = m < M;
-                const int64_t ncol0 = int64_t(nb) * kBN + half * kCols;
-                const int64_t n_end = min(int64_t(p.N), ncol0 + kCols);
+                const int64_t ncol0 = int64_t(nb) * tile_n + half * kCols;
+                const int64_t n_end = min(int64_t(p.N), min(ncol0 + kCols, int64_t(nb + 1) * tile_n));
                 // a pair's second half may lie past the rows that the workspace holds
-                const bool rows_in = kEpi == kEpiOut || wr.m0 < (p.M + kBM - 1) / kBM * kBM;
+                // (and a narrow tile's second half is none)
+                const bool rows_in = kEpi == kEpiOut || (wr.m0 < (p.M + kBM - 1) / kBM * kBM &&
+                                                         (!kNarrow || half * kCols < tile_n));
                 // what the row needs beside its accumulator, while the MMAs run
                 EntryCursor cur;
                 float lse2 = 0.0f, coef = 0.0f;
@@ -984,10 +991,10 @@ __global__ void __launch_bounds__(320, 1)
                 if (kEpi != kEpiOut) cur.begin();
                 if (kEpi == kEpiLse) {
                     const float4 st = lse_tile<kBf16, 2>(args, tmap_c, wr, cur, ncol0, n_end, k2, r);
-                    args.partial[m * args.half_tiles + (args.v0 + ncol0) / kCols] = st;
+                    args.partial[m * args.slots + ((args.v0 + ncol0) >> args.slot_shift)] = st;
                 } else if (kEpi == kEpiGrad) {
-                    if (few) grad_tile<kBf16, kBf16>(args, tmap_c, wr, cur, ncol0, k2, lse2, coef, r);
-                    else grad_tile<kBf16, false>(args, tmap_c, wr, cur, ncol0, k2, lse2, coef, r);
+                    if (few) grad_tile<kBf16, kBf16>(args, tmap_c, wr, cur, ncol0, n_end, k2, lse2, coef, r);
+                    else grad_tile<kBf16, false>(args, tmap_c, wr, cur, ncol0, n_end, k2, lse2, coef, r);
                 } else {
                     out_tile<!kBf16>(p, tmap_c, wr, p.sums ? plan.walk.sum_row(split, int(wr.m0)) : int(wr.m0), ncol0,
                                      out_scale, r);

@@ -162,12 +162,13 @@ __device__ __forceinline__ void sort_teacher_row(const PrepareArgs& a, int64_t t
     }
 }
 
-// kRows rows per CTA.  Each CTA counts the rows before its own and all rows
-// that count (T flags from L2: with 8 rows a CTA 33 MB in all at T = 8192), so
-// nothing waits for anything: row_map[0, count) are the rows that count, in
-// order, row_map[count, T) the others.  It then leaves what its rows need: the
-// target entries, the factor of their gradient, and in bf16 the states
-// themselves, gathered; the places of rows that do not count are zeros.
+// kRows rows per CTA, and where rows are few a share of their columns.  Each CTA
+// counts the rows before its own and all rows that count (T flags from L2: with
+// 8 rows a CTA 33 MB in all at T = 8192), so nothing waits for anything:
+// row_map[0, count) are the rows that count, in order, row_map[count, T) the
+// others.  It then leaves what its rows need: the target entries, the factor of
+// their gradient, and in bf16 the states themselves, gathered; the places of
+// rows that do not count are zeros.
 template <int kRows>
 __global__ void __launch_bounds__(256) prepare_kernel(const PrepareArgs a) {
     constexpr int kCols = 256;
@@ -232,8 +233,8 @@ __global__ void __launch_bounds__(256) prepare_kernel(const PrepareArgs a) {
             const int64_t dest = keep ? rank : mine ? a.T - 1 - (t - rank) : t;
             s_dest[lane] = dest < a.rows_pad ? int(dest) : -1;
             s_keep[lane] = keep;
-            if (mine) a.row_map[dest] = int(t);
-            if (keep) {
+            if (mine && blockIdx.y == 0) a.row_map[dest] = int(t);
+            if (keep && blockIdx.y == 0) {
                 if (a.targets) a.ent_idx[rank] = a.targets[t];
                 if (a.coef) a.coef[rank] = a.mean || !a.upstream ? 1.0f : a.upstream[t];
                 if (a.lse) a.lse2[rank] = a.lse[t] * kLog2e;
@@ -241,7 +242,7 @@ __global__ void __launch_bounds__(256) prepare_kernel(const PrepareArgs a) {
         }
     }
     __syncthreads();
-    if (blockIdx.x == gridDim.x - 1) {  // (its rows are mostly padding)
+    if (blockIdx.x == gridDim.x - 1 && blockIdx.y == 0) {  // (its rows are mostly padding)
         uint32_t top = 0;  // of the row factors (Float32 only)
         if (a.coef && !a.h) {
             for (int64_t t = tid; t < a.T; t += 256)
@@ -285,7 +286,7 @@ __global__ void __launch_bounds__(256) prepare_kernel(const PrepareArgs a) {
             }
         }
     }
-    if (!a.targets)
+    if (!a.targets && blockIdx.y == 0)
         for (int r = warp; r < kRows; r += 8)
             if (s_keep[r]) sort_teacher_row(a, t0 + r, s_dest[r], lane, s_sort[warp], s_sort[warp] + kMaxTeacher);
     if (!a.h) return;
@@ -305,7 +306,7 @@ __global__ void __launch_bounds__(256) prepare_kernel(const PrepareArgs a) {
     };
     if (a.vec) {
         const int units = int(a.ld / 8);
-        for (int u = tid; u < kRows * units; u += 256) {
+        for (int u = blockIdx.y * 256 + tid; u < kRows * units; u += gridDim.y * 256) {
             const int r = u / units, c = (u - r * units) * 8;
             uint4 v = make_uint4(0, 0, 0, 0);
             if (s_keep[r]) v = *reinterpret_cast<const uint4*>(a.h + (t0 + r) * a.sr + c);
@@ -314,7 +315,7 @@ __global__ void __launch_bounds__(256) prepare_kernel(const PrepareArgs a) {
         return;
     }
     const bool by_rows = a.sr == 1 && a.sc != 1;  // walk the unit stride fastest
-    for (int64_t c0 = 0; c0 < a.ld; c0 += kCols) {
+    for (int64_t c0 = int64_t(blockIdx.y) * kCols; c0 < a.ld; c0 += int64_t(gridDim.y) * kCols) {
         for (int u = tid; u < kRows * kCols; u += 256) {
             const int r = by_rows ? u % kRows : u / kCols, c = by_rows ? u / kRows : u % kCols;
             s_tile[r][c] = s_keep[r] && c0 + c < a.D ? a.h[(t0 + r) * a.sr + (c0 + c) * a.sc] : uint16_t(0);
@@ -476,8 +477,8 @@ __global__ void __launch_bounds__(256) split_kernel(const SplitJob j0, const Spl
 // ---- after the logits ------------------------------------------------------------
 
 struct LossArgs {
-    const float4* partial;   // [rows_pad][half_tiles]
-    int half_tiles;
+    const float4* partial;   // [rows_pad][slots]
+    int slots, slot_shift;
     int row0, rows;          // compact rows [row0, row0 + rows), a CTA each
     int all_rows;            // CTAs over all launches that write a row's loss
     HeadState* state;
@@ -511,7 +512,7 @@ struct LossArgs {
 template <bool kF32>
 __global__ void __launch_bounds__(256) loss_kernel(const LossArgs a) {
     constexpr int kSub = kF32 ? 2048 : 8192;  // columns of a batch: four loads a thread
-    __shared__ float factor[kSub / 128];
+    __shared__ float factor[kSub / 64];
     __shared__ float s_ref[8], s_sum[8], s_dot[8];
     __shared__ int s_last;
     pdl_enter();
@@ -543,7 +544,7 @@ __global__ void __launch_bounds__(256) loss_kernel(const LossArgs a) {
     };
     if (a.grad && i < count) fetch(c_begin);
     if (i < count) {
-        const float4* part = a.partial + (a.row0 + i) * a.half_tiles;
+        const float4* part = a.partial + (a.row0 + i) * a.slots;
         float ref = -INFINITY, sum = 0.0f, dot = 0.0f;
         auto add = [&](float r, float s, float d) {
             const float next = fmaxf(ref, r), base = next == -INFINITY ? 0.0f : next;
@@ -552,7 +553,7 @@ __global__ void __launch_bounds__(256) loss_kernel(const LossArgs a) {
             dot += d;
         };
 #pragma unroll 4
-        for (int t = tid; t < a.half_tiles; t += 256) {
+        for (int t = tid; t < a.slots; t += 256) {
             const float4 p = part[t];
             add(p.x, p.y, p.z);
         }
@@ -613,8 +614,8 @@ __global__ void __launch_bounds__(256) loss_kernel(const LossArgs a) {
     for (int64_t c0 = c_begin; c0 < c_end; c0 += kSub) {
         const int64_t c1 = min(c0 + kSub, c_end);
         __syncthreads();
-        for (int t = tid; t < int((c1 - c0 + 127) / 128); t += 256) {
-            const float ref = a.partial[(a.row0 + i) * a.half_tiles + c0 / 128 + t].x;
+        for (int t = tid; t < int((c1 - c0 + 63) / 64); t += 256) {
+            const float ref = a.partial[(a.row0 + i) * a.slots + ((c0 + t * 64) >> a.slot_shift)].x;
             // (a half tile of nothing but -inf stored zeros)
             factor[t] = ref == -INFINITY ? 0.0f : ex2(ref - lse2) * coef * (kF32 ? 1.0f : 1.0f / 32768.0f);
         }
@@ -627,7 +628,7 @@ __global__ void __launch_bounds__(256) loss_kernel(const LossArgs a) {
         for (int j = 0; j < 4; ++j) {
             const int64_t c = c0 + (kF32 ? 64 * warp + 512 * j : tid * 8 + 2048 * j);
             if (c >= c1) continue;
-            const float f = factor[(c - c0) / 128];
+            const float f = factor[(c - c0) / 64];
             if (kF32) {
                 float2 v = make_float2(__uint_as_float(now[j].x), __uint_as_float(now[j].y));
                 v.x = c + 2 * lane < a.V ? v.x * f : 0.0f;

@@ -142,7 +142,7 @@ int launch_gemm(const Tensors* t, GemmArgs& args, cudaStream_t stream) {
         int rc = make_map(&maps.a[q], t[q].a.ptr, t[q].a.rows, t[q].a.cols, t[q].a.ld, p.a_mn ? kBK : kBM);
         if (rc == SW_OK)
             rc = make_map(&maps.b[q], t[q].b.ptr, t[q].b.rows, t[q].b.cols, t[q].b.ld,
-                          kEpi == kEpiOut ? kBK : Cf::kBRows);
+                          kEpi == kEpiOut ? kBK : kShape == kSingle ? args.tile_n : Cf::kBRows);
         if (rc == SW_OK && t[q].c.ptr) rc = make_target_map(&maps.c[q], t[q].c);
         if (rc != SW_OK) return rc;
         p.pa = t[q].a.plane;
@@ -161,7 +161,9 @@ int launch_gemm(const Tensors* t, GemmArgs& args, cudaStream_t stream) {
     // every SM, unless it is known here that there are fewer tiles
     int64_t items = device_sms() / kCtas;
     if (args.problems == 1 && args.p[0].splits == 1)
-        items = std::min<int64_t>(items, tiles_of(args.p[0].M, args.p[0].N, kShape));
+        items = std::min<int64_t>(items, (args.p[0].M + Cf::kTileM - 1) / Cf::kTileM *
+                                             ((args.p[0].N + (kEpi == kEpiOut ? kBN : args.tile_n) - 1) /
+                                              (kEpi == kEpiOut ? kBN : args.tile_n)));
     if (items == 0) return SW_OK;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(kCtas * (unsigned)items);
@@ -248,7 +250,9 @@ struct Layout {
 
 struct Shape {
     int64_t T, D, V, rows_pad, ld_h;
-    int64_t half_tiles;      // 128-column halves of the vocabulary's tiles, each with its statistics
+    int tile_n;              // columns of a logits tile
+    int64_t slots;           // pieces of the vocabulary's tiles with statistics of their own
+    int slot_shift;
     bool f32, pack_w, grads, flags;
     int planes;
     // Gradients: `keep`: the forward's exponentials of `rows` compact rows at a
@@ -286,7 +290,7 @@ Layout lay_out(Bump& b, const Call& c, const Shape& s) {
     l.lse2 = b.take<float>(s.rows_pad);
     l.row_loss = b.take<float>(s.rows_pad);
     l.hc = b.take<uint16_t>(s.planes * s.rows_pad * s.ld_h);
-    if (c.loss) l.partial = b.take<float4>(s.half_tiles * s.rows_pad);
+    if (c.loss) l.partial = b.take<float4>(s.slots * s.rows_pad);
     if (s.keep) l.ent_s = b.take<float>(s.rows_pad * K);
     if (s.dh_sum_rows) l.dh_sums = b.take<float>(s.dh_sum_rows * s.ld_acc);
     if (s.dw_sum_rows) l.dw_sums = b.take<float>(s.dw_sum_rows * s.ld_acc);
@@ -355,8 +359,12 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
         if (!pa.h) pa.h = l.hc;  // no rows: only zeros are written
     }
     // 8 rows a CTA for parallelism; 32 where every CTA's look at all T rows would show
+    // Where there are few rows, several CTAs share the packing of 8 (2 column-major
+    // rows of 2880 against 765 classes: 50 us with one CTA, 29 so).
+    const int64_t blocks = s.rows_pad / 8, chunks = kBf16 ? (s.ld_h + 255) / 256 : 1;
+    const unsigned shares = (unsigned)std::max<int64_t>(1, std::min<int64_t>(chunks, sms / blocks));
     if (s.T <= 16384)
-        SW_CUDA_TRY(launch_pdl(prepare_kernel<8>, dim3((unsigned)(s.rows_pad / 8)), dim3(256), 0, stream, pa),
+        SW_CUDA_TRY(launch_pdl(prepare_kernel<8>, dim3((unsigned)blocks, shares), dim3(256), 0, stream, pa),
                     "linear head rows");
     else
         SW_CUDA_TRY(launch_pdl(prepare_kernel<32>, dim3((unsigned)(s.rows_pad / 32)), dim3(256), 0, stream, pa),
@@ -418,7 +426,9 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
     g.logit_scale = c.scale;
     g.ent_p = l.ent_p;
     g.ent_k = top_k;
-    g.half_tiles = (int)s.half_tiles;
+    g.slots = (int)s.slots;
+    g.slot_shift = s.slot_shift;
+    g.tile_n = s.tile_n;
     g.rows_pad = (int)s.rows_pad;
     const Target grad_out{l.grad, s.rows, ld_grad, ld_grad, false}, none{nullptr, 0, 0, 0, false};
 
@@ -450,7 +460,7 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
         a.ent_idx = l.ent_idx + r0 * g.ent_k;
         a.ent_p = l.ent_p ? l.ent_p + r0 * g.ent_k : nullptr;
         a.offs = l.offs ? l.offs + r0 : nullptr;
-        a.partial = l.partial + r0 * s.half_tiles;
+        a.partial = l.partial + r0 * s.slots;
         a.lse2 = l.lse2 + r0;
         a.coef = l.coef + r0;
         return a;
@@ -460,7 +470,8 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
         LossArgs a;
         memset(&a, 0, sizeof(a));
         a.partial = l.partial;
-        a.half_tiles = (int)s.half_tiles;
+        a.slots = (int)s.slots;
+        a.slot_shift = s.slot_shift;
         a.row0 = (int)r0;
         a.rows = (int)n;
         a.all_rows = (int)std::max<int64_t>(s.T, 1);
@@ -726,12 +737,20 @@ int check_and_run(const char* name, Call& c, void* stream_ptr) {
         const int64_t per_column = (grads ? s.planes * s.rows_pad * 2 : 0) + (s.pack_w ? s.planes * s.ld_h * 2 : 0);
         if (per_column > 0) s.piece = std::min(s.piece, std::max<int64_t>(budget / per_column / 256 * 256, 256));
     }
-    s.half_tiles = (V + kBN - 1) / kBN * 2;
     const int64_t n = std::min(s.rows, T), nv = std::min(s.piece, V);
     s.logits_shape = choose_parts(n, nv, D, terms, kSingle, false).us <
                              0.97f * choose_parts(n, nv, D, terms, kPair2, false).us
                          ? kSingle
                          : kPair2;
+    // Where 256-column tiles would leave SMs idle, narrower ones spread the weights
+    // over more of them: the loss of one token over 32000 classes at dim 4096 65 us
+    // at 256 columns, 61 at 128; Float32 33 x 1021 at dim 257 with gradients 55, 49 at 64.
+    s.tile_n = kBN;
+    if (s.logits_shape == kSingle)
+        for (const int t : {128, 64})
+            if ((n + kBM - 1) / kBM * ((nv + t - 1) / t) <= device_sms()) s.tile_n = t;
+    s.slot_shift = s.tile_n == 64 ? 6 : 7;
+    s.slots = (V + s.tile_n - 1) / s.tile_n * (s.tile_n >> s.slot_shift);
     // dw is written at once through TMA where that can describe it (rows that end
     // inside 16 bytes would be written past their end).
     const int64_t es = s.f32 ? 4 : 2;
