@@ -257,6 +257,13 @@ struct Plan {
     }
 };
 
+// One lane of a converged warp, always the same.
+__device__ __forceinline__ bool elected() {
+    uint32_t is;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(is));
+    return is != 0;
+}
+
 // D[tmem] (+)= A[smem] B[smem], 16-bit operands, fp32 accumulation.
 template <bool kPair>
 __device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
@@ -835,7 +842,8 @@ __global__ void __launch_bounds__(320, 1)
                 }
         }
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
+        // (the whole warp keeps in step and one lane issues)
+        if (rank == 0) {
             // ---------------- MMA issuer ----------------
             int stage = 0;
             uint32_t phase = 0, it = 0;
@@ -847,7 +855,11 @@ __global__ void __launch_bounds__(320, 1)
                 // K-major: 16 elements of K are 32 bytes of the swizzled row, 8-row groups 1024 bytes apart.
                 // MN-major: 16 rows of K are 2048 bytes, 64-element blocks of the other mode 8192 bytes
                 // apart, 8-row groups of K 1024.
-                const uint32_t a_step = a_mn ? 2048 : 32, a_block = a_mn ? 8192 : 0;
+                // (descriptors count in 16 bytes, and the stages stay below 2^18)
+                const uint32_t a_step = a_mn ? 2048 / 16 : 32 / 16, b_step = kBMn ? 2048 / 16 : 32 / 16;
+                const uint64_t a_desc = ptx::smem_desc(sbase, a_mn ? 8192 : 0, 1024, ptx::kLayoutSwizzle128);
+                const uint64_t b_desc =
+                    ptx::smem_desc(sbase + C::kABytes, kBMn ? 8192 : 0, 1024, ptx::kLayoutSwizzle128);
                 for (int i = 0, t; alive && (t = plan.nth(i, worker, workers)) >= 0; ++i) {
                 int mb, nb, split, k0, k1;
                 plan.item(t, mb, nb, split, k0, k1);
@@ -857,39 +869,36 @@ __global__ void __launch_bounds__(320, 1)
                     const uint32_t buf0 = C::kAccs == 1 ? it & 1 : 0, drained = (C::kAccs == 1 ? it >> 1 : it) & 1;
                     const int steps = (chunk_end(c0, k1) - c0) * args.terms;
                     for (int ks = 0; ks < steps && alive; ++ks) {
-                        if (!ptx::mbar_wait(bar_full + 8 * stage, phase)) { alive = false; break; }
+                        if (!__all_sync(0xffffffffu, ptx::mbar_wait(bar_full + 8 * stage, phase))) { alive = false; break; }
                         ptx::tc_fence_after();
 #pragma unroll
                         for (int h = 0; h < C::kAccs; ++h) {
                             const uint32_t buf = buf0 + h;
                             if (ks == 0) {
-                                if (!ptx::mbar_wait(bar_tmem_empty + 8 * buf, drained ^ 1)) { alive = false; break; }
+                                if (!__all_sync(0xffffffffu, ptx::mbar_wait(bar_tmem_empty + 8 * buf, drained ^ 1))) { alive = false; break; }
                                 ptx::tc_fence_after();
                             }
                             const uint32_t acc = tmem + buf * kBN;
-                            const uint32_t sa = sbase + stage * C::kStageBytes + h * (kBM * kBK * 2);
-                            const uint32_t sb = sbase + stage * C::kStageBytes + C::kABytes;
+                            const uint64_t ad = a_desc + uint32_t(stage * C::kStageBytes + h * (kBM * kBK * 2)) / 16;
+                            const uint64_t bd = b_desc + uint32_t(stage * C::kStageBytes) / 16;
+                            if (elected())
 #pragma unroll
-                            for (int j = 0; j < kBK / 16; ++j) {
-                                const uint64_t ad = ptx::smem_desc(sa + a_step * j, a_block, 1024, ptx::kLayoutSwizzle128);
-                                const uint64_t bd = kBMn
-                                                        ? ptx::smem_desc(sb + 2048 * j, 8192, 1024, ptx::kLayoutSwizzle128)
-                                                        : ptx::smem_desc(sb + 32 * j, 0, 1024, ptx::kLayoutSwizzle128);
-                                mma_f16<kPair>(acc, ad, bd, idesc, (ks > 0 || j > 0) ? 1u : 0u);
-                            }
-                            if (C::kAccs > 1 && ks + 1 == steps) commit<kPair>(bar_tmem_full + 8 * buf);
+                            for (int j = 0; j < kBK / 16; ++j)
+                                mma_f16<kPair>(acc, ad + a_step * j, bd + b_step * j, idesc,
+                                               (ks > 0 || j > 0) ? 1u : 0u);
+                            if (C::kAccs > 1 && ks + 1 == steps && elected()) commit<kPair>(bar_tmem_full + 8 * buf);
                         }
                         if (!alive) break;
-                        commit<kPair>(bar_empty + 8 * stage);
+                        if (elected()) commit<kPair>(bar_empty + 8 * stage);
                         if (++stage == kStages) { stage = 0; phase ^= 1; }
                     }
                     if (!alive) break;
-                    if (C::kAccs == 1) commit<kPair>(bar_tmem_full + 8 * buf0);
+                    if (C::kAccs == 1 && elected()) commit<kPair>(bar_tmem_full + 8 * buf0);
                 }
             }
             }
             // every MMA is done before TMEM is released
-            commit<kPair>(bar_drain);
+            if (elected()) commit<kPair>(bar_drain);
             ptx::mbar_wait(bar_drain, 0);
         }
     } else {
