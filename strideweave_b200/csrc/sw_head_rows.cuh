@@ -692,7 +692,7 @@ struct PlaceArgs {
     int64_t dst_row, dst_col;
     int vec;                 // dst rows are contiguous and aligned to four elements
 };
-template <bool kF32>
+template <bool kF32, int kRows>
 __global__ void __launch_bounds__(256) place_kernel(const PlaceArgs a) {
     pdl_enter();
     const int splits = a.splits > 0 ? a.splits : a.state->dh_splits;
@@ -700,39 +700,54 @@ __global__ void __launch_bounds__(256) place_kernel(const PlaceArgs a) {
     const bool few = !kF32 && a.by_count && a.state->few(a.row0);  // their remainders are further rows
     const Walk walk(few ? kFewRows + int(summed) : int(summed), int((a.cols + kBN - 1) / kBN), a.tile_m, a.workers,
                     splits);
-    // a CTA takes 1024 columns of a row at a time
-    const int64_t spans = (a.cols + 1023) / 1024;
-    for (int64_t u = blockIdx.x; u < a.rows * spans; u += gridDim.x) {
-        const int64_t m = u / spans, c = (u - m * spans) * 1024 + threadIdx.x * 4;
-        if (c >= a.cols) continue;
-        const float* p = a.sums + c;  // ld is whole groups of four
-        float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (m < summed) {
-            const int parts = walk.tile_of(int(m) / a.tile_m, int(c) / kBN) < walk.whole ? 1 : splits;
+    // a CTA takes 1024 columns of kRows rows (of one tile) at a time: with four,
+    // a thread has four reads in flight where one left it waiting (4096 x 4096:
+    // 60 us with one row, 33 so); with few rows and many parts to add, CTAs are
+    // worth more (64 x 2048: 10 us with one row, 17 with four)
+    const int64_t c = int64_t(blockIdx.x) * 1024 + threadIdx.x * 4;
+    if (c >= a.cols) return;
+    for (int64_t m0 = int64_t(blockIdx.y) * kRows; m0 < a.rows; m0 += int64_t(gridDim.y) * kRows) {
+        float4 s[kRows];
+#pragma unroll
+        for (int j = 0; j < kRows; ++j) s[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (m0 < summed) {
+            const int parts = walk.tile_of(int(m0) / a.tile_m, int(c) / kBN) < walk.whole ? 1 : splits;
             for (int rest = 0; rest <= (few ? kFewRows : 0); rest += kFewRows) {
-#pragma unroll 8
+#pragma unroll(8 / kRows)
                 for (int k = 0; k < parts; ++k) {
-                    const float4 v =
-                        *reinterpret_cast<const float4*>(p + int64_t(walk.sum_row(k, int(m) + rest)) * a.ld);
-                    s.x += v.x;
-                    s.y += v.y;
-                    s.z += v.z;
-                    s.w += v.w;
+                    // (ld is whole groups of four)
+                    const float* p = a.sums + int64_t(walk.sum_row(k, int(m0) + rest)) * a.ld + c;
+#pragma unroll
+                    for (int j = 0; j < kRows; ++j)
+                        if (m0 + j < summed) {
+                            const float4 v = *reinterpret_cast<const float4*>(p + j * a.ld);
+                            s[j].x += v.x;
+                            s[j].y += v.y;
+                            s[j].z += v.z;
+                            s[j].w += v.w;
+                        }
                 }
             }
         }
-        const int64_t at = (a.row_map ? int64_t(a.row_map[m]) : m) * a.dst_row + c * a.dst_col;
-        if (a.vec && c + 4 <= a.cols) {
-            if (kF32) *reinterpret_cast<float4*>(static_cast<float*>(a.dst) + at) = s;
-            else
-                *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.dst) + at) =
-                    make_uint2(pack2<true>(s.x, s.y), pack2<true>(s.z, s.w));
-            continue;
-        }
-        const float r[4] = {s.x, s.y, s.z, s.w};
-        for (int j = 0; j < 4 && c + j < a.cols; ++j) {
-            if (kF32) static_cast<float*>(a.dst)[at + j * a.dst_col] = r[j];
-            else static_cast<__nv_bfloat16*>(a.dst)[at + j * a.dst_col] = __float2bfloat16_rn(r[j]);
+#pragma unroll
+        for (int j = 0; j < kRows; ++j) {
+            const int64_t m = m0 + j;
+            if (m >= a.rows) break;
+            const int64_t at = (a.row_map ? int64_t(a.row_map[m]) : m) * a.dst_row + c * a.dst_col;
+            if (a.vec && c + 4 <= a.cols) {
+                if (kF32) *reinterpret_cast<float4*>(static_cast<float*>(a.dst) + at) = s[j];
+                else
+                    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.dst) + at) =
+                        make_uint2(pack2<true>(s[j].x, s[j].y), pack2<true>(s[j].z, s[j].w));
+                continue;
+            }
+            const float r[4] = {s[j].x, s[j].y, s[j].z, s[j].w};
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (c + q < a.cols) {
+                    if (kF32) static_cast<float*>(a.dst)[at + q * a.dst_col] = r[q];
+                    else static_cast<__nv_bfloat16*>(a.dst)[at + q * a.dst_col] = __float2bfloat16_rn(r[q]);
+                }
         }
     }
 }

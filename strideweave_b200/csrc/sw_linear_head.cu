@@ -533,9 +533,11 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
             sa.dst_row = dst_row;
             sa.dst_col = dst_col;
             sa.vec = dst_col == 1 && dst_row % 4 == 0 && (reinterpret_cast<uintptr_t>(dst) & (4 * esize - 1)) == 0;
-            const int64_t spans = rows * ((s.D + 1023) / 1024);
-            SW_CUDA_TRY(launch_pdl(place_kernel<kF32>, dim3((unsigned)std::min<int64_t>(spans, fill)),
-                                   dim3(256), 0, stream, sa),
+            const int64_t spans = (s.D + 1023) / 1024, per = rows * spans < 8 * sms ? 1 : 4;
+            const int64_t share = std::max<int64_t>(1, std::min<int64_t>((rows + per - 1) / per, fill / spans));
+            const dim3 grid((unsigned)spans, (unsigned)share);
+            SW_CUDA_TRY(per == 1 ? launch_pdl(place_kernel<kF32, 1>, grid, dim3(256), 0, stream, sa)
+                                 : launch_pdl(place_kernel<kF32, 4>, grid, dim3(256), 0, stream, sa),
                         "linear head sums");
             return SW_OK;
         };
