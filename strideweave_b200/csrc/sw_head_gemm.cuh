@@ -20,9 +20,11 @@
 //            for a second tile, so about 3000 cycles of a tile's epilogue are not
 //            hidden; in exchange a quarter fewer bytes come from L2, which under
 //            the power limit buys clock.
-// Warp 0 feeds a ring of 64-deep K stages by TMA (128-byte swizzle), one thread
-// of warp 1 (of the pair's first CTA) issues the MMAs, warps 2-9 drain one of
-// two TMEM accumulators while the other is being filled: warp w reads TMEM
+// Warp 0 feeds a ring of 64-deep K stages by TMA (128-byte swizzle), one elected
+// lane of warp 1 (of the pair's first CTA) issues the MMAs (from a warp that
+// stays in step: a lone thread took about 350 cycles for a stage's four MMAs, of
+// the 512 that they last; so it takes 200), warps 2-9 drain one of two TMEM
+// accumulators while the other is being filled: warp w reads TMEM
 // sub-partition w % 4 (32 rows) and one half of the tile's columns.  Results
 // pass through 4 KiB of shared memory per warp, so that they leave as whole
 // 128-byte row segments.  Float32 operands come as two f16 planes (hi + lo of a
@@ -110,9 +112,6 @@ struct HeadState {
     // Rows that count from row0 on, and whether they have remainder rows (bf16).
     __device__ __forceinline__ int rows(int row0) const { return max(count - row0, 0); }
     __device__ __forceinline__ bool few(int row0) const { return count <= kFewRows && rows(row0) > 0; }
-    __device__ __forceinline__ int rows_and_rest(int row0, bool bf16) const {
-        return bf16 && few(row0) ? kFewRows + rows(row0) : rows(row0);
-    }
 };
 
 // Power-of-two multiplier that brings values of magnitude `amax` just under
@@ -208,7 +207,9 @@ struct Cfg {
 // Estimated microseconds of a K stage, and of a tile's fill and drain that
 // nothing hides: a stage takes 0.27 us (kSingle: 128 x 256 on one SM), 0.26 (kPair2:
 // 256 x 256 on two) or 0.52 (kTall).
-__host__ __device__ inline float stage_us(int shape, int terms) { return float(terms) * (shape == kTall ? 0.52f : shape == kPair2 ? 0.26f : 0.27f); }
+__host__ __device__ inline float stage_us(int shape, int terms) {
+    return float(terms) * (shape == kTall ? 0.52f : shape == kPair2 ? 0.26f : 0.27f);
+}
 __host__ __device__ inline float fixed_us(int shape) { return shape == kTall ? 5.0f : shape == kPair2 ? 2.5f : 2.0f; }
 __host__ __device__ inline int shape_workers(int shape, int sms) { return shape == kSingle ? sms : sms / 2; }
 
@@ -537,8 +538,8 @@ struct WarpRows {
 // (11 bits down to 2^-29 of the half tile's largest; the later rounding to
 // bf16 is the one that counts) or, for Float32, as they are.
 template <bool kBf16, int kBlocks, class Rows>
-__device__ __forceinline__ float4 lse_tile(const GemmArgs& args, const void* tmap_c, Rows& wr, EntryCursor& cur, int64_t n0,
-                                           int64_t n_end, float k2, float (&r)[kBlocks][2][32]) {
+__device__ __forceinline__ float4 lse_tile(const GemmArgs& args, const void* tmap_c, Rows& wr, EntryCursor& cur,
+                                           int64_t n0, int64_t n_end, float k2, float (&r)[kBlocks][2][32]) {
     const int64_t m = wr.m0 + wr.lane;
     float dot = 0.0f, top = -INFINITY;
 #pragma unroll
@@ -687,6 +688,19 @@ __device__ __forceinline__ void out_tile(const Problem& args, const void* tmap_c
     }
 }
 
+// The contraction kernel.  A launch computes args.p[0] (kBoth: and args.p[1], half
+// of the workers each first, see Plan).  The tensor cores bound it, and under
+// long load the power limit; a tile's epilogue runs under the next tile's MMAs:
+//
+//   4096 x 32000, dim 4096: logits with statistics and their exponentials 699 us
+//   (tensor pipe 90 % busy), dh 691 (93 %), dw 685 (91 %): 1.54, 1.55, 1.57 PFLOP/s;
+//   dim 2048: 436 (75 %), 349 (96 %), 328 (89 %).  The logits of short walks stay
+//   behind: at dim 1024 a 256 x 256 tile lasts about 10000 cycles, its epilogue
+//   5400, with the exponentials' store 9500.
+//   Float32, 2048 x 32000, dim 1024, three plane pairs: 298 (80 %), 297 (86 %), 304
+//   (74 %): 1.35, 1.35, 1.32 PFLOP/s of f16 products.
+//   1 x 32000, dim 4096: 54 us, the read of w at 4.8 TB/s; 64 x 131072, dim 2048:
+//   102 us, 5.3 TB/s, both gradients in one launch 206 us, 5.2 TB/s.
 template <int kShape, bool kBf16, int kEpi, int kA>
 __global__ void __launch_bounds__(320, 1)
     head_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmArgs args) {
@@ -854,48 +868,53 @@ __global__ void __launch_bounds__(320, 1)
                 const bool a_mn = mn_major(args.p[q]);
                 // K-major: 16 elements of K are 32 bytes of the swizzled row, 8-row groups 1024 bytes apart.
                 // MN-major: 16 rows of K are 2048 bytes, 64-element blocks of the other mode 8192 bytes
-                // apart, 8-row groups of K 1024.
-                // (descriptors count in 16 bytes, and the stages stay below 2^18)
+                // apart, 8-row groups of K 1024.  Descriptors count in 16 bytes, and the stages
+                // stay below 2^18: each is the first one plus an offset.
                 const uint32_t a_step = a_mn ? 2048 / 16 : 32 / 16, b_step = kBMn ? 2048 / 16 : 32 / 16;
                 const uint64_t a_desc = ptx::smem_desc(sbase, a_mn ? 8192 : 0, 1024, ptx::kLayoutSwizzle128);
                 const uint64_t b_desc =
                     ptx::smem_desc(sbase + C::kABytes, kBMn ? 8192 : 0, 1024, ptx::kLayoutSwizzle128);
                 for (int i = 0, t; alive && (t = plan.nth(i, worker, workers)) >= 0; ++i) {
-                int mb, nb, split, k0, k1;
-                plan.item(t, mb, nb, split, k0, k1);
-                const uint32_t idesc = idesc_f16(kBf16, a_mn, kBMn, C::kAccRows, tile_cols(args.p[q], nb));
-                for (int c0 = k0; c0 < k1 && alive; c0 = chunk_end(c0, k1), ++it) {
-                    // one tile alternates between the two accumulators, a tall one fills both
-                    const uint32_t buf0 = C::kAccs == 1 ? it & 1 : 0, drained = (C::kAccs == 1 ? it >> 1 : it) & 1;
-                    const int steps = (chunk_end(c0, k1) - c0) * args.terms;
-                    for (int ks = 0; ks < steps && alive; ++ks) {
-                        if (!__all_sync(0xffffffffu, ptx::mbar_wait(bar_full + 8 * stage, phase))) { alive = false; break; }
-                        ptx::tc_fence_after();
+                    int mb, nb, split, k0, k1;
+                    plan.item(t, mb, nb, split, k0, k1);
+                    const uint32_t idesc = idesc_f16(kBf16, a_mn, kBMn, C::kAccRows, tile_cols(args.p[q], nb));
+                    for (int c0 = k0; c0 < k1 && alive; c0 = chunk_end(c0, k1), ++it) {
+                        // one tile alternates between the two accumulators, a tall one fills both
+                        const uint32_t buf0 = C::kAccs == 1 ? it & 1 : 0;
+                        const uint32_t drained = (C::kAccs == 1 ? it >> 1 : it) & 1;
+                        const int steps = (chunk_end(c0, k1) - c0) * args.terms;
+                        for (int ks = 0; ks < steps && alive; ++ks) {
+                            alive = __all_sync(0xffffffffu, ptx::mbar_wait(bar_full + 8 * stage, phase));
+                            if (!alive) break;
+                            ptx::tc_fence_after();
 #pragma unroll
-                        for (int h = 0; h < C::kAccs; ++h) {
-                            const uint32_t buf = buf0 + h;
-                            if (ks == 0) {
-                                if (!__all_sync(0xffffffffu, ptx::mbar_wait(bar_tmem_empty + 8 * buf, drained ^ 1))) { alive = false; break; }
-                                ptx::tc_fence_after();
+                            for (int h = 0; h < C::kAccs; ++h) {
+                                const uint32_t buf = buf0 + h;
+                                if (ks == 0) {
+                                    alive = __all_sync(0xffffffffu,
+                                                       ptx::mbar_wait(bar_tmem_empty + 8 * buf, drained ^ 1));
+                                    if (!alive) break;
+                                    ptx::tc_fence_after();
+                                }
+                                const uint32_t acc = tmem + buf * kBN;
+                                const uint64_t ad = a_desc + uint32_t(stage * C::kStageBytes + h * (kBM * kBK * 2)) / 16;
+                                const uint64_t bd = b_desc + uint32_t(stage * C::kStageBytes) / 16;
+                                if (elected()) {
+#pragma unroll
+                                    for (int j = 0; j < kBK / 16; ++j)
+                                        mma_f16<kPair>(acc, ad + a_step * j, bd + b_step * j, idesc,
+                                                       (ks > 0 || j > 0) ? 1u : 0u);
+                                    if (C::kAccs > 1 && ks + 1 == steps) commit<kPair>(bar_tmem_full + 8 * buf);
+                                }
                             }
-                            const uint32_t acc = tmem + buf * kBN;
-                            const uint64_t ad = a_desc + uint32_t(stage * C::kStageBytes + h * (kBM * kBK * 2)) / 16;
-                            const uint64_t bd = b_desc + uint32_t(stage * C::kStageBytes) / 16;
-                            if (elected())
-#pragma unroll
-                            for (int j = 0; j < kBK / 16; ++j)
-                                mma_f16<kPair>(acc, ad + a_step * j, bd + b_step * j, idesc,
-                                               (ks > 0 || j > 0) ? 1u : 0u);
-                            if (C::kAccs > 1 && ks + 1 == steps && elected()) commit<kPair>(bar_tmem_full + 8 * buf);
+                            if (!alive) break;
+                            if (elected()) commit<kPair>(bar_empty + 8 * stage);
+                            if (++stage == kStages) { stage = 0; phase ^= 1; }
                         }
                         if (!alive) break;
-                        if (elected()) commit<kPair>(bar_empty + 8 * stage);
-                        if (++stage == kStages) { stage = 0; phase ^= 1; }
+                        if (C::kAccs == 1 && elected()) commit<kPair>(bar_tmem_full + 8 * buf0);
                     }
-                    if (!alive) break;
-                    if (C::kAccs == 1 && elected()) commit<kPair>(bar_tmem_full + 8 * buf0);
                 }
-            }
             }
             // every MMA is done before TMEM is released
             if (elected()) commit<kPair>(bar_drain);
@@ -936,80 +955,81 @@ __global__ void __launch_bounds__(320, 1)
             const int M = kEpi == kEpiOut ? 0 : min(args.state->rows(args.row0), few ? INT_MAX : p.M);
             const float out_scale = kEpi == kEpiOut ? inverse(p) * args.state->grad_scale : 1.0f;
             for (int i = 0, t; alive && (t = plan.nth(i, worker, workers)) >= 0; ++i) {
-            int mb, nb, split, k0, k1;
-            plan.item(t, mb, nb, split, k0, k1);
+                int mb, nb, split, k0, k1;
+                plan.item(t, mb, nb, split, k0, k1);
 #pragma unroll 1
-            for (int h = 0; h < C::kAccs && alive; ++h) {
-    wr.m0 = int64_t(mb) * C::kTileM + h * C::kAccRows + rank * kBM + quarter * 32;
-                const int64_t m = wr.m0 + lane;
-                wr.row_in = m < M;
-                const int64_t ncol0 = int64_t(nb) * tile_n + half * kCols;
-                const int64_t n_end = min(int64_t(p.N), min(ncol0 + kCols, int64_t(nb + 1) * tile_n));
-                // a pair's second half may lie past the rows that the workspace holds
-                // (and a narrow tile's second half is none)
-                const bool rows_in = kEpi == kEpiOut || (wr.m0 < (p.M + kBM - 1) / kBM * kBM &&
-                                                         (!kNarrow || half * kCols < tile_n));
-                // what the row needs beside its accumulator, while the MMAs run
-                EntryCursor cur;
-                float lse2 = 0.0f, coef = 0.0f;
-                if (kEpi != kEpiOut) {
-                    wr.begin();  // the entries go where the stores' boxes are
-                    cur.fetch(args, wr.box, lane, m, wr.row_in, int(args.v0 + ncol0), int(n_end - ncol0));
-                }
-                if (kEpi == kEpiGrad && wr.row_in) {
-                    lse2 = args.lse2[m];
-                    coef = args.coef[m] * gscale;
-                }
-                const uint32_t lanes = uint32_t(quarter * 32) << 16;
-                // The half tile's row in registers: the accumulator is free again
-                // before any of the work on it.  (An empty share of K: zeros.)
-                float r[2][2][32];
-                if (k0 >= k1) {
-#pragma unroll
-                    for (int c = 0; c < 4; ++c)
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) r[c / 2][c % 2][j] = 0.0f;
-                }
-                for (int c0 = k0; c0 < k1; c0 = chunk_end(c0, k1)) {
-                    const uint32_t buf = C::kAccs == 1 ? it & 1 : h, filled = (C::kAccs == 1 ? it >> 1 : it) & 1;
-                    if (!__all_sync(0xffffffffu, ptx::mbar_wait(bar_tmem_full + 8 * buf, filled))) {
-                        alive = false;
-                        break;
+                for (int h = 0; h < C::kAccs && alive; ++h) {
+                    wr.m0 = int64_t(mb) * C::kTileM + h * C::kAccRows + rank * kBM + quarter * 32;
+                    const int64_t m = wr.m0 + lane;
+                    wr.row_in = m < M;
+                    const int64_t ncol0 = int64_t(nb) * tile_n + half * kCols;
+                    const int64_t n_end = min(int64_t(p.N), min(ncol0 + kCols, int64_t(nb + 1) * tile_n));
+                    // a pair's second half may lie past the rows that the workspace holds
+                    // (and a narrow tile's second half is none)
+                    const bool rows_in = kEpi == kEpiOut || (wr.m0 < (p.M + kBM - 1) / kBM * kBM &&
+                                                             (!kNarrow || half * kCols < tile_n));
+                    // what the row needs beside its accumulator, while the MMAs run
+                    EntryCursor cur;
+                    float lse2 = 0.0f, coef = 0.0f;
+                    if (kEpi != kEpiOut) {
+                        wr.begin();  // the entries go where the stores' boxes are
+                        cur.fetch(args, wr.box, lane, m, wr.row_in, int(args.v0 + ncol0), int(n_end - ncol0));
                     }
-                    ptx::tc_fence_after();
-                    const uint32_t acc = tmem + buf * kBN + half * kCols + lanes;
-                    if (c0 == k0) {
+                    if (kEpi == kEpiGrad && wr.row_in) {
+                        lse2 = args.lse2[m];
+                        coef = args.coef[m] * gscale;
+                    }
+                    const uint32_t lanes = uint32_t(quarter * 32) << 16;
+                    // The half tile's row in registers: the accumulator is free again
+                    // before any of the work on it.  (An empty share of K: zeros.)
+                    float r[2][2][32];
+                    if (k0 >= k1) {
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) tmem_ld_f32_x32(acc + c * 32, r[c / 2][c % 2]);
-                        ptx::tmem_ld_wait();
-                    } else if (kChunked) {
+                        for (int c = 0; c < 4; ++c)
 #pragma unroll
-                        for (int c = 0; c < 8; ++c) {
-                            uint32_t u[16];
-                            tmem_ld_32x32b_x16(acc + c * 16, u);
-                            ptx::tmem_ld_wait();
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) r[c / 4][c / 2 % 2][c % 2 * 16 + j] += __uint_as_float(u[j]);
+                            for (int j = 0; j < 32; ++j) r[c / 2][c % 2][j] = 0.0f;
+                    }
+                    for (int c0 = k0; c0 < k1; c0 = chunk_end(c0, k1)) {
+                        const uint32_t buf = C::kAccs == 1 ? it & 1 : h, filled = (C::kAccs == 1 ? it >> 1 : it) & 1;
+                        if (!__all_sync(0xffffffffu, ptx::mbar_wait(bar_tmem_full + 8 * buf, filled))) {
+                            alive = false;
+                            break;
                         }
+                        ptx::tc_fence_after();
+                        const uint32_t acc = tmem + buf * kBN + half * kCols + lanes;
+                        if (c0 == k0) {
+#pragma unroll
+                            for (int c = 0; c < 4; ++c) tmem_ld_f32_x32(acc + c * 32, r[c / 2][c % 2]);
+                            ptx::tmem_ld_wait();
+                        } else if (kChunked) {
+#pragma unroll
+                            for (int c = 0; c < 8; ++c) {
+                                uint32_t u[16];
+                                tmem_ld_32x32b_x16(acc + c * 16, u);
+                                ptx::tmem_ld_wait();
+#pragma unroll
+                                for (int j = 0; j < 16; ++j)
+                                    r[c / 4][c / 2 % 2][c % 2 * 16 + j] += __uint_as_float(u[j]);
+                            }
+                        }
+                        release(buf);
+                        if (h + 1 == C::kAccs) ++it;
                     }
-                    release(buf);
-                    if (h + 1 == C::kAccs) ++it;
-                }
-                if (!alive) break;
-                if (!rows_in) continue;
-                if (kEpi != kEpiOut) cur.begin();
-                if (kEpi == kEpiLse) {
-                    const float4 st = lse_tile<kBf16, 2>(args, tmap_c, wr, cur, ncol0, n_end, k2, r);
-                    args.partial[m * args.slots + ((args.v0 + ncol0) >> args.slot_shift)] = st;
-                } else if (kEpi == kEpiGrad) {
-                    if (few) grad_tile<kBf16, kBf16>(args, tmap_c, wr, cur, ncol0, n_end, k2, lse2, coef, r);
-                    else grad_tile<kBf16, false>(args, tmap_c, wr, cur, ncol0, n_end, k2, lse2, coef, r);
-                } else {
-                    out_tile<!kBf16>(p, tmap_c, wr, p.sums ? plan.walk.sum_row(split, int(wr.m0)) : int(wr.m0), ncol0,
-                                     out_scale, r);
+                    if (!alive) break;
+                    if (!rows_in) continue;
+                    if (kEpi != kEpiOut) cur.begin();
+                    if (kEpi == kEpiLse) {
+                        const float4 st = lse_tile<kBf16, 2>(args, tmap_c, wr, cur, ncol0, n_end, k2, r);
+                        args.partial[m * args.slots + ((args.v0 + ncol0) >> args.slot_shift)] = st;
+                    } else if (kEpi == kEpiGrad) {
+                        if (few) grad_tile<kBf16, kBf16>(args, tmap_c, wr, cur, ncol0, n_end, k2, lse2, coef, r);
+                        else grad_tile<kBf16, false>(args, tmap_c, wr, cur, ncol0, n_end, k2, lse2, coef, r);
+                    } else {
+                        const int row = p.sums ? plan.walk.sum_row(split, int(wr.m0)) : int(wr.m0);
+                        out_tile<!kBf16>(p, tmap_c, wr, row, ncol0, out_scale, r);
+                    }
                 }
             }
-        }
         }
         if (lane == 0) ptx::bulk_wait_group0();  // this warp's stores are done
     }
