@@ -33,8 +33,9 @@
 //
 // The tensor core's fp32 accumulator drops the bits below its last place, so a
 // long K walk drifts: measured 1.3e-9 per K element, 1.5e-4 over 128000.  Where
-// the result is Float32 (kChunked) the walk is cut into 8 or 16 stages, and the
-// epilogue adds the pieces in registers, rounded to nearest.
+// the result is Float32 (kChunked: logits, and Float32 gradients) the walk is cut
+// into pieces of args.chunk stages, and the epilogue adds them in registers, rounded
+// to nearest.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -162,6 +163,7 @@ struct GemmArgs {
     const HeadState* state;
     int row0;                // first compact row of this launch (the count starts there)
     int terms;               // plane pairs walked: 1, or 3 for Float32
+    int chunk;               // K stages between two sums in registers (kChunked)
     // logits epilogues
     float logit_scale;
     int64_t v0;              // first vocabulary column of this piece
@@ -711,8 +713,6 @@ __global__ void __launch_bounds__(320, 1)
     constexpr bool kPair = C::kPair;
     constexpr bool kChunked = !kBf16 || kEpi == kEpiLse;
     static_assert(C::kAccs == 1 || !kChunked, "the tall tile has no accumulator to alternate with");
-    // K stages between two register sums: 512 elements; 1024 in bf16, whose logits need 1e-6
-    constexpr int kChunkSteps = kBf16 ? 16 : 8;
     constexpr int kStages = C::kStages;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -781,7 +781,7 @@ __global__ void __launch_bounds__(320, 1)
     auto tile_cols = [&](const Problem& p, int nb) {
         return kEpi == kEpiOut ? min(kBN, (p.N - nb * kBN + 63) / 64 * 64) : tile_n;
     };
-    auto chunk_end = [&](int k0, int k1) { return kChunked ? min(k0 + kChunkSteps, k1) : k1; };
+    auto chunk_end = [&](int k0, int k1) { return kChunked ? min(k0 + args.chunk, k1) : k1; };
 
     if (warp == 0) {
         if (lane == 0) {
@@ -897,7 +897,8 @@ __global__ void __launch_bounds__(320, 1)
                                     ptx::tc_fence_after();
                                 }
                                 const uint32_t acc = tmem + buf * kBN;
-                                const uint64_t ad = a_desc + uint32_t(stage * C::kStageBytes + h * (kBM * kBK * 2)) / 16;
+                                const uint64_t ad =
+                                    a_desc + uint32_t(stage * C::kStageBytes + h * (kBM * kBK * 2)) / 16;
                                 const uint64_t bd = b_desc + uint32_t(stage * C::kStageBytes) / 16;
                                 if (elected()) {
 #pragma unroll

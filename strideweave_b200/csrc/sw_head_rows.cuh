@@ -594,7 +594,9 @@ __global__ void __launch_bounds__(256) loss_kernel(const LossArgs a) {
         for (int w = 1; w < 8; ++w) add(s_ref[w], s_sum[w], s_dot[w]);
         lse2 = ref + log2f(sum);
         if (writes && tid == 0) {
-            const float v = a.factor * ((a.entropy ? a.entropy[a.row0 + i] : 0.0f) + (lse2 - dot) * kLn2);
+            // (where the target is the largest, ref - dot is exact: a small loss keeps its digits)
+            const float v =
+                a.factor * ((a.entropy ? a.entropy[a.row0 + i] : 0.0f) + ((ref - dot) + log2f(sum)) * kLn2);
             const int64_t row = a.row_map[a.row0 + i];
             a.row_loss[a.row0 + i] = v;
             a.lse2[a.row0 + i] = lse2;

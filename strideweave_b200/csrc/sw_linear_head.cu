@@ -207,10 +207,29 @@ int launch_gemm(const Tensors* t, GemmArgs& args, cudaStream_t stream) {
     return SW_OK;
 }
 
+// K stages between two sums in registers: what the accumulator drops grows with
+// them, and each costs the epilogue about 500 cycles, for which a tile's MMAs may
+// have to wait.  Float32 results: 8 (at 4 a step of 2048 x 32000 at dim 1024 takes
+// 1335 us, not 1300).  Logits are exponents: what they are off by is the relative
+// error of a softmax.  Float32: 4 (gradients of 4663 x 1191, dim 576, off by 1.4e-6,
+// at 8 by 2.9e-6; that step 1303 us against 1290), for one row tile 2 (no slower;
+// 1 takes 348 us where 2 take 307, 5 x 8197 at dim 3802), and two pieces at least.
+// bf16: 16 (the loss of 1400 x 50001 off by 7e-7); for one row tile, whose errors
+// less averages out and which the read of w bounds, 8 (64 x 131072 with gradients 4
+// us of 397 more, 4 stages 12), or 2 where no exponentials are written (one token's
+// loss off by 8e-8, at 16 by 1.1e-5, in the same 61 us).
+int chunk_stages(bool bf16, int epi, const GemmArgs& args) {
+    const Problem& p = args.p[0];
+    if (epi == kEpiOut) return 8;
+    if (!bf16) return std::min(p.M > kBM ? 4 : 2, std::max(1, (p.K + 2 * kBK - 1) / (2 * kBK)));
+    return p.M > kBM ? 16 : args.keep ? 8 : 2;
+}
+
 // One contraction, or the gradients' two in one launch (kBoth, single CTAs' tiles).
 template <bool kBf16, int kEpi, int kA>
 int gemm(const Tensors* t, GemmArgs& args, int shape, cudaStream_t stream) {
     args.terms = kBf16 ? 1 : 3;
+    args.chunk = chunk_stages(kBf16, kEpi, args);
     if (kA == kBoth || shape == kSingle) return launch_gemm<kSingle, kBf16, kEpi, kA>(t, args, stream);
     // results summed in registers (Float32, and the statistics) have no tall tile,
     // and the logits' gradient has too much to do after a tile (4096 x 32000, dim
