@@ -207,10 +207,12 @@ struct Cfg {
 };
 
 // Estimated microseconds of a K stage, and of a tile's fill and drain that
-// nothing hides: a stage takes 0.27 us (kSingle: 128 x 256 on one SM), 0.26 (kPair2:
-// 256 x 256 on two) or 0.52 (kTall).
+// nothing hides: a stage takes 0.26 us on a pair (256 x 256) or 0.52 (tall), and on a
+// single CTA, half the work, 0.32 where all SMs draw their 48 KiB a stage from L2 (0.27
+// on a few; at 0.27 a step of 1024 x 32000 at dim 2048 takes single tiles for dw
+// and 413 us, at 0.32 pairs and 390).
 __host__ __device__ inline float stage_us(int shape, int terms) {
-    return float(terms) * (shape == kTall ? 0.52f : shape == kPair2 ? 0.26f : 0.27f);
+    return float(terms) * (shape == kTall ? 0.52f : shape == kPair2 ? 0.26f : 0.32f);
 }
 __host__ __device__ inline float fixed_us(int shape) { return shape == kTall ? 5.0f : shape == kPair2 ? 2.5f : 2.0f; }
 __host__ __device__ inline int shape_workers(int shape, int sms) { return shape == kSingle ? sms : sms / 2; }

@@ -783,7 +783,9 @@ int check_and_run(const char* name, Call& c, void* stream_ptr) {
         if (per_column > 0) s.piece = std::min(s.piece, std::max<int64_t>(budget / per_column / 256 * 256, 256));
     }
     const int64_t n = std::min(s.rows, T), nv = std::min(s.piece, V);
-    s.logits_shape = choose_parts(n, nv, D, terms, kSingle, false).us <
+    // (a pair's second half would have no row of a single row tile: 21 x 18689 at dim
+    // 2496 scored in 45 us by pairs, in 32 by single CTAs)
+    s.logits_shape = n <= kBM || choose_parts(n, nv, D, terms, kSingle, false).us <
                              0.97f * choose_parts(n, nv, D, terms, kPair2, false).us
                          ? kSingle
                          : kPair2;
