@@ -172,7 +172,7 @@ struct GemmArgs {
     const uint16_t* offs;    // [tile][rows_pad] first entry of each kEntryTile columns (null: one entry a row)
     int ent_k;
     int rows_pad;
-    float4* partial;         // kEpiLse: [rows_pad][slots] (max, sum, target term, -) in base-2 units
+    float4* partial;         // kEpiLse: [rows_pad][slots] (max, sum, target term, its remainder) in base-2 units
     int slots, slot_shift;   // a slot for each 1 << slot_shift columns: 128, or a narrow tile's 64
     int tile_n;              // logits tiles of one CTA: 256 columns, or 128 or 64 where they spread over more SMs
     float* ent_s;            // kEpiLse: base-2 logit of every target entry (null: not kept)
@@ -598,7 +598,9 @@ __device__ __forceinline__ float4 lse_tile(const GemmArgs& args, const void* tma
                         2 * (int(n0) + b * 64), 2 * (int(n0) + b * 64 + 32), int(wr.m0), false);
         }
     }
-    return make_float4(ref, sum, dot * k2, 0.0f);
+    const float term = dot * k2;
+    // (and what its rounding left)
+    return make_float4(ref, sum, term, fabsf(term) < INFINITY ? fmaf(dot, k2, -term) : 0.0f);
 }
 
 // Gradient with respect to the logits of a half tile's row: softmax minus

@@ -535,7 +535,7 @@ template <bool kF32>
 __global__ void __launch_bounds__(256) loss_kernel(const LossArgs a) {
     constexpr int kSub = kF32 ? 2048 : 8192;  // columns of a batch: four loads a thread
     __shared__ float factor[kSub / 64];
-    __shared__ float s_ref[8], s_sum[8], s_dot[8];
+    __shared__ float s_ref[8], s_sum[8], s_dot[8], s_low[8];
     __shared__ int s_last;
     pdl_enter();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -567,36 +567,40 @@ __global__ void __launch_bounds__(256) loss_kernel(const LossArgs a) {
     if (a.grad && i < count) fetch(c_begin);
     if (i < count) {
         const float4* part = a.partial + (a.row0 + i) * a.slots;
-        float ref = -INFINITY, sum = 0.0f, dot = 0.0f;
-        auto add = [&](float r, float s, float d) {
+        float ref = -INFINITY, sum = 0.0f, dot = 0.0f, low = 0.0f;
+        auto add = [&](float r, float s, float d, float l) {
             const float next = fmaxf(ref, r), base = next == -INFINITY ? 0.0f : next;
             sum = sum * ex2(ref - base) + s * ex2(r - base);
             ref = next;
             dot += d;
+            low += l;
         };
 #pragma unroll 4
         for (int t = tid; t < a.slots; t += 256) {
             const float4 p = part[t];
-            add(p.x, p.y, p.z);
+            add(p.x, p.y, p.z, p.w);
         }
         for (int o = 16; o; o >>= 1)
             add(__shfl_xor_sync(0xffffffffu, ref, o), __shfl_xor_sync(0xffffffffu, sum, o),
-                __shfl_xor_sync(0xffffffffu, dot, o));
+                __shfl_xor_sync(0xffffffffu, dot, o), __shfl_xor_sync(0xffffffffu, low, o));
         if (lane == 0) {
             s_ref[warp] = ref;
             s_sum[warp] = sum;
             s_dot[warp] = dot;
+            s_low[warp] = low;
         }
         __syncthreads();
         ref = s_ref[0];
         sum = s_sum[0];
         dot = s_dot[0];
-        for (int w = 1; w < 8; ++w) add(s_ref[w], s_sum[w], s_dot[w]);
+        low = s_low[0];
+        for (int w = 1; w < 8; ++w) add(s_ref[w], s_sum[w], s_dot[w], s_low[w]);
         lse2 = ref + log2f(sum);
         if (writes && tid == 0) {
-            // (where the target is the largest, ref - dot is exact: a small loss keeps its digits)
+            // (where the target is the largest, ref - dot is exact, and the sum is against
+            // the rounded ref as dot + low is against dot: a small loss keeps its digits)
             const float v =
-                a.factor * ((a.entropy ? a.entropy[a.row0 + i] : 0.0f) + ((ref - dot) + log2f(sum)) * kLn2);
+                a.factor * ((a.entropy ? a.entropy[a.row0 + i] : 0.0f) + ((ref - dot) + (log2f(sum) - low)) * kLn2);
             const int64_t row = a.row_map[a.row0 + i];
             a.row_loss[a.row0 + i] = v;
             a.lse2[a.row0 + i] = lse2;

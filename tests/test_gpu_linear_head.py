@@ -379,6 +379,27 @@ def test_logit_scale(dtype):
     check(call(h, w, targets=y, up=up, scale=0.125), reference(h, w, up, targets=y, scale=0.125), dtype)
 
 
+@pytest.mark.parametrize("grads", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_small_losses_keep_their_digits(dtype, grads):
+    """Losses of about 0.008 between logits of 60 and 55: a difference of two
+    rounded values of 60 (86 in base 2) would be off by up to 2^-18; the sum of the
+    exponentials, near one, is off by a few 2^-24, and a relative 2^-17 of the
+    logits by 2^-17 of the loss."""
+    T, V, D = 8, 500, 1024
+    h, w, y = states(T, V, D, dtype)
+    rows = w[y.long()].float()
+    near = (y.long() + 1) % V
+    w[near] = (0.92 * rows).to(dtype)
+    w[y.long()] = rows.to(dtype)
+    h = (60 * rows / rows.square().sum(1, keepdim=True)).to(dtype)
+    up = torch.ones(T, device="cuda")
+    out = call(h, w, targets=y, up=up if grads else None, dh="new" if grads else None, dw="new" if grads else None)
+    want = reference(h, w, up, targets=y)[0]
+    assert 1e-3 < float(want.min()) and float(want.max()) < 0.1
+    assert float((out["loss"].double() - want).abs().max()) <= 16 * 2.0 ** -24
+
+
 def test_extreme_logits():
     """Logits in the thousands: the softmax is one word or the other, and nothing overflows."""
     for dtype in DTYPES:
