@@ -172,12 +172,14 @@ struct GemmArgs {
     const uint16_t* offs;    // [tile][rows_pad] first entry of each kEntryTile columns (null: one entry a row)
     int ent_k;
     int rows_pad;
-    float4* partial;         // kEpiLse: [rows_pad][slots] (max, sum, target term, its remainder) in base-2 units
+    float4* partial;         // kEpiLse: [rows_pad][slots] (max, sum, target term, probability of the targets)
     int slots, slot_shift;   // a slot for each 1 << slot_shift columns: 128, or a narrow tile's 64
     int tile_n;              // logits tiles of one CTA: 256 columns, or 128 or 64 where they spread over more SMs
-    float* ent_s;            // kEpiLse: base-2 logit of every target entry (null: not kept)
+    float* ent_s;            // kEpiLse: h w of every target entry (null: not kept)
     int keep;                // kEpiLse: write exp2(logit - half tile's max) where the logits' gradient will be
-    const float* lse2;       // kEpiGrad: per compact row
+    // kEpiGrad: softmax(z) = exp2((z to_ref - norm.x) to_log2 - norm.y), norm per compact row
+    const float2* norm;
+    float to_ref, to_log2;
     const float* coef;
 };
 
@@ -536,28 +538,21 @@ struct WarpRows {
     }
 };
 
-// Softmax statistics of a row over the half tile in registers, in base-2
-// units: ref = max k2 z, sum of exp2(k2 z - ref), target term sum p z.  With
-// `keep` the exponentials are stored too, for the gradient: as f16 times 2^15
-// (11 bits down to 2^-29 of the half tile's largest; the later rounding to
-// bf16 is the one that counts) or, for Float32, as they are.
+// Softmax statistics of a row over the half tile in registers, of z = h w =
+// r inv: top = max z, sum of exp2(k2 (z - top)), target term sum p (z - top) and
+// sum p.  Everything is a difference of two z first and scaled after it: a
+// rounded k2 z of 60 would be off by 2^-18, of which a row sure of its target
+// has nothing left, and of 1e10 by more than exp2 can hold.  With `keep` the
+// exponentials are stored too, for the gradient: as f16 times 2^15 (11 bits down
+// to 2^-29 of the half tile's largest; the later rounding to bf16 is the one
+// that counts) or, for Float32, as they are.
 template <bool kBf16, int kBlocks, class Rows>
 __device__ __forceinline__ float4 lse_tile(const GemmArgs& args, const void* tmap_c, Rows& wr, EntryCursor& cur,
-                                           int64_t n0, int64_t n_end, float k2, float (&r)[kBlocks][2][32]) {
+                                           int64_t n0, int64_t n_end, float inv, float (&r)[kBlocks][2][32]) {
     const int64_t m = wr.m0 + wr.lane;
-    float dot = 0.0f, top = -INFINITY;
+    float top = -INFINITY;
 #pragma unroll
     for (int c = 0; c < 2 * kBlocks; ++c) {
-        cur.walk(int(args.v0 + n0) + c * 32, [&](int rel, float p) {
-            float v = 0.0f;
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-                if (j == rel) v = r[c / 2][c % 2][j];
-            if (rel >= 0) {
-                dot += p * v;
-                if (args.ent_s) args.ent_s[m * args.ent_k + cur.first + cur.i] = v * k2;
-            }
-        });
         const int ncols = (int)min(int64_t(32), n_end - (n0 + c * 32));
         if (ncols < 32) {
 #pragma unroll
@@ -567,15 +562,26 @@ __device__ __forceinline__ float4 lse_tile(const GemmArgs& args, const void* tma
 #pragma unroll
         for (int j = 0; j < 32; ++j) top = fmaxf(top, r[c / 2][c % 2][j]);
     }
-    const float ref = top * k2;
     // columns of nothing but -inf add nothing (and must not make -inf minus -inf)
-    const float base = ref == -INFINITY ? 0.0f : ref;
-    float sum = 0.0f;
+    const float base = top == -INFINITY ? 0.0f : top;
+    const float k2 = args.logit_scale * kLog2e * inv;
+    float sum = 0.0f, dot = 0.0f, weight = 0.0f;
 #pragma unroll
     for (int c = 0; c < 2 * kBlocks; ++c) {
+        cur.walk(int(args.v0 + n0) + c * 32, [&](int rel, float p) {
+            float v = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+                if (j == rel) v = r[c / 2][c % 2][j];
+            if (rel >= 0) {
+                if (p != 0.0f) dot += p * (v - base);
+                weight += p;
+                if (args.ent_s) args.ent_s[m * args.ent_k + cur.first + cur.i] = v * inv;
+            }
+        });
 #pragma unroll
         for (int j = 0; j < 32; ++j) {
-            r[c / 2][c % 2][j] = ex2(fmaf(r[c / 2][c % 2][j], k2, -base));
+            r[c / 2][c % 2][j] = ex2((r[c / 2][c % 2][j] - base) * k2);
             sum += r[c / 2][c % 2][j];
         }
     }
@@ -598,16 +604,16 @@ __device__ __forceinline__ float4 lse_tile(const GemmArgs& args, const void* tma
                         2 * (int(n0) + b * 64), 2 * (int(n0) + b * 64 + 32), int(wr.m0), false);
         }
     }
-    const float term = dot * k2;
-    // (and what its rounding left)
-    return make_float4(ref, sum, term, fabsf(term) < INFINITY ? fmaf(dot, k2, -term) : 0.0f);
+    return make_float4(top * inv, sum, dot * inv, weight);
 }
 
 // Gradient with respect to the logits of a half tile's row: softmax minus
-// target in fp32, rounded once to the type the next contractions read.
+// target in fp32, rounded once to the type the next contractions read.  The
+// logit is rounded before its lse is taken off it, as the lse was when it was
+// made of the largest (an fma would leave 2^-24 of a huge logit in the exponent).
 template <bool kBf16, bool kFew, class Rows>
 __device__ __forceinline__ void grad_tile(const GemmArgs& args, const void* tmap_c, Rows& wr, EntryCursor& cur,
-                                          int64_t n0, int64_t n_end, float k2, float lse2, float coef,
+                                          int64_t n0, int64_t n_end, float to_ref, float2 norm, float coef,
                                           float (&r)[2][2][32]) {
     if (n0 >= n_end || (kFew && wr.m0 >= kFewRows)) return;  // (the remainders' rows are written below)
 #pragma unroll
@@ -615,7 +621,7 @@ __device__ __forceinline__ void grad_tile(const GemmArgs& args, const void* tmap
         float (&x)[32] = r[c / 2][c % 2];
         const int ncols = (int)min(int64_t(32), n_end - (n0 + c * 32));
 #pragma unroll
-        for (int j = 0; j < 32; ++j) x[j] = ex2(fmaf(x[j], k2, -lse2));
+        for (int j = 0; j < 32; ++j) x[j] = ex2(fmaf(__fsub_rn(__fmul_rn(x[j], to_ref), norm.x), args.to_log2, -norm.y));
         cur.walk(int(args.v0 + n0) + c * 32, [&](int rel, float p) {
 #pragma unroll
             for (int j = 0; j < 32; ++j)
@@ -940,7 +946,7 @@ __global__ void __launch_bounds__(320, 1)
             if (p.scale_b >= 0) inv *= pow2i(-scale_exponent(args.state->amax[p.scale_b]));
             return inv;
         };
-        const float k2 = args.logit_scale * kLog2e * inverse(args.p[0]);
+        const float inv = inverse(args.p[0]);
         const float gscale = kEpi == kEpiGrad && !kBf16 ? pow2i(scale_exponent(args.state->amax[2])) : 1.0f;
         auto release = [&](uint32_t buf) {
             ptx::tc_fence_before();
@@ -975,13 +981,14 @@ __global__ void __launch_bounds__(320, 1)
                                                              (!kNarrow || half * kCols < tile_n));
                     // what the row needs beside its accumulator, while the MMAs run
                     EntryCursor cur;
-                    float lse2 = 0.0f, coef = 0.0f;
+                    float2 norm = make_float2(0.0f, 0.0f);
+                    float coef = 0.0f;
                     if (kEpi != kEpiOut) {
                         wr.begin();  // the entries go where the stores' boxes are
                         cur.fetch(args, wr.box, lane, m, wr.row_in, int(args.v0 + ncol0), int(n_end - ncol0));
                     }
                     if (kEpi == kEpiGrad && wr.row_in) {
-                        lse2 = args.lse2[m];
+                        norm = args.norm[m];
                         coef = args.coef[m] * gscale;
                     }
                     const uint32_t lanes = uint32_t(quarter * 32) << 16;
@@ -1024,11 +1031,12 @@ __global__ void __launch_bounds__(320, 1)
                     if (!rows_in) continue;
                     if (kEpi != kEpiOut) cur.begin();
                     if (kEpi == kEpiLse) {
-                        const float4 st = lse_tile<kBf16, 2>(args, tmap_c, wr, cur, ncol0, n_end, k2, r);
+                        const float4 st = lse_tile<kBf16, 2>(args, tmap_c, wr, cur, ncol0, n_end, inv, r);
                         args.partial[m * args.slots + ((args.v0 + ncol0) >> args.slot_shift)] = st;
                     } else if (kEpi == kEpiGrad) {
-                        if (few) grad_tile<kBf16, kBf16>(args, tmap_c, wr, cur, ncol0, n_end, k2, lse2, coef, r);
-                        else grad_tile<kBf16, false>(args, tmap_c, wr, cur, ncol0, n_end, k2, lse2, coef, r);
+                        const float to_ref = args.to_ref * inv;
+                        if (few) grad_tile<kBf16, kBf16>(args, tmap_c, wr, cur, ncol0, n_end, to_ref, norm, coef, r);
+                        else grad_tile<kBf16, false>(args, tmap_c, wr, cur, ncol0, n_end, to_ref, norm, coef, r);
                     } else {
                         const int row = p.sums ? plan.walk.sum_row(split, int(wr.m0)) : int(wr.m0);
                         out_tile<!kBf16>(p, tmap_c, wr, row, ncol0, out_scale, r);

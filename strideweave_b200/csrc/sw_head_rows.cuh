@@ -92,7 +92,7 @@ struct PrepareArgs {
     float* entropy;
     uint16_t* offs;
     float* coef;             // null: no gradients
-    float* lse2;
+    float2* norm;            // what the logits' gradient subtracts, from `lse`
     HeadState* state;
     // the contraction of dh: rows of a launch at most, dim, columns of a piece
     int64_t dh_rows, dh_cols, dh_k;
@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(256) prepare_kernel(const PrepareArgs a) {
             if (keep && blockIdx.y == 0) {
                 if (a.targets) a.ent_idx[rank] = a.targets[t];
                 if (a.coef) a.coef[rank] = a.mean || !a.upstream ? 1.0f : a.upstream[t];
-                if (a.lse) a.lse2[rank] = a.lse[t] * kLog2e;
+                if (a.lse) a.norm[rank] = make_float2(a.lse[t], 0.0f);
             }
         }
     }
@@ -505,8 +505,9 @@ struct LossArgs {
     int ignore_index;
     const float* entropy;    // distillation, or null
     float factor;            // f
+    float logit_scale;
     float* row_loss;         // compact
-    float* lse2;             // compact: for gradients that start from the logits again
+    float2* norm;            // compact: for gradients that start from the logits again
     float* loss;             // per row, or the mean; null: neither
     int mean;
     float* lse;              // per row, or null
@@ -521,10 +522,12 @@ struct LossArgs {
 };
 
 // A row's statistics from its half tiles', its loss, and (grad) the gradient of
-// its logits: exp2(k2 z - ref) 2^(ref - lse2) is the softmax, in place of the
-// stored exponentials, and the target entries are written from their own
-// Float32 logits (where the softmax is near p, the stored 11 bits of it would
-// not be enough).  A thread takes 8 columns (bf16), a warp a block of 64
+// its logits: exp2(k2 (z - top)) of a half tile times exp2(k2 (top - ref)) / sum
+// is the softmax, in place of the stored exponentials, and the target entries
+// are written from their own Float32 z (where the softmax is near p, the stored
+// 11 bits of it would not be enough).  A row's largest z and the logarithm of
+// its sum stay apart until the end: added up, their rounding is all that a row
+// sure of its target would have left.  A thread takes 8 columns (bf16), a warp a block of 64
 // (Float32: hi and lo values replace the block they were computed from).  The
 // last row to be done adds up the mean, in a fixed order.  Bound by the
 // exponentials' read and write, part of them still in L2: 4096 x 32000 109 us, 4.8
@@ -535,7 +538,7 @@ template <bool kF32>
 __global__ void __launch_bounds__(256) loss_kernel(const LossArgs a) {
     constexpr int kSub = kF32 ? 2048 : 8192;  // columns of a batch: four loads a thread
     __shared__ float factor[kSub / 64];
-    __shared__ float s_ref[8], s_sum[8], s_dot[8], s_low[8];
+    __shared__ float s_ref[8], s_sum[8], s_dot[8], s_weight[8];
     __shared__ int s_last;
     pdl_enter();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -544,7 +547,8 @@ __global__ void __launch_bounds__(256) loss_kernel(const LossArgs a) {
     const int64_t i = int64_t(gridDim.x) - 1 - blockIdx.x;
     const bool writes = blockIdx.y == 0;
     const int count = a.state->rows(a.row0);
-    float lse2 = 0.0f;
+    const float k2 = a.logit_scale * kLog2e;
+    float ref = -INFINITY, log2_sum = 0.0f;
     // the first 8192 columns' exponentials are on their way while the statistics
     // are added up, and later each batch while the one before it is written
     const int64_t c_begin = int64_t(blockIdx.y) * a.seg, c_end = min(c_begin + a.seg, a.V);
@@ -567,13 +571,15 @@ __global__ void __launch_bounds__(256) loss_kernel(const LossArgs a) {
     if (a.grad && i < count) fetch(c_begin);
     if (i < count) {
         const float4* part = a.partial + (a.row0 + i) * a.slots;
-        float ref = -INFINITY, sum = 0.0f, dot = 0.0f, low = 0.0f;
-        auto add = [&](float r, float s, float d, float l) {
+        float sum = 0.0f, dot = 0.0f, weight = 0.0f;
+        auto add = [&](float r, float s, float d, float w) {
             const float next = fmaxf(ref, r), base = next == -INFINITY ? 0.0f : next;
-            sum = sum * ex2(ref - base) + s * ex2(r - base);
+            sum = sum * ex2((ref - base) * k2) + s * ex2((r - base) * k2);
+            // (terms are against their own largest z, or against 0 beside nothing but -inf)
+            if (weight != 0.0f) dot += weight * ((ref == -INFINITY ? 0.0f : ref) - base);
+            if (w != 0.0f) dot += d + w * ((r == -INFINITY ? 0.0f : r) - base);
             ref = next;
-            dot += d;
-            low += l;
+            weight += w;
         };
 #pragma unroll 4
         for (int t = tid; t < a.slots; t += 256) {
@@ -582,30 +588,29 @@ __global__ void __launch_bounds__(256) loss_kernel(const LossArgs a) {
         }
         for (int o = 16; o; o >>= 1)
             add(__shfl_xor_sync(0xffffffffu, ref, o), __shfl_xor_sync(0xffffffffu, sum, o),
-                __shfl_xor_sync(0xffffffffu, dot, o), __shfl_xor_sync(0xffffffffu, low, o));
+                __shfl_xor_sync(0xffffffffu, dot, o), __shfl_xor_sync(0xffffffffu, weight, o));
         if (lane == 0) {
             s_ref[warp] = ref;
             s_sum[warp] = sum;
             s_dot[warp] = dot;
-            s_low[warp] = low;
+            s_weight[warp] = weight;
         }
         __syncthreads();
         ref = s_ref[0];
         sum = s_sum[0];
         dot = s_dot[0];
-        low = s_low[0];
-        for (int w = 1; w < 8; ++w) add(s_ref[w], s_sum[w], s_dot[w], s_low[w]);
-        lse2 = ref + log2f(sum);
+        weight = s_weight[0];
+        for (int w = 1; w < 8; ++w) add(s_ref[w], s_sum[w], s_dot[w], s_weight[w]);
+        log2_sum = log2f(sum);
         if (writes && tid == 0) {
-            // (where the target is the largest, ref - dot is exact, and the sum is against
-            // the rounded ref as dot + low is against dot: a small loss keeps its digits)
-            const float v =
-                a.factor * ((a.entropy ? a.entropy[a.row0 + i] : 0.0f) + ((ref - dot) + (log2f(sum) - low)) * kLn2);
+            // (where the target is the largest, dot is 0: a small loss keeps its digits)
+            const float v = a.factor * ((a.entropy ? a.entropy[a.row0 + i] : 0.0f) +
+                                        (log2_sum * kLn2 - dot * a.logit_scale));
             const int64_t row = a.row_map[a.row0 + i];
             a.row_loss[a.row0 + i] = v;
-            a.lse2[a.row0 + i] = lse2;
+            a.norm[a.row0 + i] = make_float2(ref, log2_sum);
             if (a.loss && !a.mean) a.loss[row] = v;
-            if (a.lse) a.lse[row] = lse2 * kLn2;
+            if (a.lse) a.lse[row] = __fadd_rn(__fmul_rn(ref, a.logit_scale), log2_sum * kLn2);
         }
     } else if (writes && tid == 0 && i < a.rows) {
         const int64_t row = a.row_map[a.row0 + i];
@@ -643,9 +648,11 @@ __global__ void __launch_bounds__(256) loss_kernel(const LossArgs a) {
         const int64_t c1 = min(c0 + kSub, c_end);
         __syncthreads();
         for (int t = tid; t < int((c1 - c0 + 63) / 64); t += 256) {
-            const float ref = a.partial[(a.row0 + i) * a.slots + ((c0 + t * 64) >> a.slot_shift)].x;
+            const float top = a.partial[(a.row0 + i) * a.slots + ((c0 + t * 64) >> a.slot_shift)].x;
             // (a half tile of nothing but -inf stored zeros)
-            factor[t] = ref == -INFINITY ? 0.0f : ex2(ref - lse2) * coef * (kF32 ? 1.0f : 1.0f / 32768.0f);
+            factor[t] = top == -INFINITY
+                            ? 0.0f
+                            : ex2((top - ref) * k2 - log2_sum) * coef * (kF32 ? 1.0f : 1.0f / 32768.0f);
         }
         __syncthreads();
         uint4 now[4];
@@ -690,7 +697,7 @@ __global__ void __launch_bounds__(256) loss_kernel(const LossArgs a) {
         if (col < c_begin || col >= c_end || (k > 0 && a.ent_idx[at - 1] == col)) continue;
         float p = a.ent_p ? a.ent_p[at] : 1.0f;
         for (int j = 1; k + j < a.ent_k && a.ent_idx[at + j] == col; ++j) p += a.ent_p[at + j];
-        const float g = (ex2(a.ent_s[at] - lse2) - p) * coef;
+        const float g = (ex2((a.ent_s[at] - ref) * k2 - log2_sum) - p) * coef;
         if (kF32) {
             uint16_t* d = row + (col & ~63) * int64_t(2) + (col & 63);
             const __half hi = __float2half_rn(g);

@@ -279,7 +279,7 @@ struct Layout {
     float* entropy;
     uint16_t* offs;
     float* coef;
-    float* lse2;
+    float2* norm;
     float* row_loss;
     float* ent_s;
     uint16_t* hc;
@@ -330,7 +330,7 @@ Layout lay_out(Bump& b, const Call& c, const Shape& s) {
         l.offs = b.take<uint16_t>(s.rows_pad * ((s.V + kEntryTile - 1) / kEntryTile + 1));
     }
     l.coef = b.take<float>(s.rows_pad);
-    l.lse2 = b.take<float>(s.rows_pad);
+    l.norm = b.take<float2>(s.rows_pad);
     l.row_loss = b.take<float>(s.rows_pad);
     l.hc = b.take<uint16_t>(s.planes * s.rows_pad * s.ld_h);
     if (c.loss) l.partial = b.take<float4>(s.slots * s.rows_pad);
@@ -381,7 +381,7 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
     pa.entropy = l.entropy;
     pa.offs = l.offs;
     pa.coef = s.grads ? l.coef : nullptr;
-    pa.lse2 = l.lse2;
+    pa.norm = l.norm;
     pa.state = l.state;
     if (c.dh) {
         pa.dh_rows = s.rows;
@@ -504,7 +504,10 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
         a.ent_p = l.ent_p ? l.ent_p + r0 * g.ent_k : nullptr;
         a.offs = l.offs ? l.offs + r0 : nullptr;
         a.partial = l.partial + r0 * s.slots;
-        a.lse2 = l.lse2 + r0;
+        // what the row subtracts: the kept lse of the logits, or the largest z and the sum's logarithm
+        a.norm = l.norm + r0;
+        a.to_ref = c.loss ? 1.0f : c.scale;
+        a.to_log2 = c.loss ? c.scale * kLog2e : kLog2e;
         a.coef = l.coef + r0;
         return a;
     };
@@ -525,7 +528,8 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
         a.entropy = l.entropy;
         a.factor = c.factor;
         a.row_loss = l.row_loss;
-        a.lse2 = l.lse2;
+        a.logit_scale = c.scale;
+        a.norm = l.norm;
         a.loss = c.loss;
         a.mean = p.reduction == SW_HEAD_MEAN;
         a.lse = c.lse;
