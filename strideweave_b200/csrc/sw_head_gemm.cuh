@@ -7,6 +7,8 @@
 //             and the target terms: the logits themselves are not stored
 //   kEpiGrad  logits tile -> gradient of the loss with respect to the logits,
 //             rounded once to the operand type
+//   kEpiGradCut  the same in bf16 where the K walk is cut into pieces (below): the
+//             registers of that cost 4 % of a call whose walk is one piece, dim 1024
 //   kEpiOut   the product itself: a gradient of the states or of the weights
 //
 // Tile shapes (kShape), on persistent CTAs:
@@ -35,7 +37,10 @@
 // long K walk drifts: measured 1.3e-9 per K element, 1.5e-4 over 128000.  Where
 // the result is Float32 (kChunked: logits, and Float32 gradients) the walk is cut
 // into pieces of args.chunk stages, and the epilogue adds them in registers, rounded
-// to nearest.
+// to nearest.  Logits computed again for their gradient are cut as they were for
+// their lse: what both drift by cancels in exp(s - lse), where at s = 60 the drift
+// of one alone, 1e-4 over a dim of 2048, would be more than a row sure of its
+// target has left.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -60,8 +65,9 @@ constexpr int kEntryTile = 256;         // columns per entry of the target offse
 constexpr int kFewRows = 64;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kLargeExponent = 1048576.0f;  // from here on the rounding of an exponent may be 1/16 and more
 
-enum { kEpiLse = 0, kEpiGrad = 1, kEpiOut = 2 };
+enum { kEpiLse = 0, kEpiGrad = 1, kEpiOut = 2, kEpiGradCut = 3 };
 enum { kCountM, kCountK };
 enum { kKMajor, kMnMajor, kBoth };       // A in memory; kBoth: of two contractions, each its own
 
@@ -177,9 +183,11 @@ struct GemmArgs {
     int tile_n;              // logits tiles of one CTA: 256 columns, or 128 or 64 where they spread over more SMs
     float* ent_s;            // kEpiLse: h w of every target entry (null: not kept)
     int keep;                // kEpiLse: write exp2(logit - half tile's max) where the logits' gradient will be
-    // kEpiGrad: softmax(z) = exp2((z to_ref - norm.x) to_log2 - norm.y), norm per compact row
+    // kEpiGrad: softmax(z) = exp2((z to_ref - norm.x) to_log2 - norm.y), norm per compact
+    // row; exp2's factor of z is logit_scale log2(e) rounded, and to_ref to_log2 less
+    // that, over to_ref, is factor_rest
     const float2* norm;
-    float to_ref, to_log2;
+    float to_ref, to_log2, factor_rest;
     const float* coef;
 };
 
@@ -540,9 +548,11 @@ struct WarpRows {
 
 // Softmax statistics of a row over the half tile in registers, of z = h w =
 // r inv: top = max z, sum of exp2(k2 (z - top)), target term sum p (z - top) and
-// sum p.  Everything is a difference of two z first and scaled after it: a
-// rounded k2 z of 60 would be off by 2^-18, of which a row sure of its target
-// has nothing left, and of 1e10 by more than exp2 can hold.  With `keep` the
+// sum p.  Everything is a difference of two z: a rounded k2 z of 60 is off by
+// 2^-18, of which a row sure of its target has nothing left.  The exponentials'
+// fma takes the rounded k2 top off, and what that rounding left is a factor of the
+// row (1400 x 50001, dim 2048: 206.6 us; subtracting z first 210); only where it
+// would be large (logits above 10^6) the difference comes first.  With `keep` the
 // exponentials are stored too, for the gradient: as f16 times 2^15 (11 bits down
 // to 2^-29 of the half tile's largest; the later rounding to bf16 is the one
 // that counts) or, for Float32, as they are.
@@ -550,9 +560,20 @@ template <bool kBf16, int kBlocks, class Rows>
 __device__ __forceinline__ float4 lse_tile(const GemmArgs& args, const void* tmap_c, Rows& wr, EntryCursor& cur,
                                            int64_t n0, int64_t n_end, float inv, float (&r)[kBlocks][2][32]) {
     const int64_t m = wr.m0 + wr.lane;
-    float top = -INFINITY;
+    float top = -INFINITY, dot = 0.0f, weight = 0.0f;
 #pragma unroll
     for (int c = 0; c < 2 * kBlocks; ++c) {
+        cur.walk(int(args.v0 + n0) + c * 32, [&](int rel, float p) {
+            float v = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+                if (j == rel) v = r[c / 2][c % 2][j];
+            if (rel >= 0) {
+                if (p != 0.0f) dot += p * v;
+                weight += p;
+                if (args.ent_s) args.ent_s[m * args.ent_k + cur.first + cur.i] = v * inv;
+            }
+        });
         const int ncols = (int)min(int64_t(32), n_end - (n0 + c * 32));
         if (ncols < 32) {
 #pragma unroll
@@ -565,28 +586,25 @@ __device__ __forceinline__ float4 lse_tile(const GemmArgs& args, const void* tma
     // columns of nothing but -inf add nothing (and must not make -inf minus -inf)
     const float base = top == -INFINITY ? 0.0f : top;
     const float k2 = args.logit_scale * kLog2e * inv;
-    float sum = 0.0f, dot = 0.0f, weight = 0.0f;
+    float sum = 0.0f, ref = __fmul_rn(base, k2), rest = fmaf(base, k2, -ref);
+    if (!(fabsf(ref) < kLargeExponent)) {
+#pragma unroll
+        for (int c = 0; c < 2 * kBlocks; ++c)
+#pragma unroll
+            for (int j = 0; j < 32; ++j) r[c / 2][c % 2][j] -= base;
+        ref = rest = 0.0f;
+    }
+    const float fix = ex2(-rest);
 #pragma unroll
     for (int c = 0; c < 2 * kBlocks; ++c) {
-        cur.walk(int(args.v0 + n0) + c * 32, [&](int rel, float p) {
-            float v = 0.0f;
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-                if (j == rel) v = r[c / 2][c % 2][j];
-            if (rel >= 0) {
-                if (p != 0.0f) dot += p * (v - base);
-                weight += p;
-                if (args.ent_s) args.ent_s[m * args.ent_k + cur.first + cur.i] = v * inv;
-            }
-        });
 #pragma unroll
         for (int j = 0; j < 32; ++j) {
-            r[c / 2][c % 2][j] = ex2((r[c / 2][c % 2][j] - base) * k2);
+            r[c / 2][c % 2][j] = ex2(fmaf(r[c / 2][c % 2][j], k2, -ref));
             sum += r[c / 2][c % 2][j];
         }
     }
     if (args.keep && n0 < n_end) {  // (blocks of 64 columns are written whole)
-        const float up = !wr.row_in ? 0.0f : kBf16 ? 32768.0f : 1.0f;
+        const float up = !wr.row_in ? 0.0f : kBf16 ? 32768.0f * fix : fix;
         if (kBf16) {
             wr.send_two(
                 tmap_c,
@@ -600,35 +618,64 @@ __device__ __forceinline__ float4 lse_tile(const GemmArgs& args, const void* tma
             for (int b = 0; b < kBlocks; ++b)
                 if (n0 + b * 64 < n_end)
                     wr.send_two(
-                        tmap_c, [&](int c, int j) { return wr.row_in ? __float_as_uint(r[b][c][j]) : 0u; }, true,
+                        tmap_c, [&](int c, int j) { return __float_as_uint(r[b][c][j] * up); }, true,
                         2 * (int(n0) + b * 64), 2 * (int(n0) + b * 64 + 32), int(wr.m0), false);
         }
     }
-    return make_float4(top * inv, sum, dot * inv, weight);
+    return make_float4(top * inv, sum * fix, (weight != 0.0f ? fmaf(-weight, base, dot) : 0.0f) * inv, weight);
 }
 
+// What a row's logits' gradient needs: (exp2(k2 z - ref) - p fix) coef.
+struct SoftmaxRow {
+    float ref, fix, coef;
+
+    __device__ __forceinline__ SoftmaxRow() : ref(0.0f), fix(1.0f), coef(0.0f) {}
+    __device__ __forceinline__ void load(const GemmArgs& args, int64_t m, float gscale) {
+        const float2 norm = args.norm[m];
+        const float top = __fmul_rn(norm.x, args.to_log2);
+        ref = top + norm.y;
+        const float part = ref - top;  // (the sum and its rounding error, exactly)
+        const float rest = fmaf(norm.x, args.to_log2, -top) + ((top - (ref - part)) + (norm.y - part)) -
+                           norm.x * args.factor_rest;
+        const bool large = !(fabsf(ref) < kLargeExponent);
+        fix = large ? 1.0f : ex2(rest);
+        coef = args.coef[m] * gscale * (large ? 1.0f : ex2(-rest));
+    }
+};
+
 // Gradient with respect to the logits of a half tile's row: softmax minus
-// target in fp32, rounded once to the type the next contractions read.  The
-// logit is rounded before its lse is taken off it, as the lse was when it was
-// made of the largest (an fma would leave 2^-24 of a huge logit in the exponent).
+// target in fp32, rounded once to the type the next contractions read.  As
+// above, what rounding the exponent's constant left is a factor of the row.
 template <bool kBf16, bool kFew, class Rows>
 __device__ __forceinline__ void grad_tile(const GemmArgs& args, const void* tmap_c, Rows& wr, EntryCursor& cur,
-                                          int64_t n0, int64_t n_end, float to_ref, float2 norm, float coef,
+                                          int64_t n0, int64_t n_end, float inv, const SoftmaxRow& row,
                                           float (&r)[2][2][32]) {
     if (n0 >= n_end || (kFew && wr.m0 >= kFewRows)) return;  // (the remainders' rows are written below)
+    float k2 = args.logit_scale * kLog2e * inv, ref = row.ref;
+    if (!(fabsf(ref) < kLargeExponent)) {
+        const float2 norm = args.norm[wr.m0 + wr.lane];  // (a row that exists: others have ref 0)
+        const float to_ref = args.to_ref * inv;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+                r[c / 2][c % 2][j] = __fsub_rn(__fmul_rn(r[c / 2][c % 2][j], to_ref), norm.x);
+        k2 = args.to_log2;
+        ref = norm.y;
+    }
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
         float (&x)[32] = r[c / 2][c % 2];
         const int ncols = (int)min(int64_t(32), n_end - (n0 + c * 32));
 #pragma unroll
-        for (int j = 0; j < 32; ++j) x[j] = ex2(fmaf(__fsub_rn(__fmul_rn(x[j], to_ref), norm.x), args.to_log2, -norm.y));
+        for (int j = 0; j < 32; ++j) x[j] = ex2(fmaf(x[j], k2, -ref));
         cur.walk(int(args.v0 + n0) + c * 32, [&](int rel, float p) {
 #pragma unroll
             for (int j = 0; j < 32; ++j)
-                if (j == rel) x[j] -= p;
+                if (j == rel) x[j] -= p * row.fix;
         });
 #pragma unroll
-        for (int j = 0; j < 32; ++j) x[j] *= coef;  // (0 in a row that does not exist)
+        for (int j = 0; j < 32; ++j) x[j] *= row.coef;  // (0 in a row that does not exist)
         if (ncols < 32) {
 #pragma unroll
             for (int j = 0; j < 32; ++j)
@@ -717,11 +764,12 @@ template <int kShape, bool kBf16, int kEpi, int kA>
 __global__ void __launch_bounds__(320, 1)
     head_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmArgs args) {
     constexpr bool kBMn = kEpi == kEpiOut;  // logits contract K-major operands
+    constexpr bool kGrad = kEpi == kEpiGrad || kEpi == kEpiGradCut;
     constexpr int kProblems = kA == kBoth ? 2 : 1;
     auto mn_major = [](const Problem& p) { return kA == kBoth ? p.a_mn != 0 : kA == kMnMajor; };
     using C = Cfg<kShape>;
     constexpr bool kPair = C::kPair;
-    constexpr bool kChunked = !kBf16 || kEpi == kEpiLse;
+    constexpr bool kChunked = !kBf16 || kEpi == kEpiLse || kEpi == kEpiGradCut;
     static_assert(C::kAccs == 1 || !kChunked, "the tall tile has no accumulator to alternate with");
     constexpr int kStages = C::kStages;
     extern __shared__ uint8_t smem_raw[];
@@ -753,7 +801,7 @@ __global__ void __launch_bounds__(320, 1)
         for (int q = 0; q < args.problems; ++q) {
             ptx::prefetch_tmap(&maps.a[q]);
             ptx::prefetch_tmap(&maps.b[q]);
-            if (kEpi == kEpiGrad || kEpi == kEpiOut || args.keep) ptx::prefetch_tmap(&maps.c[q]);
+            if (kGrad || kEpi == kEpiOut || args.keep) ptx::prefetch_tmap(&maps.c[q]);
         }
     }
     if (warp == 1) tmem_alloc<kPair>(ptx::smem_addr(tmem_slot), C::kTmemCols);
@@ -947,7 +995,7 @@ __global__ void __launch_bounds__(320, 1)
             return inv;
         };
         const float inv = inverse(args.p[0]);
-        const float gscale = kEpi == kEpiGrad && !kBf16 ? pow2i(scale_exponent(args.state->amax[2])) : 1.0f;
+        const float gscale = kGrad && !kBf16 ? pow2i(scale_exponent(args.state->amax[2])) : 1.0f;
         auto release = [&](uint32_t buf) {
             ptx::tc_fence_before();
             __syncwarp();
@@ -981,16 +1029,12 @@ __global__ void __launch_bounds__(320, 1)
                                                              (!kNarrow || half * kCols < tile_n));
                     // what the row needs beside its accumulator, while the MMAs run
                     EntryCursor cur;
-                    float2 norm = make_float2(0.0f, 0.0f);
-                    float coef = 0.0f;
+                    SoftmaxRow row;
                     if (kEpi != kEpiOut) {
                         wr.begin();  // the entries go where the stores' boxes are
                         cur.fetch(args, wr.box, lane, m, wr.row_in, int(args.v0 + ncol0), int(n_end - ncol0));
                     }
-                    if (kEpi == kEpiGrad && wr.row_in) {
-                        norm = args.norm[m];
-                        coef = args.coef[m] * gscale;
-                    }
+                    if (kGrad && wr.row_in) row.load(args, m, gscale);
                     const uint32_t lanes = uint32_t(quarter * 32) << 16;
                     // The half tile's row in registers: the accumulator is free again
                     // before any of the work on it.  (An empty share of K: zeros.)
@@ -1033,13 +1077,12 @@ __global__ void __launch_bounds__(320, 1)
                     if (kEpi == kEpiLse) {
                         const float4 st = lse_tile<kBf16, 2>(args, tmap_c, wr, cur, ncol0, n_end, inv, r);
                         args.partial[m * args.slots + ((args.v0 + ncol0) >> args.slot_shift)] = st;
-                    } else if (kEpi == kEpiGrad) {
-                        const float to_ref = args.to_ref * inv;
-                        if (few) grad_tile<kBf16, kBf16>(args, tmap_c, wr, cur, ncol0, n_end, to_ref, norm, coef, r);
-                        else grad_tile<kBf16, false>(args, tmap_c, wr, cur, ncol0, n_end, to_ref, norm, coef, r);
+                    } else if (kGrad) {
+                        if (few) grad_tile<kBf16, kBf16>(args, tmap_c, wr, cur, ncol0, n_end, inv, row, r);
+                        else grad_tile<kBf16, false>(args, tmap_c, wr, cur, ncol0, n_end, inv, row, r);
                     } else {
-                        const int row = p.sums ? plan.walk.sum_row(split, int(wr.m0)) : int(wr.m0);
-                        out_tile<!kBf16>(p, tmap_c, wr, row, ncol0, out_scale, r);
+                        const int y = p.sums ? plan.walk.sum_row(split, int(wr.m0)) : int(wr.m0);
+                        out_tile<!kBf16>(p, tmap_c, wr, y, ncol0, out_scale, r);
                     }
                 }
             }

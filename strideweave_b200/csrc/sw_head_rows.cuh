@@ -538,7 +538,8 @@ template <bool kF32>
 __global__ void __launch_bounds__(256) loss_kernel(const LossArgs a) {
     constexpr int kSub = kF32 ? 2048 : 8192;  // columns of a batch: four loads a thread
     __shared__ float factor[kSub / 64];
-    __shared__ float s_ref[8], s_sum[8], s_dot[8], s_weight[8];
+    __shared__ float4 s_stat[8];
+    __shared__ float s_part[8];
     __shared__ int s_last;
     pdl_enter();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -571,36 +572,31 @@ __global__ void __launch_bounds__(256) loss_kernel(const LossArgs a) {
     if (a.grad && i < count) fetch(c_begin);
     if (i < count) {
         const float4* part = a.partial + (a.row0 + i) * a.slots;
-        float sum = 0.0f, dot = 0.0f, weight = 0.0f;
-        auto add = [&](float r, float s, float d, float w) {
-            const float next = fmaxf(ref, r), base = next == -INFINITY ? 0.0f : next;
-            sum = sum * ex2((ref - base) * k2) + s * ex2((r - base) * k2);
-            // (terms are against their own largest z, or against 0 beside nothing but -inf)
-            if (weight != 0.0f) dot += weight * ((ref == -INFINITY ? 0.0f : ref) - base);
-            if (w != 0.0f) dot += d + w * ((r == -INFINITY ? 0.0f : r) - base);
-            ref = next;
-            weight += w;
-        };
-#pragma unroll 4
+        // against the largest z of a warp's slots, and then of all (a half tile of
+        // nothing but -inf has its terms against 0)
+        auto finite = [](float r) { return r == -INFINITY ? 0.0f : r; };
+        for (int t = tid; t < a.slots; t += 256) ref = fmaxf(ref, part[t].x);
+        ref = warp_max(ref);
+        float sum = 0.0f, dot = 0.0f, weight = 0.0f, base = finite(ref);
         for (int t = tid; t < a.slots; t += 256) {
             const float4 p = part[t];
-            add(p.x, p.y, p.z, p.w);
+            sum += p.y * ex2((p.x - base) * k2);
+            if (p.w != 0.0f) dot += p.z + p.w * (finite(p.x) - base);
+            weight += p.w;
         }
-        for (int o = 16; o; o >>= 1)
-            add(__shfl_xor_sync(0xffffffffu, ref, o), __shfl_xor_sync(0xffffffffu, sum, o),
-                __shfl_xor_sync(0xffffffffu, dot, o), __shfl_xor_sync(0xffffffffu, weight, o));
-        if (lane == 0) {
-            s_ref[warp] = ref;
-            s_sum[warp] = sum;
-            s_dot[warp] = dot;
-            s_weight[warp] = weight;
-        }
+        sum = warp_sum(sum);
+        dot = warp_sum(dot);
+        weight = warp_sum(weight);
+        if (lane == 0) s_stat[warp] = make_float4(ref, sum, dot, weight);
         __syncthreads();
-        ref = s_ref[0];
-        sum = s_sum[0];
-        dot = s_dot[0];
-        weight = s_weight[0];
-        for (int w = 1; w < 8; ++w) add(s_ref[w], s_sum[w], s_dot[w], s_weight[w]);
+        for (int w = 0; w < 8; ++w) ref = fmaxf(ref, s_stat[w].x);
+        base = finite(ref);
+        sum = dot = 0.0f;
+        for (int w = 0; w < 8; ++w) {
+            const float4 p = s_stat[w];
+            sum += p.y * ex2((p.x - base) * k2);
+            if (p.w != 0.0f) dot += p.z + p.w * (finite(p.x) - base);
+        }
         log2_sum = log2f(sum);
         if (writes && tid == 0) {
             // (where the target is the largest, dot is 0: a small loss keeps its digits)
@@ -610,7 +606,7 @@ __global__ void __launch_bounds__(256) loss_kernel(const LossArgs a) {
             a.row_loss[a.row0 + i] = v;
             a.norm[a.row0 + i] = make_float2(ref, log2_sum);
             if (a.loss && !a.mean) a.loss[row] = v;
-            if (a.lse) a.lse[row] = __fadd_rn(__fmul_rn(ref, a.logit_scale), log2_sum * kLn2);
+            if (a.lse) a.lse[row] = fmaf(ref, a.logit_scale, log2_sum * kLn2);
         }
     } else if (writes && tid == 0 && i < a.rows) {
         const int64_t row = a.row_map[a.row0 + i];
@@ -631,11 +627,11 @@ __global__ void __launch_bounds__(256) loss_kernel(const LossArgs a) {
             for (int r = tid; r < a.state->count; r += 256) s += __ldcg(a.row_loss + r);
             s = warp_sum(s);
             __syncthreads();
-            if (lane == 0) s_dot[warp] = s;
+            if (lane == 0) s_part[warp] = s;
             __syncthreads();
             if (tid == 0) {
                 s = 0.0f;
-                for (int w = 0; w < 8; ++w) s += s_dot[w];
+                for (int w = 0; w < 8; ++w) s += s_part[w];
                 *a.loss = a.state->bad ? NAN : s / float(a.state->count);
             }
         }

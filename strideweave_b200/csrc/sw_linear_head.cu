@@ -217,7 +217,8 @@ int launch_gemm(const Tensors* t, GemmArgs& args, cudaStream_t stream) {
 // bf16: 16 (the loss of 1400 x 50001 off by 7e-7); for one row tile, whose errors
 // less averages out and which the read of w bounds, 8 (64 x 131072 with gradients 4
 // us of 397 more, 4 stages 12), or 2 where no exponentials are written (one token's
-// loss off by 8e-8, at 16 by 1.1e-5, in the same 61 us).
+// loss off by 8e-8, at 16 by 1.1e-5, in the same 61 us).  The same for the logits of a
+// gradient from a kept lse as for the loss that left it: both drift alike.
 int chunk_stages(bool bf16, int epi, const GemmArgs& args) {
     const Problem& p = args.p[0];
     if (epi == kEpiOut) return 8;
@@ -508,6 +509,7 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
         a.norm = l.norm + r0;
         a.to_ref = c.loss ? 1.0f : c.scale;
         a.to_log2 = c.loss ? c.scale * kLog2e : kLog2e;
+        a.factor_rest = c.loss ? 0.0f : float((double(c.scale) * kLog2e - double(c.scale * kLog2e)) / c.scale);
         a.coef = l.coef + r0;
         return a;
     };
@@ -686,7 +688,10 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
         if ((rc = weights(v0, n, &w)) != SW_OK) return rc;
         GemmArgs a = logits(0, s.T, v0, n);
         const Tensors t{states(0, s.rows_pad), w, grad_out};
-        if ((rc = gemm<kBf16, kEpiGrad, kKMajor>(&t, a, s.logits_shape, stream)) != SW_OK) return rc;
+        const bool cut = kBf16 && s.D > int64_t(kBK) * chunk_stages(true, kEpiGradCut, a);
+        rc = cut ? gemm<kBf16, kBf16 ? kEpiGradCut : kEpiGrad, kKMajor>(&t, a, s.logits_shape, stream)
+                 : gemm<kBf16, kEpiGrad, kKMajor>(&t, a, s.logits_shape, stream);
+        if (rc != SW_OK) return rc;
         if ((rc = gradients(0, s.T, v0, n, w, v0 == 0, v0 + n == s.V, true, true)) != SW_OK) return rc;
     }
     return SW_OK;
