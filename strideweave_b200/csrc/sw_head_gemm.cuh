@@ -30,8 +30,13 @@
 // sub-partition w % 4 (32 rows) and one half of the tile's columns.  Results
 // pass through 4 KiB of shared memory per warp, so that they leave as whole
 // 128-byte row segments.  Float32 operands come as two f16 planes (hi + lo of a
-// power-of-two multiple of the value): the K walk then runs over three plane
-// pairs, hi lo + lo hi + hi hi, which keeps 22 bits of each factor.
+// power-of-two multiple of the value, one for a whole matrix): the K walk then runs
+// over three plane pairs, hi lo + lo hi + hi hi, which keeps 22 bits of each factor
+// down to 2^-18 of the matrix's largest, and 2^-40 of that below.  Where a row is
+// so far below the others that this would show in it (HeadState::wide), the planes
+// are bf16 instead, which have Float32's range: three of an operand (24 bits) and
+// two of the logits' gradient (16), multiplied pair by pair down to 2^-16 of the
+// largest product.
 //
 // The tensor core's fp32 accumulator drops the bits below its last place, so a
 // long K walk drifts: measured 1.3e-9 per K element, 1.5e-4 over 128000.  Where
@@ -111,7 +116,10 @@ struct Walk {
 struct HeadState {
     int count;               // rows that count (compact rows)
     int bad;                 // a target outside the vocabulary was seen
-    uint32_t amax[3];        // largest finite |h|, |w|, |row factor| as float bits (Float32 only)
+    // Float32 only, as float bits: largest finite |h|, |w|, |row factor|, and the least
+    // of a row that is not zero
+    uint32_t amax[3], least[3];
+    int wide;                // rows too far apart for f16 planes (from the first split on)
     float grad_scale;        // common factor of every row's gradient, applied to dh and dw in fp32
     int dh_splits;           // parts of the K walk of dh, chosen for the rows that count
     int done;                // rows whose loss is written
@@ -121,12 +129,28 @@ struct HeadState {
     __device__ __forceinline__ bool few(int row0) const { return count <= kFewRows && rows(row0) > 0; }
 };
 
+// Rows this many powers of two below the largest keep 22 bits and more of their
+// own largest element in f16 planes (2^-40 of the matrix's largest).  A row's
+// gradient with a factor that far below is a sum over the vocabulary of entries
+// that are 2^12 coarser: 2^-28 sqrt(131072) = 2^-19 of it.  bf16 planes cost 2008 us
+// for 1325 (a step of 2048 x 32000, dim 1024), so they are only for what needs them.
+constexpr int kSpread = 16, kFactorSpread = 12;
+__device__ __forceinline__ bool rows_far_apart(const HeadState* s) {
+    bool far = false;
+    for (int q = 0; q < 3; ++q) {
+        const uint32_t most = s->amax[q], least = s->least[q];
+        far |= least < most && int(most >> 23) - int(least >> 23) > (q == 2 ? kFactorSpread : kSpread);
+    }
+    return far;
+}
+
 // Power-of-two multiplier that brings values of magnitude `amax` just under
-// 2^15 (f16 holds up to 65504): exponent q, so that x 2^q is the value split.
-__device__ __forceinline__ int scale_exponent(uint32_t amax_bits) {
+// 2^15 (f16 holds up to 65504; bf16 planes are for small rows, which 2^23 keeps
+// from the subnormals): exponent q, so that x 2^q is the value split.
+__device__ __forceinline__ int scale_exponent(uint32_t amax_bits, bool wide) {
     if (amax_bits == 0) return 0;
     const int e = int(amax_bits >> 23) - 127;
-    return min(14 - e, 126);
+    return min((wide ? 22 : 14) - e, 126);
 }
 __device__ __forceinline__ float pow2i(int q) { return __uint_as_float(uint32_t(q + 127) << 23); }
 
@@ -162,13 +186,28 @@ struct alignas(64) Maps {
     CUtensorMap a[2], b[2], c[2];
 };
 
+// Plane of an operand in product `term` of the planes' products, the smallest
+// first (lists of hexadecimal digits, the first product's last): bf16 values have
+// one plane; f16 planes (0, 1), (1, 0), (0, 0); bf16 planes of Float32 the six, or
+// with a gradient's two planes five, whose numbers add up to 2 at most.
+struct Products {
+    int terms;
+    uint32_t a, b;
+};
+__device__ __forceinline__ Products products(bool f32, bool wide, bool gradient) {
+    if (!f32) return Products{1, 0, 0};
+    if (!wide) return Products{3, 0x010, 0x001};
+    return gradient ? Products{5, 0x01010, 0x00112} : Products{6, 0x010210, 0x001012};
+}
+__device__ __forceinline__ int plane_of(uint32_t list, int term) { return list >> (4 * term) & 15; }
+
 struct GemmArgs {
     Problem p[2];            // two at once: the gradients of states and weights of few rows
     int problems;
     int alternate;           // every second worker takes the second one first
     const HeadState* state;
     int row0;                // first compact row of this launch (the count starts there)
-    int terms;               // plane pairs walked: 1, or 3 for Float32
+    int terms;               // plane pairs walked, for estimates: 1, or 3 for Float32
     int chunk;               // K stages between two sums in registers (kChunked)
     // logits epilogues
     float logit_scale;
@@ -178,7 +217,7 @@ struct GemmArgs {
     const uint16_t* offs;    // [tile][rows_pad] first entry of each kEntryTile columns (null: one entry a row)
     int ent_k;
     int rows_pad;
-    float4* partial;         // kEpiLse: [rows_pad][slots] (max, sum, target term, probability of the targets)
+    float4* partial;         // kEpiLse: [rows_pad][slots] (max, sum, target term, unused: one store)
     int slots, slot_shift;   // a slot for each 1 << slot_shift columns: 128, or a narrow tile's 64
     int tile_n;              // logits tiles of one CTA: 256 columns, or 128 or 64 where they spread over more SMs
     float* ent_s;            // kEpiLse: h w of every target entry (null: not kept)
@@ -475,6 +514,26 @@ struct EntryCursor {
     }
 };
 
+// Two values' hi parts in the type of a Float32 operand's planes; x and y keep
+// what that leaves.
+template <bool kWide>
+__device__ __forceinline__ uint32_t split2(float& x, float& y) {
+    if (kWide) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+        x -= __low2float(h);
+        y -= __high2float(h);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    const __half2 h = __floats2half2_rn(x, y);
+    x -= __low2float(h);
+    y -= __high2float(h);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+__device__ __forceinline__ uint32_t split2(bool wide, float& x, float& y) {
+    return wide ? split2<true>(x, y) : split2<false>(x, y);
+}
+
 template <bool kBf16>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
     if (kBf16) {
@@ -547,9 +606,9 @@ struct WarpRows {
 };
 
 // Softmax statistics of a row over the half tile in registers, of z = h w =
-// r inv: top = max z, sum of exp2(k2 (z - top)), target term sum p (z - top) and
-// sum p.  Everything is a difference of two z: a rounded k2 z of 60 is off by
-// 2^-18, of which a row sure of its target has nothing left.  The exponentials'
+// r inv: top = max z, sum of exp2(k2 (z - top)), target term sum p z.  What follows
+// starts from differences of z: a rounded k2 z of 60 is off by 2^-18, of which a
+// row sure of its target has nothing left.  The exponentials'
 // fma takes the rounded k2 top off, and what that rounding left is a factor of the
 // row (1400 x 50001, dim 2048: 206.6 us; subtracting z first 210); only where it
 // would be large (logits above 10^6) the difference comes first.  With `keep` the
@@ -560,7 +619,7 @@ template <bool kBf16, int kBlocks, class Rows>
 __device__ __forceinline__ float4 lse_tile(const GemmArgs& args, const void* tmap_c, Rows& wr, EntryCursor& cur,
                                            int64_t n0, int64_t n_end, float inv, float (&r)[kBlocks][2][32]) {
     const int64_t m = wr.m0 + wr.lane;
-    float top = -INFINITY, dot = 0.0f, weight = 0.0f;
+    float top = -INFINITY, dot = 0.0f;
 #pragma unroll
     for (int c = 0; c < 2 * kBlocks; ++c) {
         cur.walk(int(args.v0 + n0) + c * 32, [&](int rel, float p) {
@@ -570,7 +629,6 @@ __device__ __forceinline__ float4 lse_tile(const GemmArgs& args, const void* tma
                 if (j == rel) v = r[c / 2][c % 2][j];
             if (rel >= 0) {
                 if (p != 0.0f) dot += p * v;
-                weight += p;
                 if (args.ent_s) args.ent_s[m * args.ent_k + cur.first + cur.i] = v * inv;
             }
         });
@@ -587,7 +645,7 @@ __device__ __forceinline__ float4 lse_tile(const GemmArgs& args, const void* tma
     const float base = top == -INFINITY ? 0.0f : top;
     const float k2 = args.logit_scale * kLog2e * inv;
     float sum = 0.0f, ref = __fmul_rn(base, k2), rest = fmaf(base, k2, -ref);
-    if (!(fabsf(ref) < kLargeExponent)) {
+    if (__builtin_expect(!(fabsf(ref) < kLargeExponent), 0)) {
 #pragma unroll
         for (int c = 0; c < 2 * kBlocks; ++c)
 #pragma unroll
@@ -622,7 +680,7 @@ __device__ __forceinline__ float4 lse_tile(const GemmArgs& args, const void* tma
                         2 * (int(n0) + b * 64), 2 * (int(n0) + b * 64 + 32), int(wr.m0), false);
         }
     }
-    return make_float4(top * inv, sum * fix, (weight != 0.0f ? fmaf(-weight, base, dot) : 0.0f) * inv, weight);
+    return make_float4(top * inv, sum * fix, dot * inv, 0.0f);
 }
 
 // What a row's logits' gradient needs: (exp2(k2 z - ref) - p fix) coef.
@@ -648,11 +706,11 @@ struct SoftmaxRow {
 // above, what rounding the exponent's constant left is a factor of the row.
 template <bool kBf16, bool kFew, class Rows>
 __device__ __forceinline__ void grad_tile(const GemmArgs& args, const void* tmap_c, Rows& wr, EntryCursor& cur,
-                                          int64_t n0, int64_t n_end, float inv, const SoftmaxRow& row,
+                                          int64_t n0, int64_t n_end, float inv, const SoftmaxRow& row, bool wide,
                                           float (&r)[2][2][32]) {
     if (n0 >= n_end || (kFew && wr.m0 >= kFewRows)) return;  // (the remainders' rows are written below)
     float k2 = args.logit_scale * kLog2e * inv, ref = row.ref;
-    if (!(fabsf(ref) < kLargeExponent)) {
+    if (__builtin_expect(!(fabsf(ref) < kLargeExponent), 0)) {
         const float2 norm = args.norm[wr.m0 + wr.lane];  // (a row that exists: others have ref 0)
         const float to_ref = args.to_ref * inv;
 #pragma unroll
@@ -703,21 +761,21 @@ __device__ __forceinline__ void grad_tile(const GemmArgs& args, const void* tmap
                 n0 + 64 < n_end, int(n0), int(n0) + 64, int(wr.m0) + kFewRows, false);
     } else {
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
-            if (n0 + b * 64 < n_end)
+        for (int b = 0; b < 2; ++b) {
+            if (n0 + b * 64 >= n_end) continue;
+            // (the second plane from what the first one leaves)
+            const int x0 = 2 * (int(n0) + b * 64);
+            if (wide)
                 wr.send_two(
                     tmap_c,
-                    [&](int plane, int j) {
-                        float& x = r[b][j / 16][2 * (j % 16)];
-                        float& y = r[b][j / 16][2 * (j % 16) + 1];
-                        const __half2 h = __floats2half2_rn(x, y);
-                        if (plane == 0) {  // what the hi values leave
-                            x -= __low2float(h);
-                            y -= __high2float(h);
-                        }
-                        return *reinterpret_cast<const uint32_t*>(&h);
-                    },
-                    true, 2 * (int(n0) + b * 64), 2 * (int(n0) + b * 64) + 64, int(wr.m0), false);
+                    [&](int, int j) { return split2<true>(r[b][j / 16][2 * (j % 16)], r[b][j / 16][2 * (j % 16) + 1]); },
+                    true, x0, x0 + 64, int(wr.m0), false);
+            else
+                wr.send_two(
+                    tmap_c,
+                    [&](int, int j) { return split2<false>(r[b][j / 16][2 * (j % 16)], r[b][j / 16][2 * (j % 16) + 1]); },
+                    true, x0, x0 + 64, int(wr.m0), false);
+        }
     }
 }
 
@@ -817,6 +875,8 @@ __global__ void __launch_bounds__(320, 1)
     const int tile_n = kNarrow ? args.tile_n : kBN;
     // rows that count, and for the gradients of few rows their remainders
     const bool few = kBf16 && kEpi != kEpiLse && args.state->few(args.row0);
+    const bool wide = !kBf16 && args.state->wide;
+    const Products pairs = products(!kBf16, wide, kEpi == kEpiOut);
     auto plan_of = [&](const Problem& p) {
         int rows = args.state->rows(args.row0);
         if (!few) rows = min(rows, p.count_is == kCountM ? p.M : p.K);
@@ -863,10 +923,8 @@ __global__ void __launch_bounds__(320, 1)
                     const uint32_t bytes =
                         (kPair ? 2 : 1) * (C::kABytes + (kEpi == kEpiOut ? boxes * 64 : b_cols) * kBK * 2);
                     for (int c0 = k0; c0 < k1 && alive; c0 = chunk_end(c0, k1))
-                        for (int term = 0; term < args.terms && alive; ++term) {
-                            // plane pairs, the small products first: (hi, lo), (lo, hi), (hi, hi)
-                            const int pa = args.terms == 3 && term == 1;
-                            const int pb = args.terms == 3 && term == 0;
+                        for (int term = 0; term < pairs.terms && alive; ++term) {
+                            const int pa = plane_of(pairs.a, term), pb = plane_of(pairs.b, term);
                             const int xa = pa * p.pa.x_plane, ya = pa * p.pa.y_plane;
                             const int xb = pb * p.pb.x_plane, yb = pb * p.pb.y_plane;
                             const int c1 = chunk_end(c0, k1);
@@ -935,12 +993,12 @@ __global__ void __launch_bounds__(320, 1)
                 for (int i = 0, t; alive && (t = plan.nth(i, worker, workers)) >= 0; ++i) {
                     int mb, nb, split, k0, k1;
                     plan.item(t, mb, nb, split, k0, k1);
-                    const uint32_t idesc = idesc_f16(kBf16, a_mn, kBMn, C::kAccRows, tile_cols(args.p[q], nb));
+                    const uint32_t idesc = idesc_f16(kBf16 || wide, a_mn, kBMn, C::kAccRows, tile_cols(args.p[q], nb));
                     for (int c0 = k0; c0 < k1 && alive; c0 = chunk_end(c0, k1), ++it) {
                         // one tile alternates between the two accumulators, a tall one fills both
                         const uint32_t buf0 = C::kAccs == 1 ? it & 1 : 0;
                         const uint32_t drained = (C::kAccs == 1 ? it >> 1 : it) & 1;
-                        const int steps = (chunk_end(c0, k1) - c0) * args.terms;
+                        const int steps = (chunk_end(c0, k1) - c0) * pairs.terms;
                         for (int ks = 0; ks < steps && alive; ++ks) {
                             alive = __all_sync(0xffffffffu, ptx::mbar_wait(bar_full + 8 * stage, phase));
                             if (!alive) break;
@@ -990,12 +1048,12 @@ __global__ void __launch_bounds__(320, 1)
         // inverse of the operands' power-of-two scales
         auto inverse = [&](const Problem& p) {
             float inv = 1.0f;
-            if (p.scale_a >= 0) inv *= pow2i(-scale_exponent(args.state->amax[p.scale_a]));
-            if (p.scale_b >= 0) inv *= pow2i(-scale_exponent(args.state->amax[p.scale_b]));
+            if (p.scale_a >= 0) inv *= pow2i(-scale_exponent(args.state->amax[p.scale_a], wide));
+            if (p.scale_b >= 0) inv *= pow2i(-scale_exponent(args.state->amax[p.scale_b], wide));
             return inv;
         };
         const float inv = inverse(args.p[0]);
-        const float gscale = kGrad && !kBf16 ? pow2i(scale_exponent(args.state->amax[2])) : 1.0f;
+        const float gscale = kGrad && !kBf16 ? pow2i(scale_exponent(args.state->amax[2], wide)) : 1.0f;
         auto release = [&](uint32_t buf) {
             ptx::tc_fence_before();
             __syncwarp();
@@ -1078,8 +1136,8 @@ __global__ void __launch_bounds__(320, 1)
                         const float4 st = lse_tile<kBf16, 2>(args, tmap_c, wr, cur, ncol0, n_end, inv, r);
                         args.partial[m * args.slots + ((args.v0 + ncol0) >> args.slot_shift)] = st;
                     } else if (kGrad) {
-                        if (few) grad_tile<kBf16, kBf16>(args, tmap_c, wr, cur, ncol0, n_end, inv, row, r);
-                        else grad_tile<kBf16, false>(args, tmap_c, wr, cur, ncol0, n_end, inv, row, r);
+                        if (few) grad_tile<kBf16, kBf16>(args, tmap_c, wr, cur, ncol0, n_end, inv, row, wide, r);
+                        else grad_tile<kBf16, false>(args, tmap_c, wr, cur, ncol0, n_end, inv, row, wide, r);
                     } else {
                         const int y = p.sums ? plan.walk.sum_row(split, int(wr.m0)) : int(wr.m0);
                         out_tile<!kBf16>(p, tmap_c, wr, y, ncol0, out_scale, r);

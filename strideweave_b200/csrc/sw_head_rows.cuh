@@ -49,6 +49,8 @@ __host__ __device__ inline float spread_cost(int64_t M, int64_t N, int64_t K, in
     return us;
 }
 
+constexpr uint32_t kNoMagnitude = 0x7f800000u;  // least magnitude of no rows
+
 // ---- preparation ---------------------------------------------------------------
 
 // flags[t] = 1 when the teacher's row has an entry: a warp per row, one read of
@@ -87,6 +89,8 @@ struct PrepareArgs {
     float factor;            // c f
     const float* lse;        // a kept lse to start from, or null
     int* row_map;            // compact rows, then the rows that do not count
+    uint32_t* row_top;       // to be zeroed for amax_kernel
+    int row_tops;
     int* ent_idx;
     float* ent_p;
     float* entropy;
@@ -246,15 +250,21 @@ __global__ void __launch_bounds__(256) prepare_kernel(const PrepareArgs a) {
     }
     __syncthreads();
     if (blockIdx.x == gridDim.x - 1 && blockIdx.y == 0) {  // (its rows are mostly padding)
-        uint32_t top = 0;  // of the row factors (Float32 only)
+        for (int i = tid; i < a.row_tops; i += 256) a.row_top[i] = 0;
+        uint32_t top = 0, least = kNoMagnitude;  // of the row factors (Float32 only)
         if (a.coef && !a.h) {
             for (int64_t t = tid; t < a.T; t += 256)
                 if (counts(t)) {
                     const float g = a.mean || !a.upstream ? 1.0f : a.upstream[t];
                     if (isfinite(g)) top = max(top, __float_as_uint(fabsf(g)));
+                    if (isfinite(g) && g != 0.0f) least = min(least, __float_as_uint(fabsf(g)));
                 }
             top = __reduce_max_sync(0xffffffffu, top);
-            if (lane == 0) s_total[warp] = int(top);
+            least = __reduce_min_sync(0xffffffffu, least);
+            if (lane == 0) {
+                s_total[warp] = int(top);
+                s_before[warp] = int(least);
+            }
         }
         __syncthreads();
         if (warp == 0) {
@@ -271,12 +281,18 @@ __global__ void __launch_bounds__(256) prepare_kernel(const PrepareArgs a) {
             }
             if (lane == 0) {
                 if (a.coef && !a.h)
-                    for (int w = 0; w < 8; ++w) top = max(top, uint32_t(s_total[w]));
+                    for (int w = 0; w < 8; ++w) {
+                        top = max(top, uint32_t(s_total[w]));
+                        least = min(least, uint32_t(s_before[w]));
+                    }
                 HeadState s;
                 s.count = total;
                 s.bad = bad;
                 s.amax[0] = s.amax[1] = 0;
                 s.amax[2] = top;
+                s.least[0] = s.least[1] = kNoMagnitude;
+                s.least[2] = least;
+                s.wide = 0;
                 // what every row's gradient is multiplied by stays out of the
                 // 16-bit logits' gradient: a target's -1 is exact there, where
                 // the common factor would round it the same way in every row
@@ -342,74 +358,147 @@ struct SplitJob {
     int scale_of;            // index of its magnitude in HeadState::amax
     uint16_t* dst;
     int64_t ld, rows_pad;
+    // amax_kernel, contiguous columns: parts of a row, and where there is more than one
+    // the rows' magnitudes and how many parts of 32 rows are in them
+    int parts;
+    uint32_t *row_top, *parts_in;
     unsigned ctas;           // the first CTAs of the grid belong to the first job
 };
 
 // Largest finite magnitudes of one or two matrices, for the power of two that
-// brings them into f16's range: a warp per row, or per column where columns are
-// contiguous.  Bound by one read (32000 x 1024 Float32 29 us, 4.8 TB/s; rows that
-// are not whole vectors, 60000 x 1001, 67 us with eight reads a lane in flight, 86
-// with four).
-__global__ void __launch_bounds__(256) amax_kernel(const SplitJob j0, const SplitJob j1, HeadState* state) {
+// brings them into f16's range, and of their rows, for whether that will do: a
+// warp per row, or where columns are contiguous a CTA per 32 rows, or per part of
+// them where rows are few.  Bound by one read (32000 x 1024
+// Float32 29 us, 4.8 TB/s; rows that are not whole vectors, 60000 x 1001, 67 us with
+// eight reads a lane in flight, 86 with four).
+__global__ void __launch_bounds__(256, 5) amax_kernel(const SplitJob j0, const SplitJob j1, HeadState* state) {
+    __shared__ uint32_t s_top[8], s_least[8], s_row[8][32];
     pdl_enter();
     const bool second = blockIdx.x >= j0.ctas;
     const SplitJob& j = second ? j1 : j0;
     const float* x = static_cast<const float*>(j.src);
     const int64_t rows = j.row_map ? state->count : j.rows;
-    const bool by_rows = j.sr == 1 && j.sc != 1;  // walk the unit stride fastest
-    const int64_t outer = by_rows ? j.cols : rows, inner = by_rows ? rows : j.cols;
-    const int64_t so = by_rows ? j.sc : j.sr, si = by_rows ? j.sr : j.sc;
-    const int lane = threadIdx.x & 31;
-    const int64_t first = int64_t(blockIdx.x - (second ? j0.ctas : 0)) * 8 + (threadIdx.x >> 5);
-    uint32_t top = 0;
-    auto take = [&](float v) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int64_t cta = blockIdx.x - (second ? j0.ctas : 0);
+    uint32_t top = 0, least = kNoMagnitude, row = 0;
+    auto take = [](uint32_t& row, float v) {
         v = fabsf(v);
-        if (v <= 3.402823466e38f) top = max(top, __float_as_uint(v));
+        if (v <= 3.402823466e38f) row = max(row, __float_as_uint(v));
     };
-    for (int64_t o = first; o < outer; o += int64_t(j.ctas) * 8) {
-        const float* p = x + (by_rows ? o : j.row_map ? int64_t(j.row_map[o]) : o) * so;
-        if (j.vec) {
-#pragma unroll 4
-            for (int64_t i = lane * 4; i < inner; i += 128) {
-                const float4 v = *reinterpret_cast<const float4*>(p + i);
-                take(v.x);
-                take(v.y);
-                take(v.z);
-                take(v.w);
-            }
-        } else {
-            for (int64_t i = lane; i < inner; i += 256) {
-                float v[8];
+    auto row_done = [&](uint32_t m) {
+        top = max(top, m);
+        if (m) least = min(least, m);
+    };
+    if (j.sr == 1 && j.sc != 1) {  // read along the unit stride: a lane a row
+        const int64_t per = (j.cols + j.parts - 1) / j.parts, items = (rows + 31) / 32 * j.parts;
+        for (int64_t t = cta; t < items; t += j.ctas) {
+            const int64_t r = t / j.parts * 32 + lane, c0 = t % j.parts * per, c1 = min(c0 + per, j.cols);
+            row = 0;
+            if (r < rows) {
+                const float* p = x + (j.row_map ? int64_t(j.row_map[r]) : r);
+                for (int64_t c = c0 + warp; c < c1; c += 64) {
+                    float v[8];
 #pragma unroll
-                for (int u = 0; u < 8; ++u) {
-                    const int64_t e = i + 32 * u;
-                    v[u] = e < inner ? p[(by_rows && j.row_map ? int64_t(j.row_map[e]) : e) * si] : 0.0f;
+                    for (int u = 0; u < 8; ++u) v[u] = c + 8 * u < c1 ? p[(c + 8 * u) * j.sc] : 0.0f;
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) take(row, v[u]);
                 }
+            }
+            s_row[warp][lane] = row;
+            __syncthreads();
+            if (warp == 0) {
+                for (int w = 1; w < 8; ++w) row = max(row, s_row[w][lane]);
+                bool last = true;
+                if (j.parts > 1) {
+                    if (row) atomicMax(&j.row_top[r], row);
+                    __threadfence();
+                    __syncwarp();
+                    uint32_t before = 0;
+                    if (lane == 0) before = atomicAdd(&j.parts_in[t / j.parts], 1u);
+                    last = __shfl_sync(0xffffffffu, before, 0) == uint32_t(j.parts - 1);
+                    __threadfence();
+                    if (last && r < rows) row = __ldcg(j.row_top + r);
+                }
+                if (last) row_done(row);
+            }
+            __syncthreads();
+        }
+    } else {
+        const int64_t step = int64_t(j.ctas) * 8;
+        auto start = [&](int64_t o) { return x + (j.row_map ? int64_t(j.row_map[o]) : o) * j.sr; };
+        for (int64_t o = cta * 8 + warp; o < rows; o += 2 * step) {
+            const float* p = start(o);
+            row = 0;
+            if (j.vec) {  // two rows at a time, so that one's reads cover the other's reduction
+                const bool two = o + step < rows;
+                const float* p2 = two ? start(o + step) : p;
+                uint32_t row2 = 0;
+#pragma unroll 4
+                for (int64_t i = lane * 4; i < j.cols; i += 128) {
+                    const float4 v = *reinterpret_cast<const float4*>(p + i);
+                    const float4 v2 = *reinterpret_cast<const float4*>(p2 + i);
+                    take(row, v.x);
+                    take(row, v.y);
+                    take(row, v.z);
+                    take(row, v.w);
+                    take(row2, v2.x);
+                    take(row2, v2.y);
+                    take(row2, v2.z);
+                    take(row2, v2.w);
+                }
+                row_done(__reduce_max_sync(0xffffffffu, row));
+                row_done(__reduce_max_sync(0xffffffffu, row2));
+                continue;
+            }
+            for (int64_t q = o; q < rows && q <= o + step; q += step) {
+                p = start(q);
+                row = 0;
+                for (int64_t i = lane; i < j.cols; i += 256) {
+                    float v[8];
 #pragma unroll
-                for (int u = 0; u < 8; ++u) take(v[u]);
+                    for (int u = 0; u < 8; ++u) v[u] = i + 32 * u < j.cols ? p[(i + 32 * u) * j.sc] : 0.0f;
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) take(row, v[u]);
+                }
+                row_done(__reduce_max_sync(0xffffffffu, row));
             }
         }
     }
     top = __reduce_max_sync(0xffffffffu, top);
-    if (lane == 0 && top) atomicMax(&state->amax[j.scale_of], top);
+    least = __reduce_min_sync(0xffffffffu, least);
+    if (lane == 0) {
+        s_top[warp] = top;
+        s_least[warp] = least;
+    }
+    __syncthreads();
+    if (tid == 0) {
+        for (int w = 1; w < 8; ++w) {
+            top = max(top, s_top[w]);
+            least = min(least, s_least[w]);
+        }
+        if (top) atomicMax(&state->amax[j.scale_of], top);
+        atomicMin(&state->least[j.scale_of], least);
+    }
 }
 
 // One or two matrices into operands [rows_pad][ld]: a copy of bf16 values, or
 // two f16 planes of a Float32 value times 2^q (hi rounded to nearest, lo the
-// rest).  Rows past the ones that count are zero.  Bound by a read and a write of
+// rest), or three bf16 ones.  Rows past the ones that count are zero.  Bound by a read and a write of
 // the matrix (32000 x 1024 Float32 with its 2048 states 55 us, 5.0 TB/s; bf16
 // 60000 x 1001, which TMA cannot read, 56 us, 4.3 TB/s).  Rows that are not whole
 // vectors are read element by element: aligned vectors shifted into place took
 // the same time.
 template <bool kF32>
-__global__ void __launch_bounds__(256) split_kernel(const SplitJob j0, const SplitJob j1, const HeadState* state) {
+__global__ void __launch_bounds__(256) split_kernel(const SplitJob j0, const SplitJob j1, HeadState* state) {
     __shared__ float tile[32][33];
     pdl_enter();
     const bool second = blockIdx.x >= j0.ctas;
     const SplitJob& j = second ? j1 : j0;
     const int64_t cta = blockIdx.x - (second ? j0.ctas : 0);
     const int64_t valid = j.row_map ? min(j.rows, int64_t(state->count)) : j.rows;
-    const float scale = kF32 ? pow2i(scale_exponent(state->amax[j.scale_of])) : 1.0f;
+    const bool wide = kF32 && rows_far_apart(state);
+    if (kF32 && blockIdx.x == 0 && threadIdx.x == 0) state->wide = wide;
+    const float scale = kF32 ? pow2i(scale_exponent(state->amax[j.scale_of], wide)) : 1.0f;
     if (j.sc == 1) {
         // a thread writes 8 columns; it reads them as vectors where rows are
         // aligned, else one by one (neighbouring threads share the sectors)
@@ -417,7 +506,7 @@ __global__ void __launch_bounds__(256) split_kernel(const SplitJob j0, const Spl
 #pragma unroll 2
         for (int64_t u = cta * 256 + threadIdx.x; u < j.rows_pad * units; u += int64_t(j.ctas) * 256) {
             const int64_t r = u / units, c = (u - r * units) * 8;
-            uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
+            uint4 hi = make_uint4(0, 0, 0, 0), lo = hi, third = hi;
             if (r < valid) {
                 const int64_t at = (j.row_map ? int64_t(j.row_map[r]) : r) * j.sr + c;
                 if (kF32) {
@@ -430,16 +519,17 @@ __global__ void __launch_bounds__(256) split_kernel(const SplitJob j0, const Spl
 #pragma unroll
                         for (int q = 0; q < 8; ++q) v[q] = c + q < j.cols ? p[q] : 0.0f;
                     }
-                    uint32_t h[4], l[4];
+                    auto plane = [&]() {
+                        uint32_t h[4];
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const float x = v[2 * q] * scale, y = v[2 * q + 1] * scale;
-                        const __half2 b2 = __floats2half2_rn(x, y);
-                        h[q] = *reinterpret_cast<const uint32_t*>(&b2);
-                        l[q] = pack2<false>(x - __low2float(b2), y - __high2float(b2));
-                    }
-                    hi = make_uint4(h[0], h[1], h[2], h[3]);
-                    lo = make_uint4(l[0], l[1], l[2], l[3]);
+                        for (int q = 0; q < 4; ++q) h[q] = split2(wide, v[2 * q], v[2 * q + 1]);
+                        return make_uint4(h[0], h[1], h[2], h[3]);
+                    };
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) v[q] *= scale;
+                    hi = plane();
+                    lo = plane();
+                    if (wide) third = plane();
                 } else {
                     const uint16_t* p = static_cast<const uint16_t*>(j.src) + at;
                     if (j.vec) {
@@ -454,6 +544,7 @@ __global__ void __launch_bounds__(256) split_kernel(const SplitJob j0, const Spl
             }
             *reinterpret_cast<uint4*>(j.dst + r * j.ld + c) = hi;
             if (kF32) *reinterpret_cast<uint4*>(j.dst + (j.rows_pad + r) * j.ld + c) = lo;
+            if (wide) *reinterpret_cast<uint4*>(j.dst + (2 * j.rows_pad + r) * j.ld + c) = third;
         }
         return;
     }
@@ -479,10 +570,9 @@ __global__ void __launch_bounds__(256) split_kernel(const SplitJob j0, const Spl
             if (r < j.rows_pad && c < j.ld) {
                 const float v = tile[y][x];
                 if (kF32) {
-                    const float s = v * scale;
-                    const __half hi = __float2half_rn(s);
-                    j.dst[r * j.ld + c] = __half_as_ushort(hi);
-                    j.dst[(j.rows_pad + r) * j.ld + c] = __half_as_ushort(__float2half_rn(s - __half2float(hi)));
+                    float s = v * scale, none = 0.0f;
+                    for (int plane = 0; plane < (wide ? 3 : 2); ++plane)
+                        j.dst[(plane * j.rows_pad + r) * j.ld + c] = uint16_t(split2(wide, s, none));
                 } else {
                     j.dst[r * j.ld + c] = __bfloat16_as_ushort(__float2bfloat16_rn(v));
                 }
@@ -535,7 +625,7 @@ struct LossArgs {
 // half tile would spare this pass, at the cost of one more 16-bit rounding, of
 // the states in dw, and of a target's exact -1: not taken.
 template <bool kF32>
-__global__ void __launch_bounds__(256) loss_kernel(const LossArgs a) {
+__global__ void __launch_bounds__(256, kF32 ? 4 : 3) loss_kernel(const LossArgs a) {
     constexpr int kSub = kF32 ? 2048 : 8192;  // columns of a batch: four loads a thread
     __shared__ float factor[kSub / 64];
     __shared__ float4 s_stat[8];
@@ -572,36 +662,35 @@ __global__ void __launch_bounds__(256) loss_kernel(const LossArgs a) {
     if (a.grad && i < count) fetch(c_begin);
     if (i < count) {
         const float4* part = a.partial + (a.row0 + i) * a.slots;
-        // against the largest z of a warp's slots, and then of all (a half tile of
-        // nothing but -inf has its terms against 0)
+        // against the largest z of a thread's slots, of a warp's, and then of all
         auto finite = [](float r) { return r == -INFINITY ? 0.0f : r; };
-        for (int t = tid; t < a.slots; t += 256) ref = fmaxf(ref, part[t].x);
-        ref = warp_max(ref);
-        float sum = 0.0f, dot = 0.0f, weight = 0.0f, base = finite(ref);
+        float sum = 0.0f, dot = 0.0f;
+#pragma unroll 4
         for (int t = tid; t < a.slots; t += 256) {
             const float4 p = part[t];
-            sum += p.y * ex2((p.x - base) * k2);
-            if (p.w != 0.0f) dot += p.z + p.w * (finite(p.x) - base);
-            weight += p.w;
+            const float next = fmaxf(ref, p.x), base = finite(next);
+            sum = sum * ex2((ref - base) * k2) + p.y * ex2((p.x - base) * k2);
+            dot += p.z;
+            ref = next;
         }
-        sum = warp_sum(sum);
+        const float own = ref;
+        ref = warp_max(ref);
+        sum = warp_sum(sum * ex2((own - finite(ref)) * k2));
         dot = warp_sum(dot);
-        weight = warp_sum(weight);
-        if (lane == 0) s_stat[warp] = make_float4(ref, sum, dot, weight);
+        if (lane == 0) s_stat[warp] = make_float4(ref, sum, dot, 0.0f);
         __syncthreads();
         for (int w = 0; w < 8; ++w) ref = fmaxf(ref, s_stat[w].x);
-        base = finite(ref);
         sum = dot = 0.0f;
         for (int w = 0; w < 8; ++w) {
             const float4 p = s_stat[w];
-            sum += p.y * ex2((p.x - base) * k2);
-            if (p.w != 0.0f) dot += p.z + p.w * (finite(p.x) - base);
+            sum += p.y * ex2((p.x - finite(ref)) * k2);
+            dot += p.z;
         }
         log2_sum = log2f(sum);
         if (writes && tid == 0) {
-            // (where the target is the largest, dot is 0: a small loss keeps its digits)
+            // (where the target is the largest, ref - dot is 0: a small loss keeps its digits)
             const float v = a.factor * ((a.entropy ? a.entropy[a.row0 + i] : 0.0f) +
-                                        (log2_sum * kLn2 - dot * a.logit_scale));
+                                        (log2_sum * kLn2 + (ref - dot) * a.logit_scale));
             const int64_t row = a.row_map[a.row0 + i];
             a.row_loss[a.row0 + i] = v;
             a.norm[a.row0 + i] = make_float2(ref, log2_sum);
@@ -637,8 +726,8 @@ __global__ void __launch_bounds__(256) loss_kernel(const LossArgs a) {
         }
     }
     if (!a.grad || i >= count) return;
-    const float coef = a.coef[a.row0 + i] * (kF32 ? pow2i(scale_exponent(a.state->amax[2])) : 1.0f);
-    const bool few = !kF32 && a.state->few(a.row0);
+    const bool few = !kF32 && a.state->few(a.row0), wide = kF32 && a.state->wide;
+    const float coef = a.coef[a.row0 + i] * (kF32 ? pow2i(scale_exponent(a.state->amax[2], wide)) : 1.0f);
     uint16_t* rest = row + kFewRows * a.ld_grad;
     for (int64_t c0 = c_begin; c0 < c_end; c0 += kSub) {
         const int64_t c1 = min(c0 + kSub, c_end);
@@ -664,11 +753,10 @@ __global__ void __launch_bounds__(256) loss_kernel(const LossArgs a) {
                 float2 v = make_float2(__uint_as_float(now[j].x), __uint_as_float(now[j].y));
                 v.x = c + 2 * lane < a.V ? v.x * f : 0.0f;
                 v.y = c + 2 * lane + 1 < a.V ? v.y * f : 0.0f;
-                const __half2 hi = __floats2half2_rn(v.x, v.y);
-                const __half2 lo = __floats2half2_rn(v.x - __low2float(hi), v.y - __high2float(hi));
+                const uint32_t hi = split2(wide, v.x, v.y), lo = split2(wide, v.x, v.y);
                 __syncwarp();  // (the whole block was read before any of it is replaced)
-                reinterpret_cast<__half2*>(row + 2 * c)[lane] = hi;
-                reinterpret_cast<__half2*>(row + 2 * c + 64)[lane] = lo;
+                reinterpret_cast<uint32_t*>(row + 2 * c)[lane] = hi;
+                reinterpret_cast<uint32_t*>(row + 2 * c + 64)[lane] = lo;
             } else {
                 const uint32_t e[4] = {now[j].x, now[j].y, now[j].z, now[j].w};
                 uint32_t hi[4], lo[4];
@@ -693,12 +781,12 @@ __global__ void __launch_bounds__(256) loss_kernel(const LossArgs a) {
         if (col < c_begin || col >= c_end || (k > 0 && a.ent_idx[at - 1] == col)) continue;
         float p = a.ent_p ? a.ent_p[at] : 1.0f;
         for (int j = 1; k + j < a.ent_k && a.ent_idx[at + j] == col; ++j) p += a.ent_p[at + j];
-        const float g = (ex2((a.ent_s[at] - ref) * k2 - log2_sum) - p) * coef;
+        float g = (ex2((a.ent_s[at] - ref) * k2 - log2_sum) - p) * coef;
         if (kF32) {
             uint16_t* d = row + (col & ~63) * int64_t(2) + (col & 63);
-            const __half hi = __float2half_rn(g);
-            d[0] = __half_as_ushort(hi);
-            d[64] = __half_as_ushort(__float2half_rn(g - __half2float(hi)));
+            float none = 0.0f;
+            d[0] = uint16_t(split2(wide, g, none));
+            d[64] = uint16_t(split2(wide, g, none));
         } else {
             const __nv_bfloat16 hi = __float2bfloat16_rn(g);
             row[col] = __bfloat16_as_ushort(hi);

@@ -284,6 +284,7 @@ struct Layout {
     float* row_loss;
     float* ent_s;
     uint16_t* hc;
+    uint32_t* row_top;
     float4* partial;
     float* dh_sums;
     float* dw_sums;
@@ -298,7 +299,12 @@ struct Shape {
     int64_t slots;           // pieces of the vocabulary's tiles with statistics of their own
     int slot_shift;
     bool f32, pack_w, grads, flags;
-    int planes;
+    int planes;              // 16-bit planes of the logits' gradient: 1, Float32 2
+    int op_planes;           // of the states and packed weights, at most: 1, Float32 3
+    int h_parts, w_parts;    // of a row, where contiguous columns are measured by row
+    // words that measuring in parts takes: a row's magnitude, a count for 32 rows
+    static int64_t measured(int64_t rows, int parts) { return parts > 1 ? rows + (rows + 31) / 32 : 0; }
+    int64_t row_tops() const { return measured(T, h_parts) + measured(V, w_parts); }
     // Gradients: `keep`: the forward's exponentials of `rows` compact rows at a
     // time stay in the workspace and become the logits' gradient.  Otherwise
     // the logits are computed again, `piece` columns of the vocabulary at a
@@ -333,13 +339,14 @@ Layout lay_out(Bump& b, const Call& c, const Shape& s) {
     l.coef = b.take<float>(s.rows_pad);
     l.norm = b.take<float2>(s.rows_pad);
     l.row_loss = b.take<float>(s.rows_pad);
-    l.hc = b.take<uint16_t>(s.planes * s.rows_pad * s.ld_h);
+    l.hc = b.take<uint16_t>(s.op_planes * s.rows_pad * s.ld_h);
+    l.row_top = b.take<uint32_t>(s.row_tops());
     if (c.loss) l.partial = b.take<float4>(s.slots * s.rows_pad);
     if (s.keep) l.ent_s = b.take<float>(s.rows_pad * K);
     if (s.dh_sum_rows) l.dh_sums = b.take<float>(s.dh_sum_rows * s.ld_acc);
     if (s.dw_sum_rows) l.dw_sums = b.take<float>(s.dw_sum_rows * s.ld_acc);
     if (s.dw_padded) l.dw_rows = b.take<uint8_t>(std::min(s.piece, s.V) * round_up(s.D * (s.f32 ? 4 : 2), 16));
-    if (s.pack_w) l.wp = b.take<uint16_t>(s.planes * round_up(s.piece, kBK) * s.ld_h);
+    if (s.pack_w) l.wp = b.take<uint16_t>(s.op_planes * round_up(s.piece, kBK) * s.ld_h);
     if (s.grads) l.grad = b.take<uint16_t>(s.planes * s.rows * round_up(s.piece, 64));
     return l;
 }
@@ -377,6 +384,8 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
     pa.factor = c.scale * c.factor;
     pa.lse = c.loss ? nullptr : c.lse;
     pa.row_map = l.row_map;
+    pa.row_top = l.row_top;
+    pa.row_tops = (int)s.row_tops();
     pa.ent_idx = l.ent_idx;
     pa.ent_p = l.ent_p;
     pa.entropy = l.entropy;
@@ -428,6 +437,7 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
         j.dst = dst;
         j.ld = s.ld_h;
         j.rows_pad = rows_pad;
+        j.parts = 1;
         const int64_t units = j.vec ? rows_pad * (s.D / 8) / 256 : (rows_pad + 31) / 32 * ((s.ld_h + 31) / 32);
         j.ctas = (unsigned)std::max<int64_t>(std::min<int64_t>(units, fill), 1);
         return j;
@@ -449,9 +459,15 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
                    round_up(n, kBK));
     };
     if (kF32) {
-        const SplitJob jh = job(c.h, s.T, p.h_row, p.h_col, l.row_map, 0, l.hc, s.rows_pad);
+        SplitJob jh = job(c.h, s.T, p.h_row, p.h_col, l.row_map, 0, l.hc, s.rows_pad);
         const int64_t n = std::min(s.piece, s.V);
         SplitJob jw = weight_job(0, n), all = job(c.w, s.V, p.w_row, p.w_col, nullptr, 1, nullptr, s.V);
+        jh.parts = s.h_parts;
+        jh.row_top = l.row_top;
+        jh.parts_in = jh.row_top + s.T;
+        all.parts = s.w_parts;
+        all.row_top = l.row_top + s.measured(s.T, s.h_parts);
+        all.parts_in = all.row_top + s.V;
         SW_CUDA_TRY(launch_pdl(amax_kernel, dim3(jh.ctas + all.ctas), dim3(256), 0, stream, jh, all, l.state),
                     "linear head scales");
         if ((rc = split(jh, jw)) != SW_OK) return rc;
@@ -460,7 +476,7 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
     const Plane dense{kBK, 0, 0};
     // rows [r0, r0 + n) of the gathered states
     auto states = [&](int64_t r0, int64_t n) {
-        return Operand{l.hc + r0 * s.ld_h, kF32 ? s.rows_pad + n : n, s.D, s.ld_h, Plane{kBK, 0, (int)s.rows_pad}};
+        return Operand{l.hc + r0 * s.ld_h, (s.op_planes - 1) * s.rows_pad + n, s.D, s.ld_h, Plane{kBK, 0, (int)s.rows_pad}};
     };
     const int64_t ld_grad = s.planes * round_up(s.piece, 64);
 
@@ -485,7 +501,7 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
         const int64_t rows = round_up(n, kBK);
         if (packed != v0 && (rc = split(weight_job(v0, n), none_job)) != SW_OK) return rc;
         packed = v0;
-        *out = Operand{l.wp, s.planes * rows, s.D, s.ld_h, Plane{kBK, 0, (int)rows}};
+        *out = Operand{l.wp, s.op_planes * rows, s.D, s.ld_h, Plane{kBK, 0, (int)rows}};
         return SW_OK;
     };
     // logits of compact rows [r0, r0 + n) and columns [v0, v0 + nv)
@@ -759,6 +775,15 @@ int check_and_run(const char* name, Call& c, void* stream_ptr) {
     s.V = V;
     s.f32 = p->dtype == SW_HEAD_F32;
     s.planes = s.f32 ? 2 : 1;
+    s.op_planes = s.f32 ? 3 : 1;
+    // 32 rows a CTA, and where that leaves SMs idle parts of at least 64 columns
+    auto parts = [&](int64_t rows, int64_t sr, int64_t sc) {
+        if (!s.f32 || sr != 1 || sc == 1) return 1;
+        const int64_t items = (rows + 31) / 32, want = 4 * device_sms();
+        return (int)std::max<int64_t>(1, items * 2 > want ? 1 : std::min((D + 63) / 64, want / std::max<int64_t>(items, 1)));
+    };
+    s.h_parts = parts(T, p->h_row, p->h_col);
+    s.w_parts = parts(V, p->w_row, p->w_col);
     s.rows_pad = std::max<int64_t>(round_up(T, kBM), kBM);
     s.ld_h = round_up(D, 8);
     s.flags = !c.targets && T * c.top_k > kInlineFlags;
@@ -768,7 +793,7 @@ int check_and_run(const char* name, Call& c, void* stream_ptr) {
     s.pack_w = s.f32 || p->w_col != 1 || p->w_row % 8 != 0 || p->w_row < D ||
                (reinterpret_cast<uintptr_t>(c.w) & 15) != 0;
     const int64_t budget = p->workspace_limit > 0 ? p->workspace_limit : kDefaultWorkspace;
-    const int64_t packed = s.pack_w ? s.planes * round_up(V, kBK) * s.ld_h * 2 : 0;
+    const int64_t packed = s.pack_w ? s.op_planes * round_up(V, kBK) * s.ld_h * 2 : 0;
     const int64_t grad_row = s.planes * round_up(V, 256) * 2;
     const int terms = s.f32 ? 3 : 1;
     // One call for the loss and the gradients keeps the logits' exponentials
@@ -788,7 +813,7 @@ int check_and_run(const char* name, Call& c, void* stream_ptr) {
     s.piece = round_up(V, 256);
     if (!s.keep) {
         // as wide as the limit allows, in whole 256-column tiles
-        const int64_t per_column = (grads ? s.planes * s.rows_pad * 2 : 0) + (s.pack_w ? s.planes * s.ld_h * 2 : 0);
+        const int64_t per_column = (grads ? s.planes * s.rows_pad * 2 : 0) + (s.pack_w ? s.op_planes * s.ld_h * 2 : 0);
         if (per_column > 0) s.piece = std::min(s.piece, std::max<int64_t>(budget / per_column / 256 * 256, 256));
     }
     const int64_t n = std::min(s.rows, T), nv = std::min(s.piece, V);

@@ -84,3 +84,51 @@ def test_a_row_of_huge_logits_is_finite_and_stays_alone(path):
     tol = 2.0 ** -8 + 1e-5 * (1 + float(others))
     assert bool((row_errors(out["dh"], dh) <= tol).all())
     assert bool((row_errors(out["dw"], dw) <= tol).all())
+
+
+def columns(x):
+    return x.t().contiguous().t()
+
+
+@pytest.mark.parametrize("path", ["one call", "kept lse", "pieces"])
+@pytest.mark.parametrize("kind", ["a state of 1e13", "states of 1e9", "a word of 1e9", "factors from 1e-6",
+                                  "factors from 1e-12", "all"])
+@pytest.mark.parametrize("T,V,D,layout", [(60, 700, 96, "rows"), (300, 3000, 200, "rows"), (60, 700, 96, "columns"),
+                                          (40, 9600, 65, "columns")])
+def test_float32_rows_far_apart(T, V, D, layout, kind, path):
+    """What one row holds is no other row's loss: states, words and upstream factors 1e6 to 1e13 apart."""
+    h, w, y = states(T, V, D, torch.float32)
+    h[:, 0] = 1.0 + h[:, 0].abs()
+    up = torch.rand(T, device="cuda") + 0.5
+    big = torch.zeros(T, dtype=torch.bool, device="cuda")
+    if kind in ("a state of 1e13", "all"):
+        big[7] = True
+        h[7] *= 1e13
+    if kind == "states of 1e9":
+        big[2::3] = True
+        h[big] *= 1e9
+    if kind in ("a word of 1e9", "all"):  # never likely: its logits are below -1e9
+        y[y == 11] = 12
+        w[11] = 0.0
+        w[11, 0] = -1e9
+    if kind.startswith("factors") or kind == "all":
+        up = torch.logspace(-6 if kind.endswith("1e-6") else -12, 0, T, device="cuda")
+    if layout == "columns":
+        h, w = columns(h), columns(w)
+    loss, lse, dh, dw, _, _ = reference(h, w, up, targets=y)
+    out = call(h, w, targets=y, up=up, limit=1 if path == "pieces" else 0)
+    s = (h.double() @ w.double().t()).abs()
+    touched = s.argmax(1)[big]  # words whose gradient the large states are
+    s[:, 11] = 0.0
+    top = s.amax(1)
+    assert bool(((out["loss"].double() - loss).abs() <= 1e-5 * (1 + top)).all())
+    assert bool(((out["lse"].double() - lse).abs() <= 1e-5 * (1 + top)).all())
+    if path == "kept lse":
+        out = call(h, w, targets=y, up=up, lse_in=out["lse"])
+    assert bool(torch.isfinite(out["dh"]).all()) and bool(torch.isfinite(out["dw"]).all())
+    tol = 2e-5 * (1 + top / 4)
+    assert bool((row_errors(out["dh"], dh) <= tol)[~big].all())
+    words = torch.ones(V, dtype=torch.bool, device="cuda")
+    words[touched] = False
+    words[y[big].long()] = False
+    assert bool((row_errors(out["dw"], dw) <= float(tol[~big].max()))[words].all())
