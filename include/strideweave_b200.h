@@ -533,7 +533,7 @@ typedef struct {
   int64_t tokens, dim, vocab;
   int64_t h_row, h_col, w_row, w_col;
   int64_t dh_row, dh_col, dw_row, dw_col;
-  int64_t workspace_limit; /* bytes that logits' gradients and packed weights may take (0: the default, 4 GiB) */
+  int64_t workspace_limit; /* bytes of scratch that a call may take (0: the default, 8 GiB); see sw_linear_xent */
 } sw_linear_head;
 
 /* Softmax cross entropy of a linear head, without keeping the logits:
@@ -547,9 +547,20 @@ typedef struct {
  *
  * `loss` is Float32 [tokens] or [1]; `lse` is Float32 [tokens] and optional.
  * With loss NULL the call computes only gradients, from the `lse` an earlier
- * call returned (the backward node of an autograd graph).  Scratch comes from
- * the device's stream-ordered pool.  No reference counterpart: the reference's
- * losses take whole predictions (src/strideweave/nn/modules.py:129-200). */
+ * call returned (the backward node of an autograd graph).  No output may overlap
+ * an input or another output.
+ *
+ * Scratch comes from the device's stream-ordered default pool, workspace_limit
+ * bytes of it at most: under a smaller limit the rows or the vocabulary go in
+ * pieces, which takes longer.  What every plan takes is the least: the states
+ * gathered (2 bytes an element, Float32 6), the statistics of min(tokens, 1024)
+ * rows (all rows where weights are packed in pieces) at vocab / 8 bytes, logits'
+ * gradients of 256 columns (2 bytes, Float32 4) and as many rows of packed
+ * weights, and fp32 sums of dh; a call that needs more than its limit for these
+ * takes them all the same.  The first call sets the pool's release threshold to
+ * keep what was freed, for the next one (as sw_alloc does). No reference
+ * counterpart: the reference's losses take whole predictions
+ * (src/strideweave/nn/modules.py:129-200). */
 int sw_linear_xent(const sw_linear_head* plan, const void* h, const void* w,
                    const int32_t* targets, int32_t ignore_index, float logit_scale,
                    float* loss, float* lse, const float* upstream,

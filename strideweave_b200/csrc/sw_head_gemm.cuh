@@ -217,7 +217,7 @@ struct GemmArgs {
     const uint16_t* offs;    // [tile][rows_pad] first entry of each kEntryTile columns (null: one entry a row)
     int ent_k;
     int rows_pad;
-    float4* partial;         // kEpiLse: [rows_pad][slots] (max, sum, target term, unused: one store)
+    float4* partial;         // kEpiLse: [rows][slots] (max, sum, target term, unused: one store)
     int slots, slot_shift;   // a slot for each 1 << slot_shift columns: 128, or a narrow tile's 64
     int tile_n;              // logits tiles of one CTA: 256 columns, or 128 or 64 where they spread over more SMs
     float* ent_s;            // kEpiLse: h w of every target entry (null: not kept)

@@ -49,6 +49,24 @@ __host__ __device__ inline float spread_cost(int64_t M, int64_t N, int64_t K, in
     return us;
 }
 
+// Parts that a K walk may be cut into (as above).
+__host__ __device__ inline int most_parts(int64_t K) {
+    const int64_t s = (K + kBK - 1) / kBK / 4;
+    return int(s < 1 ? 1 : s < kMaxParts ? s : kMaxParts);
+}
+// Rows of fp32 sums that up to `parts` parts of any row count up to M take: all rows,
+// and those of the parts past the first, of at most two tiles a worker where the
+// tiles do not fill a wave, else of the row groups that the last wave reaches.
+__host__ __device__ inline int64_t sum_rows(int64_t M, int64_t N, int parts, int shape, int sms) {
+    const int64_t cols = (N + kBN - 1) / kBN, tile_m = shape_rows(shape), all = (M + tile_m - 1) / tile_m * tile_m;
+    const int64_t workers = shape_workers(shape, sms), group = 2048 / tile_m;
+    const int64_t few = (2 * workers / cols + 1) * tile_m, every = (parts - 1) * all;
+    const int64_t reach = (workers / (group * cols) + 2) * group * tile_m;
+    const int64_t tail = (reach < all ? reach : all) * ((parts < kMaxTailParts ? parts : kMaxTailParts) - 1);
+    const int64_t first = few < every ? few : every;
+    return all + (first > tail ? first : tail);
+}
+
 constexpr uint32_t kNoMagnitude = 0x7f800000u;  // least magnitude of no rows
 
 // ---- preparation ---------------------------------------------------------------
@@ -585,7 +603,7 @@ __global__ void __launch_bounds__(256) split_kernel(const SplitJob j0, const Spl
 // ---- after the logits ------------------------------------------------------------
 
 struct LossArgs {
-    const float4* partial;   // [rows_pad][slots]
+    const float4* partial;   // [rows][slots]
     int slots, slot_shift;
     int row0, rows;          // compact rows [row0, row0 + rows), a CTA each
     int all_rows;            // CTAs over all launches that write a row's loss
@@ -661,7 +679,7 @@ __global__ void __launch_bounds__(256, kF32 ? 4 : 3) loss_kernel(const LossArgs 
     };
     if (a.grad && i < count) fetch(c_begin);
     if (i < count) {
-        const float4* part = a.partial + (a.row0 + i) * a.slots;
+        const float4* part = a.partial + i * a.slots;
         // against the largest z of a thread's slots, of a warp's, and then of all
         auto finite = [](float r) { return r == -INFINITY ? 0.0f : r; };
         float sum = 0.0f, dot = 0.0f;
@@ -733,7 +751,7 @@ __global__ void __launch_bounds__(256, kF32 ? 4 : 3) loss_kernel(const LossArgs 
         const int64_t c1 = min(c0 + kSub, c_end);
         __syncthreads();
         for (int t = tid; t < int((c1 - c0 + 63) / 64); t += 256) {
-            const float top = a.partial[(a.row0 + i) * a.slots + ((c0 + t * 64) >> a.slot_shift)].x;
+            const float top = a.partial[i * a.slots + ((c0 + t * 64) >> a.slot_shift)].x;
             // (a half tile of nothing but -inf stored zeros)
             factor[t] = top == -INFINITY
                             ? 0.0f

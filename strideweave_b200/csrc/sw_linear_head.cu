@@ -57,9 +57,9 @@ namespace sw {
 namespace head {
 namespace {
 
-// What the pieces may take unless the plan says otherwise: the exponentials of
-// 16384 rows over a vocabulary of 131072.
-constexpr int64_t kDefaultWorkspace = int64_t(4) << 30;
+// What a call may take unless the plan says otherwise: the exponentials of 16384
+// rows over a vocabulary of 131072 are half of it.
+constexpr int64_t kDefaultWorkspace = int64_t(8) << 30;
 
 // ---- host ----------------------------------------------------------------------
 
@@ -112,18 +112,6 @@ Spread choose_parts(int64_t M, int64_t N, int64_t K, int terms, int shape, bool 
         if (us < best.us * 0.97f) best = Spread{s, us};
     }
     return best;
-}
-
-// Rows of fp32 sums that the parts of any row count up to M may take: all rows,
-// and those of the parts past the first, of at most two tiles per worker where
-// the tiles do not fill a wave, else of the row groups that the last wave
-// reaches.
-int64_t sum_rows(int64_t M, int64_t N, int shape) {
-    const int64_t cols = (N + kBN - 1) / kBN, tile_m = shape_rows(shape), all = round_up(M, tile_m);
-    const int64_t workers = shape_workers(shape, device_sms()), group = 2048 / tile_m;
-    const int64_t few = (2 * workers / cols + 1) * tile_m;
-    const int64_t tail = std::min(all, (workers / (group * cols) + 2) * group * tile_m) * (kMaxTailParts - 1);
-    return all + std::max(few, tail);
 }
 
 // Where a contraction writes through its output map: 16-bit or Float32 values,
@@ -309,8 +297,9 @@ struct Shape {
     // time stay in the workspace and become the logits' gradient.  Otherwise
     // the logits are computed again, `piece` columns of the vocabulary at a
     // time.  Packed weights are laid out `piece` columns at a time too.
+    // A loss alone takes its statistics stat_rows compact rows at a time.
     bool keep;
-    int64_t rows, piece;
+    int64_t rows, piece, stat_rows;
     // Few rows (one row tile): the gradients' contractions share a launch, which
     // reads the weights while it writes their gradient.
     bool together;
@@ -341,7 +330,7 @@ Layout lay_out(Bump& b, const Call& c, const Shape& s) {
     l.row_loss = b.take<float>(s.rows_pad);
     l.hc = b.take<uint16_t>(s.op_planes * s.rows_pad * s.ld_h);
     l.row_top = b.take<uint32_t>(s.row_tops());
-    if (c.loss) l.partial = b.take<float4>(s.slots * s.rows_pad);
+    if (c.loss) l.partial = b.take<float4>(s.slots * (s.keep ? s.rows : s.stat_rows));
     if (s.keep) l.ent_s = b.take<float>(s.rows_pad * K);
     if (s.dh_sum_rows) l.dh_sums = b.take<float>(s.dh_sum_rows * s.ld_acc);
     if (s.dw_sum_rows) l.dw_sums = b.take<float>(s.dw_sum_rows * s.ld_acc);
@@ -520,7 +509,7 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
         a.ent_idx = l.ent_idx + r0 * g.ent_k;
         a.ent_p = l.ent_p ? l.ent_p + r0 * g.ent_k : nullptr;
         a.offs = l.offs ? l.offs + r0 : nullptr;
-        a.partial = l.partial + r0 * s.slots;
+        a.partial = l.partial;
         // what the row subtracts: the kept lse of the logits, or the largest z and the sum's logarithm
         a.norm = l.norm + r0;
         a.to_ref = c.loss ? 1.0f : c.scale;
@@ -687,15 +676,18 @@ int run(const Call& c, const Shape& s, const Layout& l, cudaStream_t stream) {
     }
     if (c.loss) {
         const int64_t step = s.pack_w ? s.piece : s.V;
-        for (int64_t v0 = 0; v0 < s.V; v0 += step) {
-            const int64_t n = std::min(step, s.V - v0);
-            Operand w;
-            if ((rc = weights(v0, n, &w)) != SW_OK) return rc;
-            GemmArgs a = logits(0, s.T, v0, n);
-            const Tensors t{states(0, s.rows_pad), w, none};
-            if ((rc = gemm<kBf16, kEpiLse, kKMajor>(&t, a, s.logits_shape, stream)) != SW_OK) return rc;
+        for (int64_t r0 = 0; r0 == 0 || r0 < s.T; r0 += s.stat_rows) {
+            const int64_t nr = std::min(s.stat_rows, s.T - r0);
+            for (int64_t v0 = 0; v0 < s.V; v0 += step) {
+                const int64_t n = std::min(step, s.V - v0);
+                Operand w;
+                if ((rc = weights(v0, n, &w)) != SW_OK) return rc;
+                GemmArgs a = logits(r0, nr, v0, n);
+                const Tensors t{states(r0, round_up(std::max<int64_t>(nr, 1), kBM)), w, none};
+                if ((rc = gemm<kBf16, kEpiLse, kKMajor>(&t, a, s.logits_shape, stream)) != SW_OK) return rc;
+            }
+            if ((rc = losses(r0, nr, false)) != SW_OK) return rc;
         }
-        if ((rc = losses(0, s.T, false)) != SW_OK) return rc;
     }
     if (!s.grads) return SW_OK;
     for (int64_t v0 = 0; v0 < s.V; v0 += s.piece) {
@@ -723,6 +715,139 @@ bool strides_ok(int64_t rows, int64_t cols, int64_t sr, int64_t sc, bool distinc
     if (cols > 1 && sc == 0) return false;
     if (rows == 1 || cols == 1) return true;
     return sr <= sc ? sc > (rows - 1) * sr : sr > (cols - 1) * sc;
+}
+
+// A call's plan: `keep` with the exponentials of `rows` compact rows at a time, or
+// the logits' gradient of `piece` columns of the vocabulary, and the statistics of
+// a loss alone of `stat_rows` rows at a time.
+Shape make_plan(const Call& c, bool keep, int64_t rows, int64_t piece, int64_t stat_rows) {
+    const sw_linear_head* p = c.plan;
+    const int64_t T = p->tokens, D = p->dim, V = p->vocab;
+    const bool grads = c.dh || c.dw;
+    Shape s;
+    s.T = T;
+    s.D = D;
+    s.V = V;
+    s.f32 = p->dtype == SW_HEAD_F32;
+    s.planes = s.f32 ? 2 : 1;
+    s.op_planes = s.f32 ? 3 : 1;
+    // 32 rows a CTA, and where that leaves SMs idle parts of at least 64 columns
+    auto parts = [&](int64_t rows, int64_t sr, int64_t sc) {
+        if (!s.f32 || sr != 1 || sc == 1) return 1;
+        const int64_t items = (rows + 31) / 32, want = 4 * device_sms();
+        return (int)std::max<int64_t>(1, items * 2 > want ? 1 : std::min((D + 63) / 64, want / std::max<int64_t>(items, 1)));
+    };
+    s.h_parts = parts(T, p->h_row, p->h_col);
+    s.w_parts = parts(V, p->w_row, p->w_col);
+    s.rows_pad = std::max<int64_t>(round_up(T, kBM), kBM);
+    s.ld_h = round_up(D, 8);
+    s.flags = !c.targets && T * c.top_k > kInlineFlags;
+    s.grads = grads;
+    s.ld_acc = round_up(D, 4);
+    // weights are read in place when TMA can: bf16, unit stride, 16-byte rows
+    s.pack_w = s.f32 || p->w_col != 1 || p->w_row % 8 != 0 || p->w_row < D ||
+               (reinterpret_cast<uintptr_t>(c.w) & 15) != 0;
+    const int terms = s.f32 ? 3 : 1;
+    s.keep = keep;
+    s.rows = rows;
+    s.piece = piece;
+    s.stat_rows = stat_rows;
+    const int64_t n = std::min(s.rows, T), nv = std::min(s.piece, V), nl = grads ? n : std::min(stat_rows, T);
+    // (a pair's second half would have no row of a single row tile: 21 x 18689 at dim
+    // 2496 scored in 45 us by pairs, in 32 by single CTAs)
+    s.logits_shape = nl <= kBM || choose_parts(nl, nv, D, terms, kSingle, false).us <
+                              0.97f * choose_parts(nl, nv, D, terms, kPair2, false).us
+                         ? kSingle
+                         : kPair2;
+    // Where 256-column tiles would leave SMs idle, narrower ones spread the weights
+    // over more of them: the loss of one token over 32000 classes at dim 4096 65 us
+    // at 256 columns, 61 at 128; Float32 33 x 1021 at dim 257 with gradients 55, 49 at 64.
+    s.tile_n = kBN;
+    if (s.logits_shape == kSingle)
+        for (const int t : {128, 64})
+            if ((nl + kBM - 1) / kBM * ((nv + t - 1) / t) <= device_sms()) s.tile_n = t;
+    s.slot_shift = s.tile_n == 64 ? 6 : 7;
+    s.slots = (V + s.tile_n - 1) / s.tile_n * (s.tile_n >> s.slot_shift);
+    // dw is written at once through TMA where that can describe it (rows that end
+    // inside 16 bytes would be written past their end).
+    const int64_t es = s.f32 ? 4 : 2;
+    const bool direct = p->dw_col == 1 && p->dw_row * es % 16 == 0 && D * es % 16 == 0 && p->dw_row >= D &&
+                        (reinterpret_cast<uintptr_t>(c.dw) & 15) == 0;
+    const bool one_part = s.rows >= T;  // nothing to add to what is written
+    const float sum_us = one_part ? float(nv) * float(D) * float(8 + es) / 6.0e6f : 0.0f;
+    s.together = c.dh && c.dw && n <= kBM;
+    s.dh_shape = s.dw_shape = kSingle;
+    s.dw_splits = 1;
+    float dh_us = 1e30f, dw_us = 1e30f;
+    for (int shape = s.together ? kSingle : s.f32 ? kPair2 : kTall; grads && shape >= kSingle; --shape) {
+        const Spread dh = choose_parts(n, D, nv, terms, shape, true);
+        const Spread dw = choose_parts(nv, D, n, terms, shape, true, sum_us);
+        if (dh.us < dh_us * 0.97f) {
+            dh_us = dh.us;
+            s.dh_shape = shape;
+        }
+        if (dw.us < dw_us * 0.97f) {
+            dw_us = dw.us;
+            s.dw_shape = shape;
+            s.dw_splits = dw.splits;
+        }
+    }
+    s.dh_sum_rows = c.dh && T > 0 ? sum_rows(n, D, most_parts(nv), s.dh_shape, device_sms()) : 0;
+    s.dw_sum_rows = c.dw && (!one_part || s.dw_splits > 1) ? sum_rows(nv, D, s.dw_splits, s.dw_shape, device_sms()) : 0;
+    s.dw_padded = c.dw && !s.dw_sum_rows && !direct;
+    return s;
+}
+
+int64_t scratch_bytes(const Call& c, const Shape& s) {
+    Bump measure{nullptr, 0};
+    lay_out(measure, c, s);
+    return measure.used;
+}
+
+// The plan that does least within the workspace limit.  One call for the loss and
+// the gradients keeps the logits' exponentials of all rows, or of as many as fit,
+// 1024 (or all) at least, beside the fp32 sums of dw that blocks of rows need (6
+// T V D operations and one more pass over them).  From a kept lse, or where that
+// does not fit, the logits are computed again (8 T V D), in pieces of the
+// vocabulary as wide as fit, in whole 256-column tiles.  The least there is - one
+// such piece, and the statistics of 1024 rows - is taken even if it does not fit.
+Shape choose_plan(const Call& c) {
+    const sw_linear_head* p = c.plan;
+    const bool grads = c.dh || c.dw;
+    const int64_t limit = p->workspace_limit > 0 ? p->workspace_limit : kDefaultWorkspace;
+    const int64_t all = std::max<int64_t>(round_up(p->tokens, kBM), kBM), fewest = std::min<int64_t>(all, 1024);
+    const int64_t whole = round_up(p->vocab, 256);
+    auto bytes = [&](const Shape& s) { return scratch_bytes(c, s); };
+    // the largest multiple of `unit` from `least` to `most` whose plan fits; the bytes grow with it
+    auto largest = [&](int64_t least, int64_t most, int64_t unit, auto&& plan) {
+        int64_t lo = least / unit, hi = (most + unit - 1) / unit;
+        while (lo < hi) {
+            const int64_t mid = (lo + hi + 1) / 2;
+            if (bytes(plan(std::min(mid * unit, most))) <= limit) lo = mid;
+            else hi = mid - 1;
+        }
+        return std::min(lo * unit, most);
+    };
+    if (c.loss && grads) {
+        auto kept = [&](int64_t rows) { return make_plan(c, true, rows, whole, rows); };
+        const Shape s = kept(all);
+        if (bytes(s) <= limit) return s;
+        if (fewest < all && bytes(kept(fewest)) <= limit) {
+            const int64_t rows = largest(fewest, all - kBM, kBM, kept), blocks = (all + rows - 1) / rows;
+            const Shape even = kept(round_up((all + blocks - 1) / blocks, kBM));
+            return bytes(even) <= limit ? even : kept(rows);
+        }
+    }
+    auto again = [&](int64_t piece, int64_t stat_rows) { return make_plan(c, false, all, piece, stat_rows); };
+    Shape s = again(whole, all);
+    if (bytes(s) <= limit) return s;
+    // packed weights are packed once for all rows' statistics, so in pieces these are not blocked
+    if (!grads && (!s.pack_w || bytes(again(whole, fewest)) <= limit))
+        return again(whole, largest(fewest, all, kBM, [&](int64_t rows) { return again(whole, rows); }));
+    const int64_t stats = s.pack_w ? all : fewest;
+    const int64_t piece = largest(256, whole, 256, [&](int64_t columns) { return again(columns, stats); });
+    if (s.pack_w || !c.loss) return again(piece, stats);
+    return again(piece, largest(fewest, all, kBM, [&](int64_t rows) { return again(piece, rows); }));
 }
 
 int check_and_run(const char* name, Call& c, void* stream_ptr) {
@@ -769,109 +894,18 @@ int check_and_run(const char* name, Call& c, void* stream_ptr) {
         return fail(SW_ERR_INVALID, "%s: a vector is not aligned to its elements", name);
     cudaStream_t stream = (cudaStream_t)stream_ptr;
 
-    Shape s;
-    s.T = T;
-    s.D = D;
-    s.V = V;
-    s.f32 = p->dtype == SW_HEAD_F32;
-    s.planes = s.f32 ? 2 : 1;
-    s.op_planes = s.f32 ? 3 : 1;
-    // 32 rows a CTA, and where that leaves SMs idle parts of at least 64 columns
-    auto parts = [&](int64_t rows, int64_t sr, int64_t sc) {
-        if (!s.f32 || sr != 1 || sc == 1) return 1;
-        const int64_t items = (rows + 31) / 32, want = 4 * device_sms();
-        return (int)std::max<int64_t>(1, items * 2 > want ? 1 : std::min((D + 63) / 64, want / std::max<int64_t>(items, 1)));
-    };
-    s.h_parts = parts(T, p->h_row, p->h_col);
-    s.w_parts = parts(V, p->w_row, p->w_col);
-    s.rows_pad = std::max<int64_t>(round_up(T, kBM), kBM);
-    s.ld_h = round_up(D, 8);
-    s.flags = !c.targets && T * c.top_k > kInlineFlags;
-    s.grads = grads;
-    s.ld_acc = round_up(D, 4);
-    // weights are read in place when TMA can: bf16, unit stride, 16-byte rows
-    s.pack_w = s.f32 || p->w_col != 1 || p->w_row % 8 != 0 || p->w_row < D ||
-               (reinterpret_cast<uintptr_t>(c.w) & 15) != 0;
-    const int64_t budget = p->workspace_limit > 0 ? p->workspace_limit : kDefaultWorkspace;
-    const int64_t packed = s.pack_w ? s.op_planes * round_up(V, kBK) * s.ld_h * 2 : 0;
-    const int64_t grad_row = s.planes * round_up(V, 256) * 2;
-    const int terms = s.f32 ? 3 : 1;
-    // One call for the loss and the gradients keeps the logits' exponentials
-    // of as many rows as the workspace limit allows (6 T V D operations and one
-    // more pass over them); from a kept lse, or where not even 1024 rows (or
-    // all) fit, the logits are computed again (8 T V D).
-    s.rows = s.rows_pad;
-    s.keep = false;
-    if (c.loss && grads && packed < budget) {
-        const int64_t fit = (budget - packed) / grad_row / kBM * kBM;
-        if (fit >= std::min<int64_t>(s.rows_pad, 1024)) {
-            s.keep = true;
-            const int64_t chunks = (s.rows_pad + fit - 1) / fit;
-            s.rows = std::min(s.rows_pad, round_up((s.rows_pad + chunks - 1) / chunks, kBM));
-        }
-    }
-    s.piece = round_up(V, 256);
-    if (!s.keep) {
-        // as wide as the limit allows, in whole 256-column tiles
-        const int64_t per_column = (grads ? s.planes * s.rows_pad * 2 : 0) + (s.pack_w ? s.op_planes * s.ld_h * 2 : 0);
-        if (per_column > 0) s.piece = std::min(s.piece, std::max<int64_t>(budget / per_column / 256 * 256, 256));
-    }
-    const int64_t n = std::min(s.rows, T), nv = std::min(s.piece, V);
-    // (a pair's second half would have no row of a single row tile: 21 x 18689 at dim
-    // 2496 scored in 45 us by pairs, in 32 by single CTAs)
-    s.logits_shape = n <= kBM || choose_parts(n, nv, D, terms, kSingle, false).us <
-                             0.97f * choose_parts(n, nv, D, terms, kPair2, false).us
-                         ? kSingle
-                         : kPair2;
-    // Where 256-column tiles would leave SMs idle, narrower ones spread the weights
-    // over more of them: the loss of one token over 32000 classes at dim 4096 65 us
-    // at 256 columns, 61 at 128; Float32 33 x 1021 at dim 257 with gradients 55, 49 at 64.
-    s.tile_n = kBN;
-    if (s.logits_shape == kSingle)
-        for (const int t : {128, 64})
-            if ((n + kBM - 1) / kBM * ((nv + t - 1) / t) <= device_sms()) s.tile_n = t;
-    s.slot_shift = s.tile_n == 64 ? 6 : 7;
-    s.slots = (V + s.tile_n - 1) / s.tile_n * (s.tile_n >> s.slot_shift);
-    // dw is written at once through TMA where that can describe it (rows that end
-    // inside 16 bytes would be written past their end).
-    const int64_t es = s.f32 ? 4 : 2;
-    const bool direct = p->dw_col == 1 && p->dw_row * es % 16 == 0 && D * es % 16 == 0 && p->dw_row >= D &&
-                        (reinterpret_cast<uintptr_t>(c.dw) & 15) == 0;
-    const bool one_part = s.rows >= T;  // nothing to add to what is written
-    const float sum_us = one_part ? float(nv) * float(D) * float(8 + es) / 6.0e6f : 0.0f;
-    s.together = c.dh && c.dw && n <= kBM;
-    s.dh_shape = s.dw_shape = kSingle;
-    s.dw_splits = 1;
-    float dh_us = 1e30f, dw_us = 1e30f;
-    for (int shape = s.together ? kSingle : s.f32 ? kPair2 : kTall; grads && shape >= kSingle; --shape) {
-        const Spread dh = choose_parts(n, D, nv, terms, shape, true);
-        const Spread dw = choose_parts(nv, D, n, terms, shape, true, sum_us);
-        if (dh.us < dh_us * 0.97f) {
-            dh_us = dh.us;
-            s.dh_shape = shape;
-        }
-        if (dw.us < dw_us * 0.97f) {
-            dw_us = dw.us;
-            s.dw_shape = shape;
-            s.dw_splits = dw.splits;
-        }
-    }
-    s.dh_sum_rows = c.dh && T > 0 ? sum_rows(n, D, s.dh_shape) : 0;
-    s.dw_sum_rows = c.dw && (!one_part || s.dw_splits > 1) ? sum_rows(nv, D, s.dw_shape) : 0;
-    s.dw_padded = c.dw && !s.dw_sum_rows && !direct;
-
-    Bump measure{nullptr, 0};
-    lay_out(measure, c, s);
+    const Shape s = choose_plan(c);
+    const int64_t bytes = scratch_bytes(c, s);
     void* ws = nullptr;
     int dev = 0;
     SW_CUDA_TRY(cudaGetDevice(&dev), "cudaGetDevice");
     const int pooled = keep_pool_memory(dev);
     if (pooled != SW_OK) return pooled;
-    cudaError_t err = cudaMallocAsync(&ws, (size_t)measure.used, stream);
+    cudaError_t err = cudaMallocAsync(&ws, (size_t)bytes, stream);
     if (err == cudaErrorMemoryAllocation) {
         cudaGetLastError();
         return fail(SW_ERR_NOMEM, "%s: out of device memory for %lld bytes of workspace", name,
-                    (long long)measure.used);
+                    (long long)bytes);
     }
     SW_CUDA_TRY(err, "cudaMallocAsync (linear head workspace)");
     Bump real{static_cast<uint8_t*>(ws), 0};
