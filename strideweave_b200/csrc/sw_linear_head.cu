@@ -46,6 +46,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <numeric>
 #include <type_traits>
 
 #include "sw_common.cuh"
@@ -714,7 +715,9 @@ bool strides_ok(int64_t rows, int64_t cols, int64_t sr, int64_t sc, bool distinc
     if (rows > 1 && sr == 0) return false;
     if (cols > 1 && sc == 0) return false;
     if (rows == 1 || cols == 1) return true;
-    return sr <= sc ? sc > (rows - 1) * sr : sr > (cols - 1) * sc;
+    // i sr = j sc first for i = sc / g, j = sr / g
+    const int64_t g = std::gcd(sr, sc);
+    return sc / g >= rows || sr / g >= cols;
 }
 
 // A call's plan: `keep` with the exponentials of `rows` compact rows at a time, or
