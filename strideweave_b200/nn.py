@@ -39,7 +39,7 @@ import numpy as np
 from . import _native as N
 from ._host import (BFloat16, DType, Layout, Operation, Shape, Stride, Tensor, require_capability,
                     resolve_operation_plan)
-from .layout_plan import canonical_layout, mode_leaves, mode_size, single_stride
+from .layout_plan import canonical_layout, mode_leaves, mode_size, single_stride, swizzle_stages
 
 
 def _compact(t: Any, name: str) -> tuple[int, int]:
@@ -176,6 +176,25 @@ def _head_vector(t: Any, name: str, dtype: Any, size: int) -> int:
     return t.carrier.data_ptr + 4 * t.offset
 
 
+def _head_upstream(t: Any, size: int) -> tuple[int, Any]:
+    """Address of a gradient's `size` Float32 elements, and what keeps them: the
+    gradient itself where it is contiguous, else a copy (a broadcast sum's
+    gradient has stride 0)."""
+    from . import kernels
+    from .carrier import CUDA
+
+    if (isinstance(t, Tensor) and len(t.layout) == 1 and isinstance(t.carrier, CUDA)
+            and t.carrier.dtype() is DType.Float32 and t.size() == size):
+        leaves = mode_leaves(t.layout, 0)
+        if single_stride(leaves) not in ((size, 1), (1, 0)) or t.carrier.swizzle is not None:
+            t._require_single_subtensor("CUDA linear head loss")
+            dense = CUDA(size, dtype=DType.Float32, empty=True, device=t.carrier.device)
+            kernels.copy_view_f32(t.carrier.data_ptr, t.carrier.size(), t.offset, leaves, [(1, 0)], dense.data_ptr,
+                                  size, 0, [(size, 1)], [(1, 0)], swizzle=swizzle_stages(t.carrier))
+            return dense.data_ptr, dense
+    return _head_vector(t, "gradient", DType.Float32, size), t
+
+
 class _LinearHeadLoss(Operation):
     """What the two losses of a linear head share; see `linear_cross_entropy`."""
 
@@ -226,9 +245,10 @@ class _LinearHeadLoss(Operation):
     def backward(self, gradient: Any) -> tuple[Any, Any]:
         x, weight = self.inputs()
         head, T = self._shape(x, weight)
-        up = _head_vector(gradient, "gradient", DType.Float32, 1 if self.reduction == "mean" else T)
+        up, held = _head_upstream(gradient, 1 if self.reduction == "mean" else T)
         dx, dw, where = self._gradients(x, weight)
         self._run(head, lse_ptr=self.ctx["lse"].data_ptr, upstream_ptr=up, **where)
+        del held  # (released in stream order)
         return dx, dw
 
     def loss_and_gradients(self, x: Any, weight: Any) -> tuple[Tensor, Tensor, Tensor]:

@@ -110,6 +110,21 @@ def one_call():
             assert torch.equal(values(dx).to(dtype), raw["dh"]) and torch.equal(values(dw).to(dtype), raw["dw"])
 
 
+def upstream_placements():
+    """A gradient per row at another stride, behind an offset, or the same for every row."""
+    for dtype, h, w, op, kw in cases(("rows",)):
+        base = torch.rand(3 * T, device="cuda") + 0.5
+        for up in (base[::3], base[1:2].expand(T), base[5:5 + T]):
+            x, weight = tensor(h, True), tensor(w, True)
+            loss = loss_of(op, x, weight, kw, "none")
+            gradient = tensor(base)
+            gradient.offset, gradient.layout = up.storage_offset(), Layout(Shape(T), Stride(up.stride()[0]))
+            loss.backward(gradient)
+            want = reference(h, w, up, **kw)
+            near(values(x.grad), want[2], dtype)
+            near(values(weight.grad), want[3], dtype)
+
+
 if __name__ == "__main__":
     for name in sys.argv[1:]:
         globals()[name]()
