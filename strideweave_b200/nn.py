@@ -280,9 +280,12 @@ class CudaLinearDistillation(_LinearHeadLoss):
     def _run(self, head: tuple, **kw: Any) -> None:
         from . import kernels
 
-        if not isinstance(self.index, Tensor) or len(self.index.layout) != 2:
-            raise ValueError("index must have a two-mode layout [tokens, entries]")
+        for t, name in ((self.index, "index"), (self.logits, "logits")):
+            if not isinstance(t, Tensor) or len(t.layout) != 2:
+                raise ValueError(f"{name} must have a two-mode layout [tokens, entries]")
         top_k = mode_size(self.index.layout, 1)
+        if mode_size(self.logits.layout, 1) != top_k:
+            raise ValueError(f"logits must have {top_k} entries a row, as index has")
         kernels.linear_distillation(*head, _head_vector(self.index, "index", DType.Int32, head[5] * top_k),
                                     _head_vector(self.logits, "logits", DType.Float32, head[5] * top_k), top_k,
                                     temperature=self.temperature, reduction=self.reduction, **kw)

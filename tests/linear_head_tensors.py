@@ -125,6 +125,29 @@ def upstream_placements():
             near(values(weight.grad), want[3], dtype)
 
 
+def refused(error, match, f):
+    try:
+        f()
+    except error as e:
+        assert match in str(e), e
+        return
+    raise AssertionError(f"not refused: {match}")
+
+
+def teacher_shapes():
+    """Logits of as many elements as the index, in other rows."""
+    for dtype, h, w, op, kw in cases(("rows",)):
+        if op != "distill":
+            continue
+        x, weight, index = tensor(h), tensor(w), tensor(kw["index"])
+        flat = kw["logits"].reshape(-1)
+        for logits in (flat.reshape(K, T), flat.reshape(1, T * K)):
+            refused(ValueError, "entries a row", lambda: nn.linear_distillation(x, weight, index, tensor(logits)))
+        refused(ValueError, "two-mode layout", lambda: nn.linear_distillation(x, weight, index, tensor(flat)))
+        refused(ValueError, "index must have", lambda: nn.linear_distillation(x, weight, tensor(kw["index"][:5]),
+                                                                              tensor(kw["logits"])))
+
+
 if __name__ == "__main__":
     for name in sys.argv[1:]:
         globals()[name]()
