@@ -176,7 +176,14 @@ def _head_vector(t: Any, name: str, dtype: Any, size: int) -> int:
     return t.carrier.data_ptr + 4 * t.offset
 
 
-def _head_upstream(t: Any, size: int) -> tuple[int, Any]:
+def _same_device(x: Tensor, *others: tuple[Any, str]) -> None:
+    """Refuses a tensor on another device than x's: a kernel cannot reach its memory."""
+    for t, name in others:
+        if t.carrier.device != x.carrier.device:
+            raise ValueError(f"{name} is on device {t.carrier.device}, x on device {x.carrier.device}")
+
+
+def _head_upstream(t: Any, size: int, x: Tensor) -> tuple[int, Any]:
     """Address of a gradient's `size` Float32 elements, and what keeps them: the
     gradient itself where it is contiguous, else a copy (a broadcast sum's
     gradient has stride 0)."""
@@ -188,11 +195,14 @@ def _head_upstream(t: Any, size: int) -> tuple[int, Any]:
         leaves = mode_leaves(t.layout, 0)
         if single_stride(leaves) not in ((size, 1), (1, 0)) or t.carrier.swizzle is not None:
             t._require_single_subtensor("CUDA linear head loss")
+            _same_device(x, (t, "gradient"))
             dense = CUDA(size, dtype=DType.Float32, empty=True, device=t.carrier.device)
             kernels.copy_view_f32(t.carrier.data_ptr, t.carrier.size(), t.offset, leaves, [(1, 0)], dense.data_ptr,
                                   size, 0, [(size, 1)], [(1, 0)], swizzle=swizzle_stages(t.carrier))
             return dense.data_ptr, dense
-    return _head_vector(t, "gradient", DType.Float32, size), t
+    ptr = _head_vector(t, "gradient", DType.Float32, size)
+    _same_device(x, (t, "gradient"))
+    return ptr, t
 
 
 class _LinearHeadLoss(Operation):
@@ -210,7 +220,12 @@ class _LinearHeadLoss(Operation):
             raise ValueError("Matmul inner dimensions must match")
         if dtype != dtype2:
             raise TypeError("x and weight must share their dtype")
+        _same_device(x, (weight, "weight"), *self._others(T))
         return (dtype, xp, xs, wp, ws, T, V, D), T
+
+    def _others(self, T: int) -> tuple[tuple[Any, str], ...]:
+        """Checks the tensors beside x and weight, of T rows, and names them."""
+        raise NotImplementedError
 
     def _outputs(self, x: Any, T: int) -> tuple[Tensor, Any]:
         from .carrier import CUDA
@@ -245,7 +260,7 @@ class _LinearHeadLoss(Operation):
     def backward(self, gradient: Any) -> tuple[Any, Any]:
         x, weight = self.inputs()
         head, T = self._shape(x, weight)
-        up, held = _head_upstream(gradient, 1 if self.reduction == "mean" else T)
+        up, held = _head_upstream(gradient, 1 if self.reduction == "mean" else T, x)
         dx, dw, where = self._gradients(x, weight)
         self._run(head, lse_ptr=self.ctx["lse"].data_ptr, upstream_ptr=up, **where)
         del held  # (released in stream order)
@@ -264,6 +279,10 @@ class CudaLinearCrossEntropy(_LinearHeadLoss):
     ignore_index = -100
     logit_scale = 1.0
 
+    def _others(self, T: int) -> tuple[tuple[Any, str], ...]:
+        _head_vector(self.targets, "targets", DType.Int32, T)
+        return ((self.targets, "targets"),)
+
     def _run(self, head: tuple, **kw: Any) -> None:
         from . import kernels
 
@@ -277,15 +296,21 @@ class CudaLinearDistillation(_LinearHeadLoss):
     logits: Any = None
     temperature = 1.0
 
-    def _run(self, head: tuple, **kw: Any) -> None:
-        from . import kernels
-
+    def _others(self, T: int) -> tuple[tuple[Any, str], ...]:
         for t, name in ((self.index, "index"), (self.logits, "logits")):
             if not isinstance(t, Tensor) or len(t.layout) != 2:
                 raise ValueError(f"{name} must have a two-mode layout [tokens, entries]")
         top_k = mode_size(self.index.layout, 1)
         if mode_size(self.logits.layout, 1) != top_k:
             raise ValueError(f"logits must have {top_k} entries a row, as index has")
+        _head_vector(self.index, "index", DType.Int32, T * top_k)
+        _head_vector(self.logits, "logits", DType.Float32, T * top_k)
+        return (self.index, "index"), (self.logits, "logits")
+
+    def _run(self, head: tuple, **kw: Any) -> None:
+        from . import kernels
+
+        top_k = mode_size(self.index.layout, 1)
         kernels.linear_distillation(*head, _head_vector(self.index, "index", DType.Int32, head[5] * top_k),
                                     _head_vector(self.logits, "logits", DType.Float32, head[5] * top_k), top_k,
                                     temperature=self.temperature, reduction=self.reduction, **kw)

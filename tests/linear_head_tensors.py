@@ -148,6 +148,30 @@ def teacher_shapes():
                                                                               tensor(kw["logits"])))
 
 
+def devices():
+    """A carrier that says it is on another device is refused before anything is launched."""
+
+    def elsewhere(t):
+        t.carrier._device = 1
+        return t
+
+    for dtype, h, w, op, kw in cases(("rows",)):
+        x, weight = tensor(h), tensor(w)
+        refused(ValueError, "weight is on device 1", lambda: loss_of(op, x, elsewhere(tensor(w)), kw, "mean"))
+        if op == "xent":
+            refused(ValueError, "targets is on device 1",
+                    lambda: nn.linear_cross_entropy(x, weight, elsewhere(tensor(kw["targets"]))))
+        else:
+            for bad in ("index", "logits"):
+                two = {n: elsewhere(tensor(kw[n])) if n == bad else tensor(kw[n]) for n in ("index", "logits")}
+                refused(ValueError, f"{bad} is on device 1", lambda: nn.linear_distillation(x, weight, **two))
+        loss = loss_of(op, x, weight, kw, "none")
+        refused(ValueError, "gradient is on device 1",
+                lambda: loss.backward(elsewhere(tensor(torch.ones(T, device="cuda")))))
+        refused(ValueError, "gradient is on device 1",
+                lambda: loss.backward(elsewhere(tensor(torch.ones(2 * T, device="cuda")[::2]))))
+
+
 if __name__ == "__main__":
     for name in sys.argv[1:]:
         globals()[name]()

@@ -15,7 +15,7 @@ pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
 
-@pytest.mark.parametrize("check", ["autograd", "one_call", "upstream_placements", "teacher_shapes"])
+@pytest.mark.parametrize("check", ["autograd", "one_call", "upstream_placements", "teacher_shapes", "devices"])
 def test_tensors(check):
     script = Path(__file__).resolve().parent / "linear_head_tensors.py"
     out = subprocess.run([sys.executable, str(script), check], capture_output=True, text=True, timeout=300)
