@@ -209,8 +209,18 @@ def _linear_head(dtype: str, h_strides: Sequence[int], w_strides: Sequence[int],
         raise ValueError(f"unknown reduction {reduction!r}")
     dh = (dim, 1) if dh_strides is None else dh_strides
     dw = (dim, 1) if dw_strides is None else dw_strides
+    for name, pair in (("h", h_strides), ("w", w_strides), ("dh", dh), ("dw", dw)):
+        if len(pair) != 2:
+            raise ValueError(f"{name}_strides must be the strides of rows and columns (got {len(pair)})")
     return N.LinearHead(HEAD_DTYPES[dtype], HEAD_REDUCTIONS[reduction], tokens, dim, vocab, *h_strides, *w_strides,
                         *dh, *dw, workspace_limit)
+
+
+def _int32(value: int, name: str) -> int:
+    """A value that the C call takes as 32 bits (ctypes would drop the others)."""
+    if not -(2 ** 31) <= value < 2 ** 31:
+        raise ValueError(f"{name} must fit 32 bits (got {value})")
+    return value
 
 
 def linear_cross_entropy(dtype: str, h_ptr: int, h_strides: Sequence[int], w_ptr: int, w_strides: Sequence[int],
@@ -226,9 +236,9 @@ def linear_cross_entropy(dtype: str, h_ptr: int, h_strides: Sequence[int], w_ptr
     lse at ``lse_ptr``.  See sw_linear_xent."""
     plan = _linear_head(dtype, h_strides, w_strides, tokens, vocab, dim, reduction, dh_strides, dw_strides,
                         workspace_limit)
-    N.check(N.lib.sw_linear_xent(byref(plan), h_ptr or None, w_ptr or None, targets_ptr or None, ignore_index,
-                                 logit_scale, loss_ptr or None, lse_ptr or None, upstream_ptr or None, dh_ptr or None,
-                                 dw_ptr or None, stream or None))
+    N.check(N.lib.sw_linear_xent(byref(plan), h_ptr or None, w_ptr or None, targets_ptr or None,
+                                 _int32(ignore_index, "ignore_index"), logit_scale, loss_ptr or None, lse_ptr or None,
+                                 upstream_ptr or None, dh_ptr or None, dw_ptr or None, stream or None))
 
 
 def linear_distillation(dtype: str, h_ptr: int, h_strides: Sequence[int], w_ptr: int, w_strides: Sequence[int],
@@ -244,5 +254,5 @@ def linear_distillation(dtype: str, h_ptr: int, h_strides: Sequence[int], w_ptr:
     plan = _linear_head(dtype, h_strides, w_strides, tokens, vocab, dim, reduction, dh_strides, dw_strides,
                         workspace_limit)
     N.check(N.lib.sw_linear_distill(byref(plan), h_ptr or None, w_ptr or None, index_ptr or None, logits_ptr or None,
-                                    top_k, temperature, loss_ptr or None, lse_ptr or None, upstream_ptr or None,
-                                    dh_ptr or None, dw_ptr or None, stream or None))
+                                    _int32(top_k, "top_k"), temperature, loss_ptr or None, lse_ptr or None,
+                                    upstream_ptr or None, dh_ptr or None, dw_ptr or None, stream or None))
