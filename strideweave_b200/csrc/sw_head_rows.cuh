@@ -907,7 +907,7 @@ __global__ void __launch_bounds__(256) unpad_kernel(const E* src, int64_t ld, in
         for (int64_t v = first; v < vectors; v += step) {
             const int64_t f = head + v * kPer;
             int64_t r = f / cols, c = f - r * cols;
-            E e[kPer];
+            __align__(16) E e[kPer];
 #pragma unroll
             for (int j = 0; j < kPer; ++j) {
                 e[j] = src[r * ld + c];
