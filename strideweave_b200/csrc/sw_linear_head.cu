@@ -762,9 +762,10 @@ Shape make_plan(const Call& c, bool keep, int64_t rows, int64_t piece, int64_t s
                               0.97f * choose_parts(nl, nv, D, terms, kPair2, false).us
                          ? kSingle
                          : kPair2;
-    // Where 256-column tiles would leave SMs idle, narrower ones spread the weights
-    // over more of them: the loss of one token over 32000 classes at dim 4096 65 us
-    // at 256 columns, 61 at 128; Float32 33 x 1021 at dim 257 with gradients 55, 49 at 64.
+    // Where 256-column tiles would leave SMs idle, and 128 or 64 columns still make one
+    // wave, those spread the weights over more of them: the loss of one token over 16000
+    // classes at dim 4096 44.1 us at 256 columns, 41.0 at 128, over 8000 40.2, 34.6 at 64;
+    // Float32 33 x 1021 at dim 257 with gradients 53.3, 47.6 at 64.
     s.tile_n = kBN;
     if (s.logits_shape == kSingle)
         for (const int t : {128, 64})
