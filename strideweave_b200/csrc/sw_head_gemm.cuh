@@ -809,15 +809,15 @@ __device__ __forceinline__ void out_tile(const Problem& args, const void* tmap_c
 // of the workers each first, see Plan).  The tensor cores bound it, and under
 // long load the power limit; a tile's epilogue runs under the next tile's MMAs:
 //
-//   4096 x 32000, dim 4096: logits with statistics and their exponentials 699 us
-//   (tensor pipe 90 % busy), dh 691 (93 %), dw 685 (91 %): 1.54, 1.55, 1.57 PFLOP/s;
-//   dim 2048: 436 (75 %), 349 (96 %), 328 (89 %).  The logits of short walks stay
-//   behind: at dim 1024 a 256 x 256 tile lasts about 10000 cycles, its epilogue
+//   4096 x 32000, dim 4096: logits with statistics and their exponentials 710 us
+//   (tensor pipe 91 % busy), dh 694 (93 %), dw 686 (91 %): 1.51, 1.55, 1.57 PFLOP/s;
+//   3891 rows, dim 2048: 430 (76 %), 349 (96 %), 326 (89 %).  The logits of short walks
+//   stay behind: at dim 1024 a 256 x 256 tile lasts about 10000 cycles, its epilogue
 //   5400, with the exponentials' store 9500.
-//   Float32, 2048 x 32000, dim 1024, three plane pairs: 298 (80 %), 297 (86 %), 304
-//   (74 %): 1.35, 1.35, 1.32 PFLOP/s of f16 products.
-//   1 x 32000, dim 4096: 54 us, the read of w at 4.8 TB/s; 64 x 131072, dim 2048:
-//   102 us, 5.3 TB/s, both gradients in one launch 206 us, 5.2 TB/s.
+//   Float32, 2048 x 32000, dim 1024, three plane pairs: 308 (75 %), 295 (88 %), 301
+//   (75 %): 1.31, 1.36, 1.34 PFLOP/s of f16 products.
+//   1 x 32000, dim 4096: 52 us, the read of w at 5.0 TB/s; 64 x 131072, dim 2048:
+//   105 us, 5.1 TB/s, both gradients in one launch 208 us, 5.2 TB/s.
 template <int kShape, bool kBf16, int kEpi, int kA>
 __global__ void __launch_bounds__(320, 1)
     head_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmArgs args) {

@@ -192,7 +192,7 @@ __device__ __forceinline__ void sort_teacher_row(const PrepareArgs& a, int64_t t
 // others.  It then leaves what its rows need: the target entries, the factor of
 // their gradient, and in bf16 the states themselves, gathered; the places of
 // rows that do not count are zeros.  Bound by the states' way through (4096 x
-// 4096: 18.8 us, 3.6 TB/s read and written), else by latency (64 rows of 32
+// 4096: 17.5 us, 3.8 TB/s read and written), else by latency (64 rows of 32
 // teacher entries 16 us, most of it the ranks, K comparisons for each entry).
 template <int kRows>
 __global__ void __launch_bounds__(256) prepare_kernel(const PrepareArgs a) {
@@ -386,9 +386,9 @@ struct SplitJob {
 // Largest finite magnitudes of one or two matrices, for the power of two that
 // brings them into f16's range, and of their rows, for whether that will do: a
 // warp per row, or where columns are contiguous a CTA per 32 rows, or per part of
-// them where rows are few.  Bound by one read (32000 x 1024
-// Float32 29 us, 4.8 TB/s; rows that are not whole vectors, 60000 x 1001, 67 us with
-// eight reads a lane in flight, 86 with four).
+// them where rows are few.  Bound by one read (32000 x 2048 Float32 with 900 states
+// 51 us, 5.3 TB/s; rows that are not whole vectors, 60000 x 1001, 67 us with eight
+// reads a lane in flight, 86 with four).
 __global__ void __launch_bounds__(256, 5) amax_kernel(const SplitJob j0, const SplitJob j1, HeadState* state) {
     __shared__ uint32_t s_top[8], s_least[8], s_row[8][32];
     pdl_enter();
@@ -502,7 +502,7 @@ __global__ void __launch_bounds__(256, 5) amax_kernel(const SplitJob j0, const S
 // One or two matrices into operands [rows_pad][ld]: a copy of bf16 values, or
 // two f16 planes of a Float32 value times 2^q (hi rounded to nearest, lo the
 // rest), or three bf16 ones.  Rows past the ones that count are zero.  Bound by a read and a write of
-// the matrix (32000 x 1024 Float32 with its 2048 states 55 us, 5.0 TB/s; bf16
+// the matrix (32000 x 1024 Float32 with its 2048 states 57 us, 4.9 TB/s; bf16
 // 60000 x 1001, which TMA cannot read, 56 us, 4.3 TB/s).  Rows that are not whole
 // vectors are read element by element: aligned vectors shifted into place took
 // the same time.
@@ -638,8 +638,8 @@ struct LossArgs {
 // sure of its target would have left.  A thread takes 8 columns (bf16), a warp a block of 64
 // (Float32: hi and lo values replace the block they were computed from).  The
 // last row to be done adds up the mean, in a fixed order.  Bound by the
-// exponentials' read and write, part of them still in L2: 4096 x 32000 109 us, 4.8
-// TB/s (Float32 2048 x 32000 115).  One reference for a whole row instead of one a
+// exponentials' read and write, part of them still in L2: 4096 x 32000 110 us, 4.8
+// TB/s (Float32 2048 x 32000 116).  One reference for a whole row instead of one a
 // half tile would spare this pass, at the cost of one more 16-bit rounding, of
 // the states in dw, and of a target's exact -1: not taken.
 template <bool kF32>

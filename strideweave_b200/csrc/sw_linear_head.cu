@@ -19,8 +19,8 @@
 // A loss with gradients in one call: the tiles also leave exp2(s - max) of
 // their own maxima, 16 bits each (Float32: 32), loss_kernel turns them into G
 // in place once it knows the row's sum, and two contractions take G to dh and
-// dw: 6 T V D and one pass over T V values.  That pass costs 109 us of the
-// 1440 of 4096 x 32000 x 2048; computing the logits again 430.  Where the
+// dw: 6 T V D and one pass over T V values.  That pass costs 110 us of the
+// 1464 of 4096 x 32000 x 2048; computing the logits again 430.  Where the
 // workspace limit holds fewer rows, the rows go in blocks, dh and dw added up
 // in fp32.
 //
@@ -36,10 +36,10 @@
 // out there.
 //
 // What bounds it: the contractions on the tensor cores, under the power limit
-// for the large steps (8192 x 131072 x 4096: 21.7 ms on a GPU that runs a
-// library's three products alone in 19.1, and 2.69 against 2.39 ms at 4096 x
-// 32000 x 4096); for few rows the bytes of w (64 x 131072 x 2048: 394 us for two
-// reads and a write of it, 4.1 TB/s).
+// for the large steps (8192 x 131072 x 4096: 21.1 ms on a GPU that runs a
+// library's three products alone in 19.1, and 2.71 against 2.39 ms at 4096 x
+// 32000 x 4096); for few rows the bytes of w (64 x 131072 x 2048: 405 us for two
+// reads and a write of it, 4.0 TB/s).
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -206,7 +206,8 @@ int launch_gemm(const Tensors* t, GemmArgs& args, cudaStream_t stream) {
 // bf16: 16 (the loss of 1400 x 50001 off by 7e-7); for one row tile, whose errors
 // less averages out and which the read of w bounds, 8 (64 x 131072 with gradients 4
 // us of 397 more, 4 stages 12), or 2 where no exponentials are written (one token's
-// loss off by 8e-8, at 16 by 1.1e-5, in the same 61 us).  The same for the logits of a
+// loss, over 40 inputs, off by 3.1e-6 at most, as a plain Float32 product's by 5.4e-6;
+// at 16 one of them by 1.1e-5, in the same time).  The same for the logits of a
 // gradient from a kept lse as for the loss that left it: both drift alike.
 int chunk_stages(bool bf16, int epi, const GemmArgs& args) {
     const Problem& p = args.p[0];
